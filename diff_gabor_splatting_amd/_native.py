@@ -217,6 +217,38 @@ _SIGNATURES = {
     "gs_profile_read": (_c_int, [_c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_c_i64)]),
     "gs_diagnostics_query": (_c_int, [ctypes.POINTER(_c_int), ctypes.POINTER(_c_int)]),
     "gs_diagnostics_set": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr]),
+    "gs_checkpoint8_write": (_c_int, [_c_int, _c_ptr] + [_c_i64] * 3 + [_c_ptr] * 3),
+    "gs_checkpoint8_read": (_c_int, [_c_int] + [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 2),
+    "gs_activation_forward": (
+        _c_int, [_c_int, _c_int, _c_float, _c_ptr] + [_c_i64] * 3 + [_c_ptr] * 4,
+    ),
+    "gs_activation_backward": (
+        _c_int,
+        [_c_int, _c_int, _c_float, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 2,
+    ),
+    "gs_layer_norm_forward": (
+        _c_int,
+        [_c_int, _c_int, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_float] + [_c_i64] * 2
+        + [_c_ptr] * 5,
+    ),
+    "gs_layer_norm_backward_workspace_size": (_c_size, [_c_i64] * 2),
+    "gs_layer_norm_backward": (
+        _c_int,
+        [_c_int, _c_int, _c_ptr, _c_i64, _c_ptr, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 2
+        + [_c_ptr] * 4 + [_c_size, _c_ptr],
+    ),
+    "gs_linear_forward": (
+        _c_int, [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 3 + [_c_ptr] * 4,
+    ),
+    "gs_linear_backward_input": (
+        _c_int, [_c_int, _c_ptr, _c_i64, _c_ptr] + [_c_i64] * 3 + [_c_ptr] * 2,
+    ),
+    "gs_linear_backward_weight_workspace_size": (_c_size, [_c_int] + [_c_i64] * 3),
+    "gs_linear_backward_weight": (
+        _c_int,
+        [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 3 + [_c_ptr] * 3
+        + [_c_size, _c_ptr],
+    ),
 }
 
 PROFILE_FAMILIES = {

@@ -9,8 +9,8 @@ library links the HIP runtime by its SONAME (``libamdhip64.so.7``), so when it
 is loaded after ``import torch`` it binds to the runtime torch already loaded
 and shares torch's streams and allocations.
 
-The renderer's host functions (``csrc/host.cpp``) are a Python extension
-module, ``diff_gabor_splatting_amd/_host*.so``, compiled with the host C++
+The host functions (``csrc/host.cpp`` for the renderer, ``csrc/layers_host.cpp``
+for the decoder's layers) are a Python extension module, ``diff_gabor_splatting_amd/_host*.so``, compiled with the host C++
 compiler against the installed torch (:func:`build_host`); it calls the HIP
 library's C ABI through function addresses handed over at import.
 
@@ -35,7 +35,7 @@ INCLUDE_DIR = REPO_DIR / "include"
 BUILD_DIR = REPO_DIR / "_build"
 LIBRARY = PACKAGE_DIR / "libgabor_hip.so"
 DIAGNOSTICS_LIBRARY = PACKAGE_DIR / "libgabor_hip_diag.so"
-HOST_SOURCE = SOURCE_DIR / "host.cpp"
+HOST_SOURCES = [SOURCE_DIR / "host.cpp", SOURCE_DIR / "layers_host.cpp"]
 HOST_EXTENSION = PACKAGE_DIR / ("_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 ROCM_DIR = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("GABOR_HIP_ARCH", "gfx950")
@@ -112,7 +112,7 @@ def build_library(verbose: bool = False, diagnostics: bool = False) -> Path:
 
 
 def build_host(verbose: bool = False) -> Path:
-    """Compile the renderer's C++ host functions into the ``_host`` extension
+    """Compile the C++ host functions into the ``_host`` extension
     module (no device code: the host compiler and torch's headers)."""
     import torch
     from torch.utils import cpp_extension
@@ -123,21 +123,33 @@ def build_host(verbose: bool = False) -> Path:
     torch_libraries = cpp_extension.library_paths()
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
                 str(ROCM_DIR / "include"), str(INCLUDE_DIR)]
-    temporary = HOST_EXTENSION.with_name(HOST_EXTENSION.name + ".tmp")
-    cmd = [
-        compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
         "-DTORCH_EXTENSION_NAME=_host", "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *(f"-I{path}" for path in includes),
-        str(HOST_SOURCE), "-o", str(temporary),
-        *(f"-L{path}" for path in torch_libraries),
-        *(f"-Wl,-rpath,{path}" for path in torch_libraries),
-        "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lamdhip64",
     ]
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if result.returncode != 0:
-        raise RuntimeError(f"{compiler} failed on {HOST_SOURCE.name}:\n{result.stdout}{result.stderr}")
+
+    def run(arguments, what):
+        result = subprocess.run([compiler, *arguments], capture_output=True, text=True)
+        if result.returncode != 0:
+            raise RuntimeError(f"{compiler} failed on {what}:\n{result.stdout}{result.stderr}")
+
+    def compile_source(source):
+        obj = BUILD_DIR / (source.stem + "_cpp.o")
+        run([*flags, "-c", str(source), "-o", str(obj)], source.name)
+        return obj
+
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(len(HOST_SOURCES)) as pool:
+        objects = list(pool.map(compile_source, HOST_SOURCES))
+    temporary = HOST_EXTENSION.with_name(HOST_EXTENSION.name + ".tmp")
+    run(["-shared", *map(str, objects), "-o", str(temporary),
+         *(f"-L{path}" for path in torch_libraries),
+         *(f"-Wl,-rpath,{path}" for path in torch_libraries),
+         "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lamdhip64"],
+        HOST_EXTENSION.name)
     os.replace(temporary, HOST_EXTENSION)
     if verbose:
         print(f"built {HOST_EXTENSION}", file=sys.stderr)

@@ -1,0 +1,379 @@
+// 8-bit checkpoints written and read, and activations that keep their input
+// in that form (see kept8.hpp for the format).
+//
+//   activation: y = f(z);  dz = dy f'(z8), z8 the kept z
+//     sine  f = sin(omega z)      f' = omega cos(omega z)
+//     gelu  f = z Phi(z)          f' = Phi(z) + z phi(z)
+//     silu  f = z s, s = 1 / (1 + exp(-z))   f' = s (1 + z (1 - s))
+//
+// All four kernels read and write each byte once; a lane takes eight
+// features (16 bytes of a 2-byte type), so four lanes hold a group and its
+// largest magnitude takes two quad permutations, no memory.
+#include "kept8.hpp"
+#include "layers_api.hpp"
+
+namespace gs {
+namespace {
+
+constexpr int kBlock = 256;
+
+// Where a lane's chunk lies. Flat: rows follow each other without padding
+// and hold whole groups, so that the chunk's number is its place. Otherwise
+// the block's first chunk is divided into row and chunk once, in 64 bits and
+// for all lanes alike, and the lanes divide what remains in 32 bits.
+struct Rows {
+  int64_t rows, features, stride;
+  uint32_t per_row;  // chunks of a row, padding included
+};
+
+struct Place {
+  int64_t row;
+  uint32_t chunk;
+};
+
+__device__ __forceinline__ Place place(const Rows& r, int64_t first, uint32_t local) {
+  const int64_t row0 = first / r.per_row;
+  const uint32_t rest = uint32_t(first - row0 * r.per_row) + local;
+  const uint32_t down = rest / r.per_row;
+  return {row0 + down, rest - down * r.per_row};
+}
+
+// What a launch does with each chunk: Op::apply(in, out, ...) is inlined
+// into one loop over the thread's chunks.
+enum Kind { kSine = GS_ACTIVATION_SINE, kGelu = GS_ACTIVATION_GELU, kSilu = GS_ACTIVATION_SILU };
+
+// sin and cos of 2 pi r for r = z (high + low), high + low = omega / 2 pi:
+// the product's fraction is taken with fused multiply-adds, so the phase
+// has no rounding error of its size. |f| <= 1/2 revolution.
+__device__ __forceinline__ float turn(float z, float high, float low) {
+  const float k = rintf(z * high);
+  return __builtin_fmaf(z, low, __builtin_fmaf(z, high, -k));
+}
+
+// sin(2 pi f), |f| <= 1/2 and a rounding error more: reflected at 1/4, then
+// the Taylor polynomial of sin to the 13th degree on [-pi/2, pi/2], whose
+// first omitted term is below 7e-10.
+__device__ __forceinline__ float sine_of_turn(float f) {
+  const float a = fabsf(f);
+  const float r = copysignf(a > 0.25f ? 0.5f - a : a, f) * 6.283185307179586f;
+  const float s = r * r;
+  float p = 1.6059043836821613e-10f;
+  p = __builtin_fmaf(p, s, -2.5052108385441720e-8f);
+  p = __builtin_fmaf(p, s, 2.7557319223985893e-6f);
+  p = __builtin_fmaf(p, s, -1.9841269841269841e-4f);
+  p = __builtin_fmaf(p, s, 8.3333333333333333e-3f);
+  p = __builtin_fmaf(p, s, -1.6666666666666667e-1f);
+  return __builtin_fmaf(p * s, r, r);
+}
+
+struct Parameters {
+  float omega, high, low;
+};
+
+// Phi(z) and exp(-z^2/2): Abramowitz and Stegun 7.1.26 for erf(|z| / sqrt 2)
+// (absolute error below 1.5e-7), which shares its exponential with phi.
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& bell) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+  bell = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  float p = 1.061405429f;
+  p = __builtin_fmaf(p, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * p * t * bell;  // Phi(-|z|)
+  cdf = z < 0.f ? tail : 1.f - tail;
+}
+
+template <typename T, int K>
+__device__ __forceinline__ float value(float z, const Parameters& c) {
+  if constexpr (K == kSine) {
+    return sine_of_turn(turn(z, c.high, c.low));
+  } else if constexpr (K == kGelu) {
+    float cdf, bell;
+    normal_cdf(z, cdf, bell);
+    return z * cdf;
+  } else {
+    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+  }
+}
+
+template <typename T, int K>
+__device__ __forceinline__ float slope(float z, const Parameters& c) {
+  if constexpr (K == kSine) {
+    const float f = turn(z, c.high, c.low);
+    // cos(2 pi f) = sin(2 pi (1/4 - |f|))
+    return c.omega * sine_of_turn(0.25f - fabsf(f));
+  } else if constexpr (K == kGelu) {
+    float cdf, bell;
+    normal_cdf(z, cdf, bell);
+    return __builtin_fmaf(z * bell, 0.39894228040143268f, cdf);
+  } else {
+    const float s =
+        __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    return s * __builtin_fmaf(z, 1.f - s, 1.f);
+  }
+}
+
+constexpr int kNone = -1;
+
+// Writes the checkpoint of x (where values is not null) and, with an
+// activation, y.
+template <typename T, int K, bool Whole, bool Flat, int Each>
+__global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, Rows r,
+                                                      T* __restrict__ y,
+                                                      uint8_t* __restrict__ values,
+                                                      uint8_t* __restrict__ exponents,
+                                                      Parameters c) {
+  const int64_t total = r.rows * r.per_row;
+  const int64_t first = int64_t(blockIdx.x) * (kBlock * Each);
+  float v[Each][kChunk];
+  Place at[Each];
+  int valid[Each];
+#pragma unroll
+  for (int i = 0; i < Each; ++i) {
+    const uint32_t local = i * kBlock + threadIdx.x;
+    const bool live = first + local < total;
+    if constexpr (Flat) {
+      valid[i] = live ? kChunk : 0;
+      load8<T, true>(x + (first + local) * kChunk, valid[i], v[i]);
+    } else {
+      at[i] = place(r, first, local);
+      const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
+      valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
+      load8<T, Whole>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i], v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Each; ++i) {
+    const uint32_t local = i * kBlock + threadIdx.x;
+    if (first + local >= total) break;
+    const int64_t chunk = first + local;  // rows of the checkpoint follow each other
+    if (values) {
+      uint32_t exponent;
+      const uint2 bytes = keep8<T>(v[i], exponent);
+      *reinterpret_cast<uint2*>(values + chunk * kChunk) = bytes;
+      if ((threadIdx.x & 3) == 0) exponents[chunk >> 2] = uint8_t(exponent);
+    }
+    if constexpr (K != kNone) {
+      float f[kChunk];
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) f[j] = value<T, K>(v[i][j], c);
+      if constexpr (Flat)
+        store8<T, true>(y + chunk * kChunk, kChunk, f);
+      else
+        store8<T, Whole>(y + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
+                         f);
+    }
+  }
+}
+
+// Reads a checkpoint back, or applies an activation's derivative at it to dy.
+template <typename T, int K, bool Whole, bool Flat, int Each>
+__global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict__ values,
+                                                      const uint8_t* __restrict__ exponents,
+                                                      const T* __restrict__ dy, Rows r,
+                                                      T* __restrict__ out, Parameters c) {
+  const int64_t total = r.rows * r.per_row;
+  const int64_t first = int64_t(blockIdx.x) * (kBlock * Each);
+  float g[Each][kChunk];
+  uint2 bytes[Each];
+  uint32_t exponent[Each];
+  Place at[Each];
+  int valid[Each];
+#pragma unroll
+  for (int i = 0; i < Each; ++i) {
+    const uint32_t local = i * kBlock + threadIdx.x;
+    const int64_t chunk = first + local;
+    const bool live = chunk < total;
+    bytes[i] = make_uint2(0, 0);
+    exponent[i] = 0;
+    if (live) {
+      bytes[i] = *reinterpret_cast<const uint2*>(values + chunk * kChunk);
+      exponent[i] = exponents[chunk >> 2];
+    }
+    if constexpr (Flat) {
+      valid[i] = live ? kChunk : 0;
+      if constexpr (K != kNone) load8<T, true>(dy + chunk * kChunk, valid[i], g[i]);
+    } else {
+      at[i] = place(r, first, local);
+      const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
+      valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
+      if constexpr (K != kNone)
+        load8<T, Whole>(dy + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i],
+                        g[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Each; ++i) {
+    if (valid[i] <= 0) continue;
+    float v[kChunk];
+    read8(bytes[i], exponent[i], v);
+    if constexpr (K != kNone) {
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) v[j] = g[i][j] * slope<T, K>(v[j], c);
+    }
+    if constexpr (Flat)
+      store8<T, true>(out + (first + i * kBlock + threadIdx.x) * kChunk, kChunk, v);
+    else
+      store8<T, Whole>(out + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
+                       v);
+  }
+}
+
+// Chunks from which a thread takes four of them; below, one each fills more
+// of the chip.
+constexpr int64_t kFour = int64_t(4) * 256 * kBlock;
+
+template <typename F>
+int with_layout(const char* name, const Rows& r, bool whole, bool flat, F&& launch) {
+  const int64_t total = r.rows * r.per_row;
+  const bool four = total >= kFour;
+  const int64_t blocks = ceil_div(total, four ? 4 * kBlock : kBlock);
+  GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "%s: too many rows", name);
+  using std::bool_constant;
+  using one = std::integral_constant<int, 1>;
+  using all = std::integral_constant<int, 4>;
+  const dim3 grid{unsigned(blocks)};
+  if (flat)
+    four ? launch(grid, bool_constant<true>{}, bool_constant<true>{}, all{})
+         : launch(grid, bool_constant<true>{}, bool_constant<true>{}, one{});
+  else if (whole)
+    four ? launch(grid, bool_constant<true>{}, bool_constant<false>{}, all{})
+         : launch(grid, bool_constant<true>{}, bool_constant<false>{}, one{});
+  else
+    four ? launch(grid, bool_constant<false>{}, bool_constant<false>{}, all{})
+         : launch(grid, bool_constant<false>{}, bool_constant<false>{}, one{});
+  GS_LAUNCHED(name);
+  return GS_OK;
+}
+
+template <typename F>
+int with_kind(int32_t kind, F&& call) {
+  switch (kind) {
+    case kSine: return call(std::integral_constant<int, kSine>{});
+    case kGelu: return call(std::integral_constant<int, kGelu>{});
+    default: return call(std::integral_constant<int, kSilu>{});
+  }
+}
+
+Parameters parameters(float omega) {
+  const double turns = double(omega) / 6.283185307179586476925;
+  const float high = float(turns);
+  return {omega, high, float(turns - double(high))};
+}
+
+Rows rows_of(int64_t rows, int64_t features, int64_t stride) {
+  return {rows, features, stride, uint32_t(kept_groups(features) * (kGroup / kChunk))};
+}
+
+template <typename T, int K>
+int keep_rows(const char* name, const void* x, int64_t rows, int64_t features, int64_t stride,
+              void* y, void* values, void* exponents, float omega, hipStream_t s) {
+  const Rows r = rows_of(rows, features, stride);
+  const bool whole = whole_rows<T>(x, features, stride) &&
+                     (K == kNone || whole_rows<T>(y, features, features));
+  const bool flat = whole && stride == features && features % kGroup == 0;
+  return with_layout(name, r, whole, flat, [&](dim3 grid, auto w, auto f, auto each) {
+    keep_kernel<T, K, w.value, f.value, each.value><<<grid, kBlock, 0, s>>>(
+        static_cast<const T*>(x), r, static_cast<T*>(y), static_cast<uint8_t*>(values),
+        static_cast<uint8_t*>(exponents), parameters(omega));
+  });
+}
+
+template <typename T, int K>
+int read_rows(const char* name, const void* values, const void* exponents, const void* dy,
+              int64_t rows, int64_t features, int64_t stride, void* out, float omega,
+              hipStream_t s) {
+  const Rows r = rows_of(rows, features, stride);
+  const bool whole = whole_rows<T>(out, features, features) &&
+                     (K == kNone || whole_rows<T>(dy, features, stride));
+  const bool flat = whole && features % kGroup == 0 && (K == kNone || stride == features);
+  return with_layout(name, r, whole, flat, [&](dim3 grid, auto w, auto f, auto each) {
+    read_kernel<T, K, w.value, f.value, each.value><<<grid, kBlock, 0, s>>>(
+        static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),
+        static_cast<const T*>(dy), r, static_cast<T*>(out), parameters(omega));
+  });
+}
+
+int check_activation(int32_t kind, float omega) {
+  GS_REQUIRE(kind == kSine || kind == kGelu || kind == kSilu, GS_ERR_ARGUMENT,
+             "unknown activation %d", int(kind));
+  GS_REQUIRE(std::isfinite(omega), GS_ERR_ARGUMENT, "omega must be finite");
+  return GS_OK;
+}
+
+}  // namespace
+}  // namespace gs
+
+extern "C" {
+
+int gs_checkpoint8_write(int32_t dtype, const void* x, int64_t row_stride, int64_t rows,
+                         int64_t features, void* values, void* exponents, void* stream) {
+  using namespace gs;
+  clear_error();
+  GS_CHECK(check_rows("gs_checkpoint8_write", dtype, rows, features, row_stride));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && values && exponents, GS_ERR_ARGUMENT,
+             "null pointer passed to gs_checkpoint8_write");
+  return with_type(dtype, [&](auto zero) {
+    return keep_rows<decltype(zero), kNone>("checkpoint8 write", x, rows, features, row_stride,
+                                            nullptr, values, exponents, 0.f,
+                                            static_cast<hipStream_t>(stream));
+  });
+}
+
+int gs_checkpoint8_read(int32_t dtype, const void* values, const void* exponents, int64_t rows,
+                        int64_t features, void* out, void* stream) {
+  using namespace gs;
+  clear_error();
+  GS_CHECK(check_rows("gs_checkpoint8_read", dtype, rows, features, features));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(values && exponents && out, GS_ERR_ARGUMENT,
+             "null pointer passed to gs_checkpoint8_read");
+  return with_type(dtype, [&](auto zero) {
+    return read_rows<decltype(zero), kNone>("checkpoint8 read", values, exponents, nullptr, rows,
+                                            features, features, out, 0.f,
+                                            static_cast<hipStream_t>(stream));
+  });
+}
+
+int gs_activation_forward(int32_t dtype, int32_t kind, float omega, const void* x,
+                          int64_t row_stride, int64_t rows, int64_t features, void* y,
+                          void* values, void* exponents, void* stream) {
+  using namespace gs;
+  clear_error();
+  GS_CHECK(check_rows("gs_activation_forward", dtype, rows, features, row_stride));
+  GS_CHECK(check_activation(kind, omega));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && y && !values == !exponents, GS_ERR_ARGUMENT,
+             "null pointer passed to gs_activation_forward");
+  return with_type(dtype, [&](auto zero) {
+    return with_kind(kind, [&](auto k) {
+      return keep_rows<decltype(zero), k.value>("activation forward", x, rows, features,
+                                                row_stride, y, values, exponents, omega,
+                                                static_cast<hipStream_t>(stream));
+    });
+  });
+}
+
+int gs_activation_backward(int32_t dtype, int32_t kind, float omega, const void* grad_y,
+                           int64_t grad_stride, const void* values, const void* exponents,
+                           int64_t rows, int64_t features, void* grad_x, void* stream) {
+  using namespace gs;
+  clear_error();
+  GS_CHECK(check_rows("gs_activation_backward", dtype, rows, features, grad_stride));
+  GS_CHECK(check_activation(kind, omega));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(grad_y && values && exponents && grad_x, GS_ERR_ARGUMENT,
+             "null pointer passed to gs_activation_backward");
+  return with_type(dtype, [&](auto zero) {
+    return with_kind(kind, [&](auto k) {
+      return read_rows<decltype(zero), k.value>("activation backward", values, exponents, grad_y,
+                                                rows, features, grad_stride, grad_x, omega,
+                                                static_cast<hipStream_t>(stream));
+    });
+  });
+}
+
+}  // extern "C"

@@ -17,12 +17,6 @@
 // that when it switches to another build of the same sources (the
 // diagnostics library) these calls follow.
 
-#include <torch/extension.h>
-
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <hip/hip_runtime_api.h>
-
 #include <algorithm>
 #include <array>
 #include <atomic>
@@ -33,8 +27,10 @@
 #include <vector>
 
 #include "gabor_hip.h"
+#include "host.hpp"
 
 namespace py = pybind11;
+using namespace gs_host;
 
 namespace {
 
@@ -76,15 +72,6 @@ struct Api {
 Api api;
 bool bound = false;
 
-template <typename F>
-void take(const py::dict& table, const char* name, F& slot) {
-  if (!table.contains(name))
-    throw std::runtime_error(std::string("the entry point table lacks ") + name);
-  const auto address = table[name].cast<uintptr_t>();
-  if (address == 0) throw std::runtime_error(std::string("null address for ") + name);
-  slot = reinterpret_cast<F>(address);
-}
-
 // Entry point addresses by name (the library's exported symbols).
 void bind(const py::dict& table) {
   Api next;
@@ -111,12 +98,13 @@ void bind(const py::dict& table) {
   take(table, "gs_render_backward_workspace_size", next.render_backward_workspace_size);
   take(table, "gs_render_forward", next.render_forward);
   take(table, "gs_render_backward", next.render_backward);
+  bind_layers(table);
   api = next;
   bound = true;
 }
 
 std::vector<std::string> entry_points() {
-  return {"gs_last_error", "gs_check_values", "gs_scan_workspace_size", "gs_pack_visible",
+  std::vector<std::string> names = {"gs_last_error", "gs_check_values", "gs_scan_workspace_size", "gs_pack_visible",
           "gs_records_forward", "gs_records_backward_workspace_size", "gs_records_backward",
           "gs_bin_order_workspace_size", "gs_bin_order_count", "gs_bin_order_sort",
           "gs_bin_tiles_workspace_size", "gs_bin_tiles", "gs_bin_tiles_bounded",
@@ -124,12 +112,8 @@ std::vector<std::string> entry_points() {
           "gs_bin_blocks_tiles_workspace_size", "gs_bin_blocks_tiles",
           "gs_bin_blocks_tiles_bounded", "gs_render_workspace_size",
           "gs_render_backward_workspace_size", "gs_render_forward", "gs_render_backward"};
-}
-
-[[noreturn]] void fail(const std::string& message) { throw std::runtime_error(message); }
-
-inline void require(bool ok, const char* message) {
-  if (!ok) fail(message);
+  for (const std::string& name : layer_entry_points()) names.push_back(name);
+  return names;
 }
 
 void check(int status) {
@@ -145,28 +129,6 @@ void check_hip(hipError_t status, const char* what) {
 
 void require_bound() {
   if (!bound) fail("the HIP library's entry points are not bound (_host.bind)");
-}
-
-inline void* stream_of(const at::Device& device) {
-  return c10::hip::getCurrentHIPStream(device.index()).stream();
-}
-
-template <typename T>
-inline T* ptr(const at::Tensor& t) {
-  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
-}
-
-template <typename T>
-inline T* ptr(const std::optional<at::Tensor>& t) {
-  return t ? ptr<T>(*t) : nullptr;
-}
-
-inline at::TensorOptions on(const at::Device& device, at::ScalarType type) {
-  return at::TensorOptions().dtype(type).device(device);
-}
-
-at::Tensor workspace(size_t bytes, const at::Device& device) {
-  return at::empty({std::max<int64_t>(int64_t(bytes), 1)}, on(device, at::kByte));
 }
 
 void check_float(const at::Tensor& value, const at::Tensor& geometry) {
@@ -1166,4 +1128,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("rasterize_forward", &rasterize_forward);
   m.def("zero_accumulators", &zero_accumulators);
   m.def("rasterize_backward", &rasterize_backward);
+  define_layers(m);
 }

@@ -1,0 +1,773 @@
+"""The decoder layers against their formulas in 64 bits (oracle/layers.py).
+
+CPU: the 8-bit form's definition, argument errors of the C entry points and
+of the Python functions. GPU: every operator over types, widths, row counts,
+strides and special values.
+
+Tolerances are worst-case rounding bounds. With u the unit roundoff of the
+output type (2^-8 bfloat16, 2^-11 float16, 2^-24 float32; half a unit in the
+last place, relative) and e = 2^-24, an output that is computed in float32
+and rounded once is off by at most u |out| + the float32 error, and a
+float32 sum of n terms t by at most n e sum |t|.
+"""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle import layers as oracle
+
+gpu = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+E = 2.0 ** -24
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+# Below a type's normal range the spacing is fixed: half of it.
+FLOOR = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def layers():
+    from diff_gabor_splatting_amd import layers as module
+
+    return module
+
+
+def generator(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(*shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=generator(seed)) * scale).to(dtype)
+
+
+def near(got, expected, error, dtype):
+    """|got - expected| <= rounding to dtype + the float32 error, everywhere."""
+    got = got.detach().cpu().double()
+    assert got.shape == expected.shape
+    bound = UNIT[dtype] * (expected.abs() + error) + error + FLOOR[dtype]
+    off = (got - expected).abs()
+    worst = (off / bound).max().item() if got.numel() else 0.0
+    assert torch.isfinite(got).all() and worst <= 1.0, f"{worst:.3g} times the bound"
+
+
+# --------------------------------------------------------------------------
+# CPU
+
+
+def test_oracle_kept_is_the_first_exponent_that_is_enough():
+    x = torch.tensor([[127.5, 1.0] + [0.0] * 30, [127.49, -63.5] + [0.0] * 30,
+                      [0.0] * 32, [64.0, 0.5] + [0.0] * 30])
+    q, b, v = oracle.kept(x)
+    assert b[:, 0].tolist() == [128, 127, 1, 127]
+    assert q[0, :2].tolist() == [64, 0]      # 127.5 / 2 and 1 / 2, ties to even
+    assert q[1, :2].tolist() == [127, -64]   # 63.5 to the even 64
+    assert q[3, :2].tolist() == [64, 0]
+    assert v[0, 0] == 128 and v[2].abs().max() == 0
+
+
+def test_oracle_kept_error_is_within_a_step():
+    x = normal(50, 100, seed=3)
+    _, _, v = oracle.kept(x)
+    groups = torch.nn.functional.pad(x, (0, 28)).view(50, 4, 32).abs().amax(-1)
+    limit = groups.repeat_interleave(32, 1)[:, :100].double() / 127
+    assert ((v - x.double()).abs() <= limit).all()
+
+
+def test_oracle_gradients_match_autograd():
+    x, g = normal(6, 40, seed=4).double(), normal(6, 40, seed=5).double()
+    w, b = normal(40, seed=6).double(), normal(40, seed=7).double()
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = torch.nn.functional.layer_norm(x, (40,), w, b)
+    expected = torch.autograd.grad(y, (x, w, b), g)
+    dx, dw, db, _, _ = oracle.layer_norm_backward(x.detach(), g, w.detach())
+    torch.testing.assert_close(oracle.layer_norm(x, w, b)[0], y)
+    for got, want in zip((dx, dw, db), expected):
+        torch.testing.assert_close(got, want)
+    for kind, function in (("gelu", torch.nn.functional.gelu), ("silu", torch.nn.functional.silu),
+                           ("sine", lambda z: torch.sin(30 * z))):
+        y = function(x)
+        torch.testing.assert_close(oracle.activation(x, kind, 30.0), y)
+        torch.testing.assert_close(oracle.slope(x, kind, 30.0),
+                                   torch.autograd.grad(y.sum(), x)[0])
+
+
+def test_c_entry_points_refuse_bad_arguments():
+    from diff_gabor_splatting_amd import _native
+
+    lib, p = _native.lib, ctypes.c_void_p(256)
+
+    def refused(status, code, text):
+        assert status == code and text in lib.gs_last_error().decode(), lib.gs_last_error()
+
+    refused(lib.gs_checkpoint8_write(3, p, 8, 1, 8, p, p, None), 1, "unknown type")
+    refused(lib.gs_checkpoint8_write(0, p, 8, -1, 8, p, p, None), 1, "negative")
+    refused(lib.gs_checkpoint8_write(0, p, 8, 1, 0, p, p, None), 1, "features")
+    refused(lib.gs_checkpoint8_write(0, p, 7, 2, 8, p, p, None), 1, "overlap")
+    refused(lib.gs_checkpoint8_write(0, p, 8, 1 << 60, 8, p, p, None), 2, "too many rows")
+    refused(lib.gs_checkpoint8_write(0, None, 8, 1, 8, p, p, None), 1, "null")
+    refused(lib.gs_checkpoint8_read(0, p, None, 1, 8, p, None), 1, "null")
+    refused(lib.gs_activation_forward(0, 9, 1.0, p, 8, 1, 8, p, p, p, None), 1, "activation")
+    refused(lib.gs_activation_forward(0, 0, math.inf, p, 8, 1, 8, p, p, p, None), 1, "omega")
+    refused(lib.gs_activation_forward(0, 0, 1.0, p, 8, 1, 8, p, p, None, None), 1, "null")
+    refused(lib.gs_activation_backward(0, 0, 1.0, p, 8, None, p, 1, 8, p, None), 1, "null")
+    refused(lib.gs_layer_norm_forward(1, 2, p, 8, p, p, 1e-5, 1, 8, p, p, None, None, None), 1,
+            "parameters")
+    refused(lib.gs_layer_norm_forward(0, 0, p, 8, p, p, -1.0, 1, 8, p, p, None, None, None), 1,
+            "eps")
+    refused(lib.gs_layer_norm_forward(0, 0, p, 16385, p, p, 1e-5, 1, 16385, p, p, None, None,
+                                      None), 1, "at most 16384")
+    refused(lib.gs_layer_norm_forward(0, 0, p, 8, p, p, 1e-5, 1, 8, p, None, p, p, None), 1,
+            "null")
+    # Either x or what was kept, and a workspace for the parameters' gradients.
+    refused(lib.gs_layer_norm_backward(0, 0, p, 8, p, 8, p, p, p, p, 1, 8, p, p, p, p, 1 << 20,
+                                       None), 1, "null")
+    need = lib.gs_layer_norm_backward_workspace_size(100, 8)
+    refused(lib.gs_layer_norm_backward(0, 0, p, 8, p, 8, None, None, p, p, 100, 8, p, p, p, p,
+                                       need - 1, None), 4, "workspace")
+    refused(lib.gs_linear_forward(0, p, 8, None, None, 1, 8, 8, p, None, None, None), 1, "null")
+    refused(lib.gs_linear_forward(0, p, 8, p, None, 1, 8, 0, p, None, None, None), 1, "features")
+    refused(lib.gs_linear_forward(0, p, 8, p, None, 1, 8, 1 << 20, p, None, None, None), 1,
+            "at most")
+    refused(lib.gs_linear_backward_input(0, p, 3, p, 2, 8, 4, p, None), 1, "overlap")
+    need = lib.gs_linear_backward_weight_workspace_size(0, 100, 8, 4)
+    assert need > 0
+    refused(lib.gs_linear_backward_weight(0, p, 4, p, p, 100, 8, 4, p, p, p, need - 1, None), 4,
+            "workspace")
+    # No rows: nothing to do and nothing touched.
+    assert lib.gs_checkpoint8_write(0, None, 8, 0, 8, None, None, None) == 0
+    assert lib.gs_linear_forward(0, None, 8, None, None, 0, 8, 8, None, None, None, None) == 0
+    assert lib.gs_last_error() == b""
+
+
+def test_python_functions_refuse_cpu_tensors_and_bad_options():
+    m = layers()
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    for call in (lambda: m.quantize(x), lambda: m.activation(x), lambda: m.layer_norm(x),
+                 lambda: m.linear(x, w)):
+        with pytest.raises(ValueError, match="on a HIP device"):
+            call()
+    with pytest.raises(TypeError, match="x must be a torch.Tensor"):
+        m.quantize([1.0])
+    with pytest.raises(TypeError, match="must be a Checkpoint"):
+        m.dequantize(x)
+    with pytest.raises(ValueError, match="kind must be one of"):
+        m.activation(x, "tanh")
+    with pytest.raises(ValueError, match="omega"):
+        m.activation(x, omega=math.nan)
+    with pytest.raises(ValueError, match="checkpoint must be"):
+        m.layer_norm(x, checkpoint="4bit")
+    with pytest.raises(ValueError, match="eps"):
+        m.layer_norm(x, eps=-1.0)
+
+
+# --------------------------------------------------------------------------
+# GPU: the 8-bit form
+
+
+def gpu_test(function):
+    for mark in gpu:
+        function = mark(function)
+    return function
+
+
+def same_bytes(x, dtype):
+    m = layers()
+    kept = m.quantize(x.cuda())
+    q, b, v = oracle.kept(x.reshape(-1, x.shape[-1]))
+    assert torch.equal(kept.values.cpu(), q) and torch.equal(kept.exponents.cpu(), b)
+    back = m.dequantize(kept)
+    assert back.dtype == dtype and back.shape == x.shape
+    assert torch.equal(back.cpu().double().nan_to_num(7e77),
+                       v.reshape(x.shape).nan_to_num(7e77))
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 31), (3, 32), (5, 33), (2, 8), (7, 40), (7, 187),
+                                   (1000, 64), (513, 1000), (2, 3, 5, 96), (30000, 96),
+                                   (40000, 100)])
+def test_checkpoint_bytes(dtype, shape):
+    same_bytes(normal(*shape, seed=sum(shape), dtype=dtype, scale=3.0), dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_checkpoint_of_special_values(dtype):
+    most = torch.finfo(dtype).max
+    rows = [[0.0], [-0.0, 1.0], [most, -most, most / 3], [most / 1.01], [2.0 ** -24, 2.0 ** -20],
+            [torch.finfo(dtype).tiny, torch.finfo(dtype).smallest_normal / 4], [127.5, 0.25, 0.75],
+            [127.0, 63.5, 62.5, -0.5, 1.5], [127.49, 2.5], [math.inf, 1.0], [1.0, math.nan],
+            [-math.inf, math.inf], [1e-6, 1.0], [255.0], [254.9, 3.0]]
+    x = torch.zeros(len(rows), 70)
+    for i, row in enumerate(rows):
+        x[i, :len(row)] = torch.tensor(row)
+        x[i, 40:40 + len(row)] = torch.tensor(row) / 3
+    same_bytes(x.to(dtype), dtype)
+
+
+@gpu_test
+def test_checkpoint_reads_back_in_another_type():
+    m = layers()
+    x = normal(9, 50, seed=1, dtype=torch.bfloat16)
+    _, _, v = oracle.kept(x)
+    assert torch.equal(m.dequantize(m.quantize(x.cuda()), torch.float32).cpu().double(), v)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_checkpoint_of_strided_rows(dtype):
+    m = layers()
+    base = normal(12, 4, 200, seed=2, dtype=dtype)
+    views = {
+        "rows apart": lambda t: t[:, 1, :96],
+        "misaligned": lambda t: t[:, 2, 3:100],
+        "collapsing": lambda t: t[..., :64],
+        "not collapsing": lambda t: t[:, :3, 8:72],
+        "transposed": lambda t: t.transpose(0, 2),
+        "expanded": lambda t: t[:1, 0, :40].expand(6, 40),
+        "one feature": lambda t: t[:, :, :1],
+        "vector": lambda t: t[3, 1],
+        "every second": lambda t: t[:, 0, ::2],
+    }
+    for name, view in views.items():
+        got = m.quantize(view(base.cuda()))
+        want = view(base)
+        q, b, _ = oracle.kept(want.reshape(-1, want.shape[-1]))
+        assert torch.equal(got.values.cpu(), q) and torch.equal(got.exponents.cpu(), b), name
+
+
+# --------------------------------------------------------------------------
+# GPU: activations
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["sine", "gelu", "silu"])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 57), (64, 128), (5, 1000), (2, 4, 40), (9000, 256)])
+def test_activation(dtype, kind, shape):
+    m = layers()
+    scale = 0.2 if kind == "sine" else 3.0
+    x = normal(*shape, seed=11, dtype=dtype, scale=scale)
+    g = normal(*shape, seed=12, dtype=dtype)
+    on = x.cuda().requires_grad_()
+    y = m.activation(on, kind)
+    (dx,) = torch.autograd.grad(y, on, g.cuda())
+    z = oracle.kept(x.reshape(-1, shape[-1]))[2].reshape(shape)
+    want, slope = oracle.activation(x, kind, 30.0), oracle.slope(z, kind, 30.0)
+    # sine: the phase's fraction and the polynomial to a few units of 2^-24
+    # of their largest value; gelu: 1.5e-7 on erf (half of that on Phi), the
+    # hardware's exp2 and reciprocal; silu: the same two.
+    error = {"sine": 16 * E, "gelu": 8e-8 + 16 * E, "silu": 16 * E}[kind]
+    size = 1.0 if kind == "sine" else 1 + x.double().abs()
+    near(y, want, error * size, dtype)
+    wide = 30.0 if kind == "sine" else 1 + z.abs() + z * z
+    near(dx, g.double() * slope, g.double().abs() * error * wide, dtype)
+    # Without a gradient nothing is kept and the values are the same.
+    assert torch.equal(m.activation(x.cuda(), kind), y.detach())
+
+
+@gpu_test
+def test_activation_of_special_values():
+    m = layers()
+    x = torch.zeros(4, 64)
+    x[0, 0], x[1, 40], x[2, 3] = math.inf, -math.inf, math.nan
+    x[3, :4] = torch.tensor([1e30, -1e30, 88.0, -88.0])
+    for kind in ("gelu", "silu"):
+        on = x.cuda().requires_grad_()
+        y = m.activation(on, kind)
+        (dx,) = torch.autograd.grad(y, on, torch.ones_like(y))
+        assert y[0, 0] == math.inf and y[2, 3].isnan()
+        torch.testing.assert_close(y[3, :4].cpu(), torch.tensor([1e30, 0.0, 88.0, 0.0]),
+                                   atol=1e-30, rtol=1e-6)
+        # The whole group of a non-finite input has no derivative, no other.
+        lost = dx.isnan().cpu()
+        expected = torch.zeros(4, 64, dtype=torch.bool)
+        expected[0, :32] = expected[1, 32:] = expected[2, :32] = True
+        assert torch.equal(lost, expected)
+
+
+@gpu_test
+def test_sine_of_large_phases():
+    """The phase's fraction is taken without rounding the phase: at phases of
+    thousands the sine is as exact as at small ones."""
+    m = layers()
+    x = normal(64, 64, seed=13, scale=300.0)
+    y = m.activation(x.cuda(), "sine", 30.0).cpu().double()
+    assert (y - torch.sin(30 * x.double())).abs().max() < 1e-6
+
+
+# --------------------------------------------------------------------------
+# GPU: layer norm
+
+
+def norm_case(shape, dtype, weights, eight, seed=21, parameters=True, offset=0.5):
+    m = layers()
+    features = shape[-1]
+    x = (normal(*shape, seed=seed) + offset * normal(*shape[:-1], 1, seed=seed + 1)).to(dtype)
+    g = normal(*shape, seed=seed + 2, dtype=dtype)
+    w = (1 + 0.1 * normal(features, seed=seed + 3)).to(weights) if parameters else None
+    b = normal(features, seed=seed + 4, dtype=weights) if parameters else None
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b) if t is not None]
+    y = m.layer_norm(*inputs, checkpoint="8bit" if eight else "full")
+    grads = torch.autograd.grad(y, inputs, g.cuda())
+    check_norm(x.reshape(-1, features), g.reshape(-1, features), w, b, eight,
+               y.reshape(-1, features), [grads[0].reshape(-1, features), *grads[1:]])
+    with torch.no_grad():
+        assert torch.equal(m.layer_norm(*inputs), y)
+
+
+def check_norm(x, g, w, b, eight, y, grads, eps=1e-5):
+    rows, features = x.shape
+    dtype = x.dtype
+    want, h, r = oracle.layer_norm(x, w, b, eps)
+    # A lane adds at most 32 values in turn and then the lanes', 6 + 16 steps:
+    # the mean is off by n e of the mean magnitude, the variance, its root and
+    # h by as much relatively.
+    n = 64
+    size = x.double().abs().amax(1, keepdim=True) * r
+    spread = n * E * (size + h.abs())
+    scale = 1.0 if w is None else w.double().abs()
+    near(y, want, spread * scale + 4 * E * want.abs(), dtype)
+    dx, dw, db, h, r = oracle.layer_norm_backward(x, g, w, eps, eight)
+    a = g.double().abs() * scale
+    along = (a * h.abs()).mean(1, keepdim=True)
+    error = r * (n * E * (a + a.mean(1, keepdim=True) + h.abs() * along)
+                 + spread * along + h.abs() * (a * spread).mean(1, keepdim=True))
+    near(grads[0], dx, error, dtype)
+    if w is not None:
+        terms = n + rows / 16
+        near(grads[1], dw, (g.double().abs() * (terms * E * h.abs() + spread)).sum(0), w.dtype)
+        near(grads[2], db, terms * E * g.double().abs().sum(0), w.dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("features", [1, 7, 8, 31, 33, 64, 96, 187, 256, 512, 513, 520, 1000, 1024,
+                                      2048, 2056, 4099, 8192, 8200, 16384])
+def test_layer_norm_widths(features, eight):
+    # One feature leaves h = 0 and no variance: eps alone sets r.
+    norm_case((5, features), torch.float32, torch.float32, eight)
+    norm_case((67, features), torch.bfloat16, torch.bfloat16, eight, seed=31)
+
+
+@gpu_test
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("dtype,weights", [(torch.float32, torch.float32),
+                                           (torch.bfloat16, torch.float32),
+                                           (torch.bfloat16, torch.bfloat16),
+                                           (torch.float16, torch.float32),
+                                           (torch.float16, torch.float16)])
+@pytest.mark.parametrize("shape", [(1, 64), (2, 3, 5, 48), (4099, 40), (20011, 72)])
+def test_layer_norm(dtype, weights, eight, shape):
+    norm_case(shape, dtype, weights, eight)
+
+
+@gpu_test
+@pytest.mark.parametrize("eight", [False, True])
+def test_layer_norm_without_parameters_and_with_a_large_mean(eight):
+    norm_case((33, 128), torch.float32, torch.float32, eight, parameters=False)
+    norm_case((33, 128), torch.float32, torch.float32, eight, offset=300.0)
+
+
+@gpu_test
+def test_layer_norm_of_one_parameter():
+    m = layers()
+    x, w = normal(9, 48, seed=1).cuda(), normal(48, seed=2).cuda()
+    g = normal(9, 48, seed=3).cuda()
+    for name, other in (("weight", "bias"), ("bias", "weight")):
+        p = w.clone().requires_grad_()
+        y = m.layer_norm(x, **{name: p})
+        (got,) = torch.autograd.grad(y, p, g)
+        both = {name: w.clone().requires_grad_(),
+                other: (torch.ones_like(w) if other == "weight" else torch.zeros_like(w))}
+        z = m.layer_norm(x, **both)
+        assert torch.equal(y, z)
+        assert torch.equal(got, torch.autograd.grad(z, both[name], g)[0])
+
+
+@gpu_test
+@pytest.mark.parametrize("eight", [False, True])
+def test_layer_norm_keeps_a_bad_row_to_itself(eight):
+    """Rows with NaN or infinities give NaN in their own outputs and input
+    gradients, and leave other rows' untouched; a constant row is all bias."""
+    m = layers()
+    x = normal(40, 96, seed=5)
+    bad = x.clone()
+    bad[3, 7], bad[20, 95], bad[39, 0] = math.nan, math.inf, -math.inf
+    bad[10] = 0.25
+    x[10] = 0.25
+    w, b, g = normal(96, seed=6), normal(96, seed=7), normal(40, 96, seed=8)
+    outs = []
+    for t in (x, bad):
+        inputs = [v.cuda().requires_grad_() for v in (t, w, b)]
+        y = m.layer_norm(*inputs, checkpoint="8bit" if eight else "full")
+        outs.append((y, torch.autograd.grad(y, inputs, g.cuda())))
+    rows = torch.ones(40, dtype=torch.bool)
+    rows[[3, 20, 39]] = False
+    assert torch.equal(outs[0][0][rows.cuda()], outs[1][0][rows.cuda()])
+    assert torch.equal(outs[0][1][0][rows.cuda()], outs[1][1][0][rows.cuda()])
+    assert outs[1][0][~rows.cuda()].isnan().all() and outs[1][1][0][~rows.cuda()].isnan().all()
+    assert torch.equal(outs[1][0][10].cpu(), b)
+    assert torch.equal(outs[0][1][2], outs[1][1][2])  # the bias's gradient reads dy alone
+
+
+# --------------------------------------------------------------------------
+# GPU: linear layers
+
+
+def linear_case(shape, outputs, dtype, bias=True, seed=41):
+    m = layers()
+    features = shape[-1]
+    x = normal(*shape, seed=seed, dtype=dtype)
+    w = normal(outputs, features, seed=seed + 1, dtype=dtype, scale=features ** -0.5)
+    b = normal(outputs, seed=seed + 2, dtype=dtype) if bias else None
+    g = normal(*shape[:-1], outputs, seed=seed + 3, dtype=dtype)
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b) if t is not None]
+    y = m.linear(*inputs)
+    grads = torch.autograd.grad(y, inputs, g.cuda())
+    with torch.no_grad():
+        assert torch.equal(m.linear(*inputs), y)
+    assert y.shape == (*shape[:-1], outputs) and grads[0].shape == shape
+    x, g = x.reshape(-1, features), g.reshape(-1, outputs)
+    rows = x.shape[0]
+    size = oracle.linear(x.abs(), w.abs(), None if b is None else b.abs())
+    near(y.reshape(rows, outputs), oracle.linear(x, w, b), (features + 2) * E * size, dtype)
+    dx, dw, db = oracle.linear_backward(x, w, g)
+    near(grads[0].reshape(rows, features), dx,
+         (outputs + 2) * E * (g.double().abs() @ w.double().abs()), dtype)
+    held = oracle.kept(x)[2].abs()
+    near(grads[1], dw, (rows + 2) * E * (g.double().abs().t() @ held), dtype)
+    if bias:
+        near(grads[2], db, (rows + 2) * E * g.double().abs().sum(0), dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs", [
+    (1, 1, 1), (1, 64, 64), (1, 1000, 57), (2, 33, 18), (5, 8, 8), (16, 128, 128), (17, 31, 129),
+    (64, 96, 57), (127, 130, 63), (128, 64, 256), (129, 256, 130), (300, 187, 18),
+    (1000, 40, 72), (2500, 264, 136)])
+def test_linear(dtype, rows, features, outputs):
+    linear_case((rows, features), outputs, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_shapes_and_no_bias(dtype):
+    linear_case((2, 3, 4, 48), 24, dtype)
+    linear_case((40,), 24, dtype)
+    linear_case((50, 64), 32, dtype, bias=False)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_whole_numbers_is_exact(dtype):
+    """Small whole numbers: every product and sum is exact in float32, the
+    kept rows are the rows, so all outputs equal the formula's, in any order
+    of summation (and a wrong lane or a lost row shows)."""
+    m = layers()
+    gen = generator(9)
+    x = torch.randint(-3, 4, (700, 200), generator=gen).to(dtype)
+    w = torch.randint(-1, 2, (140, 200), generator=gen).to(dtype)
+    g = torch.randint(-1, 2, (700, 140), generator=gen).to(dtype)
+    inputs = [t.cuda().requires_grad_() for t in (x, w)]
+    y = m.linear(*inputs)
+    dx, dw = torch.autograd.grad(y, inputs, g.cuda())
+    for got, want in ((y, x.double() @ w.double().t()), (dx, g.double() @ w.double()),
+                      (dw, g.double().t() @ x.double())):
+        assert torch.equal(got.cpu(), want.to(dtype))
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_keeps_bad_values_to_their_place(dtype):
+    m = layers()
+    x, w, g = (normal(*s, seed=i, dtype=dtype) for i, s in enumerate(((200, 96), (40, 96),
+                                                                       (200, 40))))
+    x[150, 70] = math.inf
+    inputs = [t.cuda().requires_grad_() for t in (x, w)]
+    y = m.linear(*inputs)
+    dx, dw = torch.autograd.grad(y, inputs, g.cuda())
+    finite = torch.isfinite(y).all(1).cpu()
+    assert not finite[150] and finite.sum() == 199
+    assert torch.isfinite(dx).all()
+    # The infinity's group of features, and no other.
+    assert dw[:, 64:].isnan().all() and torch.isfinite(dw[:, :64]).all()
+
+
+# --------------------------------------------------------------------------
+# GPU: gradients against differences, and how the operators are called
+
+
+def loss_of(name, x, w, b, g):
+    if name == "layer_norm":
+        return (oracle.layer_norm(x, w, b)[0] * g).sum()
+    return (oracle.linear(x, w, b) * g).sum()
+
+
+@gpu_test
+@pytest.mark.parametrize("name", ["layer_norm", "linear"])
+def test_gradients_against_differences(name):
+    """Directional derivatives of the formulas by central differences in 64
+    bits (step 1e-5: truncation and rounding both below 1e-8 relative),
+    against float32 gradients of inputs that 8 bits keep without error, so
+    the kept rows are the rows."""
+    m = layers()
+    gen = generator(17)
+    x = torch.randint(-100, 101, (24, 64), generator=gen).float()
+    x[:, ::32] = 100.0
+    x[:, 1::32] = -100.0  # the middle of each row's range is 0
+    outputs = 64 if name == "layer_norm" else 40
+    w = normal(64, seed=1) if name == "layer_norm" else normal(40, 64, seed=1)
+    b, g = normal(outputs, seed=2), normal(24, outputs, seed=3)
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = m.layer_norm(*inputs, checkpoint="8bit") if name == "layer_norm" else m.linear(*inputs)
+    grads = torch.autograd.grad(y, inputs, g.cuda())
+    values = [t.double() for t in (x, w, b)]
+    for i, grad in enumerate(grads):
+        for seed in range(3):
+            v = normal(*values[i].shape, seed=50 + seed).double()
+            ends = []
+            for sign in (1, -1):
+                moved = list(values)
+                moved[i] = values[i] + sign * 1e-5 * v
+                ends.append(loss_of(name, *moved, g.double()))
+            slope = ((ends[0] - ends[1]) / 2e-5).item()
+            terms = grad.cpu().double() * v
+            assert abs(terms.sum().item() - slope) <= 1e-5 * terms.abs().sum().item() + 1e-6
+
+
+@gpu_test
+@pytest.mark.parametrize("kind", ["sine", "gelu", "silu"])
+def test_activation_gradient_against_differences(kind):
+    m = layers()
+    x, g = normal(20, 64, seed=1, scale=0.3), normal(20, 64, seed=2)
+    on = x.cuda().requires_grad_()
+    (dx,) = torch.autograd.grad(m.activation(on, kind), on, g.cuda())
+    z = oracle.kept(x)[2]
+    ends = [oracle.activation(z + sign * 1e-6, kind, 30.0) for sign in (1, -1)]
+    want = g.double() * (ends[0] - ends[1]) / 2e-6
+    # Truncation: 30^3 1e-12 / 6; rounding: 1e-16 / 1e-6; float32: 30 16 E.
+    assert (dx.cpu().double() - want).abs().max() <= 1e-4 * 30 * g.abs().max()
+
+
+def every_operator(dtype=torch.bfloat16, rows=300, features=72):
+    """Calls that give all outputs and gradients of each operator."""
+    m = layers()
+    x, g = normal(rows, features, seed=1, dtype=dtype), normal(rows, features, seed=2, dtype=dtype)
+    w, b = normal(features, seed=3, dtype=dtype), normal(features, seed=4, dtype=dtype)
+    big = normal(features, features, seed=5, dtype=dtype)
+    x, g, w, b, big = (t.cuda() for t in (x, g, w, b, big))
+
+    def train(call, *inputs):
+        inputs = [t.detach().requires_grad_() for t in inputs]
+        y = call(*inputs)
+        return (y.detach(), *torch.autograd.grad(y, inputs, g))
+
+    return {
+        "checkpoint": lambda: (m.dequantize(m.quantize(x)),),
+        "layer_norm": lambda: train(m.layer_norm, x, w, b),
+        "layer_norm 8 bits": lambda: train(
+            lambda *a: m.layer_norm(*a, checkpoint="8bit"), x, w, b),
+        "sine": lambda: train(m.activation, x),
+        "gelu": lambda: train(lambda z: m.activation(z, "gelu"), x),
+        "linear": lambda: train(m.linear, x, big, b),
+    }, (x, g, w, b, big)
+
+
+@gpu_test
+def test_results_repeat_bit_for_bit_on_any_stream():
+    calls, _ = every_operator()
+    first = {name: call() for name, call in calls.items()}
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        second = {name: call() for name, call in calls.items()}
+    stream.synchronize()
+    for name in first:
+        for a, b in zip(first[name], second[name]):
+            assert torch.equal(a, b), name
+
+
+@gpu_test
+def test_operators_in_a_graph():
+    """Captured forward and backward passes replay with new inputs: each
+    replay equals the eager result, with eager work between."""
+    calls, inputs = every_operator()
+    for name, call in calls.items():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = call()
+        for seed in range(3):
+            for i, t in enumerate(inputs):
+                t.copy_(normal(*t.shape, seed=100 * seed + i, dtype=t.dtype))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in outputs]
+            for a, b in zip(got, call()):
+                assert torch.equal(a, b), (name, seed)
+
+
+@gpu_test
+def test_expanded_and_strided_gradients():
+    m = layers()
+    x = normal(50, 96, seed=1).cuda()
+    w, b = normal(96, seed=2).cuda(), normal(96, seed=3).cuda()
+    big = normal(40, 96, seed=4).cuda()
+    for call, outputs in ((lambda t: m.layer_norm(t, w, b, checkpoint="8bit"), 96),
+                          (m.activation, 96), (lambda t: m.linear(t, big), 40)):
+        scalar = torch.full((1, 1), 0.5).cuda()
+        wide = normal(50, 3 * outputs, seed=5).cuda()
+        for g in (scalar.expand(50, outputs), wide[:, outputs:2 * outputs],
+                  normal(outputs, 50, seed=6).cuda().t()):
+            results = []
+            for grad in (g, g.contiguous()):
+                on = x.clone().requires_grad_()
+                results.append(torch.autograd.grad(call(on), on, grad)[0])
+            assert torch.equal(*results)
+
+
+@gpu_test
+def test_strided_inputs_and_weights():
+    m = layers()
+    base = normal(60, 300, seed=1).cuda()
+    w = normal(96, 40, seed=2).cuda().t()  # a transposed weight
+    for x in (base[:, 10:106], base[::2, 8:104], base.view(3, 20, 300)[:, 2:9, :96]):
+        for call in (lambda t: m.linear(t, w), m.activation, m.layer_norm,
+                     lambda t: m.layer_norm(t, checkpoint="8bit")):
+            results = []
+            for t in (x, x.contiguous()):
+                on = t.detach().requires_grad_()
+                y = call(on)
+                results.append((y, *torch.autograd.grad(y, on, torch.ones_like(y))))
+            for a, b in zip(*results):
+                assert torch.equal(a, b)
+
+
+@gpu_test
+def test_shared_and_broadcast_inputs():
+    """An input used twice and a weight expanded from fewer values: autograd
+    adds what the operators return."""
+    m = layers()
+    x, w = normal(30, 64, seed=1).cuda(), normal(64, 64, seed=2).cuda()
+    on = x.clone().requires_grad_()
+    y = m.linear(m.layer_norm(on), w) + m.layer_norm(on)
+    (both,) = torch.autograd.grad(y, on, torch.ones_like(y))
+    on1, on2 = x.clone().requires_grad_(), x.clone().requires_grad_()
+    y = m.linear(m.layer_norm(on1), w) + m.layer_norm(on2)
+    one, two = torch.autograd.grad(y, (on1, on2), torch.ones_like(y))
+    torch.testing.assert_close(both, one + two, atol=1e-5, rtol=1e-5)
+    scale = torch.tensor([1.5]).cuda().requires_grad_()
+    y = m.layer_norm(x, scale.expand(64))
+    (g,) = torch.autograd.grad(y.square().sum(), scale)
+    h = m.layer_norm(x)
+    torch.testing.assert_close(g[0], (2 * 1.5 * h.square()).sum(), atol=1e-2, rtol=1e-5)
+
+
+@gpu_test
+def test_no_rows():
+    m = layers()
+    for dtype in DTYPES:
+        x = torch.zeros(0, 48, dtype=dtype).cuda().requires_grad_()
+        w = torch.ones(48, dtype=dtype).cuda().requires_grad_()
+        big = torch.ones(20, 48, dtype=dtype).cuda().requires_grad_()
+        b = torch.ones(20, dtype=dtype).cuda().requires_grad_()
+        assert m.dequantize(m.quantize(x.detach())).shape == (0, 48)
+        y = m.activation(x)
+        assert torch.autograd.grad(y, x, torch.zeros_like(y))[0].shape == (0, 48)
+        y = m.layer_norm(x, w, w.detach(), checkpoint="8bit")
+        dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+        assert dx.shape == (0, 48) and torch.equal(dw, torch.zeros_like(dw))
+        y = m.linear(x, big, b)
+        dx, dw, db = torch.autograd.grad(y, (x, big, b), torch.zeros_like(y))
+        assert y.shape == (0, 20) and dx.shape == (0, 48)
+        assert torch.equal(dw, torch.zeros_like(dw)) and torch.equal(db, torch.zeros_like(db))
+
+
+@gpu_test
+def test_second_derivatives_are_refused():
+    m = layers()
+    x = normal(4, 32, seed=1).cuda().requires_grad_()
+    w = normal(8, 32, seed=2).cuda().requires_grad_()
+    for call in (m.layer_norm, m.activation, lambda t: m.linear(t, w)):
+        y = call(x)
+        (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            dx.sum().backward()
+
+
+@gpu_test
+def test_refusals():
+    m = layers()
+    x = torch.zeros(4, 32, device="cuda")
+    bf = x.bfloat16()
+    cases = [
+        (lambda: m.quantize(x.double()), "float32, bfloat16 or float16"),
+        (lambda: m.quantize(x.int()), "float32, bfloat16 or float16"),
+        (lambda: m.quantize(x[:, :0]), "at least one feature"),
+        (lambda: m.quantize(torch.zeros((), device="cuda")), "at least one feature"),
+        (lambda: m.dequantize(m.Checkpoint(x.char(), x[:, :1].byte(), (4, 33), x.dtype)),
+         "do not hold a checkpoint"),
+        (lambda: m.dequantize(m.quantize(x), torch.int32), "reads back as"),
+        (lambda: m.layer_norm(x, torch.zeros(31, device="cuda")), r"shape \(32,\)"),
+        (lambda: m.layer_norm(x, torch.zeros(32)), "device of x"),
+        (lambda: m.layer_norm(x, torch.zeros(32, device="cuda").half()), "type of x or float32"),
+        (lambda: m.layer_norm(bf, torch.zeros(32, device="cuda"),
+                              torch.zeros(32, device="cuda").bfloat16()), "one type"),
+        (lambda: m.linear(x, torch.zeros(8, 31, device="cuda")), r"shape \(8, 32\)"),
+        (lambda: m.linear(x, torch.zeros(32, device="cuda")), r"\(outputs, features\)"),
+        (lambda: m.linear(bf, torch.zeros(8, 32, device="cuda")), "type of x"),
+        (lambda: m.linear(x, torch.zeros(8, 32, device="cuda"), torch.zeros(9, device="cuda")),
+         r"shape \(8,\)"),
+    ]
+    for call, text in cases:
+        with pytest.raises(ValueError, match=text):
+            call()
+    with pytest.raises(RuntimeError, match="at most 16384"):
+        m.layer_norm(torch.zeros(2, 16385, device="cuda"))
+
+
+@gpu_test
+def test_offsets_past_32_bits():
+    """Rows whose offsets pass 2^31 values: the last ones are what they are
+    when they are alone."""
+    m = layers()
+    rows, features = (1 << 31) // 256 + 77, 256
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    tail = torch.randn(300, features, generator=gen, device="cuda").bfloat16()
+    x = torch.zeros(rows, features, device="cuda", dtype=torch.bfloat16)
+    x[-300:] = tail
+    kept, alone = m.quantize(x), m.quantize(tail)
+    assert torch.equal(kept.values[-300:], alone.values)
+    assert torch.equal(kept.exponents[-300:], alone.exponents)
+    assert torch.equal(m.dequantize(kept)[-300:], m.dequantize(alone))
+    del kept
+    w = torch.randn(64, features, generator=gen, device="cuda").bfloat16() / 16
+    g = torch.zeros(rows, 64, device="cuda", dtype=torch.bfloat16)
+    g[-300:] = torch.randn(300, 64, generator=gen, device="cuda").bfloat16()
+    for call, grad in ((lambda t, v: m.linear(t, v), g),
+                       (lambda t, v: m.layer_norm(t, v[0], checkpoint="8bit"), None),
+                       (lambda t, v: m.activation(t), None)):
+        results = []
+        for t in (x, tail):
+            on, v = t.detach().requires_grad_(), w.detach().requires_grad_()
+            y = call(on, v)
+            dy = (grad[-len(t):] if grad is not None else
+                  torch.zeros_like(t).index_copy_(0, torch.arange(len(t) - 300, len(t),
+                                                                  device="cuda"), tail))
+            dx, dv = torch.autograd.grad(y, (on, v), dy, allow_unused=True)
+            results.append((y[-300:].detach().clone(), dx[-300:].clone(), dv))
+            del y, dx, dy, on
+        (y1, dx1, dw1), (y2, dx2, dw2) = results
+        assert torch.equal(y1, y2) and torch.equal(dx1, dx2)
+        if dw1 is not None:
+            # The same few terms, summed in another order: one unit in
+            # bfloat16's last place.
+            assert (dw1.float() - dw2.float()).abs().max() <= 2.0 ** -7 * dw2.float().abs().max()
