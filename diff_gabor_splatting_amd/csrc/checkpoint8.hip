@@ -119,7 +119,7 @@ constexpr int kNone = -1;
 
 // Writes the checkpoint of x (where values is not null) and, with an
 // activation, y.
-template <typename T, int K, bool Whole, bool Flat, int Each>
+template <typename T, int K, bool Flat, int Each>
 __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, Rows r,
                                                       T* __restrict__ y,
                                                       uint8_t* __restrict__ values,
@@ -136,12 +136,12 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
     const bool live = first + local < total;
     if constexpr (Flat) {
       valid[i] = live ? kChunk : 0;
-      load8<T, true>(x + (first + local) * kChunk, valid[i], v[i]);
+      load8<T>(x + (first + local) * kChunk, valid[i], v[i]);
     } else {
       at[i] = place(r, first, local);
       const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
       valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
-      load8<T, Whole>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i], v[i]);
+      load8<T>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i], v[i]);
     }
   }
 #pragma unroll
@@ -160,16 +160,16 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) f[j] = value<T, K>(v[i][j], c);
       if constexpr (Flat)
-        store8<T, true>(y + chunk * kChunk, kChunk, f);
+        store8<T>(y + chunk * kChunk, kChunk, f);
       else
-        store8<T, Whole>(y + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
+        store8<T>(y + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
                          f);
     }
   }
 }
 
 // Reads a checkpoint back, or applies an activation's derivative at it to dy.
-template <typename T, int K, bool Whole, bool Flat, int Each>
+template <typename T, int K, bool Flat, int Each>
 __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict__ values,
                                                       const uint8_t* __restrict__ exponents,
                                                       const T* __restrict__ dy, Rows r,
@@ -194,13 +194,13 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
     }
     if constexpr (Flat) {
       valid[i] = live ? kChunk : 0;
-      if constexpr (K != kNone) load8<T, true>(dy + chunk * kChunk, valid[i], g[i]);
+      if constexpr (K != kNone) load8<T>(dy + chunk * kChunk, valid[i], g[i]);
     } else {
       at[i] = place(r, first, local);
       const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
       valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
       if constexpr (K != kNone)
-        load8<T, Whole>(dy + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i],
+        load8<T>(dy + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i],
                         g[i]);
     }
   }
@@ -214,9 +214,9 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
       for (int j = 0; j < kChunk; ++j) v[j] = g[i][j] * slope<T, K>(v[j], c);
     }
     if constexpr (Flat)
-      store8<T, true>(out + (first + i * kBlock + threadIdx.x) * kChunk, kChunk, v);
+      store8<T>(out + (first + i * kBlock + threadIdx.x) * kChunk, kChunk, v);
     else
-      store8<T, Whole>(out + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
+      store8<T>(out + at[i].row * r.features + int64_t(at[i].chunk) * kChunk, valid[i],
                        v);
   }
 }
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
 constexpr int64_t kFour = int64_t(4) * 256 * kBlock;
 
 template <typename F>
-int with_layout(const char* name, const Rows& r, bool whole, bool flat, F&& launch) {
+int with_layout(const char* name, const Rows& r, bool flat, F&& launch) {
   const int64_t total = r.rows * r.per_row;
   const bool four = total >= kFour;
   const int64_t blocks = ceil_div(total, four ? 4 * kBlock : kBlock);
@@ -236,14 +236,10 @@ int with_layout(const char* name, const Rows& r, bool whole, bool flat, F&& laun
   using all = std::integral_constant<int, 4>;
   const dim3 grid{unsigned(blocks)};
   if (flat)
-    four ? launch(grid, bool_constant<true>{}, bool_constant<true>{}, all{})
-         : launch(grid, bool_constant<true>{}, bool_constant<true>{}, one{});
-  else if (whole)
-    four ? launch(grid, bool_constant<true>{}, bool_constant<false>{}, all{})
-         : launch(grid, bool_constant<true>{}, bool_constant<false>{}, one{});
+    four ? launch(grid, bool_constant<true>{}, all{}) : launch(grid, bool_constant<true>{}, one{});
   else
-    four ? launch(grid, bool_constant<false>{}, bool_constant<false>{}, all{})
-         : launch(grid, bool_constant<false>{}, bool_constant<false>{}, one{});
+    four ? launch(grid, bool_constant<false>{}, all{})
+         : launch(grid, bool_constant<false>{}, one{});
   GS_LAUNCHED(name);
   return GS_OK;
 }
@@ -271,11 +267,9 @@ template <typename T, int K>
 int keep_rows(const char* name, const void* x, int64_t rows, int64_t features, int64_t stride,
               void* y, void* values, void* exponents, float omega, hipStream_t s) {
   const Rows r = rows_of(rows, features, stride);
-  const bool whole = whole_rows<T>(x, features, stride) &&
-                     (K == kNone || whole_rows<T>(y, features, features));
-  const bool flat = whole && stride == features && features % kGroup == 0;
-  return with_layout(name, r, whole, flat, [&](dim3 grid, auto w, auto f, auto each) {
-    keep_kernel<T, K, w.value, f.value, each.value><<<grid, kBlock, 0, s>>>(
+  const bool flat = (stride == features || rows == 1) && features % kGroup == 0;
+  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto each) {
+    keep_kernel<T, K, f.value, each.value><<<grid, kBlock, 0, s>>>(
         static_cast<const T*>(x), r, static_cast<T*>(y), static_cast<uint8_t*>(values),
         static_cast<uint8_t*>(exponents), parameters(omega));
   });
@@ -286,11 +280,9 @@ int read_rows(const char* name, const void* values, const void* exponents, const
               int64_t rows, int64_t features, int64_t stride, void* out, float omega,
               hipStream_t s) {
   const Rows r = rows_of(rows, features, stride);
-  const bool whole = whole_rows<T>(out, features, features) &&
-                     (K == kNone || whole_rows<T>(dy, features, stride));
-  const bool flat = whole && features % kGroup == 0 && (K == kNone || stride == features);
-  return with_layout(name, r, whole, flat, [&](dim3 grid, auto w, auto f, auto each) {
-    read_kernel<T, K, w.value, f.value, each.value><<<grid, kBlock, 0, s>>>(
+  const bool flat = features % kGroup == 0 && (K == kNone || stride == features || rows == 1);
+  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto each) {
+    read_kernel<T, K, f.value, each.value><<<grid, kBlock, 0, s>>>(
         static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),
         static_cast<const T*>(dy), r, static_cast<T*>(out), parameters(omega));
   });

@@ -18,6 +18,8 @@
 // 32-byte aligned whatever F is.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace gs {
@@ -49,34 +51,102 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v) {
   return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), Ctrl, 0xf, 0xf, true));
 }
 
-// Eight consecutive features, zero past `valid`. Whole: one or two 16-byte
-// loads (the address is 16-byte aligned and valid is 8 or 0).
-template <typename T, bool Whole>
-__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[kChunk]) {
-  if constexpr (Whole) {
-    vec<T, 8> raw = T(0);
-    if (valid > 0) raw = *reinterpret_cast<const vec<T, 8>*>(p);
+// A vector in memory at any element's address: the global loads and stores
+// of gfx950 take 16 bytes from any of them, so rows of odd widths are read as
+// wide as others.
+template <typename T, int N>
+struct Packed {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <typename T, int N>
+__device__ __forceinline__ vec<T, N> load_packed(const T* p) {
+  return *reinterpret_cast<const typename Packed<T, N>::type*>(p);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_packed(T* p, vec<T, N> v) {
+  *reinterpret_cast<typename Packed<T, N>::type*>(p) = v;
+}
+
+// The first `valid` < N values at p, zero after them: 4, 2 and 1 at a time.
+template <typename T, int N>
+__device__ __forceinline__ vec<T, N> load_part(const T* p, int valid) {
+  vec<T, N> v = T(0);
+  int at = 0;
+  if (N > 4 && (valid & 4)) {
+    const vec<T, 4> four = load_packed<T, 4>(p);
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) v[j] = float(raw[j]);
-  } else {
+    for (int j = 0; j < 4; ++j) v[j] = four[j];
+    at = 4;
+  }
+  if (valid & 2) {
+    const vec<T, 2> two = load_packed<T, 2>(p + at);
+    if (N > 4 && at) {
+      v[N > 4 ? 4 : 0] = two[0];
+      v[N > 4 ? 5 : 1] = two[1];
+    } else {
+      v[0] = two[0];
+      v[1] = two[1];
+    }
+    at += 2;
+  }
+  if (valid & 1) {
+    const T one = p[at];
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) v[j] = j < valid ? float(p[j]) : 0.f;
+    for (int j = 0; j < N; j += 2)
+      if (at == j) v[j] = one;
+  }
+  return v;
+}
+
+// N consecutive values, `valid` of them in the row (none below 1).
+template <typename T, int N>
+__device__ __forceinline__ vec<T, N> load_valid(const T* p, int valid) {
+  if (valid >= N) return load_packed<T, N>(p);
+  if (valid > 0) return load_part<T, N>(p, valid);
+  return vec<T, N>(T(0));
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_valid(T* p, int valid, vec<T, N> v) {
+  if (valid >= N) {
+    store_packed<T, N>(p, v);
+  } else if (valid > 0) {
+    int at = 0;
+    if (N > 4 && (valid & 4)) {
+      store_packed<T, 4>(p, vec<T, 4>{v[0], v[1], v[2], v[3]});
+      at = 4;
+    }
+    if (valid & 2) {
+      store_packed<T, 2>(p + at, N > 4 && at ? vec<T, 2>{v[N > 4 ? 4 : 0], v[N > 4 ? 5 : 1]}
+                                             : vec<T, 2>{v[0], v[1]});
+      at += 2;
+    }
+    if (valid & 1) {
+      T one = v[0];
+#pragma unroll
+      for (int j = 2; j < N; j += 2)
+        if (at == j) one = v[j];
+      p[at] = one;
+    }
   }
 }
 
-template <typename T, bool Whole>
+// Eight consecutive features as float32, zero past `valid`.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[kChunk]) {
+  const vec<T, 8> raw = load_valid<T, 8>(p, valid);
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) v[j] = float(raw[j]);
+}
+
+template <typename T>
 __device__ __forceinline__ void store8(T* p, int valid, const float (&v)[kChunk]) {
-  if constexpr (Whole) {
-    if (valid <= 0) return;
-    vec<T, 8> raw;
+  vec<T, 8> raw;
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) raw[j] = T(v[j]);
-    *reinterpret_cast<vec<T, 8>*>(p) = raw;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j)
-      if (j < valid) p[j] = T(v[j]);
-  }
+  for (int j = 0; j < kChunk; ++j) raw[j] = T(v[j]);
+  store_valid<T, 8>(p, valid, raw);
 }
 
 // Exponent byte of a group from its largest magnitude's bits. Adding 2^16
@@ -87,6 +157,54 @@ __device__ __forceinline__ uint32_t kept_exponent(uint32_t largest) {
   const int b = int((largest + 0x10000u) >> 23) - 6;
   const int within = min(max(b, KeptRange<T>::least), KeptRange<T>::most);
   return largest >= 0x7f800000u ? 255u : uint32_t(within);
+}
+
+// The largest magnitude of N values, as float32 bits. The 2-byte types'
+// magnitudes compare as 16-bit integers, two at a time.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest_of(vec<T, N> v) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    return most;
+  } else {
+    typedef vec<uint16_t, 2> pair;
+    vec<uint32_t, N / 2> words = __builtin_bit_cast(vec<uint32_t, N / 2>, v);
+    pair most = {0, 0};
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j)
+      most = __builtin_elementwise_max(most,
+                                       __builtin_bit_cast(pair, words[j] & 0x7fff7fffu));
+    const uint16_t one = most[0] > most[1] ? most[0] : most[1];
+    if constexpr (std::is_same_v<T, bf16>)
+      return uint32_t(one) << 16;
+    else
+      return __float_as_uint(float(__builtin_bit_cast(f16, one)));
+  }
+}
+
+// N values over a group's power of two, as bytes, four to a word.
+template <int N>
+__device__ __forceinline__ void keep_bytes(const float (&v)[N], uint32_t exponent,
+                                           uint32_t (&out)[N / 4]) {
+  const float inverse = exponent == 255 ? 0.f : __uint_as_float((254u - exponent) << 23);
+  // v 2^-e + 1.5 2^23 rounds v 2^-e to an integer (ties to even) whose low
+  // byte is q; the clamp acts only at `most`.
+  constexpr float magic = 12582912.f;
+  uint32_t bits[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float t = __builtin_fmaf(v[j], inverse, magic);
+    bits[j] = __float_as_uint(__builtin_amdgcn_fmed3f(t, magic - 127.f, magic + 127.f));
+  }
+  const uint32_t fine = exponent == 255 ? 0u : ~0u;
+#pragma unroll
+  for (int j = 0; j < N; j += 4)
+    out[j / 4] = fine & __builtin_amdgcn_perm(
+                            __builtin_amdgcn_perm(bits[j + 3], bits[j + 2], 0x0c0c0400u),
+                            __builtin_amdgcn_perm(bits[j + 1], bits[j], 0x0c0c0400u),
+                            0x05040100u);
 }
 
 // The eight values of this lane, as bytes; the quad of lanes that holds the
@@ -100,27 +218,9 @@ __device__ __forceinline__ uint2 keep8(const float (&v)[kChunk], uint32_t& expon
   largest = max(largest, dpp<0xB1>(largest));  // quad_perm [1,0,3,2]
   largest = max(largest, dpp<0x4E>(largest));  // quad_perm [2,3,0,1]
   exponent = kept_exponent<T>(largest);
-  const float inverse = exponent == 255 ? 0.f : __uint_as_float((254u - exponent) << 23);
-  // v 2^-e + 1.5 2^23 rounds v 2^-e to an integer (ties to even) whose low
-  // byte is q; the clamp acts only at `most`.
-  constexpr float magic = 12582912.f;
-  uint32_t bits[kChunk];
-#pragma unroll
-  for (int j = 0; j < kChunk; ++j) {
-    const float t = __builtin_fmaf(v[j], inverse, magic);
-    bits[j] = __float_as_uint(__builtin_amdgcn_fmed3f(t, magic - 127.f, magic + 127.f));
-  }
-  uint2 out;
-  out.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400u),
-                                __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u),
-                                0x05040100u);
-  out.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[7], bits[6], 0x0c0c0400u),
-                                __builtin_amdgcn_perm(bits[5], bits[4], 0x0c0c0400u),
-                                0x05040100u);
-  const uint32_t fine = exponent == 255 ? 0u : ~0u;
-  out.x &= fine;
-  out.y &= fine;
-  return out;
+  uint32_t bytes[2];
+  keep_bytes<kChunk>(v, exponent, bytes);
+  return make_uint2(bytes[0], bytes[1]);
 }
 
 // q 2^e of four bytes, exact. b = 255 makes the scale infinite, and 0 times
@@ -134,13 +234,6 @@ __device__ __forceinline__ void read8(uint2 bytes, uint32_t exponent, float (&v)
   const float scale = __uint_as_float(exponent << 23);
   read4(bytes.x, scale, v);
   read4(bytes.y, scale, v + 4);
-}
-
-// Whether rows of this type can be read and written in whole 16-byte pieces.
-template <typename T>
-inline bool whole_rows(const void* p, int64_t features, int64_t stride) {
-  return features % kChunk == 0 && stride % kChunk == 0 &&
-         reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 
 inline int64_t kept_groups(int64_t features) { return ceil_div(features, kGroup); }

@@ -100,7 +100,7 @@ __device__ __forceinline__ int valid_of(int column, int features) {
   return left < 0 ? 0 : left < kChunk ? left : kChunk;
 }
 
-template <typename T, typename W, int Chunks, int Waves, bool Whole>
+template <typename T, typename W, int Chunks, int Waves>
 __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     const T* __restrict__ x, int64_t stride, const W* __restrict__ weight,
     const W* __restrict__ bias, float eps, int64_t rows, int features, int lanes,
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     float sum = 0.f, low = __builtin_inff(), high = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
-      load8<T, Whole>(x + row * stride + column_of<Waves>(i, lane, lanes), live ? valid[i] : 0,
+      load8<T>(x + row * stride + column_of<Waves>(i, lane, lanes), live ? valid[i] : 0,
                       v[i]);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
@@ -148,10 +148,18 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     float squares = 0.f;
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
+      if (valid[i] == kChunk) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) {
-        const float d = v[i][j] - mean;
-        if (Whole ? valid[i] > 0 : j < valid[i]) squares = __builtin_fmaf(d, d, squares);
+        for (int j = 0; j < kChunk; ++j) {
+          const float d = v[i][j] - mean;
+          squares = __builtin_fmaf(d, d, squares);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const float d = j < valid[i] ? v[i][j] - mean : 0.f;
+          squares = __builtin_fmaf(d, d, squares);
+        }
       }
     across2<Add, Add, Waves>(squares, unused, lanes, turn);
     const float inverse = rsqrtf(__builtin_fmaf(squares, inverse_count, eps));
@@ -160,11 +168,10 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
 #pragma unroll
       for (int i = 0; i < Chunks; ++i)
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j)
-          if (Whole ? valid[i] > 0 : j < valid[i]) {
-            low = Low::of(low, v[i][j]);
-            high = High::of(high, v[i][j]);
-          }
+        for (int j = 0; j < kChunk; ++j) {
+          low = Low::of(low, j < valid[i] ? v[i][j] : low);
+          high = High::of(high, j < valid[i] ? v[i][j] : high);
+        }
       across2<Low, High, Waves>(low, high, lanes, turn);
       centre = 0.5f * low + 0.5f * high;
     }
@@ -176,7 +183,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
         out[j] = __builtin_fmaf((v[i][j] - mean) * inverse, w[i][j], b[i][j]);
-      store8<T, Whole>(y + row * features + column, live ? valid[i] : 0, out);
+      store8<T>(y + row * features + column, live ? valid[i] : 0, out);
       if (values) {
         // The last group's lanes past the row keep zeros.
 #pragma unroll
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
 }
 
 // Partial sums: [gridDim.x][2][features] float32, dw then db.
-template <typename T, typename W, int Chunks, int Waves, bool Whole>
+template <typename T, typename W, int Chunks, int Waves>
 __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
     const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride,
     const uint8_t* __restrict__ values, const uint8_t* __restrict__ exponents,
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
       const int column = column_of<Waves>(i, lane, lanes);
-      load8<T, Whole>(dy + row * dy_stride + column, live ? valid[i] : 0, g[i]);
+      load8<T>(dy + row * dy_stride + column, live ? valid[i] : 0, g[i]);
       if (values) {
         uint2 bytes = make_uint2(0, 0);
         uint32_t exponent = 0;
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
         }
         read8(bytes, exponent, h[i]);
       } else {
-        load8<T, Whole>(x + row * x_stride + column, live ? valid[i] : 0, h[i]);
+        load8<T>(x + row * x_stride + column, live ? valid[i] : 0, h[i]);
       }
     }
     float sum = 0.f, product = 0.f;
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
         out[j] = s.y * (__builtin_fmaf(g[i][j], w[i][j], -sum) - h[i][j] * product);
-      store8<T, Whole>(dx + row * features + column_of<Waves>(i, lane, lanes),
+      store8<T>(dx + row * features + column_of<Waves>(i, lane, lanes),
                        live ? valid[i] : 0, out);
     }
   }
@@ -363,25 +370,22 @@ int64_t blocks_of(int64_t rows, int64_t features, bool backward) {
   return std::min(ceil_div(rows, per_block), most);
 }
 
-template <typename T, typename W, typename F>
-int with_shape(int64_t features, bool whole, F&& launch) {
-  using std::bool_constant;
+template <typename F>
+void with_shape(int64_t features, F&& launch) {
   using std::integral_constant;
-  auto by_whole = [&](auto chunks, auto waves) {
-    whole ? launch(chunks, waves, bool_constant<true>{})
-          : launch(chunks, waves, bool_constant<false>{});
-  };
+  using one = integral_constant<int, 1>;
+  using two = integral_constant<int, 2>;
+  using four = integral_constant<int, 4>;
   if (features <= 512)
-    by_whole(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    launch(one{}, one{});
   else if (features <= 1024)
-    by_whole(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    launch(two{}, one{});
   else if (features <= 2048)
-    by_whole(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    launch(four{}, one{});
   else if (features <= 8192)
-    by_whole(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    launch(four{}, four{});
   else
-    by_whole(integral_constant<int, 2>{}, integral_constant<int, 16>{});
-  return GS_OK;
+    launch(two{}, integral_constant<int, 16>{});
 }
 
 template <typename F>
@@ -422,11 +426,9 @@ int gs_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const void* x, in
   return with_types(dtype, weight_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    const bool whole = whole_rows<T>(x, features, row_stride) &&
-                       whole_rows<T>(y, features, features);
     const dim3 grid{unsigned(blocks_of(rows, features, false))};
-    with_shape<T, W>(features, whole, [&](auto chunks, auto waves, auto w) {
-      layer_norm_forward_kernel<T, W, chunks.value, waves.value, w.value>
+    with_shape(features, [&](auto chunks, auto waves) {
+      layer_norm_forward_kernel<T, W, chunks.value, waves.value>
           <<<grid, kThreads<waves.value>, 0, s>>>(
               static_cast<const T*>(x), row_stride, static_cast<const W*>(weight),
               static_cast<const W*>(bias), eps, rows, int(features), lanes_of(features),
@@ -470,12 +472,9 @@ int gs_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const void* grad
     using W = decltype(u);
     const int64_t blocks = rows > 0 ? blocks_of(rows, features, true) : 0;
     if (rows > 0) {
-      const bool whole = whole_rows<T>(grad_y, features, grad_stride) &&
-                         whole_rows<T>(grad_x, features, features) &&
-                         (!x || whole_rows<T>(x, features, row_stride));
-      with_shape<T, W>(features, whole, [&](auto chunks, auto waves, auto w) {
+      with_shape(features, [&](auto chunks, auto waves) {
         const size_t shared = waves.value == 1 ? 2 * size_t(features) * sizeof(float) : 0;
-        layer_norm_backward_kernel<T, W, chunks.value, waves.value, w.value>
+        layer_norm_backward_kernel<T, W, chunks.value, waves.value>
             <<<dim3{unsigned(blocks)}, kThreads<waves.value>, shared, s>>>(
                 static_cast<const T*>(grad_y), grad_stride, static_cast<const T*>(x), row_stride,
                 static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),

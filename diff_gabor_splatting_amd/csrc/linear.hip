@@ -89,7 +89,7 @@ struct KeptSide {
 
 // A tile of a side on its way from memory to LDS, eight columns to a chunk:
 // Rows x Columns from (row, column) on, zero outside the side.
-template <typename T, int Rows, int Columns, bool Whole>
+template <typename T, int Rows, int Columns>
 struct Staged {
   static constexpr int count = Rows * Columns / kChunk / kThreads;
   static constexpr int across = Columns / kChunk;
@@ -101,17 +101,9 @@ struct Staged {
     for (int i = 0; i < count; ++i) {
       const int id = i * kThreads + threadIdx.x;
       const int64_t r = row + id / across, c = column + (id % across) * kChunk;
-      const T* p = s.data + r * s.stride + c;
-      v[i] = T(0);
-      if (r < end) {
-        if constexpr (Whole) {
-          if (c < s.columns) v[i] = *reinterpret_cast<const vec<T, 8>*>(p);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j)
-            if (c + j < s.columns) v[i][j] = p[j];
-        }
-      }
+      const int64_t left = s.columns - c;
+      v[i] = load_valid<T, 8>(s.data + r * s.stride + c,
+                              r < end ? int(left < kChunk ? left : kChunk) : 0);
     }
   }
 
@@ -183,21 +175,15 @@ __device__ __forceinline__ typename Mma<T>::Fragment fragment(const T* lds, int 
   }
 }
 
-// Columns [n, n + 16) of a row of C.
-template <typename T, bool Whole>
+// Columns [n, n + 16) of a row of C, `left` of them inside.
+template <typename T>
 __device__ __forceinline__ void store_row(T* p, int64_t left, const float (&c)[16]) {
-  if (Whole && left >= 16) {
 #pragma unroll
-    for (int h = 0; h < 16; h += 8) {
-      vec<T, 8> raw;
+  for (int h = 0; h < 16; h += 8) {
+    vec<T, 8> raw;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) raw[j] = T(c[h + j]);
-      *reinterpret_cast<vec<T, 8>*>(p + h) = raw;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < left) p[j] = T(c[j]);
+    for (int j = 0; j < 8; ++j) raw[j] = T(c[h + j]);
+    store_valid<T, 8>(p + h, int(left - h < 8 ? left - h : 8), raw);
   }
 }
 
@@ -210,8 +196,7 @@ struct Product {
 
 // out: C in T (split == k), or partial float32 C's, one per split, each
 // followed by the M side's sums over k where sums is set.
-template <typename T, bool MContiguous, bool NContiguous, typename NSide, bool WholeM,
-          bool WholeN, bool WholeC>
+template <typename T, bool MContiguous, bool NContiguous, typename NSide>
 __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns, Product p,
                                                            const T* __restrict__ bias,
                                                            T* __restrict__ out,
@@ -219,8 +204,8 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
   constexpr int depth = Mma<T>::depth;
   __shared__ __align__(16) T m_lds[kTileSize<T, MContiguous>];
   __shared__ __align__(16) T n_lds[kTileSize<T, NContiguous>];
-  Staged<T, MContiguous ? kEdge : depth, MContiguous ? depth : kEdge, WholeM> m_next;
-  Staged<T, NContiguous ? kEdge : depth, NContiguous ? depth : kEdge, WholeN> n_next;
+  Staged<T, MContiguous ? kEdge : depth, MContiguous ? depth : kEdge> m_next;
+  Staged<T, NContiguous ? kEdge : depth, NContiguous ? depth : kEdge> n_next;
   const int64_t tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x % p.tiles_n;
   const int64_t m0 = tile_m * kEdge, n0 = tile_n * kEdge;
   const int64_t k0 = int64_t(blockIdx.y) * p.split;
@@ -292,9 +277,9 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
 #pragma unroll
     for (int j = 0; j < 16; ++j) row[j] = c[i][j >> 2][j & 3] + offset[j];
     if (mine)
-      store_row<float, false>(mine + m * p.n + n, p.n - n, row);
+      store_row<float>(mine + m * p.n + n, p.n - n, row);
     else
-      store_row<T, WholeC>(out + m * p.n + n, p.n - n, row);
+      store_row<T>(out + m * p.n + n, p.n - n, row);
   }
   if constexpr (sums) {
     if (tile_n == 0) {
@@ -316,17 +301,562 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
   }
 }
 
-// Adds `count` partial results of `size` values; the first `weights` of them
-// are dW, the others db.
+// --------------------------------------------------------------------------
+// y and dx: many rows against a small matrix.
+//
+// The matrix (W, or W transposed for dx) stays in LDS, laid out as the
+// matrix instruction's fragments, for all the rows that a workgroup takes.
+// A wave takes TM * 16 rows at a time and needs no other wave: no barriers
+// after the matrix is in place, and its loads are `Ahead` steps (of 128 bytes
+// of each row) ahead of its products, across tiles too.
+//
+// A fragment's lanes lie 16 rows apart in memory, and loading it so costs the
+// address unit a cycle a lane (it was busy for 83% of the kernel). Rows are
+// therefore loaded and results stored with eight lanes to 128 bytes of a row,
+// and turned through 2 KB of LDS that the wave has to itself.
+
+// Contiguous values of k in a lane's fragment, and in a step.
 template <typename T>
+constexpr int kPart = 16 / sizeof(T);
+template <typename T>
+constexpr int kStep = 8 * kPart<T>;  // two fragments: 128 bytes of a row
+
+constexpr int kRowThreads = 512;  // eight waves: what 256 registers allow
+constexpr int kRowWaves = kRowThreads / 64;
+constexpr size_t kRowLds = 128 * 1024;  // of the matrix
+
+struct RowsProduct {
+  int64_t rows, stride;
+  int k, n;          // length of the sum and columns of C
+  int panels;        // workgroups side by side, each with its columns of C
+  int workers;       // workgroups to a panel
+  int steps;         // of the sum, see steps_of
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 multiply(vec<T, kPart<T>> a, vec<T, kPart<T>> b, f32x4 c) {
+  return Mma<T>::of(a, b, c);
+}
+
+// Where column n of a panel is among its fragments: fragment t, row i. Lane
+// group q receives rows 4 q .. 4 q + 3 of each fragment. float32: fragment t
+// is the columns from 16 t on. 2-byte types: two fragments are 32 columns, of
+// which lane group q receives eight in succession, so that a store of 16
+// bytes a lane writes 64 bytes together either way.
+struct FragmentPlace {
+  int t, i;
+};
+template <typename T>
+__device__ __forceinline__ FragmentPlace place_in_panel(int n) {
+  if constexpr (sizeof(T) == 4)
+    return {n >> 4, n & 15};
+  else
+    return {2 * (n >> 5) + ((n >> 2) & 1), 4 * ((n >> 3) & 3) + (n & 3)};
+}
+
+// The matrix as fragments. Transposed: `w` is [k][n] in memory, else [n][k].
+template <typename T, int TN, bool Transposed>
+__device__ __forceinline__ void stage_panel(const T* __restrict__ w, const RowsProduct& p, int n0,
+                                            vec<T, kPart<T>>* lds) {
+  constexpr int part = kPart<T>, columns = 16 * TN;
+  const int parts = p.steps * 8;
+  if constexpr (!Transposed) {
+    for (int id = threadIdx.x; id < columns * parts; id += kRowThreads) {
+      const int n = id / parts, c = id - n * parts, k = c * part;
+      const int left = p.k - k;
+      const vec<T, part> v =
+          load_valid<T, part>(w + int64_t(n0 + n) * p.k + k,
+                              n0 + n < p.n ? (left < part ? left : part) : 0);
+      const FragmentPlace to = place_in_panel<T>(n);
+      lds[((c >> 2) * TN + to.t) * 64 + (c & 3) * 16 + to.i] = v;
+    }
+  } else {
+    // Four columns of `part` rows at a time, turned in registers.
+    for (int id = threadIdx.x; id < columns / 4 * parts; id += kRowThreads) {
+      const int c = id / (columns / 4), g = id - c * (columns / 4);
+      const int n = n0 + 4 * g, left = p.n - n;
+      vec<T, 4> v[part];
+#pragma unroll
+      for (int j = 0; j < part; ++j) {
+        const int k = c * part + j;
+        v[j] = load_valid<T, 4>(w + int64_t(k) * p.n + n,
+                                k < p.k ? (left < 4 ? left : 4) : 0);
+      }
+      const FragmentPlace to = place_in_panel<T>(4 * g);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        vec<T, part> turned;
+#pragma unroll
+        for (int j = 0; j < part; ++j) turned[j] = v[j][b];
+        lds[((c >> 2) * TN + to.t) * 64 + (c & 3) * 16 + to.i + b] = turned;
+      }
+    }
+  }
+}
+
+// Orders a wave's own LDS writes before its other lanes' reads, and those
+// before later writes: the hardware keeps a wave's LDS order by itself, this
+// keeps the compiler's.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Place, among a wave's 128 pieces of 16 bytes, of piece c (of four) of half
+// h (of two) of row r (of 16). LDS serves eight lanes of 16 bytes at a time:
+// a row's eight pieces when written, and when read 4 lanes of one lane group
+// with 4 of the next, rows 0..3 of eight with rows 4..7; neither meet in a
+// bank.
+__device__ __forceinline__ int turn_place(int r, int h, int c) {
+  return h * 64 + c * 16 + (r ^ (4 * h + c));
+}
+
+// The 8-bit form of one step of a tile's rows, as they were loaded: lane l
+// has piece l % 8 of row 8 j + l / 8 of x[j].
+template <typename T, int Loads>
+__device__ __forceinline__ void keep_step(const vec<T, kPart<T>> (&x)[Loads], int64_t first,
+                                          int s, const RowsProduct& p,
+                                          uint8_t* __restrict__ values,
+                                          uint8_t* __restrict__ exponents) {
+  constexpr int part = kPart<T>;
+  const int lane = threadIdx.x & 63;
+  const int groups = (p.k + kGroup - 1) / kGroup;
+  const int k = s * kStep<T> + (lane & 7) * part;
+  const int group = k / kGroup;
+#pragma unroll
+  for (int j = 0; j < Loads; ++j) {
+    const int64_t row = first + 8 * j + (lane >> 3);
+    uint32_t largest = largest_of<T, part>(x[j]);
+    largest = max(largest, dpp<0xB1>(largest));  // quad_perm [1,0,3,2]
+    largest = max(largest, dpp<0x4E>(largest));  // quad_perm [2,3,0,1]
+    if constexpr (part == 4) largest = max(largest, dpp<0x141>(largest));  // row_half_mirror
+    const uint32_t exponent = kept_exponent<T>(largest);
+    float v[part];
+#pragma unroll
+    for (int i = 0; i < part; ++i) v[i] = float(x[j][i]);
+    uint32_t bytes[part / 4];
+    keep_bytes<part>(v, exponent, bytes);
+    if (row < p.rows && group < groups) {
+      uint8_t* const to = values + row * (int64_t(groups) * kGroup) + k;
+      if constexpr (part == 8)
+        *reinterpret_cast<uint2*>(to) = make_uint2(bytes[0], bytes[1]);
+      else
+        *reinterpret_cast<uint32_t*>(to) = bytes[0];
+      if (k % kGroup == 0) exponents[row * groups + group] = uint8_t(exponent);
+    }
+  }
+}
+
+// Ahead: steps on their way. Tail: k is no whole number of steps.
+template <typename T, int TM, int TN, int Ahead, bool Transposed, bool Keep, bool Tail>
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(
+    const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ bias, RowsProduct p,
+    T* __restrict__ out, uint8_t* __restrict__ values, uint8_t* __restrict__ exponents) {
+  constexpr int part = kPart<T>, step = kStep<T>, columns = 16 * TN;
+  constexpr int loads = 2 * TM;  // of eight rows each
+  typedef vec<T, part> Part;
+  extern __shared__ __align__(16) char shared[];
+  Part* const panel = reinterpret_cast<Part*>(shared);
+  __shared__ Part turns[kRowWaves][128];
+  __shared__ float offset[columns];
+  // Workgroups go to the eight XCDs in turn: those that take the same rows
+  // share one, and its L2.
+  const int xcd = blockIdx.x & 7, in_xcd = blockIdx.x >> 3;
+  const int at = in_xcd % p.panels;
+  const int worker = in_xcd / p.panels * 8 + xcd;
+  if (worker >= p.workers) return;
+  const int n0 = at * columns;
+  stage_panel<T, TN, Transposed>(w, p, n0, panel);
+  if (threadIdx.x < columns)
+    offset[threadIdx.x] =
+        bias && n0 + int(threadIdx.x) < p.n ? float(bias[n0 + threadIdx.x]) : 0.f;
+  __syncthreads();
+
+  const int lane = threadIdx.x & 63, q = lane >> 4, i16 = lane & 15;
+  const int row8 = lane >> 3, piece = lane & 7;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Part* const turn = turns[wave];
+  const int64_t tiles = (p.rows + 16 * TM - 1) / (16 * TM);
+  const int64_t each = int64_t(p.workers) * kRowWaves;
+  // Tiles go round the workgroups first, then round their waves.
+  int64_t tile = worker + int64_t(wave) * p.workers;
+  if (tile >= tiles) return;
+
+  // What is on its way: the loop below takes ring[u] and sends for the step
+  // `Ahead` later in its place. Past the last tile it sends for that one
+  // again, so that the number of loads under way is always the same.
+  Part ring[Ahead][loads];
+  const T* base;
+  uint32_t from[loads];
+  int64_t sent = tile;
+  int sent_step = 0;
+  auto turn_to = [&](int64_t of) {
+    const int64_t first = of * (16 * TM);
+    const int most = int(p.rows - first < 16 * TM ? p.rows - first : 16 * TM) - 1;
+    base = x + first * p.stride;
+#pragma unroll
+    for (int j = 0; j < loads; ++j)  // rows past the end repeat the last one
+      from[j] = uint32_t(min(8 * j + row8, most) * int(p.stride) + piece * part);
+  };
+  turn_to(tile);
+  auto send = [&](Part (&to)[loads]) {
+    const T* const at_step = base + sent_step * step;
+    if (!Tail || (sent_step + 1) * step <= p.k) {
+#pragma unroll
+      for (int j = 0; j < loads; ++j) to[j] = load_packed<T, part>(at_step + from[j]);
+    } else {
+      const int left = min(p.k - sent_step * step - piece * part, part);
+#pragma unroll
+      for (int j = 0; j < loads; ++j) to[j] = load_valid<T, part>(at_step + from[j], left);
+    }
+    if (++sent_step == p.steps) {
+      sent_step = 0;
+      sent += each;
+      turn_to(sent < tiles ? sent : tile);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < Ahead; ++u) send(ring[u]);
+
+  for (; tile < tiles; tile += each) {
+    f32x4 c[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int t = 0; t < TN; ++t) c[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < p.steps; s0 += Ahead) {
+#pragma unroll
+      for (int u = 0; u < Ahead; ++u) {
+        const int s = s0 + u;
+        Part b[TM][2];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            turn[turn_place(8 * j + row8, piece >> 2, piece & 3)] = ring[u][2 * i + j];
+          wave_order();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) b[i][h] = turn[turn_place(i16, h, q)];
+          wave_order();
+        }
+        if constexpr (Keep) {
+          // The panels share the rows' 8-bit form: each keeps its turn's steps.
+          if (s % p.panels == at)
+            keep_step<T, loads>(ring[u], tile * (16 * TM), s, p, values, exponents);
+        }
+        send(ring[u]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < TN; ++t) {
+            const Part a = panel[((2 * s + h) * TN + t) * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) c[i][t] = multiply<T>(a, b[i][h], c[i][t]);
+          }
+      }
+    }
+    // Lane group q has, of every 64 bytes of the columns, the q-th 16.
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int v = 0; v < 4 * TN; v += 2 * part) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          Part r;
+#pragma unroll
+          for (int j = 0; j < part; ++j) {
+            const int from_fragment = v + h * part + j;
+            r[j] = T(c[i][from_fragment >> 2][j & 3] +
+                     offset[4 * (v + h * part) + q * part + j]);
+          }
+          turn[turn_place(i16, h, q)] = r;
+        }
+        wave_order();
+        const int n = n0 + 4 * v + piece * part;
+        const int inside = min(p.n - n, part);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t row = tile * (16 * TM) + 16 * i + 8 * j + row8;
+          const Part r = turn[turn_place(8 * j + row8, piece >> 2, piece & 3)];
+          store_valid<T, part>(out + row * p.n + n, row < p.rows ? inside : 0, r);
+        }
+        wave_order();
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
+// dW and db: the sum over many rows of dy^T x8.
+//
+// A workgroup of eight waves (two along the outputs, four along the features)
+// adds up a tile of dW over its share of the rows, 32 rows at a time: they
+// are two steps ahead in registers, then in one of two LDS buffers, row by
+// row as in memory, and the transposing LDS load makes fragments of them. One
+// barrier a step. x8 is expanded to bfloat16 (float16) on the way. float32 dy
+// is cut into three bfloat16 parts of eight bits each, whose sum it is, and
+// each is multiplied by x8, which is exact in bfloat16: three products at
+// the bfloat16 rate, a fifth of the time of float32's, and none of them
+// rounded (an infinity or a NaN is the first part alone).
+
+// What the matrix instructions multiply.
+template <typename T>
+using Factor = std::conditional_t<sizeof(T) == 4, bf16, T>;
+
+constexpr int kSumThreads = 512;
+constexpr int kSumRows = 32;
+
+struct SumProduct {
+  int64_t rows, stride;   // of dy
+  int outputs, features;
+  int tiles_m, tiles_n;   // of dW
+  int splits;
+  int64_t share;          // rows of a split, a multiple of kSumRows
+};
+
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+
+// Eight values as their parts.
+template <typename T>
+__device__ __forceinline__ void parts_of(vec<T, 8> v, vec<Factor<T>, 8> (&out)[kParts<T>]) {
+  if constexpr (sizeof(T) == 2) {
+    out[0] = v;
+  } else {
+    vec<uint32_t, 4> words[3];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      uint32_t part[3][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t first = __float_as_uint(v[j + i]) & 0xffff0000u;
+        const bool finite = (first & 0x7f800000u) != 0x7f800000u;
+        // Whole NaN payloads keep to the first part.
+        const uint32_t top =
+            finite ? first : __float_as_uint(v[j + i]) | (v[j + i] != v[j + i] ? 0x10000u : 0u);
+        const float rest = finite ? v[j + i] - __uint_as_float(first) : 0.f;
+        const uint32_t second = __float_as_uint(rest) & 0xffff0000u;
+        part[0][i] = top;
+        part[1][i] = second;
+        part[2][i] = __float_as_uint(rest - __uint_as_float(second));
+      }
+#pragma unroll
+      for (int h = 0; h < 3; ++h)
+        words[h][j / 2] = __builtin_amdgcn_perm(part[h][1], part[h][0], 0x07060302u);
+    }
+#pragma unroll
+    for (int h = 0; h < 3; ++h) out[h] = __builtin_bit_cast(vec<bf16, 8>, words[h]);
+  }
+}
+
+// The 16 columns from `first` on of 32 rows of LDS, as a fragment.
+template <typename F>
+__device__ __forceinline__ vec<F, 8> turned_fragment(const F* lds, int pitch, int first) {
+  typedef vec<short, 4> raw;
+  typedef __attribute__((address_space(3))) raw* lds_raw;
+  const int lane = threadIdx.x & 63, q = lane >> 4, i = lane & 15;
+  // Among 16 lanes, lane 4 a + b reads four columns at 4 b of row a, and
+  // lane i receives column i of the four rows.
+  const F* const p = lds + (4 * q + (i >> 2)) * pitch + first + 4 * (i & 3);
+  const raw low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_raw)p);
+  const raw high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_raw)(p + 16 * pitch));
+  return __builtin_bit_cast(vec<F, 8>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A wave's tile: 16 A outputs x 16 B features.
+template <typename T, int A, int B>
+__global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ dy,
+                                                          const uint8_t* __restrict__ values,
+                                                          const uint8_t* __restrict__ exponents,
+                                                          SumProduct p,
+                                                          float* __restrict__ partial) {
+  typedef Factor<T> F;
+  constexpr int parts = kParts<T>;
+  constexpr int tile_m = 32 * A, tile_n = 64 * B;
+  // 32 bytes past a multiple of 256: the eight rows that 32 lanes of a
+  // fragment's load read lie in different banks.
+  constexpr int pitch_m = tile_m + 16, pitch_n = tile_n + 16;
+  constexpr int buffer = kSumRows * (parts * pitch_m + pitch_n);
+  constexpr int across_m = tile_m / 8, across_n = tile_n / 16;
+  constexpr int loads_m = kSumRows * across_m / kSumThreads;  // chunks of a thread
+  constexpr bool all_n = kSumRows * across_n >= kSumThreads;
+  static_assert(loads_m >= 1 && kSumRows * across_n <= kSumThreads, "tile does not fit");
+  extern __shared__ __align__(16) char shared[];
+  F* const lds = reinterpret_cast<F*>(shared);
+
+  // Workgroups go to the eight XCDs in turn: the tiles of one share of the
+  // rows have one XCD, and its L2.
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int in_xcd = blockIdx.x >> 3;
+  const int split = in_xcd / tiles * 8 + (blockIdx.x & 7);
+  if (split >= p.splits) return;
+  const int tile = in_xcd % tiles;
+  const int m0 = tile / p.tiles_n * tile_m, n0 = tile % p.tiles_n * tile_n;
+  const int64_t k0 = split * p.share;
+  const int64_t k1 = k0 + p.share < p.rows ? k0 + p.share : p.rows;
+  const int groups = (p.features + kGroup - 1) / kGroup;
+
+  // Each thread's places: eight outputs of loads_m rows, 16 features of one.
+  const int row_m = threadIdx.x / across_m, column_m = threadIdx.x % across_m * 8;
+  const int row_n = threadIdx.x / across_n, column_n = threadIdx.x % across_n * 16;
+  const int valid_m = min(p.outputs - m0 - column_m, 8);
+  const bool has_n = (all_n || row_n < kSumRows) && n0 + column_n < groups * kGroup;
+  const T* from_m = dy + (k0 + row_m) * p.stride + m0 + column_m;
+  const uint8_t* from_n = values + (k0 + row_n) * (int64_t(groups) * kGroup) + n0 + column_n;
+  const uint8_t* from_e = exponents + (k0 + row_n) * groups + (n0 + column_n) / kGroup;
+
+  struct Load {
+    vec<T, 8> m[loads_m];
+    vec<uint32_t, 4> n;
+    uint32_t exponent;
+  };
+  Load ahead[2];
+  int64_t sent = k0;
+  auto send = [&](Load& to) {
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i) {
+      constexpr int apart = kSumThreads / across_m;
+      to.m[i] = load_valid<T, 8>(from_m + i * apart * p.stride,
+                                 sent + row_m + i * apart < k1 ? valid_m : 0);
+    }
+    to.n = vec<uint32_t, 4>{0, 0, 0, 0};
+    to.exponent = 0;
+    if (has_n && sent + row_n < k1) {
+      to.n = *reinterpret_cast<const vec<uint32_t, 4>*>(from_n);
+      to.exponent = *from_e;
+    }
+    sent += kSumRows;
+    from_m += kSumRows * p.stride;
+    from_n += kSumRows * int64_t(groups) * kGroup;
+    from_e += kSumRows * groups;
+  };
+  float sum[8] = {};
+  const bool sums = n0 == 0;
+  auto put = [&](const Load& from, F* to) {
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i) {
+      vec<F, 8> cut[parts];
+      parts_of<T>(from.m[i], cut);
+      if (sums) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += float(from.m[i][j]);
+      }
+#pragma unroll
+      for (int h = 0; h < parts; ++h)
+        *reinterpret_cast<vec<F, 8>*>(
+            to + (h * kSumRows + row_m + i * (kSumThreads / across_m)) * pitch_m + column_m) =
+            cut[h];
+    }
+    if (all_n || row_n < kSumRows) {
+      const float scale = __uint_as_float(from.exponent << 23);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f[8];
+        read4(from.n[2 * h], scale, f);
+        read4(from.n[2 * h + 1], scale, f + 4);
+        vec<F, 8> v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = F(f[j]);
+        *reinterpret_cast<vec<F, 8>*>(to + parts * kSumRows * pitch_m + row_n * pitch_n +
+                                      column_n + 8 * h) = v;
+      }
+    }
+  };
+
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave_m = (wave >> 2) * 16 * A, wave_n = (wave & 3) * 16 * B;
+  f32x4 c[A][B];
+#pragma unroll
+  for (int i = 0; i < A; ++i)
+#pragma unroll
+    for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply_step = [&](const F* from) {
+    vec<F, 8> b[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      b[j] = turned_fragment<F>(from + parts * kSumRows * pitch_m, pitch_n, wave_n + 16 * j);
+#pragma unroll
+    for (int h = 0; h < parts; ++h)
+#pragma unroll
+      for (int i = 0; i < A; ++i) {
+        const vec<F, 8> a =
+            turned_fragment<F>(from + h * kSumRows * pitch_m, pitch_m, wave_m + 16 * i);
+#pragma unroll
+        for (int j = 0; j < B; ++j) c[i][j] = Mma<F>::of(b[j], a, c[i][j]);
+      }
+  };
+
+  const int64_t steps = (k1 - k0 + kSumRows - 1) / kSumRows;
+  send(ahead[0]);
+  send(ahead[1]);
+  put(ahead[0], lds);
+  send(ahead[0]);
+  __syncthreads();
+  // Steps past the last read zeros: an odd count's last pair needs no case.
+  for (int64_t s = 0; s < steps; s += 2) {
+    put(ahead[1], lds + buffer);
+    send(ahead[1]);
+    multiply_step(lds);
+    __syncthreads();
+    put(ahead[0], lds);
+    send(ahead[0]);
+    multiply_step(lds + buffer);
+    __syncthreads();
+  }
+
+  // Lane 16 q + i holds features 4 q .. 4 q + 3 of output i of a fragment.
+  float* const mine = partial + int64_t(split) * p.outputs * (int64_t(p.features) + 1);
+  const int q = lane >> 4, i16 = lane & 15;
+#pragma unroll
+  for (int i = 0; i < A; ++i) {
+    const int m = m0 + wave_m + 16 * i + i16;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int n = n0 + wave_n + 16 * j + 4 * q;
+      store_valid<float, 4>(mine + int64_t(m) * p.features + n,
+                            m < p.outputs ? min(p.features - n, 4) : 0, c[i][j]);
+    }
+  }
+  if (sums) {
+    // The threads of a column add up in LDS, in their order.
+    float* const all = reinterpret_cast<float*>(shared);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) all[row_m * tile_m + column_m + j] = sum[j];
+    __syncthreads();
+    const int m = m0 + threadIdx.x;
+    if (int(threadIdx.x) < tile_m && m < p.outputs) {
+      float total = 0.f;
+      for (int i = 0; i < kSumThreads / across_m; ++i) total += all[i * tile_m + threadIdx.x];
+      mine[int64_t(p.outputs) * p.features + m] = total;
+    }
+  }
+}
+
+// Adds `count` partial results of `size` values; the first `weights` of them
+// are dW, the others db. A workgroup takes kThreads / Slices values; each
+// slice of its threads adds every Slices-th result, and the slices meet in
+// LDS, in their order.
+template <typename T, int Slices>
 __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict__ partial,
                                                         int count, int64_t size, int64_t weights,
                                                         T* __restrict__ dw, T* __restrict__ db) {
-  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= size) return;
+  constexpr int columns = kThreads / Slices;
+  __shared__ float sums[Slices][columns];
+  const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
+  const int64_t i = int64_t(blockIdx.x) * columns + column;
   float sum = 0.f;
+  if (i < size) {
 #pragma unroll 8
-  for (int s = 0; s < count; ++s) sum += partial[s * size + i];
+    for (int s = slice; s < count; s += Slices) sum += partial[s * size + i];
+  }
+  if constexpr (Slices > 1) {
+    sums[slice][column] = sum;
+    __syncthreads();
+    if (slice) return;
+    for (int s = 1; s < Slices; ++s) sum += sums[s][column];
+  }
+  if (i >= size) return;
   if (i < weights) {
     if (dw) dw[i] = T(sum);
   } else if (db) {
@@ -334,26 +864,106 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict_
   }
 }
 
-// Splits of dW's sum over the rows: two workgroups per compute unit, and at
-// least 256 rows to each.
-int64_t rows_of_split(int64_t rows, int64_t features, int64_t outputs) {
-  const int64_t tiles = ceil_div(features, kEdge) * ceil_div(outputs, kEdge);
-  const int64_t most = std::max<int64_t>(1, 512 / tiles);
-  const int64_t each = std::max<int64_t>(ceil_div(rows, most), 256);
-  return ceil_div(each, 64) * 64;
+// How dW's sum is cut: tiles of dW (fragments of a wave's tile along the
+// outputs and the features), and shares of the rows.
+struct SumPlan {
+  int a, b;
+  int64_t tiles_m, tiles_n, splits, share;
+};
+
+SumPlan sum_plan(size_t size, int64_t rows, int64_t features, int64_t outputs) {
+  SumPlan p{};
+  const bool large = outputs > 128 && features > 128 && rows >= 400000 / (size / 2);
+  p.a = large && size == 2 ? 8 : 4;
+  p.b = large ? 4 : 2;
+  p.tiles_m = ceil_div(outputs, 32 * p.a);
+  p.tiles_n = ceil_div(features, 64 * p.b);
+  const int64_t workgroups = large ? 256 : 512;
+  p.splits = std::max<int64_t>(1, workgroups / (p.tiles_m * p.tiles_n));
+  p.share = ceil_div(std::max<int64_t>(ceil_div(rows, p.splits), 8 * kSumRows), kSumRows) *
+            kSumRows;
+  p.splits = ceil_div(rows, p.share);
+  return p;
 }
 
-template <typename F>
-int with_flags(bool a, bool b, bool c, F&& call) {
-  using std::bool_constant;
-  auto third = [&](auto x, auto y) {
-    c ? call(x, y, bool_constant<true>{}) : call(x, y, bool_constant<false>{});
+// Steps that are under way at a time, and steps of the sum: a multiple of
+// them (the steps past k multiply zeros).
+int ahead_of(int64_t steps) { return steps == 1 ? 1 : steps % 4 == 0 ? 4 : 2; }
+int64_t steps_of(size_t size, int64_t k) {
+  const int64_t steps = ceil_div(k * int64_t(size), 128);
+  return steps > 1 ? steps + steps % 2 : steps;
+}
+
+// Fragments side by side of a panel of the matrix: the widest that its k
+// leaves room for in LDS, no wider than the columns of C ask for, at least
+// 128 bytes of a row of C; 0 where that does not fit.
+int panel_fragments(size_t size, int64_t k, int64_t n) {
+  const int least = size == 4 ? 2 : 4;
+  for (int fragments = 8; fragments >= least; fragments /= 2)
+    if (steps_of(size, k) * 2048 * fragments <= int64_t(kRowLds) &&
+        (n > 8 * fragments || fragments == least))
+      return fragments;
+  return 0;
+}
+
+// C = x matrix through rows_kernel; false where the matrix or the stride is
+// too large for it.
+template <typename T, bool Transposed>
+int launch_rows(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
+                int64_t rows, int64_t k, int64_t n, void* out, void* values, void* exponents,
+                hipStream_t stream, bool& taken) {
+  const int fragments = panel_fragments(sizeof(T), k, n);
+  const int64_t panels = fragments ? ceil_div(n, 16 * fragments) : 0;
+  taken = fragments && panels <= 32 && stride < (1 << 24);
+  if (!taken) return GS_OK;
+  using std::integral_constant;
+  auto launch = [&](auto tm, auto tn, auto ahead, auto keep, auto tail) {
+    RowsProduct p{rows, stride, int(k), int(n), int(panels), 0, int(steps_of(sizeof(T), k))};
+    const int64_t tiles = ceil_div(rows, 16 * tm.value);
+    p.workers = int(std::min<int64_t>(32 / panels * 8, tiles));
+    const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
+    const size_t lds = size_t(p.steps) * 2 * tn.value * 1024;
+    auto* const kernel =
+        &rows_kernel<T, tm.value, tn.value, ahead.value, Transposed, keep.value, tail.value>;
+    GS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+    kernel<<<grid, kRowThreads, lds, stream>>>(
+        static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), p,
+        static_cast<T*>(out), static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents));
+    GS_LAUNCHED(name);
+    return GS_OK;
   };
-  auto second = [&](auto x) {
-    b ? third(x, bool_constant<true>{}) : third(x, bool_constant<false>{});
+  using one = integral_constant<int, 1>;
+  using two = integral_constant<int, 2>;
+  using four = integral_constant<int, 4>;
+  auto by_ahead = [&](auto tm, auto tn, auto keep) {
+    const int64_t steps = steps_of(sizeof(T), k);
+    if (k != steps * kStep<T>)
+      switch (ahead_of(steps)) {
+        case 1: return launch(tm, tn, one{}, keep, std::true_type{});
+        case 2: return launch(tm, tn, two{}, keep, std::true_type{});
+        default: return launch(tm, tn, four{}, keep, std::true_type{});
+      }
+    switch (ahead_of(steps)) {
+      case 1: return launch(tm, tn, one{}, keep, std::false_type{});
+      case 2: return launch(tm, tn, two{}, keep, std::false_type{});
+      default: return launch(tm, tn, four{}, keep, std::false_type{});
+    }
   };
-  a ? second(bool_constant<true>{}) : second(bool_constant<false>{});
-  return GS_OK;
+  auto by_keep = [&](auto tm, auto tn) {
+    if constexpr (!Transposed)
+      if (values) return by_ahead(tm, tn, std::true_type{});
+    return by_ahead(tm, tn, std::false_type{});
+  };
+  switch (fragments) {
+    case 8: return by_keep(two{}, integral_constant<int, 8>{});
+    case 4: return by_keep(two{}, four{});
+    default:
+      if constexpr (sizeof(T) == 4)
+        return by_keep(two{}, two{});
+      else
+        return int(GS_OK);  // not reached: panel_fragments gives no such panel
+  }
 }
 
 int check_linear(const char* name, int32_t dtype, int64_t rows, int64_t features,
@@ -382,25 +992,26 @@ int gs_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const vo
   if (rows == 0) return GS_OK;
   GS_REQUIRE(x && weight && y && !values == !exponents, GS_ERR_ARGUMENT,
              "null pointer passed to gs_linear_forward");
-  if (values)
-    GS_CHECK(gs_checkpoint8_write(dtype, x, row_stride, rows, features, values, exponents,
-                                  stream));
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
+    bool taken = false;
+    GS_CHECK((launch_rows<T, false>("linear forward", x, row_stride, weight, bias, rows, features,
+                                    outputs, y, values, exponents,
+                                    static_cast<hipStream_t>(stream), taken)));
+    if (taken) return int(GS_OK);
+    if (values)
+      GS_CHECK(gs_checkpoint8_write(dtype, x, row_stride, rows, features, values, exponents,
+                                    stream));
     const Side<T> ms{static_cast<const T*>(x), row_stride, rows, features};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
     const Product p{rows, outputs, features, ceil_div(features, 64) * 64,
                     ceil_div(outputs, kEdge)};
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
-    const bool whole = whole_rows<T>(x, features, row_stride) &&
-                       whole_rows<T>(weight, features, features);
-    with_flags(whole, whole_rows<T>(y, outputs, outputs), false, [&](auto w, auto wc, auto) {
-      product_kernel<T, true, true, Side<T>, w.value, w.value, wc.value>
-          <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-              ms, ns, p, static_cast<const T*>(bias), static_cast<T*>(y), nullptr);
-    });
+    product_kernel<T, true, true, Side<T>>
+        <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            ms, ns, p, static_cast<const T*>(bias), static_cast<T*>(y), nullptr);
     GS_LAUNCHED("linear forward");
-    return GS_OK;
+    return int(GS_OK);
   });
 }
 
@@ -416,28 +1027,30 @@ int gs_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_str
              "null pointer passed to gs_linear_backward_input");
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
+    bool taken = false;
+    GS_CHECK((launch_rows<T, true>("linear backward input", grad_y, grad_stride, weight, nullptr,
+                                   rows, outputs, features, grad_x, nullptr, nullptr,
+                                   static_cast<hipStream_t>(stream), taken)));
+    if (taken) return int(GS_OK);
     const Side<T> ms{static_cast<const T*>(grad_y), grad_stride, rows, outputs};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
     const Product p{rows, features, outputs, ceil_div(outputs, 64) * 64,
                     ceil_div(features, kEdge)};
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
-    with_flags(whole_rows<T>(grad_y, outputs, grad_stride),
-               whole_rows<T>(weight, features, features),
-               whole_rows<T>(grad_x, features, features), [&](auto wm, auto wn, auto wc) {
-      product_kernel<T, true, false, Side<T>, wm.value, wn.value, wc.value>
-          <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-              ms, ns, p, static_cast<const T*>(nullptr), static_cast<T*>(grad_x), nullptr);
-    });
+    product_kernel<T, true, false, Side<T>>
+        <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            ms, ns, p, static_cast<const T*>(nullptr), static_cast<T*>(grad_x), nullptr);
     GS_LAUNCHED("linear backward input");
-    return GS_OK;
+    return int(GS_OK);
   });
 }
 
-size_t gs_linear_backward_weight_workspace_size(int32_t, int64_t rows, int64_t features,
+size_t gs_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows, int64_t features,
                                                 int64_t outputs) {
   using namespace gs;
   if (rows <= 0 || features <= 0 || outputs <= 0) return 0;
-  return size_t(ceil_div(rows, rows_of_split(rows, features, outputs))) *
+  const size_t size = dtype == GS_FLOAT32 ? 4 : 2;
+  return size_t(sum_plan(size, rows, features, outputs).splits) *
          size_t(outputs * (features + 1)) * sizeof(float);
 }
 
@@ -462,29 +1075,48 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
     using T = decltype(zero);
     int64_t splits = 0;
     if (rows > 0) {
-      const int64_t split = rows_of_split(rows, features, outputs);
-      splits = ceil_div(rows, split);
-      const Side<T> ms{static_cast<const T*>(grad_y), grad_stride, rows, outputs};
-      const KeptSide ns{static_cast<const uint8_t*>(values),
-                        static_cast<const uint8_t*>(exponents), kept_groups(features), rows,
-                        features};
-      const Product p{outputs, features, rows, split, ceil_div(features, kEdge)};
-      const dim3 grid{unsigned(ceil_div(outputs, kEdge) * p.tiles_n), unsigned(splits)};
-      with_flags(whole_rows<T>(grad_y, outputs, grad_stride), true, false,
-                 [&](auto wm, auto, auto) {
-        product_kernel<T, false, false, KeptSide, wm.value, true, false>
-            <<<grid, kThreads, 0, s>>>(ms, ns, p, static_cast<const T*>(nullptr),
-                                       static_cast<T*>(nullptr),
-                                       static_cast<float*>(workspace));
-      });
-      GS_LAUNCHED("linear backward weight");
+      const SumPlan plan = sum_plan(sizeof(T), rows, features, outputs);
+      splits = plan.splits;
+      const SumProduct p{rows, grad_stride, int(outputs), int(features), int(plan.tiles_m),
+                         int(plan.tiles_n), int(splits), plan.share};
+      const int64_t blocks = ceil_div(splits, 8) * 8 * plan.tiles_m * plan.tiles_n;
+      GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "linear backward weight: too large");
+      auto launch = [&](auto a, auto b) {
+        constexpr int pitches = kParts<T> * (32 * a.value + 16) + 64 * b.value + 16;
+        const size_t lds = std::max<size_t>(2 * size_t(kSumRows) * pitches * 2,
+                                            size_t(kSumThreads) * 8 * sizeof(float));
+        auto* const kernel = &sum_kernel<T, a.value, b.value>;
+        GS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+        kernel<<<dim3{unsigned(blocks)}, kSumThreads, lds, s>>>(
+            static_cast<const T*>(grad_y), static_cast<const uint8_t*>(values),
+            static_cast<const uint8_t*>(exponents), p, static_cast<float*>(workspace));
+        GS_LAUNCHED("linear backward weight");
+        return int(GS_OK);
+      };
+      using std::integral_constant;
+      using four = integral_constant<int, 4>;
+      if constexpr (sizeof(T) == 2)
+        GS_CHECK(plan.a == 8 ? launch(integral_constant<int, 8>{}, four{})
+                             : launch(four{}, integral_constant<int, 2>{}));
+      else
+        GS_CHECK(plan.b == 4 ? launch(four{}, four{})
+                             : launch(four{}, integral_constant<int, 2>{}));
     }
     const int64_t weights = outputs * features, size = weights + outputs;
-    join_kernel<T><<<dim3{unsigned(ceil_div(size, kThreads))}, kThreads, 0, s>>>(
-        static_cast<const float*>(workspace), int(splits), size, weights,
-        static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
+    // Enough workgroups to fill the chip with few values, too.
+    auto join = [&](auto slices) {
+      join_kernel<T, slices.value>
+          <<<dim3{unsigned(ceil_div(size, kThreads / slices.value))}, kThreads, 0, s>>>(
+              static_cast<const float*>(workspace), int(splits), size, weights,
+              static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
+    };
+    if (size >= 256 * kThreads)
+      join(std::integral_constant<int, 1>{});
+    else
+      join(std::integral_constant<int, 16>{});
     GS_LAUNCHED("join_kernel");
-    return GS_OK;
+    return int(GS_OK);
   });
 }
 
