@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
                                                       Parameters c) {
   const int64_t total = r.rows * r.per_row;
   const int64_t first = int64_t(blockIdx.x) * (kBlock * Each);
-  float v[Each][kChunk];
+  vec<T, kChunk> raw[Each];
   Place at[Each];
   int valid[Each];
 #pragma unroll
@@ -136,12 +136,13 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
     const bool live = first + local < total;
     if constexpr (Flat) {
       valid[i] = live ? kChunk : 0;
-      load8<T>(x + (first + local) * kChunk, valid[i], v[i]);
+      raw[i] = load_valid<T, kChunk>(x + (first + local) * kChunk, valid[i]);
     } else {
       at[i] = place(r, first, local);
       const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
       valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
-      load8<T>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i], v[i]);
+      raw[i] = load_valid<T, kChunk>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk,
+                                     valid[i]);
     }
   }
 #pragma unroll
@@ -149,16 +150,18 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
     const uint32_t local = i * kBlock + threadIdx.x;
     if (first + local >= total) break;
     const int64_t chunk = first + local;  // rows of the checkpoint follow each other
+    float v[kChunk];
+    widen<T, kChunk>(raw[i], v);
     if (values) {
       uint32_t exponent;
-      const uint2 bytes = keep8<T>(v[i], exponent);
+      const uint2 bytes = keep8<T>(v, largest_of<T, kChunk>(raw[i]), exponent);
       *reinterpret_cast<uint2*>(values + chunk * kChunk) = bytes;
       if ((threadIdx.x & 3) == 0) exponents[chunk >> 2] = uint8_t(exponent);
     }
     if constexpr (K != kNone) {
       float f[kChunk];
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) f[j] = value<T, K>(v[i][j], c);
+      for (int j = 0; j < kChunk; ++j) f[j] = value<T, K>(v[j], c);
       if constexpr (Flat)
         store8<T>(y + chunk * kChunk, kChunk, f);
       else

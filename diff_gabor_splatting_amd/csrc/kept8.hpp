@@ -133,6 +133,12 @@ __device__ __forceinline__ void store_valid(T* p, int valid, vec<T, N> v) {
   }
 }
 
+template <typename T, int N>
+__device__ __forceinline__ void widen(vec<T, N> raw, float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = float(raw[j]);
+}
+
 // Eight consecutive features as float32, zero past `valid`.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int valid, float (&v)[kChunk]) {
@@ -185,18 +191,22 @@ __device__ __forceinline__ uint32_t largest_of(vec<T, N> v) {
 }
 
 // N values over a group's power of two, as bytes, four to a word.
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void keep_bytes(const float (&v)[N], uint32_t exponent,
                                            uint32_t (&out)[N / 4]) {
   const float inverse = exponent == 255 ? 0.f : __uint_as_float((254u - exponent) << 23);
   // v 2^-e + 1.5 2^23 rounds v 2^-e to an integer (ties to even) whose low
-  // byte is q; the clamp acts only at `most`.
+  // byte is q. Only at the largest exponent of a type can q pass 127.
   constexpr float magic = 12582912.f;
   uint32_t bits[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float t = __builtin_fmaf(v[j], inverse, magic);
-    bits[j] = __float_as_uint(__builtin_amdgcn_fmed3f(t, magic - 127.f, magic + 127.f));
+  for (int j = 0; j < N; ++j)
+    bits[j] = __float_as_uint(__builtin_fmaf(v[j], inverse, magic));
+  if (__builtin_expect(__ballot(exponent == KeptRange<T>::most) != 0, 0)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      bits[j] = __float_as_uint(
+          __builtin_amdgcn_fmed3f(__uint_as_float(bits[j]), magic - 127.f, magic + 127.f));
   }
   const uint32_t fine = exponent == 255 ? 0u : ~0u;
 #pragma unroll
@@ -208,18 +218,16 @@ __device__ __forceinline__ void keep_bytes(const float (&v)[N], uint32_t exponen
 }
 
 // The eight values of this lane, as bytes; the quad of lanes that holds the
-// group calls it together. T: the type that sets the exponent's range.
+// group calls it together. `largest`: their largest magnitude's bits. T: the
+// type that sets the exponent's range.
 template <typename T>
-__device__ __forceinline__ uint2 keep8(const float (&v)[kChunk], uint32_t& exponent) {
-  uint32_t largest = 0;
-#pragma unroll
-  for (int j = 0; j < kChunk; ++j)
-    largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+__device__ __forceinline__ uint2 keep8(const float (&v)[kChunk], uint32_t largest,
+                                       uint32_t& exponent) {
   largest = max(largest, dpp<0xB1>(largest));  // quad_perm [1,0,3,2]
   largest = max(largest, dpp<0x4E>(largest));  // quad_perm [2,3,0,1]
   exponent = kept_exponent<T>(largest);
   uint32_t bytes[2];
-  keep_bytes<kChunk>(v, exponent, bytes);
+  keep_bytes<T, kChunk>(v, exponent, bytes);
   return make_uint2(bytes[0], bytes[1]);
 }
 

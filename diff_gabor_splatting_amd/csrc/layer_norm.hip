@@ -31,10 +31,10 @@ struct Add {
   static __device__ float of(float a, float b) { return a + b; }
 };
 struct Low {
-  static __device__ float of(float a, float b) { return a < b || a != a ? a : b; }
+  static __device__ float of(float a, float b) { return fminf(a, b); }
 };
 struct High {
-  static __device__ float of(float a, float b) { return a > b || a != a ? a : b; }
+  static __device__ float of(float a, float b) { return fmaxf(a, b); }
 };
 
 template <int Ctrl>
@@ -117,13 +117,23 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
   for (int i = 0; i < Chunks; ++i) {
     const int column = column_of<Waves>(i, lane, lanes);
     valid[i] = valid_of(column, features);
+    load8<W>(weight + column, weight ? valid[i] : 0, w[i]);
+    load8<W>(bias + column, bias ? valid[i] : 0, b[i]);
+    if (!weight) {
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      w[i][j] = weight && j < valid[i] ? float(weight[column + j]) : 1.f;
-      b[i][j] = bias && j < valid[i] ? float(bias[column + j]) : 0.f;
+      for (int j = 0; j < kChunk; ++j) w[i][j] = 1.f;
     }
   }
   int turn = 0;
+  // The next rows are on their way while these are worked on.
+  vec<T, kChunk> raw[Chunks];
+  auto send = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < Chunks; ++i)
+      raw[i] = load_valid<T, kChunk>(x + row * stride + column_of<Waves>(i, lane, lanes),
+                                     row < rows ? valid[i] : 0);
+  };
+  send(int64_t(blockIdx.x) * per_block + slot);
   // The trip count is the workgroup's: waves of a row meet at barriers.
   for (int64_t first = int64_t(blockIdx.x) * per_block; first < rows;
        first += int64_t(gridDim.x) * per_block) {
@@ -132,9 +142,8 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     float v[Chunks][kChunk];
     float sum = 0.f, low = __builtin_inff(), high = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < Chunks; ++i)
-      load8<T>(x + row * stride + column_of<Waves>(i, lane, lanes), live ? valid[i] : 0,
-                      v[i]);
+    for (int i = 0; i < Chunks; ++i) widen<T, kChunk>(raw[i], v[i]);
+    send(row + int64_t(gridDim.x) * per_block);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
 #pragma unroll
@@ -185,12 +194,16 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
         out[j] = __builtin_fmaf((v[i][j] - mean) * inverse, w[i][j], b[i][j]);
       store8<T>(y + row * features + column, live ? valid[i] : 0, out);
       if (values) {
-        // The last group's lanes past the row keep zeros.
+        // The last group's lanes past the row keep zeros. (A NaN that fmaxf
+        // passes over has made the row's statistics NaN.)
+        float largest = 0.f;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j)
+        for (int j = 0; j < kChunk; ++j) {
           v[i][j] = j < valid[i] ? v[i][j] - centre : 0.f;
+          largest = fmaxf(largest, fabsf(v[i][j]));
+        }
         uint32_t exponent;
-        const uint2 bytes = keep8<float>(v[i], exponent);
+        const uint2 bytes = keep8<float>(v[i], __float_as_uint(largest), exponent);
         if (live && column < groups * kGroup) {
           *reinterpret_cast<uint2*>(values + row * (int64_t(groups) * kGroup) + column) = bytes;
           if (column % kGroup == 0) exponents[row * groups + column / kGroup] = uint8_t(exponent);
@@ -201,7 +214,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
 }
 
 // Partial sums: [gridDim.x][2][features] float32, dw then db.
-template <typename T, typename W, int Chunks, int Waves>
+template <typename T, typename W, int Chunks, int Waves, bool Kept>
 __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
     const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride,
     const uint8_t* __restrict__ values, const uint8_t* __restrict__ exponents,
@@ -219,36 +232,55 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
   for (int i = 0; i < Chunks; ++i) {
     const int column = column_of<Waves>(i, lane, lanes);
     valid[i] = valid_of(column, features);
+    load8<W>(weight + column, weight ? valid[i] : 0, w[i]);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
-      w[i][j] = weight && j < valid[i] ? float(weight[column + j]) : 1.f;
+      if (!weight) w[i][j] = 1.f;
       dw[i][j] = db[i][j] = 0.f;
     }
   }
   int turn = 0;
+  // The next rows are on their way while these are worked on.
+  float2 s_next;
+  vec<T, kChunk> g_next[Chunks], x_next[Chunks];
+  uint2 kept_next[Chunks];
+  uint32_t exponent_next[Chunks];
+  auto send = [&](int64_t row) {
+    const bool live = row < rows;
+    s_next = live ? statistics[row] : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < Chunks; ++i) {
+      const int column = column_of<Waves>(i, lane, lanes);
+      g_next[i] = load_valid<T, kChunk>(dy + row * dy_stride + column, live ? valid[i] : 0);
+      if (Kept) {
+        kept_next[i] = make_uint2(0, 0);
+        exponent_next[i] = 0;
+        if (live && valid[i] > 0) {
+          kept_next[i] = *reinterpret_cast<const uint2*>(
+              values + row * (int64_t(groups) * kGroup) + column);
+          exponent_next[i] = exponents[row * groups + column / kGroup];
+        }
+      } else {
+        x_next[i] = load_valid<T, kChunk>(x + row * x_stride + column, live ? valid[i] : 0);
+      }
+    }
+  };
+  send(int64_t(blockIdx.x) * per_block + slot);
   for (int64_t first = int64_t(blockIdx.x) * per_block; first < rows;
        first += int64_t(gridDim.x) * per_block) {
     const int64_t row = first + slot;
     const bool live = row < rows;
-    const float2 s = live ? statistics[row] : make_float2(0.f, 0.f);
+    const float2 s = s_next;
     float g[Chunks][kChunk], h[Chunks][kChunk];
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
-      const int column = column_of<Waves>(i, lane, lanes);
-      load8<T>(dy + row * dy_stride + column, live ? valid[i] : 0, g[i]);
-      if (values) {
-        uint2 bytes = make_uint2(0, 0);
-        uint32_t exponent = 0;
-        if (live && valid[i] > 0) {
-          bytes = *reinterpret_cast<const uint2*>(values + row * (int64_t(groups) * kGroup) +
-                                                  column);
-          exponent = exponents[row * groups + column / kGroup];
-        }
-        read8(bytes, exponent, h[i]);
-      } else {
-        load8<T>(x + row * x_stride + column, live ? valid[i] : 0, h[i]);
-      }
+      widen<T, kChunk>(g_next[i], g[i]);
+      if (Kept)
+        read8(kept_next[i], exponent_next[i], h[i]);
+      else
+        widen<T, kChunk>(x_next[i], h[i]);
     }
+    send(row + int64_t(gridDim.x) * per_block);
     float sum = 0.f, product = 0.f;
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
@@ -474,13 +506,17 @@ int gs_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const void* grad
     if (rows > 0) {
       with_shape(features, [&](auto chunks, auto waves) {
         const size_t shared = waves.value == 1 ? 2 * size_t(features) * sizeof(float) : 0;
-        layer_norm_backward_kernel<T, W, chunks.value, waves.value>
-            <<<dim3{unsigned(blocks)}, kThreads<waves.value>, shared, s>>>(
-                static_cast<const T*>(grad_y), grad_stride, static_cast<const T*>(x), row_stride,
-                static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),
-                static_cast<const float2*>(statistics), static_cast<const W*>(weight), rows,
-                int(features), lanes_of(features), static_cast<T*>(grad_x),
-                parameters ? static_cast<float*>(workspace) : nullptr);
+        auto launch = [&](auto kept) {
+          layer_norm_backward_kernel<T, W, chunks.value, waves.value, kept.value>
+              <<<dim3{unsigned(blocks)}, kThreads<waves.value>, shared, s>>>(
+                  static_cast<const T*>(grad_y), grad_stride, static_cast<const T*>(x),
+                  row_stride, static_cast<const uint8_t*>(values),
+                  static_cast<const uint8_t*>(exponents), static_cast<const float2*>(statistics),
+                  static_cast<const W*>(weight), rows, int(features), lanes_of(features),
+                  static_cast<T*>(grad_x),
+                  parameters ? static_cast<float*>(workspace) : nullptr);
+        };
+        values ? launch(std::true_type{}) : launch(std::false_type{});
       });
       GS_LAUNCHED("layer_norm_backward_kernel");
     }

@@ -436,7 +436,7 @@ __device__ __forceinline__ void keep_step(const vec<T, kPart<T>> (&x)[Loads], in
 #pragma unroll
     for (int i = 0; i < part; ++i) v[i] = float(x[j][i]);
     uint32_t bytes[part / 4];
-    keep_bytes<part>(v, exponent, bytes);
+    keep_bytes<T, part>(v, exponent, bytes);
     if (row < p.rows && group < groups) {
       uint8_t* const to = values + row * (int64_t(groups) * kGroup) + k;
       if constexpr (part == 8)
@@ -605,14 +605,13 @@ template <typename T>
 using Factor = std::conditional_t<sizeof(T) == 4, bf16, T>;
 
 constexpr int kSumThreads = 512;
-constexpr int kSumRows = 32;
 
 struct SumProduct {
   int64_t rows, stride;   // of dy
   int outputs, features;
   int tiles_m, tiles_n;   // of dW
   int splits;
-  int64_t share;          // rows of a split, a multiple of kSumRows
+  int64_t share;          // rows of a split, a multiple of a step's
 };
 
 template <typename T>
@@ -665,7 +664,7 @@ __device__ __forceinline__ vec<F, 8> turned_fragment(const F* lds, int pitch, in
 }
 
 // A wave's tile: 16 A outputs x 16 B features.
-template <typename T, int A, int B>
+template <typename T, int A, int B, int Rows>
 __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ dy,
                                                           const uint8_t* __restrict__ values,
                                                           const uint8_t* __restrict__ exponents,
@@ -677,11 +676,12 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
   // 32 bytes past a multiple of 256: the eight rows that 32 lanes of a
   // fragment's load read lie in different banks.
   constexpr int pitch_m = tile_m + 16, pitch_n = tile_n + 16;
-  constexpr int buffer = kSumRows * (parts * pitch_m + pitch_n);
+  constexpr int buffer = Rows * (parts * pitch_m + pitch_n);
   constexpr int across_m = tile_m / 8, across_n = tile_n / 16;
-  constexpr int loads_m = kSumRows * across_m / kSumThreads;  // chunks of a thread
-  constexpr bool all_n = kSumRows * across_n >= kSumThreads;
-  static_assert(loads_m >= 1 && kSumRows * across_n <= kSumThreads, "tile does not fit");
+  constexpr int loads_m = Rows * across_m / kSumThreads;  // chunks of a thread
+  constexpr bool all_n = Rows * across_n >= kSumThreads;
+  static_assert(Rows * across_m % kSumThreads == 0 && Rows * across_n <= kSumThreads,
+                "the threads do not divide the tile");
   extern __shared__ __align__(16) char shared[];
   F* const lds = reinterpret_cast<F*>(shared);
 
@@ -701,7 +701,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
   const int row_m = threadIdx.x / across_m, column_m = threadIdx.x % across_m * 8;
   const int row_n = threadIdx.x / across_n, column_n = threadIdx.x % across_n * 16;
   const int valid_m = min(p.outputs - m0 - column_m, 8);
-  const bool has_n = (all_n || row_n < kSumRows) && n0 + column_n < groups * kGroup;
+  const bool has_n = (all_n || row_n < Rows) && n0 + column_n < groups * kGroup;
   const T* from_m = dy + (k0 + row_m) * p.stride + m0 + column_m;
   const uint8_t* from_n = values + (k0 + row_n) * (int64_t(groups) * kGroup) + n0 + column_n;
   const uint8_t* from_e = exponents + (k0 + row_n) * groups + (n0 + column_n) / kGroup;
@@ -726,10 +726,10 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
       to.n = *reinterpret_cast<const vec<uint32_t, 4>*>(from_n);
       to.exponent = *from_e;
     }
-    sent += kSumRows;
-    from_m += kSumRows * p.stride;
-    from_n += kSumRows * int64_t(groups) * kGroup;
-    from_e += kSumRows * groups;
+    sent += Rows;
+    from_m += Rows * p.stride;
+    from_n += Rows * int64_t(groups) * kGroup;
+    from_e += Rows * groups;
   };
   float sum[8] = {};
   const bool sums = n0 == 0;
@@ -745,10 +745,10 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
 #pragma unroll
       for (int h = 0; h < parts; ++h)
         *reinterpret_cast<vec<F, 8>*>(
-            to + (h * kSumRows + row_m + i * (kSumThreads / across_m)) * pitch_m + column_m) =
+            to + (h * Rows + row_m + i * (kSumThreads / across_m)) * pitch_m + column_m) =
             cut[h];
     }
-    if (all_n || row_n < kSumRows) {
+    if (all_n || row_n < Rows) {
       const float scale = __uint_as_float(from.exponent << 23);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
         vec<F, 8> v;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = F(f[j]);
-        *reinterpret_cast<vec<F, 8>*>(to + parts * kSumRows * pitch_m + row_n * pitch_n +
+        *reinterpret_cast<vec<F, 8>*>(to + parts * Rows * pitch_m + row_n * pitch_n +
                                       column_n + 8 * h) = v;
       }
     }
@@ -772,22 +772,26 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
 #pragma unroll
     for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto multiply_step = [&](const F* from) {
-    vec<F, 8> b[B];
 #pragma unroll
-    for (int j = 0; j < B; ++j)
-      b[j] = turned_fragment<F>(from + parts * kSumRows * pitch_m, pitch_n, wave_n + 16 * j);
+    for (int k = 0; k < Rows; k += 32) {
+      vec<F, 8> b[B];
 #pragma unroll
-    for (int h = 0; h < parts; ++h)
+      for (int j = 0; j < B; ++j)
+        b[j] = turned_fragment<F>(from + (parts * Rows) * pitch_m + k * pitch_n, pitch_n,
+                                  wave_n + 16 * j);
 #pragma unroll
-      for (int i = 0; i < A; ++i) {
-        const vec<F, 8> a =
-            turned_fragment<F>(from + h * kSumRows * pitch_m, pitch_m, wave_m + 16 * i);
+      for (int h = 0; h < parts; ++h)
 #pragma unroll
-        for (int j = 0; j < B; ++j) c[i][j] = Mma<F>::of(b[j], a, c[i][j]);
-      }
+        for (int i = 0; i < A; ++i) {
+          const vec<F, 8> a =
+              turned_fragment<F>(from + (h * Rows + k) * pitch_m, pitch_m, wave_m + 16 * i);
+#pragma unroll
+          for (int j = 0; j < B; ++j) c[i][j] = Mma<F>::of(b[j], a, c[i][j]);
+        }
+    }
   };
 
-  const int64_t steps = (k1 - k0 + kSumRows - 1) / kSumRows;
+  const int64_t steps = (k1 - k0 + Rows - 1) / Rows;
   send(ahead[0]);
   send(ahead[1]);
   put(ahead[0], lds);
@@ -865,23 +869,31 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict_
 }
 
 // How dW's sum is cut: tiles of dW (fragments of a wave's tile along the
-// outputs and the features), and shares of the rows.
+// outputs and the features), rows of a step, and shares of the rows.
+//
+// Tiles are as wide as dW asks for, and the widest only where there are rows
+// enough: every workgroup writes a partial tile, so 256 x 256 of them cost 64
+// MB whatever the rows (256 -> 256, bfloat16: 100k rows 45 us with 256-wide
+// tiles, 38 with 128; 1M rows 185 and 225). Two workgroups per compute unit
+// of the narrower ones; 64 rows at least to each.
 struct SumPlan {
-  int a, b;
+  int a, b, step;
   int64_t tiles_m, tiles_n, splits, share;
 };
 
 SumPlan sum_plan(size_t size, int64_t rows, int64_t features, int64_t outputs) {
   SumPlan p{};
-  const bool large = outputs > 128 && features > 128 && rows >= 400000 / (size / 2);
-  p.a = large && size == 2 ? 8 : 4;
-  p.b = large ? 4 : 2;
+  const bool large =
+      outputs > 128 && features > 128 && rows >= 400000 / (int64_t(size) / 2);
+  p.a = large ? (size == 2 ? 8 : 4) : outputs <= 64 ? 2 : 4;
+  p.b = large ? 4 : features <= 64 ? 1 : 2;
+  p.step = p.a == 2 ? 64 : 32;
   p.tiles_m = ceil_div(outputs, 32 * p.a);
   p.tiles_n = ceil_div(features, 64 * p.b);
-  const int64_t workgroups = large ? 256 : 512;
-  p.splits = std::max<int64_t>(1, workgroups / (p.tiles_m * p.tiles_n));
-  p.share = ceil_div(std::max<int64_t>(ceil_div(rows, p.splits), 8 * kSumRows), kSumRows) *
-            kSumRows;
+  const int64_t tiles = p.tiles_m * p.tiles_n;
+  p.splits = std::max<int64_t>(1, (large ? 256 : 512) / tiles);
+  const int64_t least = tiles < 8 ? 64 : 128;
+  p.share = ceil_div(std::max(ceil_div(rows, p.splits), least), p.step) * p.step;
   p.splits = ceil_div(rows, p.share);
   return p;
 }
@@ -894,16 +906,31 @@ int64_t steps_of(size_t size, int64_t k) {
   return steps > 1 ? steps + steps % 2 : steps;
 }
 
-// Fragments side by side of a panel of the matrix: the widest that its k
-// leaves room for in LDS, no wider than the columns of C ask for, at least
-// 128 bytes of a row of C; 0 where that does not fit.
-int panel_fragments(size_t size, int64_t k, int64_t n) {
+// LDS beyond 64 KB is asked for, each time: the kernel may be running on a
+// device where it was not.
+int allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return GS_OK;
+  GS_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  return GS_OK;
+}
+
+// Rows of a wave's tile, and fragments side by side of a panel of the matrix:
+// the widest panel that its k leaves room for in LDS, no wider than the
+// columns of C ask for, at least 128 bytes of a row of C; 0 where that does
+// not fit. With few rows, narrower ones, while that gives more workgroups (up
+// to one per compute unit) less to put in place.
+constexpr int kRowTile = 32;
+int panel_fragments(size_t size, int64_t rows, int64_t k, int64_t n) {
   const int least = size == 4 ? 2 : 4;
-  for (int fragments = 8; fragments >= least; fragments /= 2)
-    if (steps_of(size, k) * 2048 * fragments <= int64_t(kRowLds) &&
-        (n > 8 * fragments || fragments == least))
-      return fragments;
-  return 0;
+  int fragments = 8;
+  while (fragments >= least && steps_of(size, k) * 2048 * fragments > int64_t(kRowLds))
+    fragments /= 2;
+  if (fragments < least) return 0;
+  const int64_t tiles = ceil_div(rows, kRowTile);
+  while (fragments > least &&
+         (n <= 8 * fragments || tiles * ceil_div(n, 8 * fragments) <= 256))
+    fragments /= 2;
+  return fragments;
 }
 
 // C = x matrix through rows_kernel; false where the matrix or the stride is
@@ -912,21 +939,21 @@ template <typename T, bool Transposed>
 int launch_rows(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
                 int64_t rows, int64_t k, int64_t n, void* out, void* values, void* exponents,
                 hipStream_t stream, bool& taken) {
-  const int fragments = panel_fragments(sizeof(T), k, n);
+  const int fragments = panel_fragments(sizeof(T), rows, k, n);
   const int64_t panels = fragments ? ceil_div(n, 16 * fragments) : 0;
   taken = fragments && panels <= 32 && stride < (1 << 24);
   if (!taken) return GS_OK;
   using std::integral_constant;
   auto launch = [&](auto tm, auto tn, auto ahead, auto keep, auto tail) {
     RowsProduct p{rows, stride, int(k), int(n), int(panels), 0, int(steps_of(sizeof(T), k))};
-    const int64_t tiles = ceil_div(rows, 16 * tm.value);
+    static_assert(16 * tm.value == kRowTile, "tiles");
+    const int64_t tiles = ceil_div(rows, kRowTile);
     p.workers = int(std::min<int64_t>(32 / panels * 8, tiles));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
     const size_t lds = size_t(p.steps) * 2 * tn.value * 1024;
     auto* const kernel =
         &rows_kernel<T, tm.value, tn.value, ahead.value, Transposed, keep.value, tail.value>;
-    GS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                               hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+    GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
     kernel<<<grid, kRowThreads, lds, stream>>>(
         static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), p,
         static_cast<T*>(out), static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents));
@@ -966,6 +993,63 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
   }
 }
 
+// --------------------------------------------------------------------------
+// y of a few rows: a wave to an output, its lanes along the features. Each
+// weight is read once, by as many workgroups as a quarter of the outputs; the
+// matrix instructions would wait for a panel in LDS first (1 x 1024 -> 1024:
+// 9.7 us that way).
+
+constexpr int kFewRows = 4;
+
+template <typename T, int Rows>
+__global__ __launch_bounds__(kThreads) void few_rows_kernel(
+    const T* __restrict__ x, int64_t stride, const T* __restrict__ w, const T* __restrict__ bias,
+    int k, int n, T* __restrict__ y) {
+  const int lane = threadIdx.x & 63;
+  const int output = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (output >= n) return;
+  const T* const row = w + int64_t(output) * k;
+  float sum[Rows] = {};
+#pragma unroll 4
+  for (int c = lane * kChunk; c < k; c += 64 * kChunk) {
+    const int valid = min(k - c, kChunk);
+    float a[kChunk], b[Rows][kChunk];
+    load8<T>(row + c, valid, a);
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) load8<T>(x + r * stride + c, valid, b[r]);
+#pragma unroll
+    for (int r = 0; r < Rows; ++r)
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) sum[r] = __builtin_fmaf(a[j], b[r][j], sum[r]);
+  }
+  const float offset = bias ? float(bias[output]) : 0.f;
+#pragma unroll
+  for (int r = 0; r < Rows; ++r) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) sum[r] += __shfl_xor(sum[r], step);
+    if (lane == 0) y[int64_t(r) * n + output] = T(sum[r] + offset);
+  }
+}
+
+template <typename T>
+int launch_few_rows(const void* x, int64_t stride, const void* w, const void* bias, int64_t rows,
+                    int64_t k, int64_t n, void* y, hipStream_t stream) {
+  const dim3 grid{unsigned(ceil_div(n, kThreads / 64))};
+  auto launch = [&](auto count) {
+    few_rows_kernel<T, count.value><<<grid, kThreads, 0, stream>>>(
+        static_cast<const T*>(x), stride, static_cast<const T*>(w), static_cast<const T*>(bias),
+        int(k), int(n), static_cast<T*>(y));
+  };
+  switch (rows) {
+    case 1: launch(std::integral_constant<int, 1>{}); break;
+    case 2: launch(std::integral_constant<int, 2>{}); break;
+    case 3: launch(std::integral_constant<int, 3>{}); break;
+    default: launch(std::integral_constant<int, 4>{}); break;
+  }
+  GS_LAUNCHED("few_rows_kernel");
+  return GS_OK;
+}
+
 int check_linear(const char* name, int32_t dtype, int64_t rows, int64_t features,
                  int64_t outputs) {
   GS_CHECK(check_rows(name, dtype, rows, features, features));
@@ -994,6 +1078,13 @@ int gs_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const vo
              "null pointer passed to gs_linear_forward");
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
+    if (rows <= kFewRows) {  // with and without the 8-bit form: y is the same
+      if (values)
+        GS_CHECK(gs_checkpoint8_write(dtype, x, row_stride, rows, features, values, exponents,
+                                      stream));
+      return launch_few_rows<T>(x, row_stride, weight, bias, rows, features, outputs, y,
+                                static_cast<hipStream_t>(stream));
+    }
     bool taken = false;
     GS_CHECK((launch_rows<T, false>("linear forward", x, row_stride, weight, bias, rows, features,
                                     outputs, y, values, exponents,
@@ -1082,12 +1173,12 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
       const int64_t blocks = ceil_div(splits, 8) * 8 * plan.tiles_m * plan.tiles_n;
       GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "linear backward weight: too large");
       auto launch = [&](auto a, auto b) {
+        constexpr int step = a.value == 2 ? 64 : 32;
         constexpr int pitches = kParts<T> * (32 * a.value + 16) + 64 * b.value + 16;
-        const size_t lds = std::max<size_t>(2 * size_t(kSumRows) * pitches * 2,
+        const size_t lds = std::max<size_t>(2 * size_t(step) * pitches * 2,
                                             size_t(kSumThreads) * 8 * sizeof(float));
-        auto* const kernel = &sum_kernel<T, a.value, b.value>;
-        GS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+        auto* const kernel = &sum_kernel<T, a.value, b.value, step>;
+        GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
         kernel<<<dim3{unsigned(blocks)}, kSumThreads, lds, s>>>(
             static_cast<const T*>(grad_y), static_cast<const uint8_t*>(values),
             static_cast<const uint8_t*>(exponents), p, static_cast<float*>(workspace));
@@ -1095,13 +1186,19 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
         return int(GS_OK);
       };
       using std::integral_constant;
+      using one = integral_constant<int, 1>;
+      using two = integral_constant<int, 2>;
       using four = integral_constant<int, 4>;
-      if constexpr (sizeof(T) == 2)
-        GS_CHECK(plan.a == 8 ? launch(integral_constant<int, 8>{}, four{})
-                             : launch(four{}, integral_constant<int, 2>{}));
-      else
-        GS_CHECK(plan.b == 4 ? launch(four{}, four{})
-                             : launch(four{}, integral_constant<int, 2>{}));
+      const int shape = plan.a * 10 + plan.b;
+      if (shape == 21) GS_CHECK(launch(two{}, one{}));
+      if (shape == 22) GS_CHECK(launch(two{}, two{}));
+      if (shape == 41) GS_CHECK(launch(four{}, one{}));
+      if (shape == 42) GS_CHECK(launch(four{}, two{}));
+      if constexpr (sizeof(T) == 2) {
+        if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}));
+      } else {
+        if (shape == 44) GS_CHECK(launch(four{}, four{}));
+      }
     }
     const int64_t weights = outputs * features, size = weights + outputs;
     // Enough workgroups to fill the chip with few values, too.
