@@ -25,58 +25,108 @@
 namespace gs {
 namespace {
 
-// Lanes of a row: `lanes` (a power of two up to 64) in one wave, or Waves
-// whole waves. Sums, smallest and largest over them.
-struct Add {
-  static __device__ float of(float a, float b) { return a + b; }
-};
-struct Low {
-  static __device__ float of(float a, float b) { return fminf(a, b); }
-};
-struct High {
-  static __device__ float of(float a, float b) { return fmaxf(a, b); }
-};
-
+// Lanes of a row: Lanes (a power of two from 4 to 64) of one wave, or Waves
+// whole waves. The lower lane bits are crossed with DPP moves, the upper two
+// with the lane swaps.
 template <int Ctrl>
 __device__ __forceinline__ float swap(float v) {
   return __uint_as_float(dpp<Ctrl>(__float_as_uint(v)));
 }
 
-template <typename Op>
-__device__ __forceinline__ float across(float v, int lanes) {
-  if (lanes >= 2) v = Op::of(v, swap<0xB1>(v));    // quad_perm [1,0,3,2]
-  if (lanes >= 4) v = Op::of(v, swap<0x4E>(v));    // quad_perm [2,3,0,1]
-  if (lanes >= 8) v = Op::of(v, swap<0x141>(v));   // row_half_mirror
-  if (lanes >= 16) v = Op::of(v, swap<0x140>(v));  // row_mirror
-  if (lanes >= 32) {
+template <int Lanes>
+__device__ __forceinline__ float sum_across(float v) {
+  v += swap<0xB1>(v);                            // quad_perm [1,0,3,2]
+  v += swap<0x4E>(v);                            // quad_perm [2,3,0,1]
+  if constexpr (Lanes >= 8) v += swap<0x141>(v);   // row_half_mirror
+  if constexpr (Lanes >= 16) v += swap<0x140>(v);  // row_mirror
+  if constexpr (Lanes >= 32) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
                                                     false, false);
-    v = Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  if (lanes >= 64) {
+  if constexpr (Lanes >= 64) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
                                                     false, false);
-    v = Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
   return v;
 }
 
-// Two values at once over the row's lanes, through LDS where the row has
-// several waves (`turn` alternates the buffer, so one barrier is enough).
-template <typename First, typename Second, int Waves>
-__device__ __forceinline__ void across2(float& a, float& b, int lanes, int& turn) {
-  a = across<First>(a, lanes);
-  b = across<Second>(b, lanes);
+// Smallest and largest. As instructions, since the compiler quiets every
+// operand of fminf and fmaxf first (four instructions for one); a NaN is
+// passed over. Each s_nop is the distance that a DPP or lane swap keeps from
+// the write of what it reads.
+__device__ __forceinline__ void range_of_8(const float (&v)[kChunk], float& low, float& high) {
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(low) : "v"(v[0]), "v"(v[1]), "v"(v[2]));
+  asm("v_min3_f32 %0, %0, %1, %2" : "+v"(low) : "v"(v[3]), "v"(v[4]));
+  asm("v_min3_f32 %0, %0, %1, %2" : "+v"(low) : "v"(v[5]), "v"(v[6]));
+  asm("v_min_f32 %0, %0, %1" : "+v"(low) : "v"(v[7]));
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(high) : "v"(v[0]), "v"(v[1]), "v"(v[2]));
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(high) : "v"(v[3]), "v"(v[4]));
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(high) : "v"(v[5]), "v"(v[6]));
+  asm("v_max_f32 %0, %0, %1" : "+v"(high) : "v"(v[7]));
+}
+
+__device__ __forceinline__ void widen_range(float& low, float& high, float other_low,
+                                            float other_high) {
+  asm("v_min_f32 %0, %0, %1" : "+v"(low) : "v"(other_low));
+  asm("v_max_f32 %0, %0, %1" : "+v"(high) : "v"(other_high));
+}
+
+#define GS_RANGE_DPP(control)                                                        \
+  asm("s_nop 1\n\t"                                                                  \
+      "v_min_f32_dpp %0, %0, %0 " control " row_mask:0xf bank_mask:0xf\n\t"           \
+      "v_max_f32_dpp %1, %1, %1 " control " row_mask:0xf bank_mask:0xf\n\t"           \
+      "s_nop 1"                                                                      \
+      : "+v"(low), "+v"(high))
+
+template <int Lanes>
+__device__ __forceinline__ void range_across(float& low, float& high) {
+  GS_RANGE_DPP("quad_perm:[1,0,3,2]");
+  GS_RANGE_DPP("quad_perm:[2,3,0,1]");
+  if constexpr (Lanes >= 8) GS_RANGE_DPP("row_half_mirror");
+  if constexpr (Lanes >= 16) GS_RANGE_DPP("row_mirror");
+  if constexpr (Lanes >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(low), __float_as_uint(low),
+                                                    false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(high), __float_as_uint(high),
+                                                    false, false);
+    low = __uint_as_float(a[0]);
+    high = __uint_as_float(b[0]);
+    widen_range(low, high, __uint_as_float(a[1]), __uint_as_float(b[1]));
+    asm("s_nop 1" : "+v"(low), "+v"(high));
+  }
+  if constexpr (Lanes >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(low), __float_as_uint(low),
+                                                    false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(high), __float_as_uint(high),
+                                                    false, false);
+    low = __uint_as_float(a[0]);
+    high = __uint_as_float(b[0]);
+    widen_range(low, high, __uint_as_float(a[1]), __uint_as_float(b[1]));
+  }
+}
+#undef GS_RANGE_DPP
+
+// Two values of every wave of a row's, in LDS. `turn` alternates the buffer,
+// so that one barrier is enough.
+template <int Waves>
+struct Meet {
+  float2 part[2][Waves];
+};
+
+template <int Lanes, int Waves>
+__device__ __forceinline__ void sum2(float& a, float& b, Meet<Waves>& meet, int& turn) {
+  a = sum_across<Lanes>(a);
+  b = sum_across<Lanes>(b);
   if constexpr (Waves > 1) {
-    __shared__ float2 part[2][Waves];
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) part[turn][wave] = make_float2(a, b);
+    if ((threadIdx.x & 63) == 0) meet.part[turn][threadIdx.x >> 6] = make_float2(a, b);
     __syncthreads();
-    float2 all = part[turn][0];
+    float2 all = meet.part[turn][0];
 #pragma unroll
     for (int i = 1; i < Waves; ++i) {
-      all.x = First::of(all.x, part[turn][i].x);
-      all.y = Second::of(all.y, part[turn][i].y);
+      all.x += meet.part[turn][i].x;
+      all.y += meet.part[turn][i].y;
     }
     a = all.x;
     b = all.y;
@@ -84,15 +134,57 @@ __device__ __forceinline__ void across2(float& a, float& b, int lanes, int& turn
   }
 }
 
-// A workgroup of Block threads. Waves == 1: each wave takes 64 / lanes rows
+template <int Lanes, int Waves>
+__device__ __forceinline__ float sum1(float a, Meet<Waves>& meet, int& turn) {
+  if constexpr (Waves > 1) {
+    float unused = 0.f;
+    sum2<Lanes, Waves>(a, unused, meet, turn);
+    return a;
+  } else {
+    return sum_across<Lanes>(a);
+  }
+}
+
+template <int Lanes, int Waves>
+__device__ __forceinline__ void range2(float& low, float& high, Meet<Waves>& meet, int& turn) {
+  range_across<Lanes>(low, high);
+  if constexpr (Waves > 1) {
+    if ((threadIdx.x & 63) == 0) meet.part[turn][threadIdx.x >> 6] = make_float2(low, high);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Waves; ++i)
+      widen_range(low, high, meet.part[turn][i].x, meet.part[turn][i].y);
+    turn ^= 1;
+  }
+}
+
+// A workgroup of kThreads threads. Waves == 1: each wave takes 64 / Lanes rows
 // at a time. Waves > 1: the workgroup takes one row.
 template <int Waves>
 constexpr int kThreads = Waves == 1 ? 256 : Waves * 64;
 
-// The features of chunk i of this lane, and how many of them the row has.
+// Workgroups to a compute unit. The grid is that many for each of the 256,
+// all of them running at once (one more would wait for the rest and then run
+// by itself), and no more than memory likes: 1M x 512 bfloat16 rows, forward
+// with 3, 4, 5, 6: 398, 380, 367, 412 us; keeping 8 bits: 510, 569, 546, 539;
+// backward with 2, 3, 4, 5: 564, 572, 610, 603, from 8 bits 530, 461, 502,
+// 517. The registers of a row set the limit where it takes more lanes' worth.
+enum Pass { kForward, kForwardKept, kBackward };
+template <int Chunks, int Waves>
+constexpr int workgroups_of(Pass pass) {
+  if (Waves == 16) return 1;
+  if (Chunks == 1) return pass == kForward ? 5 : 3;
+  if (Chunks == 2) return pass == kBackward ? 2 : 3;
+  return pass == kBackward ? 1 : 2;
+}
 template <int Waves>
-__device__ __forceinline__ int column_of(int i, int lane, int lanes) {
-  return (i * (Waves == 1 ? lanes : Waves * 64) + lane) * kChunk;
+constexpr int kSimdWaves = Waves == 16 ? 4 : 1;  // of a workgroup, on each of the four
+constexpr int kUnits = 256;
+
+// The features of chunk i of this lane, and how many of them the row has.
+template <int Lanes, int Waves>
+__device__ __forceinline__ int column_of(int i, int lane) {
+  return (i * Lanes * Waves + lane) * kChunk;
 }
 
 __device__ __forceinline__ int valid_of(int column, int features) {
@@ -100,22 +192,25 @@ __device__ __forceinline__ int valid_of(int column, int features) {
   return left < 0 ? 0 : left < kChunk ? left : kChunk;
 }
 
-template <typename T, typename W, int Chunks, int Waves>
-__global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
+template <typename T, typename W, int Chunks, int Waves, int Lanes>
+__global__ __launch_bounds__(
+    kThreads<Waves>, (workgroups_of<Chunks, Waves>(kForward) * kSimdWaves<Waves>)) void layer_norm_forward_kernel(
     const T* __restrict__ x, int64_t stride, const W* __restrict__ weight,
-    const W* __restrict__ bias, float eps, int64_t rows, int features, int lanes,
+    const W* __restrict__ bias, float eps, int64_t rows, int features,
     T* __restrict__ y, float2* __restrict__ statistics, uint8_t* __restrict__ values,
     uint8_t* __restrict__ exponents) {
-  const int lane = Waves == 1 ? threadIdx.x % lanes : threadIdx.x;
-  const int per_block = Waves == 1 ? kThreads<1> / lanes : 1;
-  const int slot = Waves == 1 ? threadIdx.x / lanes : 0;
+  static_assert(Waves == 1 || Lanes == 64, "a row of several waves takes whole ones");
+  constexpr int per_block = Waves == 1 ? kThreads<1> / Lanes : 1;
+  const int lane = Waves == 1 ? threadIdx.x % Lanes : threadIdx.x;
+  const int slot = Waves == 1 ? threadIdx.x / Lanes : 0;
+  __shared__ Meet<Waves> meet;
   const int groups = (features + kGroup - 1) / kGroup;
   const float inverse_count = 1.f / float(features);
   float w[Chunks][kChunk], b[Chunks][kChunk];
   int valid[Chunks];
 #pragma unroll
   for (int i = 0; i < Chunks; ++i) {
-    const int column = column_of<Waves>(i, lane, lanes);
+    const int column = column_of<Lanes, Waves>(i, lane);
     valid[i] = valid_of(column, features);
     load8<W>(weight + column, weight ? valid[i] : 0, w[i]);
     load8<W>(bias + column, bias ? valid[i] : 0, b[i]);
@@ -130,7 +225,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
   auto send = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
-      raw[i] = load_valid<T, kChunk>(x + row * stride + column_of<Waves>(i, lane, lanes),
+      raw[i] = load_valid<T, kChunk>(x + row * stride + column_of<Lanes, Waves>(i, lane),
                                      row < rows ? valid[i] : 0);
   };
   send(int64_t(blockIdx.x) * per_block + slot);
@@ -140,7 +235,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     const int64_t row = first + slot;
     const bool live = row < rows;
     float v[Chunks][kChunk];
-    float sum = 0.f, low = __builtin_inff(), high = -__builtin_inff();
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) widen<T, kChunk>(raw[i], v[i]);
     send(row + int64_t(gridDim.x) * per_block);
@@ -148,8 +243,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
     for (int i = 0; i < Chunks; ++i)
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) sum += v[i][j];
-    float unused = 0.f;
-    across2<Add, Add, Waves>(sum, unused, lanes, turn);
+    sum = sum1<Lanes, Waves>(sum, meet, turn);
     // sum / features, rounded once: the product with the reciprocal and one
     // correction (a constant row's mean is then its value).
     float mean = sum * inverse_count;
@@ -170,24 +264,32 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
           squares = __builtin_fmaf(d, d, squares);
         }
       }
-    across2<Add, Add, Waves>(squares, unused, lanes, turn);
+    squares = sum1<Lanes, Waves>(squares, meet, turn);
     const float inverse = rsqrtf(__builtin_fmaf(squares, inverse_count, eps));
     float centre = 0.f;
     if (values) {
+      float low = __builtin_inff(), high = -low;
 #pragma unroll
-      for (int i = 0; i < Chunks; ++i)
+      for (int i = 0; i < Chunks; ++i) {
+        float in_low = __builtin_inff(), in_high = -in_low;
+        if (valid[i] == kChunk) {
+          range_of_8(v[i], in_low, in_high);
+        } else if (valid[i] > 0) {
+          // The row's last chunk, its first value in place of what it lacks.
+          float filled[kChunk];
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          low = Low::of(low, j < valid[i] ? v[i][j] : low);
-          high = High::of(high, j < valid[i] ? v[i][j] : high);
+          for (int j = 0; j < kChunk; ++j) filled[j] = j < valid[i] ? v[i][j] : v[i][0];
+          range_of_8(filled, in_low, in_high);
         }
-      across2<Low, High, Waves>(low, high, lanes, turn);
+        widen_range(low, high, in_low, in_high);
+      }
+      range2<Lanes, Waves>(low, high, meet, turn);
       centre = 0.5f * low + 0.5f * high;
     }
     if (statistics && live && lane == 0) statistics[row] = make_float2(mean - centre, inverse);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
-      const int column = column_of<Waves>(i, lane, lanes);
+      const int column = column_of<Lanes, Waves>(i, lane);
       float out[kChunk];
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
@@ -196,12 +298,15 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
       if (values) {
         // The last group's lanes past the row keep zeros. (A NaN that fmaxf
         // passes over has made the row's statistics NaN.)
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) v[i][j] -= centre;
+        if (valid[i] != kChunk) {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) v[i][j] = j < valid[i] ? v[i][j] : 0.f;
+        }
         float largest = 0.f;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          v[i][j] = j < valid[i] ? v[i][j] - centre : 0.f;
-          largest = fmaxf(largest, fabsf(v[i][j]));
-        }
+        for (int j = 0; j < kChunk; ++j) largest = fmaxf(largest, fabsf(v[i][j]));
         uint32_t exponent;
         const uint2 bytes = keep8<float>(v[i], __float_as_uint(largest), exponent);
         if (live && column < groups * kGroup) {
@@ -214,23 +319,27 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_forward_kernel(
 }
 
 // Partial sums: [gridDim.x][2][features] float32, dw then db.
-template <typename T, typename W, int Chunks, int Waves, bool Kept>
-__global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
+template <typename T, typename W, int Chunks, int Waves, int Lanes, bool Kept>
+__global__ __launch_bounds__(
+    kThreads<Waves>,
+    (workgroups_of<Chunks, Waves>(kBackward) * kSimdWaves<Waves>)) void layer_norm_backward_kernel(
     const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride,
     const uint8_t* __restrict__ values, const uint8_t* __restrict__ exponents,
     const float2* __restrict__ statistics, const W* __restrict__ weight, int64_t rows,
-    int features, int lanes, T* __restrict__ dx, float* __restrict__ partial) {
+    int features, T* __restrict__ dx, float* __restrict__ partial) {
   extern __shared__ float shared[];
-  const int lane = Waves == 1 ? threadIdx.x % lanes : threadIdx.x;
-  const int per_block = Waves == 1 ? kThreads<1> / lanes : 1;
-  const int slot = Waves == 1 ? threadIdx.x / lanes : 0;
+  static_assert(Waves == 1 || Lanes == 64, "a row of several waves takes whole ones");
+  constexpr int per_block = Waves == 1 ? kThreads<1> / Lanes : 1;
+  const int lane = Waves == 1 ? threadIdx.x % Lanes : threadIdx.x;
+  const int slot = Waves == 1 ? threadIdx.x / Lanes : 0;
+  __shared__ Meet<Waves> meet;
   const int groups = (features + kGroup - 1) / kGroup;
   const float inverse_count = 1.f / float(features);
   float w[Chunks][kChunk], dw[Chunks][kChunk], db[Chunks][kChunk];
   int valid[Chunks];
 #pragma unroll
   for (int i = 0; i < Chunks; ++i) {
-    const int column = column_of<Waves>(i, lane, lanes);
+    const int column = column_of<Lanes, Waves>(i, lane);
     valid[i] = valid_of(column, features);
     load8<W>(weight + column, weight ? valid[i] : 0, w[i]);
 #pragma unroll
@@ -250,7 +359,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
     s_next = live ? statistics[row] : make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
-      const int column = column_of<Waves>(i, lane, lanes);
+      const int column = column_of<Lanes, Waves>(i, lane);
       g_next[i] = load_valid<T, kChunk>(dy + row * dy_stride + column, live ? valid[i] : 0);
       if (Kept) {
         kept_next[i] = make_uint2(0, 0);
@@ -293,7 +402,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
         dw[i][j] = __builtin_fmaf(g[i][j], h[i][j], dw[i][j]);
         db[i][j] += g[i][j];
       }
-    across2<Add, Add, Waves>(sum, product, lanes, turn);
+    sum2<Lanes, Waves>(sum, product, meet, turn);
     sum *= inverse_count;
     product *= inverse_count;
 #pragma unroll
@@ -302,7 +411,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
         out[j] = s.y * (__builtin_fmaf(g[i][j], w[i][j], -sum) - h[i][j] * product);
-      store8<T>(dx + row * features + column_of<Waves>(i, lane, lanes),
+      store8<T>(dx + row * features + column_of<Lanes, Waves>(i, lane),
                        live ? valid[i] : 0, out);
     }
   }
@@ -311,7 +420,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
   if constexpr (Waves > 1) {
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
-      const int column = column_of<Waves>(i, lane, lanes);
+      const int column = column_of<Lanes, Waves>(i, lane);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
         if (j < valid[i]) {
@@ -323,7 +432,7 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
     // The workgroup's slots each hold sums of every feature: slots add theirs
     // to LDS one after the other's barrier, in their order. Slots of one wave
     // are added across its lanes first.
-    for (int step = lanes; step < 64; step *= 2) {
+    for (int step = Lanes; step < 64; step *= 2) {
 #pragma unroll
       for (int i = 0; i < Chunks; ++i)
 #pragma unroll
@@ -333,12 +442,12 @@ __global__ __launch_bounds__(kThreads<Waves>) void layer_norm_backward_kernel(
         }
     }
     const int wave = threadIdx.x >> 6;
-    const bool holds = (threadIdx.x & 63) < lanes;
+    const bool holds = (threadIdx.x & 63) < Lanes;
     for (int turn_of = 0; turn_of < kThreads<1> / 64; ++turn_of) {
       if (wave == turn_of && holds) {
 #pragma unroll
         for (int i = 0; i < Chunks; ++i) {
-          const int column = column_of<Waves>(i, lane, lanes);
+          const int column = column_of<Lanes, Waves>(i, lane);
 #pragma unroll
           for (int j = 0; j < kChunk; ++j)
             if (j < valid[i]) {
@@ -387,37 +496,48 @@ __global__ __launch_bounds__(kColumns* kSlices) void layer_norm_parameters_kerne
 // Rows wider than this are refused.
 constexpr int64_t kMostNormFeatures = 16384;
 
-int lanes_of(int64_t features) {
-  int lanes = 1;
-  while (lanes < 64 && lanes * kChunk < features) lanes *= 2;
-  return lanes < 4 ? 4 : lanes;  // a group of the checkpoint takes four
-}
-
-// Workgroups: enough rows at a time to fill the chip, each taking several
-// after one another, so that parameters are loaded and partial sums written
-// once for all of them.
-int64_t blocks_of(int64_t rows, int64_t features, bool backward) {
-  const int64_t per_block = features <= 2048 ? 256 / lanes_of(features) : 1;
-  const int64_t most = backward ? 1024 : 2048;
-  return std::min(ceil_div(rows, per_block), most);
-}
-
+// Chunks of a lane, waves of a row and lanes of a wave for a width. A group
+// of the checkpoint takes four lanes, so a row takes as many at least.
 template <typename F>
 void with_shape(int64_t features, F&& launch) {
   using std::integral_constant;
   using one = integral_constant<int, 1>;
   using two = integral_constant<int, 2>;
   using four = integral_constant<int, 4>;
-  if (features <= 512)
-    launch(one{}, one{});
+  using all = integral_constant<int, 64>;
+  if (features <= 32)
+    launch(one{}, one{}, four{});
+  else if (features <= 64)
+    launch(one{}, one{}, integral_constant<int, 8>{});
+  else if (features <= 128)
+    launch(one{}, one{}, integral_constant<int, 16>{});
+  else if (features <= 256)
+    launch(one{}, one{}, integral_constant<int, 32>{});
+  else if (features <= 512)
+    launch(one{}, one{}, all{});
   else if (features <= 1024)
-    launch(two{}, one{});
+    launch(two{}, one{}, all{});
   else if (features <= 2048)
-    launch(four{}, one{});
+    launch(four{}, one{}, all{});
+  else if (features <= 4096)
+    launch(two{}, four{}, all{});
   else if (features <= 8192)
-    launch(four{}, four{});
+    launch(four{}, four{}, all{});
   else
-    launch(two{}, integral_constant<int, 16>{});
+    launch(two{}, integral_constant<int, 16>{}, all{});
+}
+
+// Workgroups: as many as the chip holds, each taking several rows after one
+// another, so that parameters are loaded and partial sums written once for
+// all of them; fewer where there are not the rows.
+int64_t blocks_of(int64_t rows, int64_t features, Pass pass) {
+  int64_t blocks = 0;
+  with_shape(features, [&](auto chunks, auto waves, auto lanes) {
+    const int64_t per_block = waves.value == 1 ? kThreads<1> / lanes.value : 1;
+    const int64_t most = kUnits * workgroups_of<chunks.value, waves.value>(pass);
+    blocks = std::min(ceil_div(rows, per_block), most);
+  });
+  return blocks;
 }
 
 template <typename F>
@@ -458,12 +578,12 @@ int gs_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const void* x, in
   return with_types(dtype, weight_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    const dim3 grid{unsigned(blocks_of(rows, features, false))};
-    with_shape(features, [&](auto chunks, auto waves) {
-      layer_norm_forward_kernel<T, W, chunks.value, waves.value>
+    const dim3 grid{unsigned(blocks_of(rows, features, values ? kForwardKept : kForward))};
+    with_shape(features, [&](auto chunks, auto waves, auto lanes) {
+      layer_norm_forward_kernel<T, W, chunks.value, waves.value, lanes.value>
           <<<grid, kThreads<waves.value>, 0, s>>>(
               static_cast<const T*>(x), row_stride, static_cast<const W*>(weight),
-              static_cast<const W*>(bias), eps, rows, int(features), lanes_of(features),
+              static_cast<const W*>(bias), eps, rows, int(features),
               static_cast<T*>(y), static_cast<float2*>(statistics),
               static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents));
     });
@@ -474,7 +594,7 @@ int gs_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const void* x, in
 
 size_t gs_layer_norm_backward_workspace_size(int64_t rows, int64_t features) {
   if (rows <= 0 || features <= 0) return 0;
-  return size_t(gs::blocks_of(rows, features, true)) * 2 * size_t(features) * sizeof(float);
+  return size_t(gs::blocks_of(rows, features, gs::kBackward)) * 2 * size_t(features) * sizeof(float);
 }
 
 int gs_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const void* grad_y,
@@ -502,17 +622,17 @@ int gs_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const void* grad
   return with_types(dtype, weight_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    const int64_t blocks = rows > 0 ? blocks_of(rows, features, true) : 0;
+    const int64_t blocks = rows > 0 ? blocks_of(rows, features, kBackward) : 0;
     if (rows > 0) {
-      with_shape(features, [&](auto chunks, auto waves) {
+      with_shape(features, [&](auto chunks, auto waves, auto lanes) {
         const size_t shared = waves.value == 1 ? 2 * size_t(features) * sizeof(float) : 0;
         auto launch = [&](auto kept) {
-          layer_norm_backward_kernel<T, W, chunks.value, waves.value, kept.value>
+          layer_norm_backward_kernel<T, W, chunks.value, waves.value, lanes.value, kept.value>
               <<<dim3{unsigned(blocks)}, kThreads<waves.value>, shared, s>>>(
                   static_cast<const T*>(grad_y), grad_stride, static_cast<const T*>(x),
                   row_stride, static_cast<const uint8_t*>(values),
                   static_cast<const uint8_t*>(exponents), static_cast<const float2*>(statistics),
-                  static_cast<const W*>(weight), rows, int(features), lanes_of(features),
+                  static_cast<const W*>(weight), rows, int(features),
                   static_cast<T*>(grad_x),
                   parameters ? static_cast<float*>(workspace) : nullptr);
         };

@@ -413,37 +413,38 @@ __device__ __forceinline__ int turn_place(int r, int h, int c) {
 }
 
 // The 8-bit form of one step of a tile's rows, as they were loaded: lane l
-// has piece l % 8 of row 8 j + l / 8 of x[j].
+// has piece l % 8 of row 8 j + l / 8 of x[j]. `rows_left`: of the tile's.
 template <typename T, int Loads>
 __device__ __forceinline__ void keep_step(const vec<T, kPart<T>> (&x)[Loads], int64_t first,
-                                          int s, const RowsProduct& p,
+                                          int rows_left, int s, int groups,
                                           uint8_t* __restrict__ values,
                                           uint8_t* __restrict__ exponents) {
   constexpr int part = kPart<T>;
-  const int lane = threadIdx.x & 63;
-  const int groups = (p.k + kGroup - 1) / kGroup;
-  const int k = s * kStep<T> + (lane & 7) * part;
-  const int group = k / kGroup;
+  const int lane = threadIdx.x & 63, piece = lane & 7;
+  const int in_step = piece * part / kGroup;  // group of the step
+  const int group = s * (kStep<T> / kGroup) + in_step;
+  uint8_t* const to_values = values + first * (groups * kGroup) + s * kStep<T>;
+  uint8_t* const to_exponents = exponents + first * groups + s * (kStep<T> / kGroup);
 #pragma unroll
   for (int j = 0; j < Loads; ++j) {
-    const int64_t row = first + 8 * j + (lane >> 3);
+    const int row = 8 * j + (lane >> 3);
     uint32_t largest = largest_of<T, part>(x[j]);
     largest = max(largest, dpp<0xB1>(largest));  // quad_perm [1,0,3,2]
     largest = max(largest, dpp<0x4E>(largest));  // quad_perm [2,3,0,1]
     if constexpr (part == 4) largest = max(largest, dpp<0x141>(largest));  // row_half_mirror
     const uint32_t exponent = kept_exponent<T>(largest);
     float v[part];
-#pragma unroll
-    for (int i = 0; i < part; ++i) v[i] = float(x[j][i]);
+    widen<T, part>(x[j], v);
     uint32_t bytes[part / 4];
     keep_bytes<T, part>(v, exponent, bytes);
-    if (row < p.rows && group < groups) {
-      uint8_t* const to = values + row * (int64_t(groups) * kGroup) + k;
+    if (row < rows_left && group < groups) {
+      uint8_t* const to = to_values + uint32_t(row * groups * kGroup + piece * part);
       if constexpr (part == 8)
         *reinterpret_cast<uint2*>(to) = make_uint2(bytes[0], bytes[1]);
       else
         *reinterpret_cast<uint32_t*>(to) = bytes[0];
-      if (k % kGroup == 0) exponents[row * groups + group] = uint8_t(exponent);
+      if (piece * part % kGroup == 0)
+        to_exponents[uint32_t(row * groups + in_step)] = uint8_t(exponent);
     }
   }
 }
@@ -477,6 +478,7 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
   const int row8 = lane >> 3, piece = lane & 7;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part* const turn = turns[wave];
+  const int groups = (p.k + kGroup - 1) / kGroup;
   const int64_t tiles = (p.rows + 16 * TM - 1) / (16 * TM);
   const int64_t each = int64_t(p.workers) * kRowWaves;
   // Tiles go round the workgroups first, then round their waves.
@@ -543,7 +545,9 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
         if constexpr (Keep) {
           // The panels share the rows' 8-bit form: each keeps its turn's steps.
           if (s % p.panels == at)
-            keep_step<T, loads>(ring[u], tile * (16 * TM), s, p, values, exponents);
+            keep_step<T, loads>(ring[u], tile * (16 * TM),
+                                int(min(p.rows - tile * (16 * TM), int64_t(16 * TM))), s,
+                                groups, values, exponents);
         }
         send(ring[u]);
 #pragma unroll
@@ -883,8 +887,9 @@ struct SumPlan {
 
 SumPlan sum_plan(size_t size, int64_t rows, int64_t features, int64_t outputs) {
   SumPlan p{};
-  const bool large =
-      outputs > 128 && features > 128 && rows >= 400000 / (int64_t(size) / 2);
+  const bool large = outputs > 128 && features > 128 &&
+                     double(rows) * double(outputs) * double(features) >=
+                         (size == 2 ? 2e10 : 1e10);
   p.a = large ? (size == 2 ? 8 : 4) : outputs <= 64 ? 2 : 4;
   p.b = large ? 4 : features <= 64 ? 1 : 2;
   p.step = p.a == 2 ? 64 : 32;
