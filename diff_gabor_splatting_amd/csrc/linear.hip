@@ -2,22 +2,17 @@
 // gradients dx = dy W, dW = dy^T x8, db = the sum of dy's rows, x8 what the
 // checkpoint stands for.
 //
-// All three products are one tiled kernel: C[m][n] = sum_k M(m,k) N(n,k), on
-// the matrix cores with float32 accumulators (16x16x32 for the 2-byte types,
-// 16x16x4 for float32). A side whose k is the contiguous dimension in memory
-// is staged in LDS as it lies; one whose m or n is (W in dx, both sides of
-// dW) is staged row by row too, and the 2-byte types' fragments are read
-// with the transposing LDS load. What is kept in 8 bits is expanded while it
-// is staged: q 2^e is exact in each type.
+// All products run on the matrix cores with float32 accumulators (16x16x32
+// for the 2-byte types, 16x16x4 for float32). What bounds them is memory up to
+// about 256 features and outputs, the matrix cores beyond:
 //
-//                M side             N side               k
-//   y    rows    x  [m][k]          W  [n][k]            features
-//   dx   rows    dy [m][k]          W  [k][n]            outputs
-//   dW   outputs dy [k][m]          x8 [k][n]            rows, split
+//   few_rows_kernel  y of up to four rows: a wave to an output
+//   rows_kernel      y and dx: the matrix in LDS, rows streamed past it
+//   product_kernel   y and dx where the matrix has a side too long for that
+//   sum_kernel       dW and db: tiles of dW over shares of the rows, whose
+//                    partial sums join_kernel adds in their order
 //
-// dW's k is long and its C small: the rows are split over workgroups, each
-// writes a float32 partial C, and a second kernel adds the partials in their
-// order (no atomics: results do not depend on timing).
+// No atomics: results do not depend on timing.
 #include "kept8.hpp"
 #include "layers_api.hpp"
 
@@ -73,17 +68,11 @@ __device__ __forceinline__ int place_of(int n) {
   return (n & ~63) + 16 * ((n >> 2) & 3) + 4 * ((n >> 4) & 3) + (n & 3);
 }
 
-// A side in memory: rows x columns of T, or of the 8-bit form.
+// A side in memory: rows x columns.
 template <typename T>
 struct Side {
   const T* data;
   int64_t stride;
-  int64_t rows, columns;
-};
-struct KeptSide {
-  const uint8_t* values;
-  const uint8_t* exponents;
-  int64_t groups;
   int64_t rows, columns;
 };
 
@@ -95,32 +84,14 @@ struct Staged {
   static constexpr int across = Columns / kChunk;
   vec<T, 8> v[count];
 
-  __device__ __forceinline__ void load(const Side<T>& s, int64_t row, int64_t column,
-                                       int64_t end) {
+  __device__ __forceinline__ void load(const Side<T>& s, int64_t row, int64_t column) {
 #pragma unroll
     for (int i = 0; i < count; ++i) {
       const int id = i * kThreads + threadIdx.x;
       const int64_t r = row + id / across, c = column + (id % across) * kChunk;
       const int64_t left = s.columns - c;
       v[i] = load_valid<T, 8>(s.data + r * s.stride + c,
-                              r < end ? int(left < kChunk ? left : kChunk) : 0);
-    }
-  }
-
-  __device__ __forceinline__ void load(const KeptSide& s, int64_t row, int64_t column,
-                                       int64_t end) {
-#pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int id = i * kThreads + threadIdx.x;
-      const int64_t r = row + id / across, c = column + (id % across) * kChunk;
-      v[i] = T(0);
-      if (r < end && c < s.groups * kGroup) {
-        float f[kChunk];
-        read8(*reinterpret_cast<const uint2*>(s.values + r * s.groups * kGroup + c),
-              s.exponents[r * s.groups + c / kGroup], f);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[i][j] = T(f[j]);
-      }
+                              r < s.rows ? int(left < kChunk ? left : kChunk) : 0);
     }
   }
 
@@ -188,28 +159,25 @@ __device__ __forceinline__ void store_row(T* p, int64_t left, const float (&c)[1
 }
 
 struct Product {
-  int64_t m, n;        // C's rows and columns
-  int64_t k;           // length of the sum
-  int64_t split;       // k of one workgroup (a multiple of the depth)
+  int64_t m, n;     // C's rows and columns
+  int64_t k;        // length of the sum
   int64_t tiles_n;
 };
 
-// out: C in T (split == k), or partial float32 C's, one per split, each
-// followed by the M side's sums over k where sums is set.
-template <typename T, bool MContiguous, bool NContiguous, typename NSide>
-__global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns, Product p,
+// C[m][n] = sum_k M(m, k) N(n, k) (+ bias[n]), one 128 x 128 tile to a
+// workgroup: a step of both sides is in registers while the step before is
+// multiplied out of LDS. M is the rows, k contiguous; N the matrix, [n][k] in
+// memory (NContiguous) or [k][n].
+template <typename T, bool NContiguous>
+__global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, Side<T> ns, Product p,
                                                            const T* __restrict__ bias,
-                                                           T* __restrict__ out,
-                                                           float* __restrict__ partial) {
+                                                           T* __restrict__ out) {
   constexpr int depth = Mma<T>::depth;
-  __shared__ __align__(16) T m_lds[kTileSize<T, MContiguous>];
+  __shared__ __align__(16) T m_lds[kTileSize<T, true>];
   __shared__ __align__(16) T n_lds[kTileSize<T, NContiguous>];
-  Staged<T, MContiguous ? kEdge : depth, MContiguous ? depth : kEdge> m_next;
+  Staged<T, kEdge, depth> m_next;
   Staged<T, NContiguous ? kEdge : depth, NContiguous ? depth : kEdge> n_next;
-  const int64_t tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x % p.tiles_n;
-  const int64_t m0 = tile_m * kEdge, n0 = tile_n * kEdge;
-  const int64_t k0 = int64_t(blockIdx.y) * p.split;
-  const int64_t k1 = k0 + p.split < p.k ? k0 + p.split : p.k;
+  const int64_t m0 = blockIdx.x / p.tiles_n * kEdge, n0 = blockIdx.x % p.tiles_n * kEdge;
   const int wave = threadIdx.x >> 6;
   const int wave_m = (wave >> 1) * kWaveEdge, wave_n = (wave & 1) * kWaveEdge;
   f32x4 c[kTiles][kTiles];  // [m][n]
@@ -217,40 +185,25 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
   for (int i = 0; i < kTiles; ++i)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr bool sums = !MContiguous;
-  float sum[kChunk] = {};
-
   auto fetch = [&](int64_t k) {
-    if constexpr (MContiguous)
-      m_next.load(ms, m0, k, p.m);
-    else
-      m_next.load(ms, k, m0, k1);
+    m_next.load(ms, m0, k);
     if constexpr (NContiguous)
-      n_next.load(ns, n0, k, p.n);
+      n_next.load(ns, n0, k);
     else
-      n_next.load(ns, k, n0, k1);
+      n_next.load(ns, k, n0);
   };
-  fetch(k0);
-  for (int64_t k = k0; k < k1; k += depth) {
-    m_next.template store<kPitch<T, MContiguous>, false, MContiguous>(m_lds);
+  fetch(0);
+  for (int64_t k = 0; k < p.k; k += depth) {
+    m_next.template store<kPitch<T, true>, false, true>(m_lds);
     n_next.template store<kPitch<T, NContiguous>, true, NContiguous>(n_lds);
-    if constexpr (sums) {
-      // A thread's chunks of dy lie in the same eight columns throughout.
-      if (tile_n == 0) {
-#pragma unroll
-        for (int i = 0; i < m_next.count; ++i)
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) sum[j] += float(m_next.v[i][j]);
-      }
-    }
     __syncthreads();
-    if (k + depth < k1) fetch(k + depth);
+    if (k + depth < p.k) fetch(k + depth);
 #pragma unroll
     for (int s = 0; s < depth; s += Mma<T>::step) {
       typename Mma<T>::Fragment a[kTiles], b[kTiles];
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        a[i] = fragment<T, MContiguous>(m_lds, wave_m + 16 * i, s);
+        a[i] = fragment<T, true>(m_lds, wave_m + 16 * i, s);
         b[i] = fragment<T, NContiguous>(n_lds, wave_n + 16 * i, s);
       }
 #pragma unroll
@@ -267,8 +220,6 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
   float offset[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) offset[j] = bias && n + j < p.n ? float(bias[n + j]) : 0.f;
-  float* mine = partial ? partial + int64_t(blockIdx.y) * (p.m * p.n + (sums ? p.m : 0))
-                        : nullptr;
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     const int64_t m = m0 + wave_m + 16 * i + (lane & 15);
@@ -276,28 +227,7 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, NSide ns,
     float row[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) row[j] = c[i][j >> 2][j & 3] + offset[j];
-    if (mine)
-      store_row<float>(mine + m * p.n + n, p.n - n, row);
-    else
-      store_row<T>(out + m * p.n + n, p.n - n, row);
-  }
-  if constexpr (sums) {
-    if (tile_n == 0) {
-      // 16 threads a row of the staged tile; the 16 rows' sums meet in LDS.
-      float* all = reinterpret_cast<float*>(m_lds);
-      static_assert(sizeof(m_lds) >= 16 * kEdge * sizeof(float), "sums do not fit");
-      constexpr int across = kEdge / kChunk;
-      const int r = threadIdx.x / across, column = threadIdx.x % across * kChunk;
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j) all[r * kEdge + column + j] = sum[j];
-      __syncthreads();
-      const int64_t m = m0 + threadIdx.x;
-      if (threadIdx.x < kEdge && m < p.m) {
-        float total = 0.f;
-        for (int i = 0; i < kThreads / across; ++i) total += all[i * kEdge + threadIdx.x];
-        mine[p.m * p.n + m] = total;
-      }
-    }
+    store_row<T>(out + m * p.n + n, p.n - n, row);
   }
 }
 
@@ -479,6 +409,9 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part* const turn = turns[wave];
   const int groups = (p.k + kGroup - 1) / kGroup;
+  // Steps that lie together in memory go to one panel, whole lines of it.
+  const int keep_each = (p.steps + p.panels - 1) / p.panels;
+  const int keep_from = at * keep_each, keep_to = keep_from + keep_each;
   const int64_t tiles = (p.rows + 16 * TM - 1) / (16 * TM);
   const int64_t each = int64_t(p.workers) * kRowWaves;
   // Tiles go round the workgroups first, then round their waves.
@@ -543,8 +476,8 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
           wave_order();
         }
         if constexpr (Keep) {
-          // The panels share the rows' 8-bit form: each keeps its turn's steps.
-          if (s % p.panels == at)
+          // The panels share the rows' 8-bit form: each keeps its own steps.
+          if (s >= keep_from && s < keep_to)
             keep_step<T, loads>(ring[u], tile * (16 * TM),
                                 int(min(p.rows - tile * (16 * TM), int64_t(16 * TM))), s,
                                 groups, values, exponents);
@@ -1100,12 +1033,10 @@ int gs_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const vo
                                     stream));
     const Side<T> ms{static_cast<const T*>(x), row_stride, rows, features};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
-    const Product p{rows, outputs, features, ceil_div(features, 64) * 64,
-                    ceil_div(outputs, kEdge)};
+    const Product p{rows, outputs, features, ceil_div(outputs, kEdge)};
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
-    product_kernel<T, true, true, Side<T>>
-        <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            ms, ns, p, static_cast<const T*>(bias), static_cast<T*>(y), nullptr);
+    product_kernel<T, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        ms, ns, p, static_cast<const T*>(bias), static_cast<T*>(y));
     GS_LAUNCHED("linear forward");
     return int(GS_OK);
   });
@@ -1130,12 +1061,10 @@ int gs_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_str
     if (taken) return int(GS_OK);
     const Side<T> ms{static_cast<const T*>(grad_y), grad_stride, rows, outputs};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
-    const Product p{rows, features, outputs, ceil_div(outputs, 64) * 64,
-                    ceil_div(features, kEdge)};
+    const Product p{rows, features, outputs, ceil_div(features, kEdge)};
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
-    product_kernel<T, true, false, Side<T>>
-        <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            ms, ns, p, static_cast<const T*>(nullptr), static_cast<T*>(grad_x), nullptr);
+    product_kernel<T, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        ms, ns, p, static_cast<const T*>(nullptr), static_cast<T*>(grad_x));
     GS_LAUNCHED("linear backward input");
     return int(GS_OK);
   });

@@ -463,6 +463,53 @@ def test_linear_shapes_and_no_bias(dtype):
 
 @gpu_test
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs", [
+    (140, 1100, 40), (140, 40, 1100), (130, 1030, 1030), (6, 24, 4200), (6, 4200, 24),
+    (3, 1500, 130), (33, 512, 512), (4000, 512, 130), (2000, 130, 512), (3000, 70, 130)])
+def test_linear_wide(dtype, rows, features, outputs):
+    """Matrices with a side longer than the streaming kernel takes, panels of
+    every width, and tiles of dW of every shape."""
+    linear_case((rows, features), outputs, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_of_many_rows(dtype):
+    """Rows enough for the widest tiles of dW (2e10 and 1e10 products), against
+    the sum over parts of the rows, whose bound the parts' sizes give."""
+    m = layers()
+    rows, features, outputs = (310_000, 260, 260) if dtype == torch.bfloat16 else (
+        160_000, 260, 260)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, features, generator=gen, device="cuda").to(dtype)
+    g = torch.randn(rows, outputs, generator=gen, device="cuda").to(dtype)
+    w = torch.randn(outputs, features, generator=gen, device="cuda").to(dtype)
+    b = torch.zeros(outputs, device="cuda", dtype=dtype)
+    inputs = [t.requires_grad_() for t in (x, w, b)]
+    dw, db = torch.autograd.grad(m.linear(*inputs), inputs[1:], g)
+    held = m.dequantize(m.quantize(x.detach())).double()
+    near(dw, (g.double().t() @ held).cpu(),
+         ((rows + 2) * E * (g.double().abs().t() @ held.abs())).cpu(), dtype)
+    near(db, g.double().sum(0).cpu(), ((rows + 2) * E * g.double().abs().sum(0)).cpu(), dtype)
+
+
+@gpu_test
+def test_linear_gradients_asked_for_one_by_one():
+    m = layers()
+    x, w, b, g = (normal(*s, seed=i).cuda() for i, s in enumerate(((70, 48), (24, 48), (24,),
+                                                                   (70, 24))))
+    inputs = [t.clone().requires_grad_() for t in (x, w, b)]
+    every = torch.autograd.grad(m.linear(*inputs), inputs, g)
+    for i in range(3):
+        some = [t.clone().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+        (one,) = torch.autograd.grad(m.linear(*some), some[i], g)
+        assert torch.equal(one, every[i])
+        (one,) = torch.autograd.grad(m.linear(*inputs), inputs[i], g)
+        assert torch.equal(one, every[i])
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_of_whole_numbers_is_exact(dtype):
     """Small whole numbers: every product and sum is exact in float32, the
     kept rows are the rows, so all outputs equal the formula's, in any order
@@ -553,7 +600,7 @@ def test_activation_gradient_against_differences(kind):
     assert (dx.cpu().double() - want).abs().max() <= 1e-4 * 30 * g.abs().max()
 
 
-def every_operator(dtype=torch.bfloat16, rows=300, features=72):
+def every_operator(dtype=torch.bfloat16, rows=300, features=512):
     """Calls that give all outputs and gradients of each operator."""
     m = layers()
     x, g = normal(rows, features, seed=1, dtype=dtype), normal(rows, features, seed=2, dtype=dtype)
