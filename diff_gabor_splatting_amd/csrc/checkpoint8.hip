@@ -6,9 +6,13 @@
 //     gelu  f = z Phi(z)          f' = Phi(z) + z phi(z)
 //     silu  f = z s, s = 1 / (1 + exp(-z))   f' = s (1 + z (1 - s))
 //
-// All four kernels read and write each byte once; a lane takes eight
-// features (16 bytes of a 2-byte type), so four lanes hold a group and its
-// largest magnitude takes two quad permutations, no memory.
+// Each kernel reads and writes each byte once, and memory bounds it: a lane
+// takes eight features (16 bytes of a 2-byte type), so four lanes hold a group
+// and its largest magnitude takes two quad permutations, no LDS; a thread has
+// four such chunks on their way. 1M x 512 bfloat16: written in 284 us (5.5
+// TB/s), read back in 251 (6.2), gelu forward in 468 (5.5) and backward in 489
+// (5.3; there the vector units are busy for 88% of the time, with 25
+// instructions a value, most of them erf's).
 #include "kept8.hpp"
 #include "layers_api.hpp"
 
@@ -38,8 +42,6 @@ __device__ __forceinline__ Place place(const Rows& r, int64_t first, uint32_t lo
   return {row0 + down, rest - down * r.per_row};
 }
 
-// What a launch does with each chunk: Op::apply(in, out, ...) is inlined
-// into one loop over the thread's chunks.
 enum Kind { kSine = GS_ACTIVATION_SINE, kGelu = GS_ACTIVATION_GELU, kSilu = GS_ACTIVATION_SILU };
 
 // sin and cos of 2 pi r for r = z (high + low), high + low = omega / 2 pi:
@@ -224,8 +226,8 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
   }
 }
 
-// Chunks from which a thread takes four of them; below, one each fills more
-// of the chip.
+// Chunks from which a thread takes four of them: one a thread for 1,024
+// workgroups. Below that, one each fills more of the chip.
 constexpr int64_t kFour = int64_t(4) * 256 * kBlock;
 
 template <typename F>

@@ -164,10 +164,12 @@ struct Product {
   int64_t tiles_n;
 };
 
-// C[m][n] = sum_k M(m, k) N(n, k) (+ bias[n]), one 128 x 128 tile to a
-// workgroup: a step of both sides is in registers while the step before is
+// C[m][n] = sum_k M(m, k) N(n, k) (+ bias[n]), for matrices with a side too
+// long to stay in LDS (over 1,024 values, or over 32 panels wide): one
+// 128 x 128 tile to a workgroup; a step of both sides is in registers while the step before is
 // multiplied out of LDS. M is the rows, k contiguous; N the matrix, [n][k] in
-// memory (NContiguous) or [k][n].
+// memory (NContiguous) or [k][n]. 50k x 2048 -> 2048 bfloat16: 616 us (680
+// TFLOP/s).
 template <typename T, bool NContiguous>
 __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, Side<T> ns, Product p,
                                                            const T* __restrict__ bias,
@@ -244,6 +246,13 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, Side<T> n
 // address unit a cycle a lane (it was busy for 83% of the kernel). Rows are
 // therefore loaded and results stored with eight lanes to 128 bytes of a row,
 // and turned through 2 KB of LDS that the wave has to itself.
+//
+// 1M x 512 -> 512 bfloat16 (524 Gflop, 2.0 GB): y 580 us, with the 8-bit form
+// 735, dx 560 (930 TFLOP/s; a library product of these sizes takes 770 and
+// 711). The matrix cores are then busy for half of the time, the address unit
+// for 65%, LDS for 54%: eight waves, as many as the registers allow, do not
+// fill any of them. 100k x 256 -> 256: 23.5, 31 and 22.5 us (4.4 TB/s). float32
+// is bound by its matrix instructions: 1M x 256 -> 256 1010 us (130 TFLOP/s).
 
 // Contiguous values of k in a lane's fragment, and in a step.
 template <typename T>
@@ -536,6 +545,12 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
 // each is multiplied by x8, which is exact in bfloat16: three products at
 // the bfloat16 rate, a fifth of the time of float32's, and none of them
 // rounded (an infinity or a NaN is the first part alone).
+//
+// 1M rows, 512 -> 512 bfloat16: 595 us (880 TFLOP/s; a library product of
+// these sizes takes 2166), 100k, 256 -> 256: 29 and 9 for the partial sums.
+// With the widest tiles the matrix cores are busy for 43% of the time, the
+// vector units, which expand x8, for 28%, LDS for 32%: a step's barrier and
+// the way from LDS to its first product take the rest.
 
 // What the matrix instructions multiply.
 template <typename T>
