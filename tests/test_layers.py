@@ -494,6 +494,26 @@ def test_linear_of_many_rows(dtype):
 
 
 @gpu_test
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_linear_of_many_rows_of_whole_numbers(dtype):
+    """The widest tiles of dW (they take dW's of 250 x 250 and these rows), odd
+    shares of the rows: small whole numbers, whose sums float32 holds exactly;
+    dW itself stays within what the type holds exactly."""
+    m = layers()
+    rows = 330_001 if dtype != torch.float32 else 170_001
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randint(-2, 3, (rows, 250), generator=gen, device="cuda").to(dtype)
+    g = torch.zeros(rows, 250, device="cuda", dtype=dtype)
+    at = torch.randint(0, rows, (20_000,), generator=gen, device="cuda")
+    g[at, torch.arange(20_000, device="cuda") % 250] = 1
+    w = torch.zeros(250, 250, device="cuda", dtype=dtype).requires_grad_()
+    (dw,) = torch.autograd.grad(m.linear(x, w), w, g)
+    want = (g.double().t() @ x.double())
+    assert want.abs().max() <= 256  # exact in bfloat16's eight bits, too
+    assert torch.equal(dw.double(), want)
+
+
+@gpu_test
 def test_linear_gradients_asked_for_one_by_one():
     m = layers()
     x, w, b, g = (normal(*s, seed=i).cuda() for i, s in enumerate(((70, 48), (24, 48), (24,),
