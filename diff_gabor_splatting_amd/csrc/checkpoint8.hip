@@ -121,7 +121,7 @@ constexpr int kNone = -1;
 
 // Writes the checkpoint of x (where values is not null) and, with an
 // activation, y.
-template <typename T, int K, bool Flat, int Each>
+template <typename T, int K, bool Flat, bool Narrow, int Each>
 __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, Rows r,
                                                       T* __restrict__ y,
                                                       uint8_t* __restrict__ values,
@@ -143,8 +143,8 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
       at[i] = place(r, first, local);
       const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
       valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
-      raw[i] = load_valid<T, kChunk>(x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk,
-                                     valid[i]);
+      raw[i] = load_edge<T, kChunk, Narrow>(
+          x + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i]);
     }
   }
 #pragma unroll
@@ -152,6 +152,7 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
     const uint32_t local = i * kBlock + threadIdx.x;
     if (first + local >= total) break;
     const int64_t chunk = first + local;  // rows of the checkpoint follow each other
+    if constexpr (!Flat) raw[i] = settle<T, kChunk, Narrow>(raw[i], valid[i]);
     float v[kChunk];
     widen<T, kChunk>(raw[i], v);
     if (values) {
@@ -174,14 +175,14 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(const T* __restrict__ x, R
 }
 
 // Reads a checkpoint back, or applies an activation's derivative at it to dy.
-template <typename T, int K, bool Flat, int Each>
+template <typename T, int K, bool Flat, bool Narrow, int Each>
 __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict__ values,
                                                       const uint8_t* __restrict__ exponents,
                                                       const T* __restrict__ dy, Rows r,
                                                       T* __restrict__ out, Parameters c) {
   const int64_t total = r.rows * r.per_row;
   const int64_t first = int64_t(blockIdx.x) * (kBlock * Each);
-  float g[Each][kChunk];
+  vec<T, kChunk> g[Each];
   uint2 bytes[Each];
   uint32_t exponent[Each];
   Place at[Each];
@@ -199,14 +200,14 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
     }
     if constexpr (Flat) {
       valid[i] = live ? kChunk : 0;
-      if constexpr (K != kNone) load8<T>(dy + chunk * kChunk, valid[i], g[i]);
+      if constexpr (K != kNone) g[i] = load_valid<T, kChunk>(dy + chunk * kChunk, valid[i]);
     } else {
       at[i] = place(r, first, local);
       const int64_t left = r.features - int64_t(at[i].chunk) * kChunk;
       valid[i] = live ? int(left < 0 ? 0 : left < kChunk ? left : kChunk) : 0;
       if constexpr (K != kNone)
-        load8<T>(dy + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i],
-                        g[i]);
+        g[i] = load_edge<T, kChunk, Narrow>(
+            dy + at[i].row * r.stride + int64_t(at[i].chunk) * kChunk, valid[i]);
     }
   }
 #pragma unroll
@@ -215,8 +216,9 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
     float v[kChunk];
     read8(bytes[i], exponent[i], v);
     if constexpr (K != kNone) {
+      if constexpr (!Flat) g[i] = settle<T, kChunk, Narrow>(g[i], valid[i]);
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) v[j] = g[i][j] * slope<T, K>(v[j], c);
+      for (int j = 0; j < kChunk; ++j) v[j] = float(g[i][j]) * slope<T, K>(v[j], c);
     }
     if constexpr (Flat)
       store8<T>(out + (first + i * kBlock + threadIdx.x) * kChunk, kChunk, v);
@@ -240,11 +242,15 @@ int with_layout(const char* name, const Rows& r, bool flat, F&& launch) {
   using one = std::integral_constant<int, 1>;
   using all = std::integral_constant<int, 4>;
   const dim3 grid{unsigned(blocks)};
+  auto by_count = [&](auto flat_, auto narrow) {
+    four ? launch(grid, flat_, narrow, all{}) : launch(grid, flat_, narrow, one{});
+  };
   if (flat)
-    four ? launch(grid, bool_constant<true>{}, all{}) : launch(grid, bool_constant<true>{}, one{});
+    by_count(bool_constant<true>{}, bool_constant<false>{});
+  else if (r.features >= kChunk)
+    by_count(bool_constant<false>{}, bool_constant<false>{});
   else
-    four ? launch(grid, bool_constant<false>{}, all{})
-         : launch(grid, bool_constant<false>{}, one{});
+    by_count(bool_constant<false>{}, bool_constant<true>{});
   GS_LAUNCHED(name);
   return GS_OK;
 }
@@ -273,8 +279,8 @@ int keep_rows(const char* name, const void* x, int64_t rows, int64_t features, i
               void* y, void* values, void* exponents, float omega, hipStream_t s) {
   const Rows r = rows_of(rows, features, stride);
   const bool flat = (stride == features || rows == 1) && features % kGroup == 0;
-  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto each) {
-    keep_kernel<T, K, f.value, each.value><<<grid, kBlock, 0, s>>>(
+  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
+    keep_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
         static_cast<const T*>(x), r, static_cast<T*>(y), static_cast<uint8_t*>(values),
         static_cast<uint8_t*>(exponents), parameters(omega));
   });
@@ -286,8 +292,8 @@ int read_rows(const char* name, const void* values, const void* exponents, const
               hipStream_t s) {
   const Rows r = rows_of(rows, features, stride);
   const bool flat = features % kGroup == 0 && (K == kNone || stride == features || rows == 1);
-  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto each) {
-    read_kernel<T, K, f.value, each.value><<<grid, kBlock, 0, s>>>(
+  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
+    read_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
         static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),
         static_cast<const T*>(dy), r, static_cast<T*>(out), parameters(omega));
   });

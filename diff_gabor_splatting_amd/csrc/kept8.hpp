@@ -108,6 +108,54 @@ __device__ __forceinline__ vec<T, N> load_valid(const T* p, int valid) {
   return vec<T, N>(T(0));
 }
 
+// The same without waiting for memory: the last, partly filled piece of a
+// row is loaded N - valid values earlier, where it is whole and inside the
+// row, and `settle` moves it down once it is there. (load_part puts its pieces
+// together at once, so a load ahead of its use would not be one.) Rows of
+// fewer than N values (Narrow) have no such place and take load_valid.
+template <typename T, int N, bool Narrow>
+__device__ __forceinline__ vec<T, N> load_edge(const T* p, int valid) {
+  if constexpr (Narrow) {
+    return load_valid<T, N>(p, valid);
+  } else {
+    vec<T, N> v = T(0);
+    if (valid > 0) v = load_packed<T, N>(p - (N - valid));
+    return v;
+  }
+}
+
+template <typename T, int N, bool Narrow>
+__device__ __forceinline__ vec<T, N> settle(vec<T, N> v, int valid) {
+  if constexpr (Narrow) {
+    return v;
+  } else {
+    if (valid >= N) return v;
+    constexpr int words = N * sizeof(T) / 4;
+    vec<uint32_t, words> w = __builtin_bit_cast(vec<uint32_t, words>, v);
+    // Down by `words_down` words, 4, 2 and 1 at a time, then by half a word.
+    const int missing = N - valid, words_down = missing * int(sizeof(T)) / 4;
+#pragma unroll
+    for (int step = 4; step; step >>= 1) {
+      if (step >= words) continue;
+      const bool move = words_down & step;
+#pragma unroll
+      for (int j = 0; j < words; ++j) {
+        const uint32_t from = j + step < words ? w[j + step < words ? j + step : 0] : 0u;
+        w[j] = move ? from : w[j];
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+      const bool move = missing & 1;
+#pragma unroll
+      for (int j = 0; j < words; ++j) {
+        const uint32_t next = j + 1 < words ? w[j + 1 < words ? j + 1 : 0] : 0u;
+        w[j] = move ? __builtin_amdgcn_alignbit(next, w[j], 16) : w[j];
+      }
+    }
+    return __builtin_bit_cast(vec<T, N>, w);
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_valid(T* p, int valid, vec<T, N> v) {
   if (valid >= N) {

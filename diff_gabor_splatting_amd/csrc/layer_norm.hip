@@ -198,7 +198,7 @@ __device__ __forceinline__ int valid_of(int column, int features) {
   return left < 0 ? 0 : left < kChunk ? left : kChunk;
 }
 
-template <typename T, typename W, int Chunks, int Waves, int Lanes>
+template <typename T, typename W, int Chunks, int Waves, int Lanes, bool Narrow>
 __global__ __launch_bounds__(
     kThreads<Waves>, (workgroups_of<Chunks, Waves>(kForward) * kSimdWaves<Waves>)) void layer_norm_forward_kernel(
     const T* __restrict__ x, int64_t stride, const W* __restrict__ weight,
@@ -212,6 +212,7 @@ __global__ __launch_bounds__(
   __shared__ Meet<Waves> meet;
   const int groups = (features + kGroup - 1) / kGroup;
   const float inverse_count = 1.f / float(features);
+  const bool ragged = features % kChunk;
   float w[Chunks][kChunk], b[Chunks][kChunk];
   int valid[Chunks];
 #pragma unroll
@@ -231,8 +232,8 @@ __global__ __launch_bounds__(
   auto send = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
-      raw[i] = load_valid<T, kChunk>(x + row * stride + column_of<Lanes, Waves>(i, lane),
-                                     row < rows ? valid[i] : 0);
+      raw[i] = load_edge<T, kChunk, Narrow>(
+          x + row * stride + column_of<Lanes, Waves>(i, lane), row < rows ? valid[i] : 0);
   };
   send(int64_t(blockIdx.x) * per_block + slot);
   // The trip count is the workgroup's: waves of a row meet at barriers.
@@ -243,7 +244,10 @@ __global__ __launch_bounds__(
     float v[Chunks][kChunk];
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < Chunks; ++i) widen<T, kChunk>(raw[i], v[i]);
+    for (int i = 0; i < Chunks; ++i) {
+      if (ragged) raw[i] = settle<T, kChunk, Narrow>(raw[i], valid[i]);
+      widen<T, kChunk>(raw[i], v[i]);
+    }
     send(row + int64_t(gridDim.x) * per_block);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
@@ -325,7 +329,7 @@ __global__ __launch_bounds__(
 }
 
 // Partial sums: [gridDim.x][2][features] float32, dw then db.
-template <typename T, typename W, int Chunks, int Waves, int Lanes, bool Kept>
+template <typename T, typename W, int Chunks, int Waves, int Lanes, bool Narrow, bool Kept>
 __global__ __launch_bounds__(
     kThreads<Waves>,
     (workgroups_of<Chunks, Waves>(kBackward) * kSimdWaves<Waves>)) void layer_norm_backward_kernel(
@@ -341,6 +345,7 @@ __global__ __launch_bounds__(
   __shared__ Meet<Waves> meet;
   const int groups = (features + kGroup - 1) / kGroup;
   const float inverse_count = 1.f / float(features);
+  const bool ragged = features % kChunk;
   float w[Chunks][kChunk], dw[Chunks][kChunk], db[Chunks][kChunk];
   int valid[Chunks];
 #pragma unroll
@@ -366,7 +371,8 @@ __global__ __launch_bounds__(
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
       const int column = column_of<Lanes, Waves>(i, lane);
-      g_next[i] = load_valid<T, kChunk>(dy + row * dy_stride + column, live ? valid[i] : 0);
+      g_next[i] =
+          load_edge<T, kChunk, Narrow>(dy + row * dy_stride + column, live ? valid[i] : 0);
       if (Kept) {
         kept_next[i] = make_uint2(0, 0);
         exponent_next[i] = 0;
@@ -376,7 +382,8 @@ __global__ __launch_bounds__(
           exponent_next[i] = exponents[row * groups + column / kGroup];
         }
       } else {
-        x_next[i] = load_valid<T, kChunk>(x + row * x_stride + column, live ? valid[i] : 0);
+        x_next[i] =
+            load_edge<T, kChunk, Narrow>(x + row * x_stride + column, live ? valid[i] : 0);
       }
     }
   };
@@ -389,11 +396,14 @@ __global__ __launch_bounds__(
     float g[Chunks][kChunk], h[Chunks][kChunk];
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
+      if (ragged) g_next[i] = settle<T, kChunk, Narrow>(g_next[i], valid[i]);
       widen<T, kChunk>(g_next[i], g[i]);
-      if (Kept)
+      if (Kept) {
         read8(kept_next[i], exponent_next[i], h[i]);
-      else
+      } else {
+        if (ragged) x_next[i] = settle<T, kChunk, Narrow>(x_next[i], valid[i]);
         widen<T, kChunk>(x_next[i], h[i]);
+      }
     }
     send(row + int64_t(gridDim.x) * per_block);
     float sum = 0.f, product = 0.f;
@@ -502,7 +512,8 @@ __global__ __launch_bounds__(kColumns* kSlices) void layer_norm_parameters_kerne
 // Rows wider than this are refused.
 constexpr int64_t kMostNormFeatures = 16384;
 
-// Chunks of a lane, waves of a row and lanes of a wave for a width. A group
+// Chunks of a lane, waves of a row and lanes of a wave for a width, and whether
+// it is less than a chunk. A group
 // of the checkpoint takes four lanes, so a row takes as many at least.
 template <typename F>
 void with_shape(int64_t features, F&& launch) {
@@ -511,26 +522,29 @@ void with_shape(int64_t features, F&& launch) {
   using two = integral_constant<int, 2>;
   using four = integral_constant<int, 4>;
   using all = integral_constant<int, 64>;
-  if (features <= 32)
-    launch(one{}, one{}, four{});
+  using wide = std::false_type;
+  if (features < kChunk)
+    launch(one{}, one{}, four{}, std::true_type{});
+  else if (features <= 32)
+    launch(one{}, one{}, four{}, wide{});
   else if (features <= 64)
-    launch(one{}, one{}, integral_constant<int, 8>{});
+    launch(one{}, one{}, integral_constant<int, 8>{}, wide{});
   else if (features <= 128)
-    launch(one{}, one{}, integral_constant<int, 16>{});
+    launch(one{}, one{}, integral_constant<int, 16>{}, wide{});
   else if (features <= 256)
-    launch(one{}, one{}, integral_constant<int, 32>{});
+    launch(one{}, one{}, integral_constant<int, 32>{}, wide{});
   else if (features <= 512)
-    launch(one{}, one{}, all{});
+    launch(one{}, one{}, all{}, wide{});
   else if (features <= 1024)
-    launch(two{}, one{}, all{});
+    launch(two{}, one{}, all{}, wide{});
   else if (features <= 2048)
-    launch(four{}, one{}, all{});
+    launch(four{}, one{}, all{}, wide{});
   else if (features <= 4096)
-    launch(two{}, four{}, all{});
+    launch(two{}, four{}, all{}, wide{});
   else if (features <= 8192)
-    launch(four{}, four{}, all{});
+    launch(four{}, four{}, all{}, wide{});
   else
-    launch(two{}, integral_constant<int, 16>{}, all{});
+    launch(two{}, integral_constant<int, 16>{}, all{}, wide{});
 }
 
 // Workgroups: as many as the chip holds, each taking several rows after one
@@ -538,7 +552,7 @@ void with_shape(int64_t features, F&& launch) {
 // all of them; fewer where there are not the rows.
 int64_t blocks_of(int64_t rows, int64_t features, Pass pass) {
   int64_t blocks = 0;
-  with_shape(features, [&](auto chunks, auto waves, auto lanes) {
+  with_shape(features, [&](auto chunks, auto waves, auto lanes, auto) {
     const int64_t per_block = waves.value == 1 ? kThreads<1> / lanes.value : 1;
     const int64_t most = kUnits * workgroups_of<chunks.value, waves.value>(pass);
     blocks = std::min(ceil_div(rows, per_block), most);
@@ -585,8 +599,8 @@ int gs_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const void* x, in
     using T = decltype(t);
     using W = decltype(u);
     const dim3 grid{unsigned(blocks_of(rows, features, values ? kForwardKept : kForward))};
-    with_shape(features, [&](auto chunks, auto waves, auto lanes) {
-      layer_norm_forward_kernel<T, W, chunks.value, waves.value, lanes.value>
+    with_shape(features, [&](auto chunks, auto waves, auto lanes, auto narrow) {
+      layer_norm_forward_kernel<T, W, chunks.value, waves.value, lanes.value, narrow.value>
           <<<grid, kThreads<waves.value>, 0, s>>>(
               static_cast<const T*>(x), row_stride, static_cast<const W*>(weight),
               static_cast<const W*>(bias), eps, rows, int(features),
@@ -630,10 +644,11 @@ int gs_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const void* grad
     using W = decltype(u);
     const int64_t blocks = rows > 0 ? blocks_of(rows, features, kBackward) : 0;
     if (rows > 0) {
-      with_shape(features, [&](auto chunks, auto waves, auto lanes) {
+      with_shape(features, [&](auto chunks, auto waves, auto lanes, auto narrow) {
         const size_t shared = waves.value == 1 ? 2 * size_t(features) * sizeof(float) : 0;
         auto launch = [&](auto kept) {
-          layer_norm_backward_kernel<T, W, chunks.value, waves.value, lanes.value, kept.value>
+          layer_norm_backward_kernel<T, W, chunks.value, waves.value, lanes.value, narrow.value,
+                                     kept.value>
               <<<dim3{unsigned(blocks)}, kThreads<waves.value>, shared, s>>>(
                   static_cast<const T*>(grad_y), grad_stride, static_cast<const T*>(x),
                   row_stride, static_cast<const uint8_t*>(values),

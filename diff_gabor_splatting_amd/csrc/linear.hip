@@ -452,7 +452,8 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
     } else {
       const int left = min(p.k - sent_step * step - piece * part, part);
 #pragma unroll
-      for (int j = 0; j < loads; ++j) to[j] = load_valid<T, part>(at_step + from[j], left);
+      for (int j = 0; j < loads; ++j)
+        to[j] = load_edge<T, part, false>(at_step + from[j], left);
     }
     if (++sent_step == p.steps) {
       sent_step = 0;
@@ -473,6 +474,11 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
 #pragma unroll
       for (int u = 0; u < Ahead; ++u) {
         const int s = s0 + u;
+        if (Tail && (s + 1) * step > p.k) {
+          const int left = min(p.k - s * step - piece * part, part);
+#pragma unroll
+          for (int j = 0; j < loads; ++j) ring[u][j] = settle<T, part, false>(ring[u][j], left);
+        }
         Part b[TM][2];
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -616,7 +622,7 @@ __device__ __forceinline__ vec<F, 8> turned_fragment(const F* lds, int pitch, in
 }
 
 // A wave's tile: 16 A outputs x 16 B features.
-template <typename T, int A, int B, int Rows>
+template <typename T, int A, int B, int Rows, bool Narrow>
 __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ dy,
                                                           const uint8_t* __restrict__ values,
                                                           const uint8_t* __restrict__ exponents,
@@ -653,6 +659,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
   const int row_m = threadIdx.x / across_m, column_m = threadIdx.x % across_m * 8;
   const int row_n = threadIdx.x / across_n, column_n = threadIdx.x % across_n * 16;
   const int valid_m = min(p.outputs - m0 - column_m, 8);
+  const bool ragged = p.outputs % 8;
   const bool has_n = (all_n || row_n < Rows) && n0 + column_n < groups * kGroup;
   const T* from_m = dy + (k0 + row_m) * p.stride + m0 + column_m;
   const uint8_t* from_n = values + (k0 + row_n) * (int64_t(groups) * kGroup) + n0 + column_n;
@@ -669,8 +676,8 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
 #pragma unroll
     for (int i = 0; i < loads_m; ++i) {
       constexpr int apart = kSumThreads / across_m;
-      to.m[i] = load_valid<T, 8>(from_m + i * apart * p.stride,
-                                 sent + row_m + i * apart < k1 ? valid_m : 0);
+      to.m[i] = load_edge<T, 8, Narrow>(from_m + i * apart * p.stride,
+                                        sent + row_m + i * apart < k1 ? valid_m : 0);
     }
     to.n = vec<uint32_t, 4>{0, 0, 0, 0};
     to.exponent = 0;
@@ -685,9 +692,10 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
   };
   float sum[8] = {};
   const bool sums = n0 == 0;
-  auto put = [&](const Load& from, F* to) {
+  auto put = [&](Load& from, F* to) {
 #pragma unroll
     for (int i = 0; i < loads_m; ++i) {
+      if (ragged) from.m[i] = settle<T, 8, Narrow>(from.m[i], valid_m);
       vec<F, 8> cut[parts];
       parts_of<T>(from.m[i], cut);
       if (sums) {
@@ -890,15 +898,15 @@ int panel_fragments(size_t size, int64_t rows, int64_t k, int64_t n) {
   return fragments;
 }
 
-// C = x matrix through rows_kernel; false where the matrix or the stride is
-// too large for it.
+// C = x matrix through rows_kernel; `taken` is false where the matrix or the
+// stride is too large for it, or k less than a lane's part of a fragment.
 template <typename T, bool Transposed>
 int launch_rows(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
                 int64_t rows, int64_t k, int64_t n, void* out, void* values, void* exponents,
                 hipStream_t stream, bool& taken) {
   const int fragments = panel_fragments(sizeof(T), rows, k, n);
   const int64_t panels = fragments ? ceil_div(n, 16 * fragments) : 0;
-  taken = fragments && panels <= 32 && stride < (1 << 24);
+  taken = fragments && panels <= 32 && stride < (1 << 24) && k >= kPart<T>;
   if (!taken) return GS_OK;
   using std::integral_constant;
   auto launch = [&](auto tm, auto tn, auto ahead, auto keep, auto tail) {
@@ -1130,12 +1138,12 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
                          int(plan.tiles_n), int(splits), plan.share};
       const int64_t blocks = ceil_div(splits, 8) * 8 * plan.tiles_m * plan.tiles_n;
       GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "linear backward weight: too large");
-      auto launch = [&](auto a, auto b) {
+      auto launch = [&](auto a, auto b, auto narrow) {
         constexpr int step = a.value == 2 ? 64 : 32;
         constexpr int pitches = kParts<T> * (32 * a.value + 16) + 64 * b.value + 16;
         const size_t lds = std::max<size_t>(2 * size_t(step) * pitches * 2,
                                             size_t(kSumThreads) * 8 * sizeof(float));
-        auto* const kernel = &sum_kernel<T, a.value, b.value, step>;
+        auto* const kernel = &sum_kernel<T, a.value, b.value, step, narrow.value>;
         GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
         kernel<<<dim3{unsigned(blocks)}, kSumThreads, lds, s>>>(
             static_cast<const T*>(grad_y), static_cast<const uint8_t*>(values),
@@ -1148,14 +1156,18 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
       using two = integral_constant<int, 2>;
       using four = integral_constant<int, 4>;
       const int shape = plan.a * 10 + plan.b;
-      if (shape == 21) GS_CHECK(launch(two{}, one{}));
-      if (shape == 22) GS_CHECK(launch(two{}, two{}));
-      if (shape == 41) GS_CHECK(launch(four{}, one{}));
-      if (shape == 42) GS_CHECK(launch(four{}, two{}));
+      using wide = std::false_type;
+      using narrow = std::true_type;
+      if (shape == 21 && outputs < 8) GS_CHECK(launch(two{}, one{}, narrow{}));
+      if (shape == 22 && outputs < 8) GS_CHECK(launch(two{}, two{}, narrow{}));
+      if (shape == 21 && outputs >= 8) GS_CHECK(launch(two{}, one{}, wide{}));
+      if (shape == 22 && outputs >= 8) GS_CHECK(launch(two{}, two{}, wide{}));
+      if (shape == 41) GS_CHECK(launch(four{}, one{}, wide{}));
+      if (shape == 42) GS_CHECK(launch(four{}, two{}, wide{}));
       if constexpr (sizeof(T) == 2) {
-        if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}));
+        if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}, wide{}));
       } else {
-        if (shape == 44) GS_CHECK(launch(four{}, four{}));
+        if (shape == 44) GS_CHECK(launch(four{}, four{}, wide{}));
       }
     }
     const int64_t weights = outputs * features, size = weights + outputs;
