@@ -44,15 +44,19 @@ __device__ __forceinline__ Place place(const Rows& r, int64_t first, uint32_t lo
 
 enum Kind { kSine = GS_ACTIVATION_SINE, kGelu = GS_ACTIVATION_GELU, kSilu = GS_ACTIVATION_SILU };
 
-// sin and cos of 2 pi r for r = z (high + low), high + low = omega / 2 pi:
-// the product's fraction is taken with fused multiply-adds, so the phase
-// has no rounding error of its size. |f| <= 1/2 revolution.
+// The fraction f of z (high + low) revolutions, high + low = omega / 2 pi, for
+// sin and cos of 2 pi f: the product's fraction is taken with fused
+// multiply-adds, so the phase has no rounding error of its size. From 2^24
+// revolutions on the rounded product is a whole number further than 1/2 from
+// the product, so what is left is brought to |f| <= 1/2 once more (f is off by
+// 2^-48 of the revolutions at most; a product past float32's range gives NaN).
 __device__ __forceinline__ float turn(float z, float high, float low) {
   const float k = rintf(z * high);
-  return __builtin_fmaf(z, low, __builtin_fmaf(z, high, -k));
+  const float f = __builtin_fmaf(z, low, __builtin_fmaf(z, high, -k));
+  return f - rintf(f);
 }
 
-// sin(2 pi f), |f| <= 1/2 and a rounding error more: reflected at 1/4, then
+// sin(2 pi f), |f| <= 1/2: reflected at 1/4, then
 // the Taylor polynomial of sin to the 13th degree on [-pi/2, pi/2], whose
 // first omitted term is below 7e-10.
 __device__ __forceinline__ float sine_of_turn(float f) {

@@ -298,6 +298,30 @@ def test_sine_of_large_phases():
     assert (y - torch.sin(30 * x.double())).abs().max() < 1e-6
 
 
+@gpu_test
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sine_of_phases_past_whole_floats(dtype):
+    """Past 2^24 revolutions the rounded product with omega / 2 pi is whole,
+    and what it lacks is more than half a revolution. The fraction is off by
+    at most 2^-48 of the revolutions (omega / 2 pi as two floats: 2^-49; the
+    sum of the two small products, at most 2^-24 of the revolutions: 2^-49);
+    twice that is allowed. A sine stays a sine, whatever its phase."""
+    m = layers()
+    for size in (1e5, 1e7, 1e9, 1e12, 1e20, 1e30):
+        x = (normal(32, 64, seed=14) * size).to(dtype)
+        on = x.cuda().requires_grad_()
+        y = m.activation(on, "sine", 30.0)
+        (dx,) = torch.autograd.grad(y, on, torch.ones_like(y))
+        y, dx = y.detach().cpu().double(), dx.cpu().double()
+        assert y.abs().max() <= 1 + 1e-6 and dx.abs().max() <= 30 * (1 + 1e-6)
+        turns = 30 * x.double().abs() / (2 * math.pi)
+        error = 2 * math.pi * turns * 2.0 ** -47
+        near(y.to(dtype), oracle.activation(x, "sine", 30.0), error + 16 * E, dtype)
+        z = oracle.kept(x)[2]
+        near(dx.to(dtype), oracle.slope(z, "sine", 30.0),
+             30 * (2 * math.pi * 30 * z.abs() / (2 * math.pi) * 2.0 ** -47 + 16 * E), dtype)
+
+
 # --------------------------------------------------------------------------
 # GPU: layer norm
 
