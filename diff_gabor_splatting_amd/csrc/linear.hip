@@ -800,7 +800,10 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
 // Adds `count` partial results of `size` values; the first `weights` of them
 // are dW, the others db. A workgroup takes kThreads / Slices values; each
 // slice of its threads adds every Slices-th result, and the slices meet in
-// LDS, in their order.
+// LDS, in their order. With one slice a workgroup goes on to further values:
+// the grid stays at kJoinBlocks, far below the 2^32 threads of a launch.
+constexpr int64_t kJoinBlocks = 1 << 20;
+
 template <typename T, int Slices>
 __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict__ partial,
                                                         int count, int64_t size, int64_t weights,
@@ -808,23 +811,29 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict_
   constexpr int columns = kThreads / Slices;
   __shared__ float sums[Slices][columns];
   const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
-  const int64_t i = int64_t(blockIdx.x) * columns + column;
-  float sum = 0.f;
-  if (i < size) {
+  auto add = [&](int64_t i) {
+    float sum = 0.f;
 #pragma unroll 8
     for (int s = slice; s < count; s += Slices) sum += partial[s * size + i];
-  }
-  if constexpr (Slices > 1) {
+    return sum;
+  };
+  auto put = [&](int64_t i, float sum) {
+    if (i < weights) {
+      if (dw) dw[i] = T(sum);
+    } else if (db) {
+      db[i - weights] = T(sum);
+    }
+  };
+  int64_t i = int64_t(blockIdx.x) * columns + column;
+  if constexpr (Slices == 1) {
+    for (; i < size; i += int64_t(gridDim.x) * columns) put(i, add(i));
+  } else {
+    float sum = i < size ? add(i) : 0.f;
     sums[slice][column] = sum;
     __syncthreads();
-    if (slice) return;
+    if (slice || i >= size) return;
     for (int s = 1; s < Slices; ++s) sum += sums[s][column];
-  }
-  if (i >= size) return;
-  if (i < weights) {
-    if (dw) dw[i] = T(sum);
-  } else if (db) {
-    db[i - weights] = T(sum);
+    put(i, sum);
   }
 }
 
@@ -1174,7 +1183,8 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
     // Enough workgroups to fill the chip with few values, too.
     auto join = [&](auto slices) {
       join_kernel<T, slices.value>
-          <<<dim3{unsigned(ceil_div(size, kThreads / slices.value))}, kThreads, 0, s>>>(
+          <<<dim3{unsigned(std::min(ceil_div(size, kThreads / slices.value), kJoinBlocks))},
+             kThreads, 0, s>>>(
               static_cast<const float*>(workspace), int(splits), size, weights,
               static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
     };

@@ -538,6 +538,26 @@ def test_linear_of_many_rows_of_whole_numbers(dtype):
 
 
 @gpu_test
+def test_linear_of_a_matrix_larger_than_the_joining_grid():
+    """More than 2^20 x 256 weights: the workgroups that join dW's partial
+    sums take several stretches of it. Whole numbers: exact."""
+    m = layers()
+    rows, features, outputs = 9, 16384, 20001
+    gen = generator(67)
+    x = torch.randint(-9, 10, (rows, features), generator=gen).to(torch.bfloat16)
+    g = torch.randint(-2, 3, (rows, outputs), generator=gen).to(torch.bfloat16)
+    w = torch.zeros(outputs, features, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    b = torch.zeros(outputs, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    dw, db = torch.autograd.grad(m.linear(x.cuda(), w, b), (w, b), g.cuda())
+    assert torch.equal(db.cpu().float(), g.float().sum(0))
+    x, g = x.cuda().float(), g.cuda().float()
+    for first in range(0, outputs, 4096):
+        part = g[:, first:first + 4096]
+        want = sum(part[r, :, None] * x[r, None, :] for r in range(rows))
+        assert torch.equal(dw[first:first + 4096].float(), want), first
+
+
+@gpu_test
 def test_linear_gradients_asked_for_one_by_one():
     m = layers()
     x, w, b, g = (normal(*s, seed=i).cuda() for i, s in enumerate(((70, 48), (24, 48), (24,),
