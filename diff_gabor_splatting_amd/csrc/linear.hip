@@ -553,7 +553,7 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
 // rounded (an infinity or a NaN is the first part alone).
 //
 // 1M rows, 512 -> 512 bfloat16: 595 us (880 TFLOP/s; a library product of
-// these sizes takes 2166), 100k, 256 -> 256: 29 and 9 for the partial sums.
+// these sizes takes 2166), 100k, 256 -> 256: 29 and 6 for the partial sums.
 // With the widest tiles the matrix cores are busy for 43% of the time, the
 // vector units, which expand x8, for 28%, LDS for 32%: a step's barrier and
 // the way from LDS to its first product take the rest.
@@ -1180,7 +1180,9 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
       }
     }
     const int64_t weights = outputs * features, size = weights + outputs;
-    // Enough workgroups to fill the chip with few values, too.
+    // Enough workgroups to fill the chip with few values, too: 65,792 values of
+    // 128 partial results take 9.2 us with one slice and 6.2 with four, 147,840
+    // 7.1 and 7.2.
     auto join = [&](auto slices) {
       join_kernel<T, slices.value>
           <<<dim3{unsigned(std::min(ceil_div(size, kThreads / slices.value), kJoinBlocks))},
@@ -1188,8 +1190,10 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
               static_cast<const float*>(workspace), int(splits), size, weights,
               static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
     };
-    if (size >= 256 * kThreads)
+    if (size >= 512 * kThreads)
       join(std::integral_constant<int, 1>{});
+    else if (size >= 256 * kThreads)
+      join(std::integral_constant<int, 4>{});
     else
       join(std::integral_constant<int, 16>{});
     GS_LAUNCHED("join_kernel");
