@@ -5,6 +5,8 @@
 // Rows may have any stride as long as their features are contiguous and the
 // leading dimensions collapse into one; other inputs are copied first.
 
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -144,6 +146,22 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
   return grads;
 }
 
+// The kernels write into tensors that torch sees as empty, so what follows
+// its operators and not these calls would get that for a result: a tracer
+// (torch.jit.trace; make_fx and torch.export, whose mode is PROXY or the
+// pre-dispatch key) would record the allocation alone, and forward mode would
+// find no tangent. Both are refused, in the backward pass too.
+void check_calls(const char* name, std::initializer_list<const at::Tensor*> inputs) {
+  using c10::impl::TorchDispatchModeTLS;
+  if (at::tracer::impl::is_dispatch_enabled() ||
+      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+      TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    fail(std::string(name) + " cannot be traced");
+  for (const at::Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      fail(std::string(name) + " has no forward-mode derivative");
+}
+
 bool grad_wanted(std::initializer_list<const at::Tensor*> inputs) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : inputs)
@@ -155,6 +173,7 @@ bool grad_wanted(std::initializer_list<const at::Tensor*> inputs) {
 // Checkpoints
 
 std::vector<at::Tensor> checkpoint8_write(const at::Tensor& x) {
+  check_calls("quantize", {&x});
   check_input(x);
   const c10::DeviceGuard guard(x.device());
   const RowsOf r(x);
@@ -167,6 +186,7 @@ std::vector<at::Tensor> checkpoint8_write(const at::Tensor& x) {
 
 at::Tensor checkpoint8_read(const at::Tensor& values, const at::Tensor& exponents,
                             std::vector<int64_t> shape, at::ScalarType type) {
+  check_calls("dequantize", {});
   if (shape.empty() || shape.back() < 1) throw py::value_error("invalid checkpoint shape");
   const int64_t features = shape.back(), groups = (features + kGroup - 1) / kGroup;
   int64_t rows = 1;
@@ -215,6 +235,7 @@ struct Activation : torch::autograd::Function<Activation> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    check_calls("activation", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const c10::DeviceGuard guard(grads[0].device());
     const RowsOf g(grads[0]);
@@ -228,6 +249,7 @@ struct Activation : torch::autograd::Function<Activation> {
 };
 
 at::Tensor activation(const at::Tensor& x, int64_t kind, double omega) {
+  check_calls("activation", {&x});
   check_input(x);
   if (!grad_wanted({&x})) return activation_rows(x, kind, omega, nullptr);
   return Activation::apply(x, kind, omega);
@@ -274,6 +296,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    check_calls("layer_norm", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const bool has_weight = ctx->saved_data["weight"].toBool();
     const bool has_bias = ctx->saved_data["bias"].toBool();
@@ -309,8 +332,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 at::Tensor layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& weight,
                       const std::optional<at::Tensor>& bias, double eps, bool eight) {
-  check_input(x);
   const at::Tensor w = weight.value_or(at::Tensor()), b = bias.value_or(at::Tensor());
+  check_calls("layer_norm", {&x, &w, &b});
+  check_input(x);
   check_parameter("weight", w, {x.size(-1)}, x, true);
   check_parameter("bias", b, {x.size(-1)}, x, true);
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
@@ -352,6 +376,7 @@ struct Linear : torch::autograd::Function<Linear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    check_calls("linear", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const bool has_bias = ctx->saved_data["bias"].toBool();
     const at::Tensor& grad = grads[0];
@@ -383,10 +408,11 @@ struct Linear : torch::autograd::Function<Linear> {
 
 at::Tensor linear(const at::Tensor& x, const at::Tensor& weight,
                   const std::optional<at::Tensor>& bias) {
+  const at::Tensor b = bias.value_or(at::Tensor());
+  check_calls("linear", {&x, &weight, &b});
   check_input(x);
   if (weight.dim() != 2 || weight.size(0) < 1)
     throw py::value_error("weight must have shape (outputs, features)");
-  const at::Tensor b = bias.value_or(at::Tensor());
   check_parameter("weight", weight, {weight.size(0), x.size(-1)}, x, false);
   check_parameter("bias", b, {weight.size(0)}, x, false);
   if (!grad_wanted({&x, &weight, &b})) return linear_rows(x, weight, b, nullptr);

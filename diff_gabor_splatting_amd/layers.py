@@ -3,7 +3,7 @@ values that the renderers take.
 
 ``layer_norm``, ``linear`` and ``activation`` work on rows of features (any
 leading dimensions) in float32, bfloat16 or float16 on a HIP device, with
-first-order autograd. Over a scene's surfels it is the activations kept for
+first-order reverse-mode autograd (forward mode and tracing are refused). Over a scene's surfels it is the activations kept for
 the backward pass that fill memory, so these keep them in 8 bits: 33/32 bytes
 a value instead of two or four.
 

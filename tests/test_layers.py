@@ -162,6 +162,64 @@ def test_python_functions_refuse_cpu_tensors_and_bad_options():
         m.layer_norm(x, eps=-1.0)
 
 
+def layer_calls(device="cpu"):
+    """Each operator as a function of the rows alone, by name."""
+    m = layers()
+    w, b = torch.ones(8, device=device), torch.zeros(8, device=device)
+    big, four = torch.ones(4, 8, device=device), torch.zeros(4, device=device)
+    return {"activation": lambda t: m.activation(t),
+            "layer_norm": lambda t: m.layer_norm(t, w, b),
+            "linear": lambda t: m.linear(t, big, four)}
+
+
+def refuses_what_would_lose_a_result(calls, x):
+    """Forward mode and the tracers follow torch's operators, not these
+    calls: without a refusal a tangent is lost and a replayed trace returns
+    memory that nothing has written."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for name, call in calls.items():
+        for t in (x, x.clone().requires_grad_()):
+            for trace in (lambda: torch.jit.trace(call, (t,)), lambda: make_fx(call)(t),
+                          lambda: make_fx(call, pre_dispatch=True)(t),
+                          lambda: make_fx(call, tracing_mode="fake")(t)):
+                with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+                    trace()
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match=f"{name} has no forward-mode derivative"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode"):
+                call(dual)
+
+
+def test_forward_mode_and_tracing_are_refused():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    m = layers()
+    x = torch.zeros(2, 8)
+    refuses_what_would_lose_a_result(layer_calls(), x)
+    with forward_ad.dual_level():
+        w = forward_ad.make_dual(torch.ones(8), torch.ones(8))
+        big = forward_ad.make_dual(torch.ones(4, 8), torch.ones(4, 8))
+        for call in (lambda: m.layer_norm(x, w), lambda: m.layer_norm(x, None, w),
+                     lambda: m.linear(x, big), lambda: m.linear(x, torch.ones(8, 8), w)):
+            with pytest.raises(RuntimeError, match="no forward-mode"):
+                call()
+    kept = m.Checkpoint(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8),
+                        x.shape, x.dtype)
+    for name, trace in (("quantize", lambda: make_fx(lambda t: m.quantize(t).values)(x)),
+                        ("dequantize", lambda: torch.jit.trace(
+                            lambda t: t + m.dequantize(kept), (x,)))):
+        with pytest.raises(RuntimeError, match=f"^{name} cannot be traced"):
+            trace()
+    # Outside of them the refusal leaves no trace.
+    with pytest.raises(ValueError, match="on a HIP device"):
+        m.activation(x)
+
+
 # --------------------------------------------------------------------------
 # GPU: the 8-bit form
 
@@ -812,6 +870,38 @@ def test_second_derivatives_are_refused():
         (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiable once"):
             dx.sum().backward()
+
+
+@gpu_test
+def test_forward_mode_and_tracing_are_refused_on_the_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = normal(2, 8, seed=1).cuda()
+    calls = layer_calls("cuda")
+    refuses_what_would_lose_a_result(calls, x)
+    for name, call in calls.items():
+        on = x.clone().requires_grad_()
+        y = call(on)
+        g = torch.ones_like(y)
+
+        def back(t):
+            return torch.autograd.grad(y, on, t, retain_graph=True)[0]
+
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            make_fx(back)(g)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode"):
+            back(forward_ad.make_dual(g, torch.ones_like(g)))
+        for transform in (torch.func.vmap, torch.func.functionalize,
+                          lambda f: lambda t: torch.func.jvp(f, (t,), (t,))):
+            with pytest.raises(RuntimeError):
+                transform(call)(x)
+        with pytest.raises(RuntimeError), FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            call(mode.from_tensor(x))
+        # None of it stays behind.
+        assert torch.equal(call(x), y.detach())
+        assert torch.isfinite(back(g)).all()
 
 
 @gpu_test
