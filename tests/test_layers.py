@@ -326,6 +326,58 @@ def test_activation(dtype, kind, shape):
     assert torch.equal(m.activation(x.cuda(), kind), y.detach())
 
 
+def float32_activation(kind, x):
+    """(value, its 64-bit value, slope, its 64-bit value) of float32 rows; the
+    slope is that at the kept rows."""
+    m = layers()
+    on = x.cuda().requires_grad_()
+    y = m.activation(on, kind)
+    (dx,) = torch.autograd.grad(y, on, torch.ones_like(y))
+    z = oracle.kept(x)[2]
+    return (y.detach().cpu().double(), oracle.activation(x, kind, 30.0), dx.cpu().double(),
+            oracle.slope(z, kind, 30.0))
+
+
+def relative_rms(got, want):
+    return ((got - want).norm() / want.norm()).item()
+
+
+@gpu_test
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_float32_gelu_is_as_exact_as_its_type(scale):
+    """A rounding is off by half a unit, 2^-24, at most, with an rms of a
+    root of three less: rms relative error of three roundings (the
+    function's, Phi's, its polynomial's). The negative tail, where the value
+    is the product of z, a polynomial and the bell: by value, the units of
+    2^-24 of its operations (exp2 2, reciprocal and its argument 3, the
+    polynomial's last steps 2, the bell's correction 1, three products 3) and
+    one for the rest."""
+    y, value, dx, slope = float32_activation("gelu", normal(512, 256, seed=15, scale=scale))
+    assert relative_rms(y, value) <= E
+    assert relative_rms(dx, slope) <= E
+    x = -2 - 4 * torch.rand(64, 256, generator=generator(16))
+    y, value, _, _ = float32_activation("gelu", x)
+    assert ((y - value).abs() <= 12 * E * value.abs()).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_keeps_its_tail_in_two_bytes(dtype):
+    """Phi(-|z|) to 1.2e-5 of itself (the fit), the bell's argument (up to 26,
+    rounded twice) 2.2e-6, a dozen float32 roundings below 1e-6: 2e-5 in all,
+    and then the one rounding to the type."""
+    m = layers()
+    x = (-2 - 4 * torch.rand(64, 256, generator=generator(17))).to(dtype)
+    on = x.cuda().requires_grad_()
+    y = m.activation(on, "gelu")
+    (dx,) = torch.autograd.grad(y, on, torch.ones_like(y))
+    value = oracle.activation(x, "gelu", 0.0)
+    near(y, value, 2e-5 * value.abs(), dtype)
+    z = oracle.kept(x)[2]
+    near(dx, oracle.slope(z, "gelu", 0.0),
+         2e-5 * torch.special.ndtr(z) + 4e-6 * z.abs() * torch.exp(-z * z / 2) * 0.4, dtype)
+
+
 @gpu_test
 def test_activation_of_special_values():
     m = layers()
