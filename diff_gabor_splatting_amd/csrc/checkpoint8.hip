@@ -47,8 +47,9 @@ enum Kind { kSine = GS_ACTIVATION_SINE, kGelu = GS_ACTIVATION_GELU, kSilu = GS_A
 // Whether a type shows errors of 2^-24: float32's functions are evaluated to
 // its own rounding, which costs no time beside four bytes a value (gelu of
 // 500k x 512: 425 and 420 us, 423 and 426 with the shorter form). The 2-byte
-// types' rounding is 2^13 and 2^16 times as large, and the longer form takes
-// 569 and 574 us of 1M x 512 bfloat16 where theirs takes 461 and 450.
+// types' rounding is 2^13 and 2^16 times as large, and the longer forms take
+// time there: gelu of 1M x 512 bfloat16 569 and 574 us against 461 and 450,
+// the sine's slope 513 against 456.
 template <typename T>
 constexpr bool kFine = sizeof(T) == 4;
 
@@ -64,10 +65,9 @@ __device__ __forceinline__ float turn(float z, float high, float low) {
   return f - rintf(f);
 }
 
-// sin(2 pi f), |f| <= 1/4: the Taylor polynomial of sin to the 13th degree on
-// [-pi/2, pi/2], whose first omitted term is below 7e-10.
-__device__ __forceinline__ float sine_of_quarter(float f) {
-  const float r = f * 6.283185307179586f;
+// sin r, |r| <= pi/2: the Taylor polynomial of sin to the 13th degree, whose
+// first omitted term is below 7e-10.
+__device__ __forceinline__ float sine_of_angle(float r) {
   const float s = r * r;
   float p = 1.6059043836821613e-10f;
   p = __builtin_fmaf(p, s, -2.5052108385441720e-8f);
@@ -78,10 +78,58 @@ __device__ __forceinline__ float sine_of_quarter(float f) {
   return __builtin_fmaf(p * s, r, r);
 }
 
+// sin(2 pi f), |f| <= 1/4.
+__device__ __forceinline__ float sine_of_quarter(float f) {
+  return sine_of_angle(f * 6.283185307179586f);
+}
+
 // sin(2 pi f), |f| <= 1/2: reflected at 1/4.
 __device__ __forceinline__ float sine_of_turn(float f) {
   const float a = fabsf(f);
   return sine_of_quarter(copysignf(fminf(a, 0.5f - a), f));
+}
+
+// float32's fraction in two parts, whose sum it is to 2^-48 of the
+// revolutions: the product less the nearest whole number is exact, and so is
+// its rounding error (of the rounded product: contracted, it would count
+// twice). What passes 1/2 (from 2^24 revolutions on) comes off the second part.
+struct Turn {
+  float high, low;
+};
+
+__device__ __forceinline__ Turn fine_turn(float z, float high, float low) {
+#pragma clang fp contract(off)
+  const float p = z * high;
+  const float rest = __builtin_fmaf(z, low, __builtin_fmaf(z, high, -p));
+  return {p - rintf(p), rest - rintf(rest)};
+}
+
+// sin(2 pi (high + low)), the sum within 1/4: 2 pi too has two parts, so that
+// the angle is rounded once.
+__device__ __forceinline__ float sine_of_parts(float high, float low) {
+  constexpr float two_pi = 6.283185307179586f;
+  constexpr float rest = float(6.283185307179586 - double(two_pi));
+  return sine_of_angle(
+      __builtin_fmaf(high, two_pi, __builtin_fmaf(high, rest, low * two_pi)));
+}
+
+// sin(2 pi f) from the nearest half revolution n / 2 on, with n's sign.
+__device__ __forceinline__ float fine_sine(Turn f) {
+  constexpr float magic = 12582912.f;  // 1.5 2^23: the sum's low bit is n's
+  const float n = __builtin_fmaf(2.f, f.high + f.low, magic);
+  const float r = sine_of_parts(__builtin_fmaf(n - magic, -0.5f, f.high), f.low);
+  return __uint_as_float(__float_as_uint(r) ^ (__float_as_uint(n) << 31));
+}
+
+// cos(2 pi f) = sin(2 pi (1/4 - |f|)), |f| = high + low once both have the
+// sign that makes it so, and 1/4 - high with its rounding error.
+__device__ __forceinline__ float fine_cosine(Turn f) {
+  float high = f.high - rintf(f.high + f.low), low = f.low;
+  const bool negative = high + low < 0.f;
+  high = negative ? -high : high;
+  low = negative ? -low : low;
+  const float rest = 0.25f - high;
+  return sine_of_parts(rest, ((0.25f - rest) - high) - low);
 }
 
 struct Parameters {
@@ -152,7 +200,9 @@ __device__ __forceinline__ Normal normal(float z) {
 
 template <typename T, int K>
 __device__ __forceinline__ float value(float z, const Parameters& c) {
-  if constexpr (K == kSine) {
+  if constexpr (K == kSine && kFine<T>) {
+    return fine_sine(fine_turn(z, c.high, c.low));
+  } else if constexpr (K == kSine) {
     return sine_of_turn(turn(z, c.high, c.low));
   } else if constexpr (K == kGelu && kFine<T>) {
     const Normal n = normal(z);
@@ -168,7 +218,9 @@ __device__ __forceinline__ float value(float z, const Parameters& c) {
 
 template <typename T, int K>
 __device__ __forceinline__ float slope(float z, const Parameters& c) {
-  if constexpr (K == kSine) {
+  if constexpr (K == kSine && kFine<T>) {
+    return c.omega * fine_cosine(fine_turn(z, c.high, c.low));
+  } else if constexpr (K == kSine) {
     const float f = turn(z, c.high, c.low);
     // cos(2 pi f) = sin(2 pi (1/4 - |f|))
     return c.omega * sine_of_quarter(0.25f - fabsf(f));

@@ -343,6 +343,17 @@ def relative_rms(got, want):
 
 
 @gpu_test
+@pytest.mark.parametrize("scale", [1 / 30, 1.0, 30.0])
+def test_float32_sine_is_as_exact_as_its_type(scale):
+    """Two roundings, the phase's and the function's, at phases of 1, 30 and
+    900: an rms of 2^-24 times the root of two thirds of the largest value a
+    rounding error is half a unit of."""
+    y, value, dx, slope = float32_activation("sine", normal(512, 256, seed=18, scale=scale))
+    assert relative_rms(y, value) <= E * (2 / 3) ** 0.5
+    assert relative_rms(dx, slope) <= E * (2 / 3) ** 0.5
+
+
+@gpu_test
 @pytest.mark.parametrize("scale", [1.0, 4.0])
 def test_float32_gelu_is_as_exact_as_its_type(scale):
     """A rounding is off by half a unit, 2^-24, at most, with an rms of a
