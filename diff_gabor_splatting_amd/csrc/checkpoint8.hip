@@ -198,6 +198,26 @@ __device__ __forceinline__ Normal normal(float z) {
   return n;
 }
 
+// 1 / (1 + exp(-z)). float32: the exponent as h + l, l the rounding errors of
+// -z log2(e), z cut where the result is 0 or 1.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z, float& denominator) {
+  constexpr float rate = -1.4426950408889634f;
+  float e;
+  if constexpr (kFine<T>) {
+    constexpr float rest = float(-1.4426950408889634 - double(rate));
+    const float x = __builtin_amdgcn_fmed3f(z, -130.f, 130.f);
+    const float h = x * rate;
+    const float l = __builtin_fmaf(x, rest, __builtin_fmaf(x, rate, -h));
+    const float whole = __builtin_amdgcn_exp2f(h);
+    e = __builtin_fmaf(whole, l * 0.69314718055994531f, whole);
+  } else {
+    e = __builtin_amdgcn_exp2f(z * rate);
+  }
+  denominator = 1.f + e;
+  return __builtin_amdgcn_rcpf(denominator);
+}
+
 template <typename T, int K>
 __device__ __forceinline__ float value(float z, const Parameters& c) {
   if constexpr (K == kSine && kFine<T>) {
@@ -212,7 +232,11 @@ __device__ __forceinline__ float value(float z, const Parameters& c) {
     normal_cdf(z, cdf, bell);
     return z * cdf;
   } else {
-    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    float d;
+    const float s = sigmoid<T>(z, d), y = z * s;
+    if constexpr (!kFine<T>) return y;
+    // The quotient z / d to its rounding, where d is no infinity.
+    return fabsf(z) < 88.f ? __builtin_fmaf(__builtin_fmaf(-d, y, z), s, y) : y;
   }
 }
 
@@ -234,8 +258,8 @@ __device__ __forceinline__ float slope(float z, const Parameters& c) {
     normal_cdf(z, cdf, bell);
     return __builtin_fmaf(z * bell, 0.39894228040143268f, cdf);
   } else {
-    const float s =
-        __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    float d;
+    const float s = sigmoid<T>(z, d);
     return s * __builtin_fmaf(z, 1.f - s, 1.f);
   }
 }

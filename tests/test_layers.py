@@ -372,6 +372,19 @@ def test_float32_gelu_is_as_exact_as_its_type(scale):
 
 
 @gpu_test
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_float32_silu_is_as_exact_as_its_type(scale):
+    """rms as for the sine: two roundings (the sum 1 + exp and the quotient).
+    Where the exponential is all of the sum, by value, in units of 2^-24:
+    exp2 2, its correction 1, the sum 1, the quotient 2."""
+    y, value, _, _ = float32_activation("silu", normal(512, 256, seed=19, scale=scale))
+    assert relative_rms(y, value) <= E * (2 / 3) ** 0.5
+    x = -2 - 60 * torch.rand(64, 256, generator=generator(20))
+    y, value, _, _ = float32_activation("silu", x)
+    assert ((y - value).abs() <= 6 * E * value.abs()).all()
+
+
+@gpu_test
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_gelu_keeps_its_tail_in_two_bytes(dtype):
     """Phi(-|z|) to 1.2e-5 of itself (the fit), the bell's argument (up to 26,
