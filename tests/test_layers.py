@@ -530,6 +530,31 @@ def test_layer_norm_without_parameters_and_with_a_large_mean(eight):
 
 
 @gpu_test
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("features", [5, 57, 187, 500, 1000, 4099, 16384])
+def test_layer_norm_of_constant_rows(features, eight):
+    """A row of one value is its own mean to the last bit, whatever the value:
+    the output is the bias, h and with it dw are zero. Rows whose spread is a
+    few units of the mean's last place: the mean is off by half a unit and
+    what the n differences' sum loses, n 2^-24 of their size."""
+    m = layers()
+    at = torch.tensor([4097.3, 1000.1, -33333.3, 0.1, 1e-20, 1e20, 0.0])
+    x = at[:, None].expand(-1, features).contiguous()
+    w, b, g = normal(features, seed=61), normal(features, seed=62), normal(7, features, seed=63)
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = m.layer_norm(*inputs, checkpoint="8bit" if eight else "full")
+    dx, dw, db = torch.autograd.grad(y, inputs, g.cuda())
+    assert torch.equal(y.detach().cpu(), b.expand(7, -1))
+    assert torch.equal(dw.cpu(), torch.zeros(features))
+    unit = 2.0 ** -11  # of 4097.3
+    x = 4097.3 + unit * torch.randint(-8, 9, (40, features), generator=generator(64))
+    eps = 1.0  # the differences stay below it: r is 1 to 2^-14
+    y = m.layer_norm(x.cuda(), eps=eps).cpu().double()
+    want = oracle.layer_norm(x, eps=eps)[0]
+    assert ((y - want).abs() <= unit * (0.5 + 16 * features * E) + 2 * E).all()
+
+
+@gpu_test
 def test_layer_norm_of_one_parameter():
     m = layers()
     x, w = normal(9, 48, seed=1).cuda(), normal(48, seed=2).cuda()
