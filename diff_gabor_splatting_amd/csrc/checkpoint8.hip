@@ -379,12 +379,24 @@ __global__ __launch_bounds__(kBlock) void read_kernel(const uint8_t* __restrict_
 // workgroups. Below that, one each fills more of the chip.
 constexpr int64_t kFour = int64_t(4) * 256 * kBlock;
 
+// Chunks of a launch at most: a launch takes less than 2^32 threads, here a
+// quarter of them, and more rows take several launches.
+constexpr int64_t kMostChunks = int64_t(4) << 30;
+
+// Calls `part(first row, rows)` for each launch's rows.
+template <typename F>
+int in_parts(int64_t rows, int64_t features, F&& part) {
+  const int64_t most = kMostChunks / (kept_groups(features) * (kGroup / kChunk));
+  for (int64_t first = 0; first < rows; first += most)
+    GS_CHECK(part(first, std::min(rows - first, most)));
+  return GS_OK;
+}
+
 template <typename F>
 int with_layout(const char* name, const Rows& r, bool flat, F&& launch) {
   const int64_t total = r.rows * r.per_row;
   const bool four = total >= kFour;
   const int64_t blocks = ceil_div(total, four ? 4 * kBlock : kBlock);
-  GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "%s: too many rows", name);
   using std::bool_constant;
   using one = std::integral_constant<int, 1>;
   using all = std::integral_constant<int, 4>;
@@ -424,12 +436,18 @@ Rows rows_of(int64_t rows, int64_t features, int64_t stride) {
 template <typename T, int K>
 int keep_rows(const char* name, const void* x, int64_t rows, int64_t features, int64_t stride,
               void* y, void* values, void* exponents, float omega, hipStream_t s) {
-  const Rows r = rows_of(rows, features, stride);
   const bool flat = (stride == features || rows == 1) && features % kGroup == 0;
-  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
-    keep_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
-        static_cast<const T*>(x), r, static_cast<T*>(y), static_cast<uint8_t*>(values),
-        static_cast<uint8_t*>(exponents), parameters(omega));
+  return in_parts(rows, features, [&](int64_t first, int64_t count) {
+    const Rows r = rows_of(count, features, stride);
+    const int64_t groups = kept_groups(features);
+    const T* const from = static_cast<const T*>(x) + first * stride;
+    T* const to = y ? static_cast<T*>(y) + first * features : nullptr;
+    uint8_t* const v = values ? static_cast<uint8_t*>(values) + first * groups * kGroup : nullptr;
+    uint8_t* const e = exponents ? static_cast<uint8_t*>(exponents) + first * groups : nullptr;
+    return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
+      keep_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
+          from, r, to, v, e, parameters(omega));
+    });
   });
 }
 
@@ -437,12 +455,18 @@ template <typename T, int K>
 int read_rows(const char* name, const void* values, const void* exponents, const void* dy,
               int64_t rows, int64_t features, int64_t stride, void* out, float omega,
               hipStream_t s) {
-  const Rows r = rows_of(rows, features, stride);
   const bool flat = features % kGroup == 0 && (K == kNone || stride == features || rows == 1);
-  return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
-    read_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
-        static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents),
-        static_cast<const T*>(dy), r, static_cast<T*>(out), parameters(omega));
+  return in_parts(rows, features, [&](int64_t first, int64_t count) {
+    const Rows r = rows_of(count, features, stride);
+    const int64_t groups = kept_groups(features);
+    const uint8_t* const v = static_cast<const uint8_t*>(values) + first * groups * kGroup;
+    const uint8_t* const e = static_cast<const uint8_t*>(exponents) + first * groups;
+    const T* const g = dy ? static_cast<const T*>(dy) + first * stride : nullptr;
+    T* const to = static_cast<T*>(out) + first * features;
+    return with_layout(name, r, flat, [&](dim3 grid, auto f, auto narrow, auto each) {
+      read_kernel<T, K, f.value, narrow.value, each.value><<<grid, kBlock, 0, s>>>(
+          v, e, g, r, to, parameters(omega));
+    });
   });
 }
 

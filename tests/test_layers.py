@@ -1073,3 +1073,35 @@ def test_offsets_past_32_bits():
             # The same few terms, summed in another order: one unit in
             # bfloat16's last place.
             assert (dw1.float() - dw2.float()).abs().max() <= 2.0 ** -7 * dw2.float().abs().max()
+
+
+@gpu_test
+def test_more_rows_than_one_launch_takes():
+    """A row of one feature takes four chunks, a thread four chunks: 2^32 rows
+    would be 2^32 threads, more than a launch takes, and 2^30 rows are as many
+    as one is given. A pattern of odd length repeats over the rows, and so do
+    the results."""
+    m = layers()
+    torch.cuda.empty_cache()
+    period = 1_000_003
+    base = normal(period, seed=71, dtype=torch.bfloat16).cuda()[:, None]
+
+    def repeats(got, want, times):
+        assert torch.equal(got.reshape(times, -1), want.reshape(1, -1).expand(times, -1))
+
+    times = (1 << 32) // period + 2
+    repeats(m.activation(base.repeat(times, 1), "silu"), m.activation(base, "silu"), times)
+    torch.cuda.empty_cache()
+    times = (1 << 30) // period + 2
+    results = []
+    for x in (base, base.repeat(times, 1)):
+        on = x.requires_grad_()
+        y = m.activation(on, "silu")
+        (dx,) = torch.autograd.grad(y, on, x.detach())
+        kept = m.quantize(x)
+        results.append((y.detach(), dx, kept.values, kept.exponents, m.dequantize(kept)))
+        del on, y, dx, kept, x
+    for want, got in zip(*results):
+        repeats(got, want, times)
+    del results, got
+    torch.cuda.empty_cache()
