@@ -644,12 +644,15 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const T* __restrict__ 
   F* const lds = reinterpret_cast<F*>(shared);
 
   // Workgroups go to the eight XCDs in turn: the tiles of one share of the
-  // rows have one XCD, and its L2.
+  // rows have one XCD, and its L2. With fewer shares than XCDs the tiles go
+  // round, a workgroup each, so that their number is that of the launch.
   const int tiles = p.tiles_m * p.tiles_n;
   const int in_xcd = blockIdx.x >> 3;
-  const int split = in_xcd / tiles * 8 + (blockIdx.x & 7);
+  const bool shared_xcd = p.splits >= 8;
+  const int split = shared_xcd ? in_xcd / tiles * 8 + int(blockIdx.x & 7)
+                               : int(blockIdx.x % unsigned(p.splits));
   if (split >= p.splits) return;
-  const int tile = in_xcd % tiles;
+  const int tile = shared_xcd ? in_xcd % tiles : int(blockIdx.x / unsigned(p.splits));
   const int m0 = tile / p.tiles_n * tile_m, n0 = tile % p.tiles_n * tile_n;
   const int64_t k0 = split * p.share;
   const int64_t k1 = k0 + p.share < p.rows ? k0 + p.share : p.rows;
@@ -1035,8 +1038,12 @@ int check_linear(const char* name, int32_t dtype, int64_t rows, int64_t features
   GS_CHECK(check_rows(name, dtype, rows, outputs, outputs));
   GS_REQUIRE(outputs <= kMostFeatures / 64 && features <= kMostFeatures / 64, GS_ERR_ARGUMENT,
              "%s: at most %lld features and outputs", name, (long long)(kMostFeatures / 64));
-  GS_REQUIRE(ceil_div(rows, kEdge) * ceil_div(std::max(features, outputs), kEdge) <=
-                 0x7fffffffLL, GS_ERR_OVERFLOW, "%s: too many rows", name);
+  return GS_OK;
+}
+
+// A launch takes less than 2^32 threads.
+int check_launch(const char* name, int64_t blocks, int64_t threads) {
+  GS_REQUIRE(blocks < (int64_t(1) << 32) / threads, GS_ERR_OVERFLOW, "%s: too many rows", name);
   return GS_OK;
 }
 
@@ -1075,6 +1082,7 @@ int gs_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const vo
     const Side<T> ms{static_cast<const T*>(x), row_stride, rows, features};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
     const Product p{rows, outputs, features, ceil_div(outputs, kEdge)};
+    GS_CHECK(check_launch("gs_linear_forward", ceil_div(rows, kEdge) * p.tiles_n, kThreads));
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
     product_kernel<T, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
         ms, ns, p, static_cast<const T*>(bias), static_cast<T*>(y));
@@ -1103,6 +1111,8 @@ int gs_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_str
     const Side<T> ms{static_cast<const T*>(grad_y), grad_stride, rows, outputs};
     const Side<T> ns{static_cast<const T*>(weight), features, outputs, features};
     const Product p{rows, features, outputs, ceil_div(features, kEdge)};
+    GS_CHECK(
+        check_launch("gs_linear_backward_input", ceil_div(rows, kEdge) * p.tiles_n, kThreads));
     const dim3 grid{unsigned(ceil_div(rows, kEdge) * p.tiles_n)};
     product_kernel<T, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
         ms, ns, p, static_cast<const T*>(nullptr), static_cast<T*>(grad_x));
@@ -1145,8 +1155,9 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
       splits = plan.splits;
       const SumProduct p{rows, grad_stride, int(outputs), int(features), int(plan.tiles_m),
                          int(plan.tiles_n), int(splits), plan.share};
-      const int64_t blocks = ceil_div(splits, 8) * 8 * plan.tiles_m * plan.tiles_n;
-      GS_REQUIRE(blocks <= 0x7fffffffLL, GS_ERR_OVERFLOW, "linear backward weight: too large");
+      const int64_t blocks =
+          (splits >= 8 ? ceil_div(splits, 8) * 8 : splits) * plan.tiles_m * plan.tiles_n;
+      GS_CHECK(check_launch("gs_linear_backward_weight", blocks, kSumThreads));
       auto launch = [&](auto a, auto b, auto narrow) {
         constexpr int step = a.value == 2 ? 64 : 32;
         constexpr int pitches = kParts<T> * (32 * a.value + 16) + 64 * b.value + 16;

@@ -1105,3 +1105,23 @@ def test_more_rows_than_one_launch_takes():
         repeats(got, want, times)
     del results, got
     torch.cuda.empty_cache()
+
+
+@gpu_test
+def test_linear_of_as_many_tiles_as_a_launch_takes():
+    """2^34 weights are 2^20 tiles of dW; eight workgroups of 512 threads to
+    each would be 2^32 threads. Whole numbers: exact."""
+    m = layers()
+    torch.cuda.empty_cache()
+    rows, side = 9, 1 << 17
+    gen = torch.Generator(device="cuda").manual_seed(72)
+    x = torch.randint(-9, 10, (rows, side), generator=gen, device="cuda").to(torch.bfloat16)
+    g = torch.randint(-2, 3, (rows, side), generator=gen, device="cuda").to(torch.bfloat16)
+    w = torch.zeros(side, side, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    (dw,) = torch.autograd.grad(m.linear(x, w), w, g)
+    x, g = x.float(), g.float()
+    for first in range(0, side, 2048):
+        want = g[:, first:first + 2048].t() @ x
+        assert torch.equal(dw[first:first + 2048].float(), want), first
+    del w, dw, want
+    torch.cuda.empty_cache()
