@@ -697,6 +697,35 @@ def test_linear_of_many_rows_of_whole_numbers(dtype):
 
 
 @gpu_test
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,features,outputs", [
+    (90_001, 490, 500),   # several of the widest tiles of dW, ragged on both sides
+    (310_000, 260, 260),  # narrow ones, as the widest would be mostly empty
+    (20_001, 300, 900),   # as many shares of the rows as are no multiple of eight
+    (3_001, 2_060, 2_070)])  # fewer shares than eight
+def test_linear_of_many_dense_rows_of_whole_numbers(dtype, rows, features, outputs):
+    """Every row counts: sums of small whole numbers stay below 2^24, which
+    float32 holds exactly in any order, so each output is the exact sum,
+    rounded once to the type. (A bound of n 2^-24 of the terms' sum would let
+    a dW or db of zeros pass at these row counts.)"""
+    m = layers()
+    gen = torch.Generator(device="cuda").manual_seed(73)
+
+    def whole(low, high, *shape):
+        return torch.randint(low, high + 1, shape, generator=gen, device="cuda").to(dtype)
+
+    x, g = whole(-2, 2, rows, features), whole(-1, 2, rows, outputs)
+    w, b = whole(-1, 1, outputs, features), whole(-9, 9, outputs)
+    inputs = [t.requires_grad_() for t in (x, w, b)]
+    y = m.linear(*inputs)
+    got = (y.detach(), *torch.autograd.grad(y, inputs, g))
+    x, w, b, g = (t.detach().double() for t in (x, w, b, g))
+    want = (x @ w.t() + b, g @ w, g.t() @ x, g.sum(0))
+    for name, a, e in zip(("y", "dx", "dw", "db"), got, want):
+        assert e.abs().max() < 2 ** 24 and torch.equal(a, e.to(dtype)), name
+
+
+@gpu_test
 def test_linear_of_a_matrix_larger_than_the_joining_grid():
     """More than 2^20 x 256 weights: the workgroups that join dW's partial
     sums take several stretches of it. Whole numbers: exact."""
