@@ -85,15 +85,22 @@ void check_parameter(const char* name, const at::Tensor& t, c10::IntArrayRef sha
   }
 }
 
+// The values themselves where `t` is a view that negates them lazily (what
+// torch.imag gives of a conjugate): the kernels read memory as it is.
+at::Tensor in_memory(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+// A parameter as the kernels read it.
+at::Tensor dense(const at::Tensor& t) { return t.defined() ? in_memory(t).contiguous() : t; }
+
 // A tensor as rows of its last dimension.
 struct RowsOf {
   at::Tensor held;  // keeps a copy alive, where one was made
   int64_t rows, features, stride;
 
-  explicit RowsOf(const at::Tensor& t) : held(t) {
+  explicit RowsOf(const at::Tensor& t) : held(in_memory(t)) {
     features = t.size(-1);
     rows = t.numel() / features;
-    if (!collapses(t)) held = t.contiguous();
+    if (!collapses(held)) held = held.contiguous();
     const int64_t last = t.dim() - 2;
     stride = rows > 1 && held.dim() >= 2 ? row_stride(held, last) : features;
   }
@@ -262,8 +269,7 @@ at::Tensor norm_rows(const at::Tensor& x, const at::Tensor& weight, const at::Te
                      double eps, at::Tensor* statistics, Kept* kept) {
   const c10::DeviceGuard guard(x.device());
   const RowsOf r(x);
-  const at::Tensor w = weight.defined() ? weight.contiguous() : weight;
-  const at::Tensor b = bias.defined() ? bias.contiguous() : bias;
+  const at::Tensor w = dense(weight), b = dense(bias);
   const int32_t parameters =
       w.defined() ? type_of(w) : b.defined() ? type_of(b) : type_of(x);
   at::Tensor y = at::empty(x.sizes(), x.options());
@@ -311,7 +317,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       rows.emplace(x);
       stride = rows->stride;
     }
-    if (has_weight) w = saved[1].contiguous();
+    if (has_weight) w = dense(saved[1]);
     dx = at::empty(grad.sizes(), grad.options());
     if (has_weight && ctx->needs_input_grad(1))
       dw = at::empty({g.features}, on(grad.device(), type));
@@ -350,8 +356,7 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& weight, const at::
                        Kept* kept) {
   const c10::DeviceGuard guard(x.device());
   const RowsOf r(x);
-  const at::Tensor w = weight.contiguous();
-  const at::Tensor b = bias.defined() ? bias.contiguous() : bias;
+  const at::Tensor w = dense(weight), b = dense(bias);
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = w.size(0);
   at::Tensor y = at::empty(shape, x.options());
@@ -382,7 +387,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const at::Tensor& grad = grads[0];
     const c10::DeviceGuard guard(grad.device());
     const RowsOf g(grad);
-    const at::Tensor w = saved[0].contiguous();
+    const at::Tensor w = dense(saved[0]);
     const int64_t outputs = w.size(0), features = w.size(1);
     const int32_t type = type_of(grad);
     void* const stream = stream_of(grad.device());

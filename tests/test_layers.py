@@ -951,6 +951,34 @@ def test_strided_inputs_and_weights():
 
 
 @gpu_test
+def test_lazily_negated_views():
+    """A view whose values are the negatives of what its memory holds (the
+    imaginary part of a conjugate) is read as its values."""
+    m = layers()
+    x, g = normal(30, 64, seed=1).cuda(), normal(30, 64, seed=2).cuda()
+    w, b, big = (normal(*s, seed=3).cuda() for s in ((64,), (64,), (64, 64)))
+    pairs = [(torch.imag(torch.complex(t, t).conj()), -t) for t in (x[:, :1], x[0])]
+    pairs += [(torch._neg_view(t), -t) for t in (x, g, w, b, big)]
+    for lazy, plain in pairs:
+        assert lazy.is_neg() and torch.equal(lazy, plain)
+        a, e = m.quantize(lazy), m.quantize(plain)
+        assert torch.equal(a.values, e.values) and torch.equal(a.exponents, e.exponents)
+    _, (nx, px), (ng, pg), (nw, pw), (nb, pb), (nbig, pbig) = pairs[1:]
+    for call, lazy, plain in (
+            (m.activation, (nx,), (px,)),
+            (m.layer_norm, (nx, nw, nb), (px, pw, pb)),
+            (lambda *a: m.layer_norm(*a, checkpoint="8bit"), (nx, nw, nb), (px, pw, pb)),
+            (m.linear, (nx, nbig, nb), (px, pbig, pb))):
+        results = []
+        for inputs, grad in ((lazy, ng), (plain, pg)):
+            inputs = [t.detach().requires_grad_() for t in inputs]
+            y = call(*inputs)
+            results.append((y, *torch.autograd.grad(y, inputs, grad)))
+        for a, e in zip(*results):
+            assert torch.equal(a, e)
+
+
+@gpu_test
 def test_shared_and_broadcast_inputs():
     """An input used twice and a weight expanded from fewer values: autograd
     adds what the operators return."""
