@@ -3,9 +3,10 @@ values that the renderers take.
 
 ``layer_norm``, ``linear`` and ``activation`` work on rows of features (any
 leading dimensions) in float32, bfloat16 or float16 on a HIP device, with
-first-order reverse-mode autograd (forward mode and tracing are refused). Over a scene's surfels it is the activations kept for
-the backward pass that fill memory, so these keep them in 8 bits: 33/32 bytes
-a value instead of two or four.
+first-order reverse-mode autograd (forward mode and tracing are refused). Over
+a scene's surfels it is the activations kept for the backward pass that fill
+memory, so these keep them in 8 bits: 33/32 bytes a value instead of two or
+four.
 
 The 8-bit form (:class:`Checkpoint`, :func:`quantize`, :func:`dequantize`):
 each 32 consecutive features of a row share a power of two, the smallest with
@@ -65,6 +66,12 @@ def _tensor(name: str, value) -> Tensor:
     return value
 
 
+def _number(name: str, value) -> None:
+    # A learned one would be read here and never get its gradient.
+    if isinstance(value, Tensor) and value.requires_grad:
+        raise ValueError(f"{name} has no gradient: pass a number, or a detached tensor")
+
+
 def quantize(x: Tensor) -> Checkpoint:
     """``x`` in 8 bits, in groups of 32 features. Not differentiable."""
     values, exponents = _host.checkpoint8_write(_tensor("x", x))
@@ -86,6 +93,7 @@ def activation(x: Tensor, kind: str = "sine", omega: float = 30.0) -> Tensor:
     at the input as kept in 8 bits."""
     if kind not in ACTIVATIONS:
         raise ValueError(f"kind must be one of {', '.join(map(repr, ACTIVATIONS))}")
+    _number("omega", omega)
     if not math.isfinite(omega):
         raise ValueError("omega must be finite")
     return _host.activation(_tensor("x", x), ACTIVATIONS[kind], omega)
@@ -100,6 +108,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     kept in 8 bits ("8bit")."""
     if checkpoint not in _CHECKPOINTS:
         raise ValueError("checkpoint must be 'full' or '8bit'")
+    _number("eps", eps)
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
     return _host.layer_norm(_tensor("x", x), weight, bias, eps, _CHECKPOINTS[checkpoint])

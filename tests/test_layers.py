@@ -220,6 +220,18 @@ def test_forward_mode_and_tracing_are_refused():
         m.activation(x)
 
 
+def test_learned_numbers_are_refused():
+    """omega and eps have no gradient: one that asks for it would get none."""
+    m = layers()
+    x, learned = torch.zeros(2, 8), torch.tensor(30.0, requires_grad=True)
+    with pytest.raises(ValueError, match="omega has no gradient"):
+        m.activation(x, "sine", learned)
+    with pytest.raises(ValueError, match="eps has no gradient"):
+        m.layer_norm(x, eps=learned)
+    with pytest.raises(ValueError, match="on a HIP device"):
+        m.activation(x, "sine", learned.detach())
+
+
 # --------------------------------------------------------------------------
 # GPU: the 8-bit form
 
