@@ -258,29 +258,32 @@ __global__ __launch_bounds__(
     // correction.
     float mean = sum * inverse_count;
     mean = __builtin_fmaf(__builtin_fmaf(-mean, float(features), sum), inverse_count, mean);
+    // The differences from it, zero past the row.
+    float d[Chunks][kChunk];
+    auto differ = [&] {
+#pragma unroll
+      for (int i = 0; i < Chunks; ++i) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) d[i][j] = v[i][j] - mean;
+        if (valid[i] != kChunk) {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) d[i][j] = j < valid[i] ? d[i][j] : 0.f;
+        }
+      }
+    };
+    differ();
     float squares = 0.f;
 #pragma unroll
     for (int i = 0; i < Chunks; ++i)
-      if (valid[i] == kChunk) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const float d = v[i][j] - mean;
-          squares = __builtin_fmaf(d, d, squares);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const float d = j < valid[i] ? v[i][j] - mean : 0.f;
-          squares = __builtin_fmaf(d, d, squares);
-        }
-      }
+      for (int j = 0; j < kChunk; ++j) squares = __builtin_fmaf(d[i][j], d[i][j], squares);
     squares = sum1<Lanes, Waves>(squares, meet, turn);
     float inverse = rsqrtf(__builtin_fmaf(squares, inverse_count, eps));
     // The sum has lost units of its own last place. Where the mean is larger
     // than the deviation they show in h: the mean of the differences from it is
     // then added (a constant row's mean becomes its value) and its square taken
-    // off the variance. 1M x 512 bfloat16 rows with the 8-bit form: 490 us without
-    // the test, 511 with it, 524 where every row goes through. A row's result is
+    // off the variance. 1M x 512 bfloat16 rows with the 8-bit form: 499 us without
+    // the test, 509 with it, 524 where every row goes through. A row's result is
     // its own: rows that share a wave with such a one stay as they are.
     const bool far = mean * mean > squares * inverse_count;
     if (__any(far)) {
@@ -288,13 +291,13 @@ __global__ __launch_bounds__(
 #pragma unroll
       for (int i = 0; i < Chunks; ++i)
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j)
-          rest += j < valid[i] ? v[i][j] - mean : 0.f;
+        for (int j = 0; j < kChunk; ++j) rest += d[i][j];
       rest = sum1<Lanes, Waves>(rest, meet, turn) * inverse_count;
       const float variance = __builtin_fmaf(squares, inverse_count, -rest * rest);
       if (far) {
         mean += rest;
         inverse = rsqrtf((variance < 0.f ? 0.f : variance) + eps);
+        differ();
       }
     }
     float centre = 0.f;
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(
       float out[kChunk];
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
-        out[j] = __builtin_fmaf((v[i][j] - mean) * inverse, w[i][j], b[i][j]);
+        out[j] = __builtin_fmaf(d[i][j] * inverse, w[i][j], b[i][j]);
       store8<T>(y + row * features + column, live ? valid[i] : 0, out);
       if (values) {
         // The last group's lanes past the row keep zeros. (A NaN that fmaxf
