@@ -10,9 +10,10 @@ is loaded after ``import torch`` it binds to the runtime torch already loaded
 and shares torch's streams and allocations.
 
 The host functions (``csrc/host.cpp`` for the renderer, ``csrc/layers_host.cpp``
-for the decoder's layers) are a Python extension module, ``diff_gabor_splatting_amd/_host*.so``, compiled with the host C++
-compiler against the installed torch (:func:`build_host`); it calls the HIP
-library's C ABI through function addresses handed over at import.
+for the decoder's layers) are a Python extension module,
+``diff_gabor_splatting_amd/_host*.so``, compiled with the host C++ compiler
+against the installed torch (:func:`build_host`); it calls the HIP library's C
+ABI through function addresses handed over at import.
 
 Run ``python -m diff_gabor_splatting_amd.build`` or call :func:`build_library`
 and :func:`build_host`.

@@ -9,10 +9,11 @@
 // Each kernel reads and writes each byte once, and memory bounds it: a lane
 // takes eight features (16 bytes of a 2-byte type), so four lanes hold a group
 // and its largest magnitude takes two quad permutations, no LDS; a thread has
-// four such chunks on their way. 1M x 512 bfloat16: written in 284 us (5.5
-// TB/s), read back in 251 (6.2), gelu forward in 468 (5.5) and backward in 489
-// (5.3; there the vector units are busy for 88% of the time, with 25
-// instructions a value, most of them erf's); sine 469 and 488.
+// four such chunks on their way. 1M x 512 bfloat16: written in 285 us (5.4
+// TB/s), read back in 253 (6.1), gelu forward in 458 (5.6) and backward in 487
+// (5.3; the vector units issue for 90% and 80% of the time, 25 and 24
+// instructions a value, most of them Phi's); sine 447 and 461, silu 434 and
+// 464. 500k x 512 float32: gelu and sine 422 and 435 (6.1 and 5.9 TB/s).
 #include "kept8.hpp"
 #include "layers_api.hpp"
 

@@ -104,14 +104,15 @@ void bind(const py::dict& table) {
 }
 
 std::vector<std::string> entry_points() {
-  std::vector<std::string> names = {"gs_last_error", "gs_check_values", "gs_scan_workspace_size", "gs_pack_visible",
-          "gs_records_forward", "gs_records_backward_workspace_size", "gs_records_backward",
-          "gs_bin_order_workspace_size", "gs_bin_order_count", "gs_bin_order_sort",
-          "gs_bin_tiles_workspace_size", "gs_bin_tiles", "gs_bin_tiles_bounded",
-          "gs_bin_blocks_fit", "gs_bin_blocks_count", "gs_bin_blocks_sort",
-          "gs_bin_blocks_tiles_workspace_size", "gs_bin_blocks_tiles",
-          "gs_bin_blocks_tiles_bounded", "gs_render_workspace_size",
-          "gs_render_backward_workspace_size", "gs_render_forward", "gs_render_backward"};
+  std::vector<std::string> names = {
+      "gs_last_error", "gs_check_values", "gs_scan_workspace_size", "gs_pack_visible",
+      "gs_records_forward", "gs_records_backward_workspace_size", "gs_records_backward",
+      "gs_bin_order_workspace_size", "gs_bin_order_count", "gs_bin_order_sort",
+      "gs_bin_tiles_workspace_size", "gs_bin_tiles", "gs_bin_tiles_bounded",
+      "gs_bin_blocks_fit", "gs_bin_blocks_count", "gs_bin_blocks_sort",
+      "gs_bin_blocks_tiles_workspace_size", "gs_bin_blocks_tiles",
+      "gs_bin_blocks_tiles_bounded", "gs_render_workspace_size",
+      "gs_render_backward_workspace_size", "gs_render_forward", "gs_render_backward"};
   for (const std::string& name : layer_entry_points()) names.push_back(name);
   return names;
 }

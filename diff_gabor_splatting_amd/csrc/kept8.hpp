@@ -7,8 +7,9 @@
 // stand for q 2^(b-127): b is the smallest with which the group's largest
 // magnitude rounds to at most 127, within [least, most]. A power of two and
 // not largest / 127: v 2^-e is exact, so q is a function of the inputs alone
-// (no rounding of a scale comes before it), and q 2^e is exact in bfloat16,
-// float16 and float32, so the matrix instructions of the linear layer's
+// (no rounding of a scale comes before it), and q 2^e is exact in the type that
+// the values came from (in bfloat16 and float32 whatever they came from, in
+// float16 within its range), so the matrix instructions of the linear layer's
 // weight gradient take it without another rounding. It costs at most one of
 // the eight bits. A group that holds an infinity or a NaN keeps b = 255 and
 // reads back as NaN throughout.

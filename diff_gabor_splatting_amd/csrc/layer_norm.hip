@@ -20,11 +20,11 @@
 // writes one partial row, and a second kernel adds the partial rows in their
 // order. No atomics: the result does not depend on timing.
 //
-// Memory bounds both passes. 1M x 512 bfloat16: forward 367 us (5.6 TB/s), 510
-// with the 8-bit form (5.0; the vector units, with 187 instructions a row and
-// wave, are then busy for 60% of the time), backward 572 (5.4), 461 from the
-// 8-bit form (5.6). With 1,024 x 64 float32 rows it is launches: 3.3 us, 5.6
-// and 2.6 for the partial sums.
+// Memory bounds both passes. 1M x 512 bfloat16: forward 381 us (5.4 TB/s), 533
+// with the 8-bit form (4.8; the vector units, with 202 instructions a row and
+// wave, then issue for 73% of the time), backward 565 (5.4), 475 from the 8-bit
+// form (5.4; 63%). With 1,024 x 64 float32 rows it is launches: 3.5 us, 5.6
+// and 2.5 for the partial sums.
 #include "kept8.hpp"
 #include "layers_api.hpp"
 
@@ -172,9 +172,11 @@ constexpr int kThreads = Waves == 1 ? 256 : Waves * 64;
 // Workgroups to a compute unit. The grid is that many for each of the 256,
 // all of them running at once (one more would wait for the rest and then run
 // by itself), and no more than memory likes: 1M x 512 bfloat16 rows, forward
-// with 3, 4, 5, 6: 398, 380, 367, 412 us; keeping 8 bits: 510, 569, 546, 539;
+// with 3, 4, 5, 6: 398, 380, 367, 412 us; keeping 8 bits: 510, 569, 546, 539
+// (both before the mean's correction, which added 2% to the latter);
 // backward with 2, 3, 4, 5: 564, 572, 610, 603, from 8 bits 530, 461, 502,
-// 517. The registers of a row set the limit where it takes more lanes' worth.
+// 517. They are those of this size; fewer or shorter rows may want others. The
+// registers of a row set the limit where it takes more lanes' worth.
 enum Pass { kForward, kForwardKept, kBackward };
 template <int Chunks, int Waves>
 constexpr int workgroups_of(Pass pass) {

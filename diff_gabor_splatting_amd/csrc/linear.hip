@@ -168,8 +168,8 @@ struct Product {
 // long to stay in LDS (over 1,024 values, or over 32 panels wide): one
 // 128 x 128 tile to a workgroup; a step of both sides is in registers while the step before is
 // multiplied out of LDS. M is the rows, k contiguous; N the matrix, [n][k] in
-// memory (NContiguous) or [k][n]. 50k x 2048 -> 2048 bfloat16: 616 us (680
-// TFLOP/s).
+// memory (NContiguous) or [k][n]. 50k x 2048 -> 2048 bfloat16: y 573 us (732
+// TFLOP/s), dx 611.
 template <typename T, bool NContiguous>
 __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, Side<T> ns, Product p,
                                                            const T* __restrict__ bias,
@@ -247,12 +247,17 @@ __global__ __launch_bounds__(kThreads) void product_kernel(Side<T> ms, Side<T> n
 // therefore loaded and results stored with eight lanes to 128 bytes of a row,
 // and turned through 2 KB of LDS that the wave has to itself.
 //
-// 1M x 512 -> 512 bfloat16 (524 Gflop, 2.0 GB): y 580 us, with the 8-bit form
-// 735, dx 560 (930 TFLOP/s; a library product of these sizes takes 770 and
-// 711). The matrix cores are then busy for half of the time, the address unit
-// for 65%, LDS for 54%: eight waves, as many as the registers allow, do not
-// fill any of them. 100k x 256 -> 256: 23.5, 31 and 22.5 us (4.4 TB/s). float32
-// is bound by its matrix instructions: 1M x 256 -> 256 1010 us (130 TFLOP/s).
+// 1M x 512 -> 512 bfloat16 (524 Gflop, 2.0 GB): y 562 us, with the 8-bit form
+// 683, dx 555 (945 TFLOP/s; a library product of these sizes takes 770 and
+// 711). In dx the matrix cores are busy for 51% of the time, the address unit
+// for 50%, LDS for 55%, in y with the 8-bit form for 42%, 62% and 45%: eight
+// waves, as many as the registers allow, do not fill any of them. 100k x 256 ->
+// 256: 24, 31 to 36 and 24 to 27 us (4.3 TB/s). float32 is bound by its matrix
+// instructions: 1M x 256 -> 256 1006 us (130 TFLOP/s).
+//
+// 32 compute units of an XCD are shared by whole sets of panels: where the
+// panels are no divisor of 32 some stay idle (19 panels of float32 600 -> 600
+// leave 104 of 256), and rows of fewer tiles than XCDs leave XCDs idle.
 
 // Contiguous values of k in a lane's fragment, and in a step.
 template <typename T>
@@ -552,11 +557,12 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(
 // the bfloat16 rate, a fifth of the time of float32's, and none of them
 // rounded (an infinity or a NaN is the first part alone).
 //
-// 1M rows, 512 -> 512 bfloat16: 595 us (880 TFLOP/s; a library product of
-// these sizes takes 2166), 100k, 256 -> 256: 29 and 6 for the partial sums.
+// 1M rows, 512 -> 512 bfloat16: 637 us (823 TFLOP/s; a library product of
+// these sizes takes 2166), 100k, 256 -> 256: 30 and 6 for the partial sums.
 // With the widest tiles the matrix cores are busy for 43% of the time, the
-// vector units, which expand x8, for 28%, LDS for 32%: a step's barrier and
-// the way from LDS to its first product take the rest.
+// vector units issue for 43% (a quarter of it matrix instructions, most of the
+// rest the expansion of x8), LDS is busy for 32%: a step's barrier and the way
+// from LDS to its first product take the rest.
 
 // What the matrix instructions multiply.
 template <typename T>
@@ -846,8 +852,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict_
 // Tiles are as wide as dW asks for, and the widest only where there are rows
 // enough: every workgroup writes a partial tile, so 256 x 256 of them cost 64
 // MB whatever the rows (256 -> 256, bfloat16: 100k rows 45 us with 256-wide
-// tiles, 38 with 128; 1M rows 185 and 225). Two workgroups per compute unit
-// of the narrower ones; 64 rows at least to each.
+// tiles, 38 with 128; 1M rows 185 and 225). Shares for two workgroups per
+// compute unit of the narrower ones, which the registers allow but for float32's
+// 128 x 128 tile: its 144 allow one, so that they come in two rounds. 64 rows
+// at least to each, 128 from eight tiles on. Where the shares are no multiple of
+// the eight XCDs some XCDs have one more of them than others (600 -> 600: 20
+// shares of 25 tiles, 390 us for 200k rows where 127 would do).
 struct SumPlan {
   int a, b, step;
   int64_t tiles_m, tiles_n, splits, share;
@@ -856,7 +866,8 @@ struct SumPlan {
 SumPlan sum_plan(size_t size, int64_t rows, int64_t features, int64_t outputs) {
   SumPlan p{};
   // What of the wide tiles dW leaves empty, against the narrow ones, which
-  // take 1.3 times as long for the same area (1M, 512 -> 512: 815 and 623).
+  // take 1.3 times as long for the same area (1M, 512 -> 512: 815 and 623, the
+  // XCDs' load even in both).
   const int64_t wide = 4 * ceil_div(outputs, 256) * ceil_div(features, 256);
   const int64_t narrow = ceil_div(outputs, 128) * ceil_div(features, 128);
   const bool large = outputs > 128 && features > 128 && 10 * wide <= 13 * narrow &&

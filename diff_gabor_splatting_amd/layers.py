@@ -13,8 +13,8 @@ each 32 consecutive features of a row share a power of two, the smallest with
 which the largest of them rounds to at most 127, and each is kept as the
 nearest integer multiple of it (ties to even). The error of a value is at most
 1/127 of the largest of its group (half a step; a power of two, because then a
-kept value is exact in every type and does not depend on how a scale was
-rounded). A group with an infinity or a NaN reads back as NaN.
+kept value is exact in the type it came from and does not depend on how a scale
+was rounded). A group with an infinity or a NaN reads back as NaN.
 
 All work is queued on the current stream; nothing synchronises. Inputs whose
 features are contiguous and whose leading dimensions collapse are read in
@@ -80,7 +80,8 @@ def quantize(x: Tensor) -> Checkpoint:
 
 def dequantize(checkpoint: Checkpoint, dtype: Optional[torch.dtype] = None) -> Tensor:
     """What the checkpoint stands for, contiguous, in the type it was made from
-    or in ``dtype``."""
+    or in ``dtype`` (float16 of another type's is rounded where it has no such
+    value)."""
     if not isinstance(checkpoint, Checkpoint):
         raise TypeError("checkpoint must be a Checkpoint")
     return _host.checkpoint8_read(checkpoint.values, checkpoint.exponents,
