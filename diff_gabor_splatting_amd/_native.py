@@ -249,6 +249,14 @@ _SIGNATURES = {
         [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 3 + [_c_ptr] * 3
         + [_c_size, _c_ptr],
     ),
+    "gs_dropout": (
+        _c_int,
+        [_c_int, ctypes.c_double, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 3 + [_c_ptr] * 2,
+    ),
+    "gs_row_groups_workspace_size": (_c_size, [_c_i64] * 2),
+    "gs_row_groups": (
+        _c_int, [_c_int, _c_ptr] + [_c_i64] * 2 + [_c_ptr] * 3 + [_c_size, _c_ptr],
+    ),
 }
 
 PROFILE_FAMILIES = {

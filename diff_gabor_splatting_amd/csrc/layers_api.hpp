@@ -37,6 +37,23 @@ inline int check_rows(const char* name, int32_t dtype, int64_t rows, int64_t fea
   return GS_OK;
 }
 
+// Orders a wave's own LDS writes before its other lanes' reads, and those
+// before later writes: the hardware keeps a wave's LDS order by itself, this
+// keeps the compiler's.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// LDS beyond 64 KB is asked for, each time: the kernel may be running on a
+// device where it was not.
+inline int allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return GS_OK;
+  GS_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  return GS_OK;
+}
+
 // Calls `call` with a zero of the type.
 template <typename F>
 int with_type(int32_t dtype, F&& call) {

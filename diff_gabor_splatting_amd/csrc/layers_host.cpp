@@ -29,6 +29,9 @@ struct Api {
   decltype(&gs_linear_backward_input) linear_backward_input = nullptr;
   decltype(&gs_linear_backward_weight_workspace_size) linear_workspace = nullptr;
   decltype(&gs_linear_backward_weight) linear_backward_weight = nullptr;
+  decltype(&gs_dropout) dropout = nullptr;
+  decltype(&gs_row_groups_workspace_size) row_groups_workspace = nullptr;
+  decltype(&gs_row_groups) row_groups = nullptr;
 };
 
 Api api;
@@ -424,6 +427,72 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& weight,
   return Linear::apply(x, weight, bias);
 }
 
+// --------------------------------------------------------------------------
+// Dropout
+
+at::Tensor masked(const at::Tensor& x, double p, int64_t seed, const at::Tensor& seed_at) {
+  const c10::DeviceGuard guard(x.device());
+  const RowsOf r(x);
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  check(api.dropout(type_of(x), p, seed, data_of(seed_at), r.data(), r.stride, r.rows, r.features,
+                    y.data_ptr(), stream_of(x.device())));
+  return y;
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, double p,
+                            int64_t seed, const std::optional<at::Tensor>& seed_at) {
+    // A seed on the device is saved as it is: one that is changed before the
+    // backward pass raises there, by torch's own check.
+    ctx->save_for_backward({seed_at.value_or(at::Tensor())});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    return masked(x, p, seed, seed_at.value_or(at::Tensor()));
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    check_calls("dropout", {&grads[0]});
+    const auto saved = ctx->get_saved_variables();
+    return once({masked(grads[0], ctx->saved_data["p"].toDouble(),
+                        ctx->saved_data["seed"].toInt(), saved[0]),
+                 at::Tensor(), at::Tensor(), at::Tensor()},
+                "dropout");
+  }
+};
+
+at::Tensor dropout(const at::Tensor& x, double p, int64_t seed,
+                   const std::optional<at::Tensor>& seed_at) {
+  const at::Tensor word = seed_at.value_or(at::Tensor());
+  check_calls("dropout", {&x, &word});
+  check_input(x);
+  if (word.defined() &&
+      (word.device() != x.device() || word.scalar_type() != at::kLong || word.numel() != 1))
+    throw py::value_error("seed must be an integer, or one int64 on the device of x");
+  if (!grad_wanted({&x})) return masked(x, p, seed, word);
+  return Dropout::apply(x, p, seed, seed_at);
+}
+
+// --------------------------------------------------------------------------
+// Rows in groups
+
+std::vector<at::Tensor> row_groups(const at::Tensor& index, int64_t groups) {
+  check_calls("row_groups", {&index});
+  const bool wide = index.scalar_type() == at::kLong;
+  if (!index.is_cuda() || !(wide || index.scalar_type() == at::kInt))
+    throw py::value_error("index must be int32 or int64 on a HIP device");
+  const c10::DeviceGuard guard(index.device());
+  const at::Tensor rows = index.contiguous();
+  at::Tensor order = at::empty({rows.numel()}, on(index.device(), at::kInt));
+  at::Tensor offsets = at::empty({groups + 1}, on(index.device(), at::kInt));
+  const size_t bytes = api.row_groups_workspace(rows.numel(), groups);
+  at::Tensor space;
+  if (bytes) space = workspace(bytes, index.device());
+  check(api.row_groups(wide, rows.data_ptr(), rows.numel(), groups, order.data_ptr<int32_t>(),
+                       offsets.data_ptr<int32_t>(), const_cast<void*>(data_of(space)), bytes,
+                       stream_of(index.device())));
+  return {offsets, order};
+}
+
 }  // namespace
 
 void bind_layers(const py::dict& table) {
@@ -440,6 +509,9 @@ void bind_layers(const py::dict& table) {
   take(table, "gs_linear_backward_input", next.linear_backward_input);
   take(table, "gs_linear_backward_weight_workspace_size", next.linear_workspace);
   take(table, "gs_linear_backward_weight", next.linear_backward_weight);
+  take(table, "gs_dropout", next.dropout);
+  take(table, "gs_row_groups_workspace_size", next.row_groups_workspace);
+  take(table, "gs_row_groups", next.row_groups);
   api = next;
 }
 
@@ -448,7 +520,8 @@ std::vector<std::string> layer_entry_points() {
           "gs_activation_backward", "gs_layer_norm_forward",
           "gs_layer_norm_backward_workspace_size", "gs_layer_norm_backward", "gs_linear_forward",
           "gs_linear_backward_input", "gs_linear_backward_weight_workspace_size",
-          "gs_linear_backward_weight"};
+          "gs_linear_backward_weight", "gs_dropout", "gs_row_groups_workspace_size",
+          "gs_row_groups"};
 }
 
 void define_layers(py::module_& m) {
@@ -462,6 +535,8 @@ void define_layers(py::module_& m) {
   m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"),
         py::arg("eps"), py::arg("eight"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"));
+  m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("seed_at"));
+  m.def("row_groups", &row_groups, py::arg("index"), py::arg("groups"));
 }
 
 }  // namespace gs_host

@@ -25,7 +25,8 @@ points.
 from __future__ import annotations
 
 import math
-from typing import Optional
+import operator
+from typing import Optional, Union
 
 import torch
 from torch import Tensor
@@ -38,7 +39,8 @@ GROUP = 32
 ACTIVATIONS = {"sine": 0, "gelu": 1, "silu": 2}
 _CHECKPOINTS = {"full": False, "8bit": True}
 
-__all__ = ["Checkpoint", "quantize", "dequantize", "activation", "layer_norm", "linear"]
+__all__ = ["Checkpoint", "quantize", "dequantize", "activation", "layer_norm", "linear", "dropout",
+           "RowGroups", "row_groups"]
 
 
 class Checkpoint:
@@ -120,3 +122,68 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:
     type. The weight's gradient is taken with the input as kept in 8 bits; the
     input's gradient does not depend on it."""
     return _host.linear(_tensor("x", x), _tensor("weight", weight), bias)
+
+
+def dropout(x: Tensor, p: float = 0.5, seed: Union[int, Tensor] = 0) -> Tensor:
+    """``x / (1 - p)`` where a mask keeps a value, 0 where it does not (a NaN
+    that is dropped, too). Nothing is kept for the backward pass: the mask is
+    a function of ``seed`` and of a value's row and column (the leading
+    dimensions counted as one), from a counter-based generator
+    (Philox4x32-10; ``include/gabor_layers.h`` has the definition). The same
+    seed gives the same mask, so a program takes another for each layer and
+    step. ``seed`` is a 64-bit integer, or one int64 on the device of ``x``,
+    which is read when the call runs, in a replayed HIP graph too; it may not
+    change between the forward and the backward pass. ``p`` is rounded to a multiple
+    of 2^-16, and 1 / (1 - p) is that of the rounded one."""
+    _tensor("x", x)
+    _number("p", p)
+    if not 0 <= p <= 1:  # not for a NaN, either
+        raise ValueError("p must be 0 through 1")
+    if isinstance(seed, Tensor):
+        return _host.dropout(x, p, 0, seed)
+    seed = operator.index(seed)
+    if not -(1 << 63) <= seed < 1 << 64:
+        raise ValueError("seed must fit 64 bits")
+    return _host.dropout(x, p, (seed + (1 << 63)) % (1 << 64) - (1 << 63), None)
+
+
+class RowGroups:
+    """Rows that belong to groups: ``offsets`` int32 [groups + 1], not falling,
+    and ``order`` int32 [rows], a permutation of the rows: the rows of group g
+    are ``order[offsets[g]:offsets[g + 1]]``, those at other places of ``order``
+    are in no group. Without an order the rows lie by group themselves.
+    :func:`row_groups` makes one of each row's group."""
+
+    __slots__ = ("offsets", "order")
+
+    def __init__(self, offsets: Tensor, order: Optional[Tensor] = None):
+        _tensor("offsets", offsets)
+        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 2 or \
+                not offsets.is_contiguous():
+            raise ValueError("offsets must be contiguous int32 of shape (groups + 1,)")
+        if order is not None:
+            _tensor("order", order)
+            if order.dtype != torch.int32 or order.dim() != 1 or not order.is_contiguous():
+                raise ValueError("order must be contiguous int32 of shape (rows,)")
+            if order.device != offsets.device:
+                raise ValueError("order must be on the device of offsets")
+        self.offsets, self.order = offsets, order
+
+    @property
+    def groups(self) -> int:
+        return self.offsets.numel() - 1
+
+    def __repr__(self) -> str:
+        rows = "" if self.order is None else f", rows={self.order.numel()}"
+        return f"RowGroups(groups={self.groups}{rows})"
+
+
+def row_groups(index: Tensor, groups: int) -> RowGroups:
+    """The rows by group: ``index`` (int32 or int64, any shape) is each row's
+    group, 0 through ``groups - 1``, and any other number puts a row in none.
+    Rows keep their order within a group. At most 4096 groups and 2^31 - 1
+    rows."""
+    groups = operator.index(groups)
+    if not 1 <= groups <= 4096:
+        raise ValueError("groups must be 1 through 4096")
+    return RowGroups(*_host.row_groups(_tensor("index", index), groups))

@@ -88,6 +88,30 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
                               void* grad_bias, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* Dropout: y = x / (1 - p) where the mask keeps a value, else 0; the backward
+ * pass is the same call on grad_y. The mask is a function of the value's row
+ * and column and of the seed (seed_at where that is not null: one 64-bit
+ * word on the device, read when the kernel runs): Philox4x32-10 with the key
+ * (seed's low word, high word) and the counter (column / 8, row's low word,
+ * high word, 0) gives four words, whose eight halves, low ones first, are
+ * the bits of eight columns; a value is kept where its bits are at least
+ * t = rint(65536 p), and multiplied by 65536 / (65536 - t). */
+int gs_dropout(int32_t dtype, double p, int64_t seed, const void* seed_at, const void* x,
+               int64_t row_stride, int64_t rows, int64_t features, void* y, void* stream);
+
+/* Rows in groups. The row at position p of 0 .. rows - 1 is order[p] (p where
+ * order is null), group g has the positions offsets[g] .. offsets[g + 1] - 1,
+ * and the rows at other positions are in no group. order is a permutation of
+ * the rows, offsets [groups + 1] does not fall; both are held to the rows
+ * that exist. rows < 2^31.
+ *
+ * gs_row_groups makes both of each row's group (index, int32 or with `wide`
+ * int64; outside 0 .. groups - 1: of none, behind the last group), each
+ * group's rows in their order, for up to 4096 groups. */
+size_t gs_row_groups_workspace_size(int64_t rows, int64_t groups);
+int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups, int32_t* order,
+                  int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
