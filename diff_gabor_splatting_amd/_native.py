@@ -257,6 +257,18 @@ _SIGNATURES = {
     "gs_row_groups": (
         _c_int, [_c_int, _c_ptr] + [_c_i64] * 2 + [_c_ptr] * 3 + [_c_size, _c_ptr],
     ),
+    "gs_grouped_linear_forward": (
+        _c_int, [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 4 + [_c_ptr] * 2,
+    ),
+    "gs_grouped_linear_backward_input": (
+        _c_int, [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 3 + [_c_i64] * 4 + [_c_ptr] * 2,
+    ),
+    "gs_grouped_linear_backward_weight_workspace_size": (_c_size, [_c_int] + [_c_i64] * 4),
+    "gs_grouped_linear_backward_weight": (
+        _c_int,
+        [_c_int, _c_ptr, _c_i64, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 4 + [_c_ptr] * 3
+        + [_c_size, _c_ptr],
+    ),
 }
 
 PROFILE_FAMILIES = {

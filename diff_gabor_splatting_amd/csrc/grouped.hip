@@ -1,0 +1,690 @@
+// Linear layers whose matrix and bias are those of the row's group:
+// y_i = W_g x_i + b_g for the rows i of group g, and the gradients dx_i = W_g^T dy_i,
+// dW_g = sum dy_i x_i^T, db_g = sum dy_i. Rows of no group have y = dx = 0.
+//
+// Rows are read and written where they lie, through the groups' order: no
+// pass sorts them. Group sizes are on the device alone, so the host launches
+// grids that hold any sizes and the workgroups find their group in the offsets.
+//
+//   group_few_kernel   y of a few rows: a wave to a row's output
+//   group_tile_kernel  y and dx: a tile of one group's rows to a workgroup
+//   group_sum_kernel   dW and db: tiles of dW over shares of all rows, whose
+//                      partial sums group_join_kernel adds in their order
+//
+// No atomics: results do not depend on timing.
+#include "groups.hpp"
+#include "matrix.hpp"
+
+namespace gs {
+namespace {
+
+// --------------------------------------------------------------------------
+// y and dx, a tile of 128 x 128 to a workgroup
+
+// Tiles are numbered without the groups' counts being added up: segment s
+// begins at tile B / 128 + s, B its first position, which leaves it room
+// enough (some numbers have no rows).
+__device__ __forceinline__ int64_t tile_key(const Grouping& g, int s) {
+  return begin_of(g, s) / kEdge + s;
+}
+int64_t tile_numbers(const Grouping& g) { return g.rows / kEdge + g.groups + 2; }
+
+// A tile of rows on its way from memory to LDS, eight columns to a chunk.
+template <typename T, int Columns>
+struct StagedRows {
+  static constexpr int across = Columns / kChunk;
+  static constexpr int count = kEdge * across / kThreads;
+  const T* row[count];  // null past the segment's end
+  vec<T, 8> v[count];
+
+  __device__ __forceinline__ void place(const Grouping& g, const T* data, int64_t stride,
+                                        int first, int end) {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int position = first + (i * kThreads + int(threadIdx.x)) / across;
+      row[i] = position < end ? data + row_at(g, position) * stride : nullptr;
+    }
+  }
+  __device__ __forceinline__ void load(int64_t column, int64_t columns) {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int64_t c = column + (i * kThreads + threadIdx.x) % across * kChunk;
+      const int64_t left = columns - c;
+      v[i] = load_valid<T, 8>(row[i] + c, row[i] ? int(left < kChunk ? left : kChunk) : 0);
+    }
+  }
+  template <int Pitch>
+  __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int id = i * kThreads + threadIdx.x;
+      *reinterpret_cast<vec<T, 8>*>(lds + id / across * Pitch + id % across * kChunk) = v[i];
+    }
+  }
+};
+
+struct GroupProduct {
+  int64_t n, k;      // columns of C, length of the sum
+  int64_t tiles_n;
+  int64_t stride;    // of the rows
+};
+
+// C[i][n] = sum_k x[i][k] W_g(n, k) (+ bias[g][n]); W_g is [n][k] in memory
+// (NContiguous) or [k][n].
+template <typename T, bool NContiguous>
+__global__ __launch_bounds__(kThreads) void group_tile_kernel(
+    const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ bias, Grouping g,
+    GroupProduct p, T* __restrict__ out) {
+  constexpr int depth = Mma<T>::depth;
+  __shared__ __align__(16) T m_lds[kTileSize<T, true>];
+  __shared__ __align__(16) T n_lds[kTileSize<T, NContiguous>];
+  const int64_t number = blockIdx.x / p.tiles_n, n0 = blockIdx.x % p.tiles_n * kEdge;
+  const int s = find_segment(segments_of(g), number, [&](int i) { return tile_key(g, i); });
+  const int begin = begin_of(g, s), end = begin_of(g, s + 1);
+  const int64_t first64 = begin + (number - tile_key(g, s)) * kEdge;
+  if (first64 < begin || first64 >= end) return;  // below only where offsets fall
+  const int first = int(first64);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave_m = (wave >> 1) * kWaveEdge, wave_n = (wave & 1) * kWaveEdge;
+  const int64_t n = n0 + wave_n + 16 * (lane >> 4);
+  f32x4 c[kTiles][kTiles];  // [m][n]
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float offset[16] = {};
+  if (s > 0 && s <= g.groups) {
+    const int64_t group = s - 1;
+    const T* const matrix = w + group * p.n * p.k;
+    const Side<T> ns{matrix, NContiguous ? p.k : p.n, NContiguous ? p.n : p.k,
+                     NContiguous ? p.k : p.n};
+    StagedRows<T, depth> m_next;
+    Staged<T, NContiguous ? kEdge : depth, NContiguous ? depth : kEdge> n_next;
+    m_next.place(g, x, p.stride, first, end);
+    auto fetch = [&](int64_t k) {
+      m_next.load(k, p.k);
+      if constexpr (NContiguous)
+        n_next.load(ns, n0, k);
+      else
+        n_next.load(ns, k, n0);
+    };
+    fetch(0);
+    for (int64_t k = 0; k < p.k; k += depth) {
+      m_next.template store<kPitch<T, true>>(m_lds);
+      n_next.template store<kPitch<T, NContiguous>, true, NContiguous>(n_lds);
+      __syncthreads();
+      if (k + depth < p.k) fetch(k + depth);
+#pragma unroll
+      for (int step = 0; step < depth; step += Mma<T>::step) {
+        typename Mma<T>::Fragment a[kTiles], b[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          a[i] = fragment<T, true>(m_lds, wave_m + 16 * i, step);
+          b[i] = fragment<T, NContiguous>(n_lds, wave_n + 16 * i, step);
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) c[i][j] = Mma<T>::of(b[j], a[i], c[i][j]);
+      }
+      __syncthreads();
+    }
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        offset[j] = n + j < p.n ? float(bias[group * p.n + n + j]) : 0.f;
+    }
+  }
+  // Lane 16 q + i holds, of fragment row i, the 16 columns from 16 q on.
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    const int64_t position = int64_t(first) + wave_m + 16 * i + (lane & 15);
+    if (position >= end) continue;
+    float row[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) row[j] = c[i][j >> 2][j & 3] + offset[j];
+    store_row<T>(out + row_at(g, int(position)) * p.n + n, p.n - n, row);
+  }
+}
+
+template <typename T, bool NContiguous>
+int launch_tiles(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
+                 const Grouping& g, int64_t k, int64_t n, void* out, hipStream_t stream) {
+  const GroupProduct p{n, k, ceil_div(n, kEdge), stride};
+  const int64_t blocks = tile_numbers(g) * p.tiles_n;
+  GS_REQUIRE(blocks < (int64_t(1) << 32) / kThreads, GS_ERR_OVERFLOW, "%s: too many rows", name);
+  group_tile_kernel<T, NContiguous><<<dim3{unsigned(blocks)}, kThreads, 0, stream>>>(
+      static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), g, p,
+      static_cast<T*>(out));
+  GS_LAUNCHED(name);
+  return GS_OK;
+}
+
+// --------------------------------------------------------------------------
+// y of a few rows: a wave to a row's output, its lanes along the features.
+
+constexpr int kFewRows = 16;
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void group_few_kernel(
+    const T* __restrict__ x, int64_t stride, const T* __restrict__ w, const T* __restrict__ bias,
+    Grouping g, int k, int n, T* __restrict__ y) {
+  const int lane = threadIdx.x & 63, position = blockIdx.y;
+  const int output = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (output >= n) return;
+  const int s = find_segment(segments_of(g), position,
+                             [&](int i) { return int64_t(begin_of(g, i)); });
+  const int64_t row = row_at(g, position), group = s - 1;
+  float sum = 0.f;
+  if (s > 0 && s <= g.groups) {
+    const T* const matrix = w + (group * n + output) * k;
+    const T* const from = x + row * stride;
+#pragma unroll 4
+    for (int c = lane * kChunk; c < k; c += 64 * kChunk) {
+      const int valid = min(k - c, kChunk);
+      float a[kChunk], b[kChunk];
+      load8<T>(matrix + c, valid, a);
+      load8<T>(from + c, valid, b);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) sum = __builtin_fmaf(a[j], b[j], sum);
+    }
+#pragma unroll
+    for (int step = 32; step; step >>= 1) sum += __shfl_xor(sum, step);
+    if (bias) sum += float(bias[group * n + output]);
+  }
+  if (lane == 0) y[row * n + output] = T(sum);
+}
+
+// --------------------------------------------------------------------------
+// dW and db: the sums over each group's rows of dy^T x.
+//
+// A workgroup of eight waves (two along the outputs, four along the features)
+// adds up a tile of dW over its share of the positions, `Rows` of them at a
+// time, whatever groups they are in: where a group ends it writes what it
+// has and begins anew, and the loads, which are two steps ahead in registers
+// and one in LDS, run on across that. A share is cut from the line on which
+// each segment takes kGroupCost + its rows, so that writing a group's
+// tile counts too. A group whose part of the line lies in one share is
+// written at once; the others' parts go to the share's head (the group
+// began before it) or tail, and group_join_kernel adds them in their order.
+
+constexpr int kSumThreads = 512;
+constexpr int64_t kGroupCost = 128;  // of a group's tile, in rows
+
+__device__ __forceinline__ int64_t line_at(const Grouping& g, int s) {
+  return begin_of(g, s) + kGroupCost * s;
+}
+__host__ __device__ __forceinline__ int64_t line_length(const Grouping& g) {
+  return g.rows + kGroupCost * (int64_t(g.groups) + 2);
+}
+
+struct GroupSum {
+  int64_t dy_stride, x_stride;
+  int outputs, features;
+  int tiles_m, tiles_n;  // of dW
+  int shares;
+};
+
+// Rows of dy and x that are multiplied: the positions of one step.
+struct StepOf {
+  int first, count;
+};
+
+// Where a share stands: segment s, whose positions from `next` to `end` are its.
+struct Share {
+  int64_t from, to;  // on the line
+  int s, next, end;
+
+  __device__ __forceinline__ void open(const Grouping& g, int segment) {
+    s = segment;
+    if (s >= segments_of(g)) {
+      next = end = 0;
+      return;
+    }
+    // A row at position i of segment s lies at i + kGroupCost (s + 1).
+    const int64_t shift = kGroupCost * (s + 1);
+    const int64_t low = begin_of(g, s), high = begin_of(g, s + 1);
+    const int64_t a = from - shift > low ? from - shift : low;
+    const int64_t b = to - shift < high ? to - shift : high;
+    const bool some = a < b && s > 0 && s <= g.groups;
+    next = some ? int(a) : 0;
+    end = some ? int(b) : 0;
+  }
+  // Whether segment s begins before the share's end.
+  __device__ __forceinline__ bool inside(const Grouping& g) const {
+    return s < segments_of(g) && line_at(g, s) < to;
+  }
+};
+
+// 16 rows by 16 columns of LDS as a fragment, k along the rows, `k` the first
+// of Mma's step.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Fragment row_fragment(const T* lds, int pitch,
+                                                                  int first) {
+  if constexpr (sizeof(T) == 2) {
+    return turned_fragment<T>(lds, pitch, first);
+  } else {
+    // Value j of lane group q is row 4 j + q: with a pitch of 16 past a
+    // multiple of 64, the four lane groups read different banks.
+    const int lane = threadIdx.x & 63;
+    const T* const p = lds + (lane >> 4) * pitch + first + (lane & 15);
+    return vec<T, 4>{p[0], p[4 * pitch], p[8 * pitch], p[12 * pitch]};
+  }
+}
+
+// A wave's tile: 16 A outputs x 16 B features.
+template <typename T, int A, int B, int Rows>
+__global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x, Grouping g, GroupSum p,
+    float* __restrict__ partial, T* __restrict__ dw, T* __restrict__ db) {
+  constexpr int tile_m = 32 * A, tile_n = 64 * B;
+  // 16 values past a multiple of 64: the rows that the lanes of a fragment's
+  // load read lie in different banks.
+  constexpr int pitch_m = tile_m + 16, pitch_n = tile_n + 16;
+  constexpr int buffer = Rows * (pitch_m + pitch_n);
+  constexpr int across_m = tile_m / 8, across_n = tile_n / 8;
+  constexpr int apart_m = kSumThreads / across_m, apart_n = kSumThreads / across_n;
+  constexpr int loads_m = (Rows + apart_m - 1) / apart_m, loads_n = (Rows + apart_n - 1) / apart_n;
+  extern __shared__ __align__(16) char shared[];
+  T* const lds = reinterpret_cast<T*>(shared);
+
+  // Workgroups go to the eight XCDs in turn: the tiles of one share have one
+  // XCD, and its L2. With fewer shares than XCDs the tiles go round.
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int in_xcd = blockIdx.x >> 3;
+  const bool shared_xcd = p.shares >= 8;
+  const int share = shared_xcd ? in_xcd / tiles * 8 + int(blockIdx.x & 7)
+                               : int(blockIdx.x % unsigned(p.shares));
+  if (share >= p.shares) return;
+  const int tile = shared_xcd ? in_xcd % tiles : int(blockIdx.x / unsigned(p.shares));
+  const int m0 = tile / p.tiles_n * tile_m, n0 = tile % p.tiles_n * tile_n;
+  const int64_t length = line_length(g);
+  Share at;
+  at.from = length * share / p.shares;
+  at.to = length * (share + 1) / p.shares;
+  at.open(g, find_segment(segments_of(g), at.from, [&](int i) { return line_at(g, i); }));
+  Share ahead_at = at;
+
+  // The positions of the step after the last that this was called for.
+  auto next_step = [&]() {
+    while (ahead_at.next >= ahead_at.end && ahead_at.inside(g)) ahead_at.open(g, ahead_at.s + 1);
+    const int left = ahead_at.end - ahead_at.next;
+    const StepOf step{ahead_at.next, left < Rows ? left : Rows};
+    ahead_at.next += step.count;
+    return step;
+  };
+
+  // Each thread's places: eight outputs of loads_m rows, eight features of
+  // loads_n.
+  const int row_m = threadIdx.x / across_m, column_m = threadIdx.x % across_m * 8;
+  const int row_n = threadIdx.x / across_n, column_n = threadIdx.x % across_n * 8;
+  const int valid_m = min(p.outputs - m0 - column_m, 8);
+  const int valid_n = min(p.features - n0 - column_n, 8);
+  const T* const from_m = dy + m0 + column_m;
+  const T* const from_n = x + n0 + column_n;
+
+  struct Load {
+    vec<T, 8> m[loads_m], n[loads_n];
+  };
+  struct Ids {  // rows of a step, -1 where there is none
+    int m[loads_m], n[loads_n];
+  };
+  Load ahead[2];
+  Ids ids;
+  auto find = [&]() {
+    const StepOf step = next_step();
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i) {
+      const int r = row_m + i * apart_m;
+      ids.m[i] = r < step.count ? int(row_at(g, step.first + r)) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < loads_n; ++i) {
+      const int r = row_n + i * apart_n;
+      ids.n[i] = r < step.count ? int(row_at(g, step.first + r)) : -1;
+    }
+  };
+  auto send = [&](Load& to) {
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i)
+      to.m[i] = load_valid<T, 8>(from_m + ids.m[i] * p.dy_stride, ids.m[i] >= 0 ? valid_m : 0);
+#pragma unroll
+    for (int i = 0; i < loads_n; ++i)
+      to.n[i] = load_valid<T, 8>(from_n + ids.n[i] * p.x_stride, ids.n[i] >= 0 ? valid_n : 0);
+    find();
+  };
+  auto put = [&](const Load& from, T* to) {
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i)
+      if (apart_m * loads_m == Rows || row_m + i * apart_m < Rows)
+        *reinterpret_cast<vec<T, 8>*>(to + (row_m + i * apart_m) * pitch_m + column_m) = from.m[i];
+#pragma unroll
+    for (int i = 0; i < loads_n; ++i)
+      if (apart_n * loads_n == Rows || row_n + i * apart_n < Rows)
+        *reinterpret_cast<vec<T, 8>*>(to + Rows * pitch_m + (row_n + i * apart_n) * pitch_n +
+                                      column_n) = from.n[i];
+  };
+
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave_m = (wave >> 2) * 16 * A, wave_n = (wave & 3) * 16 * B;
+  const bool sums = db && n0 == 0;
+  f32x4 c[A][B];
+  float sum[(A + 3) / 4];  // of the outputs of fragments wave % 4, + 4, ..
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < (A + 3) / 4; ++i) sum[i] = 0.f;
+  };
+  auto multiply_step = [&](const T* from) {
+    constexpr int deep = Mma<T>::step;
+#pragma unroll
+    for (int k = 0; k < Rows; k += deep) {
+      typename Mma<T>::Fragment b[B];
+#pragma unroll
+      for (int j = 0; j < B; ++j)
+        b[j] = row_fragment<T>(from + Rows * pitch_m + k * pitch_n, pitch_n, wave_n + 16 * j);
+#pragma unroll
+      for (int i = 0; i < A; ++i) {
+        const typename Mma<T>::Fragment a =
+            row_fragment<T>(from + k * pitch_m, pitch_m, wave_m + 16 * i);
+#pragma unroll
+        for (int j = 0; j < B; ++j) c[i][j] = Mma<T>::of(b[j], a, c[i][j]);
+        if (sums && (wave & 3) == (i & 3)) {
+#pragma unroll
+          for (int j = 0; j < int(sizeof(a) / sizeof(T)); ++j) sum[i / 4] += float(a[j]);
+        }
+      }
+    }
+  };
+
+  const int q = lane >> 4, i16 = lane & 15;
+  // Writes the tile of segment at.s and goes on to the next.
+  auto finish = [&]() __attribute__((always_inline)) {
+    const int64_t low = line_at(g, at.s), high = line_at(g, at.s + 1);
+    const bool whole = low >= at.from && high <= at.to;
+    const int64_t size = int64_t(p.outputs) * (int64_t(p.features) + 1);
+    float* const mine = partial + (2 * int64_t(share) + (low < at.from ? 0 : 1)) * size;
+    const int64_t weights = int64_t(p.outputs) * p.features;
+    const bool group = at.s > 0 && at.s <= g.groups;
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      const int m = m0 + wave_m + 16 * i + i16;
+      float total = sum[i / 4];
+      if (sums && (wave & 3) == (i & 3)) {
+        total += __shfl_xor(total, 16);
+        total += __shfl_xor(total, 32);
+      }
+      if (!group || m >= p.outputs) continue;
+      // Lane 16 q + i holds features 4 q .. 4 q + 3 of output i of a fragment.
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const int n = n0 + wave_n + 16 * j + 4 * q;
+        const int valid = min(p.features - n, 4);
+        if (!whole) {
+          store_valid<float, 4>(mine + int64_t(m) * p.features + n, valid, c[i][j]);
+        } else if (dw) {
+          const vec<T, 4> v = {T(c[i][j][0]), T(c[i][j][1]), T(c[i][j][2]), T(c[i][j][3])};
+          store_valid<T, 4>(dw + (at.s - 1) * weights + int64_t(m) * p.features + n, valid, v);
+        }
+      }
+      if (sums && (wave & 3) == (i & 3) && q == 0) {
+        if (whole)
+          db[(at.s - 1) * int64_t(p.outputs) + m] = T(total);
+        else
+          mine[weights + m] = total;
+      }
+    }
+    clear();
+    at.open(g, at.s + 1);
+  };
+  // Whether a step is left; segments without another row in this share are
+  // finished on the way.
+  auto more = [&]() __attribute__((always_inline)) {
+    while (at.next >= at.end && at.inside(g)) finish();
+    return at.inside(g);
+  };
+
+  clear();
+  find();
+  send(ahead[0]);
+  send(ahead[1]);
+  put(ahead[0], lds);
+  send(ahead[0]);
+  __syncthreads();
+  while (more()) {
+    put(ahead[1], lds + buffer);
+    send(ahead[1]);
+    multiply_step(lds);
+    at.next += min(at.end - at.next, Rows);
+    __syncthreads();
+    if (!more()) return;
+    put(ahead[0], lds);
+    send(ahead[0]);
+    multiply_step(lds + buffer);
+    at.next += min(at.end - at.next, Rows);
+    __syncthreads();
+  }
+}
+
+// Adds the parts of the groups that lie in several shares. blockIdx.y: the
+// border between two shares that is the first within its group; blockIdx.x:
+// kThreads / Slices values of dW and db at a time, for which each slice of
+// the threads adds every Slices-th part.
+template <typename T, int Slices>
+__global__ __launch_bounds__(kThreads) void group_join_kernel(const float* __restrict__ partial,
+                                                              Grouping g, GroupSum p,
+                                                              T* __restrict__ dw,
+                                                              T* __restrict__ db) {
+  constexpr int columns = kThreads / Slices;
+  __shared__ float sums[Slices][columns];
+  const int64_t length = line_length(g);
+  const int border = blockIdx.y + 1;
+  const int64_t v = length * border / p.shares;
+  const int s = find_segment(segments_of(g), v, [&](int i) { return line_at(g, i); });
+  const int64_t low = line_at(g, s), high = line_at(g, s + 1);
+  if (s < 1 || s > g.groups || v <= low || length * (border - 1) / p.shares > low) return;
+  // Shares border - 1 (its tail) .. last (their heads).
+  int last = border;
+  while (last + 1 < p.shares && length * (last + 1) / p.shares < high) ++last;
+  const int count = last - border + 2;
+  const int64_t weights = int64_t(p.outputs) * p.features, size = weights + p.outputs;
+  const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
+  for (int64_t first = int64_t(blockIdx.x) * columns; first < size;
+       first += int64_t(gridDim.x) * columns) {
+    const int64_t i = first + column;
+    float sum = 0.f;
+    if (i < size) {
+#pragma unroll 8
+      for (int j = slice; j < count; j += Slices)
+        sum += partial[(j ? 2 * int64_t(border - 1 + j) : 2 * int64_t(border) - 1) * size + i];
+    }
+    if constexpr (Slices > 1) {
+      sums[slice][column] = sum;
+      __syncthreads();
+      for (int j = 1; j < Slices; ++j) sum += slice == 0 ? sums[j][column] : 0.f;
+      __syncthreads();
+    }
+    if (slice || i >= size) continue;
+    if (i < weights) {
+      if (dw) dw[(s - 1) * weights + i] = T(sum);
+    } else if (db) {
+      db[(s - 1) * int64_t(p.outputs) + (i - weights)] = T(sum);
+    }
+  }
+}
+
+// How dW's sums are cut: fragments of a wave's tile along the outputs and the
+// features, positions of a step, and shares of the line. As for one group:
+// the widest tiles where they leave little empty and there are rows enough.
+struct GroupSumPlan {
+  int a, b, step;
+  int64_t tiles_m, tiles_n, shares;
+};
+
+GroupSumPlan sum_plan(size_t size, const Grouping& g, int64_t features, int64_t outputs) {
+  GroupSumPlan p{};
+  const int64_t wide = 4 * ceil_div(outputs, 256) * ceil_div(features, 256);
+  const int64_t narrow = ceil_div(outputs, 128) * ceil_div(features, 128);
+  const bool large = size == 2 && outputs > 128 && features > 128 && 10 * wide <= 13 * narrow &&
+                     double(g.rows) * double(outputs) * double(features) >= 2e10;
+  p.a = large ? 8 : outputs <= 64 ? 2 : 4;
+  p.b = large ? 4 : features <= 64 ? 1 : 2;
+  p.step = p.a == 2 ? 64 : 32;
+  p.tiles_m = ceil_div(outputs, 32 * p.a);
+  p.tiles_n = ceil_div(features, 64 * p.b);
+  const int64_t tiles = p.tiles_m * p.tiles_n;
+  p.shares = std::max<int64_t>(1, (large ? 256 : 512) / tiles);
+  p.shares = std::min(p.shares, ceil_div(line_length(g), 2 * kGroupCost));
+  return p;
+}
+
+int check_grouped(const char* name, int32_t dtype, const void* offsets, int64_t rows,
+                  int64_t groups, int64_t features, int64_t outputs) {
+  GS_CHECK(check_grouping(name, offsets, rows, groups));
+  GS_CHECK(check_rows(name, dtype, rows, features, features));
+  GS_CHECK(check_rows(name, dtype, rows, outputs, outputs));
+  GS_REQUIRE(outputs <= kMostFeatures / 64 && features <= kMostFeatures / 64, GS_ERR_ARGUMENT,
+             "%s: at most %lld features and outputs", name, (long long)(kMostFeatures / 64));
+  return GS_OK;
+}
+
+Grouping grouping(const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups) {
+  return {order, offsets, int32_t(rows), int32_t(groups)};
+}
+
+}  // namespace
+}  // namespace gs
+
+extern "C" {
+
+int gs_grouped_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const void* weight,
+                              const void* bias, const int32_t* order, const int32_t* offsets,
+                              int64_t rows, int64_t groups, int64_t features, int64_t outputs,
+                              void* y, void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_grouped_linear_forward";
+  GS_CHECK(check_grouped(name, dtype, offsets, rows, groups, features, outputs));
+  GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && weight && y, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  const Grouping g = grouping(order, offsets, rows, groups);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    if (rows <= kFewRows) {
+      const dim3 grid{unsigned(ceil_div(outputs, kThreads / 64)), unsigned(rows)};
+      group_few_kernel<T><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+          static_cast<const T*>(x), row_stride, static_cast<const T*>(weight),
+          static_cast<const T*>(bias), g, int(features), int(outputs), static_cast<T*>(y));
+      GS_LAUNCHED(name);
+      return int(GS_OK);
+    }
+    return launch_tiles<T, true>(name, x, row_stride, weight, bias, g, features, outputs, y,
+                                 static_cast<hipStream_t>(stream));
+  });
+}
+
+int gs_grouped_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                     const void* weight, const int32_t* order,
+                                     const int32_t* offsets, int64_t rows, int64_t groups,
+                                     int64_t features, int64_t outputs, void* grad_x,
+                                     void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_grouped_linear_backward_input";
+  GS_CHECK(check_grouped(name, dtype, offsets, rows, groups, features, outputs));
+  GS_CHECK(check_rows(name, dtype, rows, outputs, grad_stride));
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(grad_y && weight && grad_x, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  const Grouping g = grouping(order, offsets, rows, groups);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return launch_tiles<T, false>(name, grad_y, grad_stride, weight, nullptr, g, outputs,
+                                  features, grad_x, static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t gs_grouped_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows,
+                                                        int64_t groups, int64_t features,
+                                                        int64_t outputs) {
+  using namespace gs;
+  if (rows < 0 || rows > kMostGroupedRows || groups <= 0 || groups > kMostGroupsOfRows ||
+      features <= 0 || outputs <= 0)
+    return 0;
+  const size_t size = dtype == GS_FLOAT32 ? 4 : 2;
+  const int64_t shares =
+      sum_plan(size, grouping(nullptr, nullptr, rows, groups), features, outputs).shares;
+  return shares == 1 ? 0 : size_t(2 * shares) * size_t(outputs * (features + 1)) * sizeof(float);
+}
+
+int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                      const void* x, int64_t row_stride, const int32_t* order,
+                                      const int32_t* offsets, int64_t rows, int64_t groups,
+                                      int64_t features, int64_t outputs, void* grad_weight,
+                                      void* grad_bias, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_grouped_linear_backward_weight";
+  GS_CHECK(check_grouped(name, dtype, offsets, rows, groups, features, outputs));
+  GS_CHECK(check_rows(name, dtype, rows, outputs, grad_stride));
+  GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
+  if (!grad_weight && !grad_bias) return GS_OK;
+  GS_REQUIRE(offsets && (rows == 0 || (grad_y && x)), GS_ERR_ARGUMENT,
+             "null pointer passed to %s", name);
+  const size_t need = gs_grouped_linear_backward_weight_workspace_size(dtype, rows, groups,
+                                                                       features, outputs);
+  GS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), GS_ERR_WORKSPACE,
+             "workspace too small for %s", name);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const Grouping g = grouping(order, offsets, rows, groups);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const GroupSumPlan plan = sum_plan(sizeof(T), g, features, outputs);
+    const GroupSum p{grad_stride,       row_stride,        int(outputs),    int(features),
+                     int(plan.tiles_m), int(plan.tiles_n), int(plan.shares)};
+    const int64_t blocks = (plan.shares >= 8 ? ceil_div(plan.shares, 8) * 8 : plan.shares) *
+                           plan.tiles_m * plan.tiles_n;
+    GS_REQUIRE(blocks < (int64_t(1) << 32) / kSumThreads, GS_ERR_OVERFLOW,
+               "%s: too many values", name);
+    T* const dw = static_cast<T*>(grad_weight);
+    T* const db = static_cast<T*>(grad_bias);
+    float* const partial = static_cast<float*>(workspace);
+    auto launch = [&](auto a, auto b) {
+      constexpr int step = a.value == 2 ? 64 : 32;
+      constexpr size_t lds = 2 * step * (32 * a.value + 16 + 64 * b.value + 16) * sizeof(T);
+      auto* const kernel = &group_sum_kernel<T, a.value, b.value, step>;
+      GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
+      kernel<<<dim3{unsigned(blocks)}, kSumThreads, lds, s>>>(
+          static_cast<const T*>(grad_y), static_cast<const T*>(x), g, p, partial, dw, db);
+      GS_LAUNCHED(name);
+      return int(GS_OK);
+    };
+    using std::integral_constant;
+    using one = integral_constant<int, 1>;
+    using two = integral_constant<int, 2>;
+    using four = integral_constant<int, 4>;
+    const int shape = plan.a * 10 + plan.b;
+    if (shape == 21) GS_CHECK(launch(two{}, one{}));
+    if (shape == 22) GS_CHECK(launch(two{}, two{}));
+    if (shape == 41) GS_CHECK(launch(four{}, one{}));
+    if (shape == 42) GS_CHECK(launch(four{}, two{}));
+    if constexpr (sizeof(T) == 2)
+      if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}));
+    if (plan.shares == 1) return int(GS_OK);
+    const int64_t size = outputs * (features + 1);
+    auto join = [&](auto slices) {
+      const dim3 grid{unsigned(std::min<int64_t>(ceil_div(size, kThreads / slices.value), 1 << 14)),
+                      unsigned(plan.shares - 1)};
+      group_join_kernel<T, slices.value><<<grid, kThreads, 0, s>>>(partial, g, p, dw, db);
+    };
+    size >= 512 * kThreads ? join(one{}) : join(four{});
+    GS_LAUNCHED("group_join_kernel");
+    return int(GS_OK);
+  });
+}
+
+}  // extern "C"

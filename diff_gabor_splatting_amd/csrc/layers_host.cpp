@@ -32,6 +32,10 @@ struct Api {
   decltype(&gs_dropout) dropout = nullptr;
   decltype(&gs_row_groups_workspace_size) row_groups_workspace = nullptr;
   decltype(&gs_row_groups) row_groups = nullptr;
+  decltype(&gs_grouped_linear_forward) grouped_forward = nullptr;
+  decltype(&gs_grouped_linear_backward_input) grouped_backward_input = nullptr;
+  decltype(&gs_grouped_linear_backward_weight_workspace_size) grouped_workspace = nullptr;
+  decltype(&gs_grouped_linear_backward_weight) grouped_backward_weight = nullptr;
 };
 
 Api api;
@@ -493,6 +497,111 @@ std::vector<at::Tensor> row_groups(const at::Tensor& index, int64_t groups) {
   return {offsets, order};
 }
 
+// How rows are grouped, as the entry points take it.
+struct Groups {
+  at::Tensor offsets, order;  // no order: the rows lie by group
+
+  const int32_t* begins() const { return offsets.data_ptr<int32_t>(); }
+  const int32_t* places() const { return order.defined() ? order.data_ptr<int32_t>() : nullptr; }
+  int64_t count() const { return offsets.numel() - 1; }
+
+  void check(const at::Tensor& x, int64_t groups) const {
+    if (offsets.device() != x.device() || (order.defined() && order.device() != x.device()))
+      throw py::value_error("groups must be on the device of x");
+    if (count() != groups)
+      throw py::value_error("groups has offsets of " + std::to_string(count()) + " groups, not " +
+                            std::to_string(groups));
+    const int64_t rows = x.numel() / x.size(-1);
+    if (rows > 0x7fffffff) throw py::value_error("x has more than 2^31 - 1 rows");
+    if (order.defined() && order.numel() != rows)
+      throw py::value_error("groups has an order of " + std::to_string(order.numel()) +
+                            " rows, x has " + std::to_string(rows));
+  }
+};
+
+at::Tensor grouped_rows(const at::Tensor& x, const at::Tensor& weight, const Groups& groups,
+                        const at::Tensor& bias) {
+  const c10::DeviceGuard guard(x.device());
+  const RowsOf r(x);
+  const at::Tensor w = dense(weight), b = dense(bias);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = w.size(1);
+  at::Tensor y = at::empty(shape, x.options());
+  check(api.grouped_forward(type_of(x), r.data(), r.stride, w.data_ptr(), data_of(b),
+                            groups.places(), groups.begins(), r.rows, groups.count(), r.features,
+                            w.size(1), y.data_ptr(), stream_of(x.device())));
+  return y;
+}
+
+struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                            const at::Tensor& weight, const at::Tensor& offsets,
+                            const std::optional<at::Tensor>& order,
+                            const std::optional<at::Tensor>& bias) {
+    const bool keep = weight.requires_grad() || (bias && bias->requires_grad());
+    const Groups groups{offsets, order.value_or(at::Tensor())};
+    at::Tensor y = grouped_rows(x, weight, groups, bias.value_or(at::Tensor()));
+    ctx->save_for_backward({keep ? x : at::Tensor(), weight, offsets, groups.order});
+    ctx->saved_data["order"] = order.has_value();
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    check_calls("grouped_linear", {&grads[0]});
+    const auto saved = ctx->get_saved_variables();
+    const bool has_order = ctx->saved_data["order"].toBool();
+    const bool has_bias = ctx->saved_data["bias"].toBool();
+    const at::Tensor& grad = grads[0];
+    const c10::DeviceGuard guard(grad.device());
+    const RowsOf g(grad);
+    const at::Tensor w = dense(saved[1]);
+    const Groups groups{saved[2], saved[3]};
+    const int64_t outputs = w.size(1), features = w.size(2);
+    const int32_t type = type_of(grad);
+    void* const stream = stream_of(grad.device());
+    at::Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) {
+      dx = at::empty(ctx->saved_data["shape"].toIntVector(), grad.options());
+      check(api.grouped_backward_input(type, g.data(), g.stride, w.data_ptr(), groups.places(),
+                                       groups.begins(), g.rows, groups.count(), features, outputs,
+                                       dx.data_ptr(), stream));
+    }
+    // A tensor that is not there is no input of the function's graph.
+    const size_t bias_at = has_order ? 4 : 3;
+    if (ctx->needs_input_grad(1)) dw = at::empty(w.sizes(), grad.options());
+    if (has_bias && ctx->needs_input_grad(bias_at))
+      db = at::empty({groups.count(), outputs}, grad.options());
+    if (dw.defined() || db.defined()) {
+      const RowsOf r(saved[0]);
+      const at::Tensor space = workspace(
+          api.grouped_workspace(type, g.rows, groups.count(), features, outputs), grad.device());
+      check(api.grouped_backward_weight(
+          type, g.data(), g.stride, r.data(), r.stride, groups.places(), groups.begins(), g.rows,
+          groups.count(), features, outputs, const_cast<void*>(data_of(dw)),
+          const_cast<void*>(data_of(db)), space.data_ptr(), size_t(space.numel()), stream));
+    }
+    return once({dx, dw, at::Tensor(), at::Tensor(), db}, "grouped_linear");
+  }
+};
+
+at::Tensor grouped_linear(const at::Tensor& x, const at::Tensor& weight,
+                          const at::Tensor& offsets, const std::optional<at::Tensor>& order,
+                          const std::optional<at::Tensor>& bias) {
+  const at::Tensor b = bias.value_or(at::Tensor());
+  const Groups groups{offsets, order.value_or(at::Tensor())};
+  check_calls("grouped_linear", {&x, &weight, &b});
+  check_input(x);
+  if (weight.dim() != 3 || weight.size(0) < 1 || weight.size(1) < 1)
+    throw py::value_error("weight must have shape (groups, outputs, features)");
+  check_parameter("weight", weight, {weight.size(0), weight.size(1), x.size(-1)}, x, false);
+  check_parameter("bias", b, {weight.size(0), weight.size(1)}, x, false);
+  groups.check(x, weight.size(0));
+  if (!grad_wanted({&x, &weight, &b})) return grouped_rows(x, weight, groups, b);
+  return GroupedLinear::apply(x, weight, offsets, order, bias);
+}
+
 }  // namespace
 
 void bind_layers(const py::dict& table) {
@@ -512,6 +621,10 @@ void bind_layers(const py::dict& table) {
   take(table, "gs_dropout", next.dropout);
   take(table, "gs_row_groups_workspace_size", next.row_groups_workspace);
   take(table, "gs_row_groups", next.row_groups);
+  take(table, "gs_grouped_linear_forward", next.grouped_forward);
+  take(table, "gs_grouped_linear_backward_input", next.grouped_backward_input);
+  take(table, "gs_grouped_linear_backward_weight_workspace_size", next.grouped_workspace);
+  take(table, "gs_grouped_linear_backward_weight", next.grouped_backward_weight);
   api = next;
 }
 
@@ -521,7 +634,9 @@ std::vector<std::string> layer_entry_points() {
           "gs_layer_norm_backward_workspace_size", "gs_layer_norm_backward", "gs_linear_forward",
           "gs_linear_backward_input", "gs_linear_backward_weight_workspace_size",
           "gs_linear_backward_weight", "gs_dropout", "gs_row_groups_workspace_size",
-          "gs_row_groups"};
+          "gs_row_groups", "gs_grouped_linear_forward", "gs_grouped_linear_backward_input",
+          "gs_grouped_linear_backward_weight_workspace_size",
+          "gs_grouped_linear_backward_weight"};
 }
 
 void define_layers(py::module_& m) {
@@ -537,6 +652,8 @@ void define_layers(py::module_& m) {
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"));
   m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("seed_at"));
   m.def("row_groups", &row_groups, py::arg("index"), py::arg("groups"));
+  m.def("grouped_linear", &grouped_linear, py::arg("x"), py::arg("weight"), py::arg("offsets"),
+        py::arg("order"), py::arg("bias"));
 }
 
 }  // namespace gs_host

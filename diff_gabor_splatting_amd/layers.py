@@ -40,7 +40,7 @@ ACTIVATIONS = {"sine": 0, "gelu": 1, "silu": 2}
 _CHECKPOINTS = {"full": False, "8bit": True}
 
 __all__ = ["Checkpoint", "quantize", "dequantize", "activation", "layer_norm", "linear", "dropout",
-           "RowGroups", "row_groups"]
+           "RowGroups", "row_groups", "grouped_linear"]
 
 
 class Checkpoint:
@@ -187,3 +187,21 @@ def row_groups(index: Tensor, groups: int) -> RowGroups:
     if not 1 <= groups <= 4096:
         raise ValueError("groups must be 1 through 4096")
     return RowGroups(*_host.row_groups(_tensor("index", index), groups))
+
+
+def _groups(groups) -> RowGroups:
+    if not isinstance(groups, RowGroups):
+        raise TypeError("groups must be a RowGroups")
+    return groups
+
+
+def grouped_linear(x: Tensor, weight: Tensor, groups: RowGroups,
+                   bias: Optional[Tensor] = None) -> Tensor:
+    """``x weight[g]^T + bias[g]`` for the rows of group g, 0 for rows of no
+    group (whose gradient is 0, too). ``weight`` [groups, outputs, features]
+    and ``bias`` [groups, outputs] have the type of ``x``. Rows are read and
+    written where they lie. The backward pass reads ``x`` itself, which the
+    parameters' gradients are those of."""
+    groups = _groups(groups)
+    return _host.grouped_linear(_tensor("x", x), _tensor("weight", weight), groups.offsets,
+                                groups.order, bias)

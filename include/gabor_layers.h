@@ -112,6 +112,31 @@ size_t gs_row_groups_workspace_size(int64_t rows, int64_t groups);
 int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups, int32_t* order,
                   int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A linear layer by group: y = x weight[g]^T + bias[g] for the rows of group g
+ * (weight [groups, outputs, features], bias [groups, outputs] or null), all of
+ * one type; rows of no group have y = 0 and grad_x = 0. groups <= 2^20. */
+int gs_grouped_linear_forward(int32_t dtype, const void* x, int64_t row_stride,
+                              const void* weight, const void* bias, const int32_t* order,
+                              const int32_t* offsets, int64_t rows, int64_t groups,
+                              int64_t features, int64_t outputs, void* y, void* stream);
+/* grad_x = grad_y weight[g]. */
+int gs_grouped_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                     const void* weight, const int32_t* order,
+                                     const int32_t* offsets, int64_t rows, int64_t groups,
+                                     int64_t features, int64_t outputs, void* grad_x,
+                                     void* stream);
+/* grad_weight[g] = the sum over group g's rows of grad_y^T x, grad_bias[g] the
+ * sum of grad_y (either may be null; zero for a group without rows). */
+size_t gs_grouped_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows,
+                                                        int64_t groups, int64_t features,
+                                                        int64_t outputs);
+int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                      const void* x, int64_t row_stride, const int32_t* order,
+                                      const int32_t* offsets, int64_t rows, int64_t groups,
+                                      int64_t features, int64_t outputs, void* grad_weight,
+                                      void* grad_bias, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

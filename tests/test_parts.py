@@ -274,3 +274,242 @@ def test_dropout_seed_refusals():
                 torch.tensor([1, 2], device="cuda")):
         with pytest.raises(ValueError, match="seed must be"):
             m.dropout(x, 0.5, bad)
+
+
+# --------------------------------------------------------------------------
+# GPU: layers by group
+
+
+def some_groups(rows, groups, seed, none=0.05, empty=True):
+    """Each row's group, sizes uneven, some groups empty, some rows in none."""
+    gen = torch.Generator().manual_seed(seed)
+    shares = torch.rand(groups, generator=gen) ** 3 + 1e-3
+    if empty and groups > 2:
+        shares[::3] = 0
+    index = torch.multinomial(shares, rows, replacement=True, generator=gen)
+    index[torch.rand(rows, generator=gen) < none] = -1
+    return index
+
+
+def grouped_by(index, groups):
+    """(the framework's groups, each group's rows)."""
+    got = layers().row_groups(index.cuda(), groups)
+    return got, oracle.members(got.offsets, got.order, index.numel())
+
+
+def check_grouped(x, w, b, g, members, y, grads):
+    rows, features, outputs = len(x), x.shape[1], w.shape[1]
+    want = oracle.grouped_linear(x, w, members, b, g)
+    size = oracle.grouped_linear(x.abs(), w.abs(), members, None if b is None else b.abs(),
+                                 g.abs())
+    most = max([len(m) for m in members] + [1])
+    near(y.reshape(rows, outputs), want[0], (features + 2) * E * size[0], x.dtype)
+    near(grads[0].reshape(rows, features), want[1], (outputs + 2) * E * size[1], x.dtype)
+    near(grads[1], want[2], (most + 2) * E * size[2], x.dtype)
+    if b is not None:
+        near(grads[2], want[3], (most + 2) * E * size[3], x.dtype)
+
+
+def grouped_case(rows, features, outputs, groups, dtype, bias=True, seed=21, index=None):
+    m = layers()
+    x = normal(rows, features, seed=seed, dtype=dtype)
+    w = normal(groups, outputs, features, seed=seed + 1, dtype=dtype, scale=features ** -0.5)
+    b = normal(groups, outputs, seed=seed + 2, dtype=dtype) if bias else None
+    g = normal(rows, outputs, seed=seed + 3, dtype=dtype)
+    index = some_groups(rows, groups, seed) if index is None else index
+    by, members = grouped_by(index, groups)
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b) if t is not None]
+    y = m.grouped_linear(inputs[0], inputs[1], by, *inputs[2:])
+    grads = torch.autograd.grad(y, inputs, g.cuda())
+    with torch.no_grad():
+        assert torch.equal(m.grouped_linear(inputs[0], inputs[1], by, *inputs[2:]), y)
+    check_grouped(x, w, b, g, members, y, grads)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs,groups", [
+    (1, 1, 1, 1), (1, 1024, 57, 8), (4, 64, 64, 8), (16, 33, 18, 3), (17, 8, 8, 5), (40, 5, 3, 2),
+    (64, 96, 57, 64), (127, 130, 63, 4), (300, 187, 18, 7), (1000, 40, 72, 300),
+    (2500, 264, 136, 6), (1024, 64, 57, 16), (5000, 128, 128, 12), (3000, 260, 300, 2),
+    (200, 1100, 40, 3), (200, 40, 1100, 3), (90, 1030, 1030, 2), (700, 512, 512, 5)])
+def test_grouped_linear(dtype, rows, features, outputs, groups):
+    grouped_case(rows, features, outputs, groups, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_linear_without_bias_and_of_special_groups(dtype):
+    grouped_case(500, 64, 40, 5, dtype, bias=False)
+    none = torch.full((200,), -1)
+    grouped_case(200, 64, 40, 5, dtype, index=none)           # no row has a group
+    grouped_case(200, 64, 40, 5, dtype, index=none + 4)       # one has all
+    grouped_case(3000, 64, 40, 5, dtype, index=torch.arange(3000) % 5)
+    grouped_case(130, 64, 40, 130, dtype, index=torch.arange(130))  # a row each
+    grouped_case(2000, 24, 8, 3000, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_linear_of_rows_that_lie_by_group(dtype):
+    """No order; rows of no group before the first group and behind the last."""
+    m = layers()
+    rows, features, outputs = 700, 48, 40
+    offsets = torch.tensor([30, 30, 200, 455, 455, 690], dtype=torch.int32)
+    x, g = normal(rows, features, seed=1, dtype=dtype), normal(rows, outputs, seed=2, dtype=dtype)
+    w, b = normal(5, outputs, features, seed=3, dtype=dtype), normal(5, outputs, seed=4, dtype=dtype)
+    inputs = [t.cuda().requires_grad_() for t in (x, w, b)]
+    by = m.RowGroups(offsets.cuda())
+    y = m.grouped_linear(inputs[0], inputs[1], by, inputs[2])
+    grads = torch.autograd.grad(y, inputs, g.cuda())
+    members = oracle.members(offsets, None, rows)
+    check_grouped(x, w, b, g, members, y, grads)
+    assert not y[:30].any() and not y[690:].any() and not grads[0][690:].any()
+    # The same through an order, and of a few rows.
+    order = torch.arange(rows, dtype=torch.int32).cuda()
+    again = m.grouped_linear(inputs[0], inputs[1], m.RowGroups(by.offsets, order), inputs[2])
+    assert torch.equal(again, y)
+    few = m.RowGroups(torch.tensor([1, 3, 3, 3, 3, 9], dtype=torch.int32).cuda())
+    got = m.grouped_linear(inputs[0][:10], inputs[1], few, inputs[2])
+    want = oracle.grouped_linear(x[:10], w, oracle.members(few.offsets, None, 10), b)
+    near(got, want, (features + 2) * E * oracle.grouped_linear(
+        x[:10].abs(), w.abs(), oracle.members(few.offsets, None, 10), b.abs()), dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs,groups", [
+    (310_001, 260, 260, 5), (150_000, 300, 40, 40), (60_001, 100, 130, 2000)])
+def test_grouped_linear_of_many_rows_of_whole_numbers(dtype, rows, features, outputs, groups):
+    """Every row counts: sums of small whole numbers stay below 2^24, which
+    float32 holds exactly in any order, so each output is the exact sum,
+    rounded once."""
+    m = layers()
+    gen = torch.Generator(device="cuda").manual_seed(7)
+
+    def whole(*shape):
+        return torch.randint(-2, 3, shape, generator=gen, device="cuda").to(dtype)
+
+    x, g = whole(rows, features).requires_grad_(), whole(rows, outputs)
+    w, b = whole(groups, outputs, features).requires_grad_(), whole(groups, outputs).requires_grad_()
+    index = some_groups(rows, groups, 5, none=0.01).cuda()
+    by = m.row_groups(index, groups)
+    y = m.grouped_linear(x, w, by, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    bounds = by.offsets.tolist()
+    inside = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for group in range(groups):
+        at = by.order[bounds[group]:bounds[group + 1]].long()
+        inside[at] = True
+        part, d, matrix = x[at].detach().double(), g[at].double(), w[group].detach().double()
+        assert torch.equal(y[at], (part @ matrix.t() + b[group].double()).to(dtype))
+        assert torch.equal(dx[at], (d @ matrix).to(dtype))
+        assert torch.equal(dw[group], (d.t() @ part).to(dtype))
+        assert torch.equal(db[group], d.sum(0).to(dtype))
+    assert not y[~inside].any() and not dx[~inside].any()
+
+
+@gpu_test
+def test_grouped_linear_gradients_asked_for_one_by_one():
+    m = layers()
+    index = some_groups(900, 6, 3)
+    by, _ = grouped_by(index, 6)
+    tensors = [normal(900, 40, seed=1), normal(6, 24, 40, seed=2), normal(6, 24, seed=3)]
+    g = normal(900, 24, seed=4).cuda()
+    for groups in (by, m.RowGroups(by.offsets)):
+        every = [t.cuda().requires_grad_() for t in tensors]
+        want = torch.autograd.grad(m.grouped_linear(every[0], every[1], groups, every[2]), every, g)
+        for i in range(3):
+            some = [t.cuda().requires_grad_(j == i) for j, t in enumerate(tensors)]
+            y = m.grouped_linear(some[0], some[1], groups, some[2])
+            (got,) = torch.autograd.grad(y, some[i], g)
+            assert torch.equal(got, want[i])
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_linear_keeps_bad_values_to_their_place(dtype):
+    """A bad row shows in its own outputs and its own group's gradients; a
+    bad row of no group nowhere."""
+    m = layers()
+    index = torch.arange(400) % 4 - 1
+    by, _ = grouped_by(index, 3)
+    x = normal(400, 64, seed=1, dtype=dtype)
+    w, g = normal(3, 32, 64, seed=2, dtype=dtype), normal(400, 32, seed=3, dtype=dtype)
+    outs = []
+    for bad in (False, True):
+        held, grad = x.clone(), g.clone()
+        if bad:
+            held[4], held[8, 3], grad[4] = math.nan, math.inf, math.inf  # rows of no group
+            held[5] = math.nan                                          # of group 0
+        inputs = [t.cuda().requires_grad_() for t in (held, w)]
+        y = m.grouped_linear(*inputs, by)
+        outs.append((y, *torch.autograd.grad(y, inputs, grad.cuda())))
+    (y0, dx0, dw0), (y1, dx1, dw1) = outs
+    rows = torch.arange(400, device="cuda") != 5
+    assert torch.equal(y0[rows], y1[rows]) and y1[5].isnan().all()
+    assert torch.equal(dx0, dx1) and torch.equal(dw0[1:], dw1[1:]) and dw1[0].isnan().all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_linear_shapes_and_strides(dtype):
+    m = layers()
+    base = normal(30, 4, 200, seed=1, dtype=dtype).cuda()
+    w = normal(3, 96, 80, seed=2, dtype=dtype).cuda()
+    for view in (lambda t: t[:, 1, :96], lambda t: t[:, 2, 3:99], lambda t: t[:, :3, 8:104],
+                 lambda t: t.transpose(0, 2)[:96].transpose(0, 1).transpose(1, 2)[..., :96],
+                 lambda t: t[:1, 0, :96].expand(60, 96)):
+        x = view(base)
+        if x.shape[-1] != 96:
+            continue
+        rows = x.numel() // 96
+        by = m.row_groups((torch.arange(rows) % 4 - 1).cuda(), 3)
+        for matrix in (w.transpose(1, 2), w.transpose(1, 2).contiguous()):  # [3, 80, 96]
+            got, want = [], []
+            for source, out in ((x, got), (x.contiguous(), want)):
+                on = source.detach().requires_grad_()
+                weight = matrix.detach().requires_grad_()
+                y = m.grouped_linear(on, weight, by)
+                out += [y, *torch.autograd.grad(y, (on, weight),
+                                                torch.ones(1, dtype=dtype, device="cuda").expand_as(y))]
+            assert got[0].shape == (*x.shape[:-1], 80)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
+@gpu_test
+def test_grouped_linear_of_no_rows():
+    m = layers()
+    x = torch.zeros(0, 8, device="cuda", requires_grad=True)
+    w = torch.ones(3, 4, 8, device="cuda", requires_grad=True)
+    b = torch.ones(3, 4, device="cuda", requires_grad=True)
+    y = m.grouped_linear(x, w, m.row_groups(torch.zeros(0, dtype=torch.int64, device="cuda"), 3), b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == (0, 4) and dx.shape == (0, 8) and not dw.any() and not db.any()
+
+
+@gpu_test
+def test_grouped_linear_refusals():
+    m = layers()
+    x, w = torch.zeros(6, 8, device="cuda"), torch.zeros(3, 4, 8, device="cuda")
+    by = m.row_groups(torch.zeros(6, dtype=torch.int32, device="cuda"), 3)
+    with pytest.raises(TypeError, match="RowGroups"):
+        m.grouped_linear(x, w, by.offsets)
+    for weight in (w[0], w[..., :7], torch.zeros(0, 4, 8, device="cuda")):
+        with pytest.raises(ValueError, match="weight must have shape"):
+            m.grouped_linear(x, weight, by)
+    with pytest.raises(ValueError, match="type of x"):
+        m.grouped_linear(x, w.half(), by)
+    with pytest.raises(ValueError, match="bias must have shape"):
+        m.grouped_linear(x, w, by, torch.zeros(4, device="cuda"))
+    with pytest.raises(ValueError, match="of 3 groups, not 2"):
+        m.grouped_linear(x, w[:2], by)
+    with pytest.raises(ValueError, match="order of 6 rows, x has 5"):
+        m.grouped_linear(x[:5], w, by)
+    with pytest.raises(ValueError, match="groups must be on the device"):
+        m.grouped_linear(x, w, m.RowGroups(by.offsets.cpu(), by.order.cpu()))
+    y = m.grouped_linear(x.requires_grad_(), w, by)
+    (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="grouped_linear is differentiable once"):
+        dx.sum().backward()
