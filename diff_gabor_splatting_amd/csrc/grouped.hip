@@ -234,13 +234,13 @@ struct StepOf {
 struct Share {
   int64_t from, to;  // on the line
   int s, next, end;
+  bool inside;  // whether segment s begins before the share's end
 
   __device__ __forceinline__ void open(const Grouping& g, int segment) {
     s = segment;
-    if (s >= segments_of(g)) {
-      next = end = 0;
-      return;
-    }
+    next = end = 0;
+    inside = s < segments_of(g) && line_at(g, s) < to;
+    if (!inside) return;
     // A row at position i of segment s lies at i + kGroupCost (s + 1).
     const int64_t shift = kGroupCost * (s + 1);
     const int64_t low = begin_of(g, s), high = begin_of(g, s + 1);
@@ -249,10 +249,6 @@ struct Share {
     const bool some = a < b && s > 0 && s <= g.groups;
     next = some ? int(a) : 0;
     end = some ? int(b) : 0;
-  }
-  // Whether segment s begins before the share's end.
-  __device__ __forceinline__ bool inside(const Grouping& g) const {
-    return s < segments_of(g) && line_at(g, s) < to;
   }
 };
 
@@ -273,7 +269,7 @@ __device__ __forceinline__ typename Mma<T>::Fragment row_fragment(const T* lds, 
 }
 
 // A wave's tile: 16 A outputs x 16 B features.
-template <typename T, int A, int B, int Rows>
+template <typename T, int A, int B, int Rows, bool Narrow>
 __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, Grouping g, GroupSum p,
     float* __restrict__ partial, T* __restrict__ dw, T* __restrict__ db) {
@@ -303,14 +299,20 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   at.from = length * share / p.shares;
   at.to = length * (share + 1) / p.shares;
   at.open(g, find_segment(segments_of(g), at.from, [&](int i) { return line_at(g, i); }));
+  // Steps come in pairs, for the two buffers: a group's last may be empty.
+  auto pairs_of = [](const Share& of) { return (of.end - of.next + 2 * Rows - 1) / (2 * Rows); };
   Share ahead_at = at;
-
+  int ahead_steps = 2 * pairs_of(at);
   // The positions of the step after the last that this was called for.
   auto next_step = [&]() {
-    while (ahead_at.next >= ahead_at.end && ahead_at.inside(g)) ahead_at.open(g, ahead_at.s + 1);
+    while (ahead_steps <= 0 && ahead_at.inside) {
+      ahead_at.open(g, ahead_at.s + 1);
+      ahead_steps = 2 * pairs_of(ahead_at);
+    }
     const int left = ahead_at.end - ahead_at.next;
     const StepOf step{ahead_at.next, left < Rows ? left : Rows};
     ahead_at.next += step.count;
+    --ahead_steps;
     return step;
   };
 
@@ -320,6 +322,7 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   const int row_n = threadIdx.x / across_n, column_n = threadIdx.x % across_n * 8;
   const int valid_m = min(p.outputs - m0 - column_m, 8);
   const int valid_n = min(p.features - n0 - column_n, 8);
+  const bool ragged = p.outputs % 8 || p.features % 8;
   const T* const from_m = dy + m0 + column_m;
   const T* const from_n = x + n0 + column_n;
 
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   };
   Load ahead[2];
   Ids ids;
-  auto find = [&]() {
+  auto find = [&](Ids& ids) {
     const StepOf step = next_step();
 #pragma unroll
     for (int i = 0; i < loads_m; ++i) {
@@ -345,15 +348,28 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
     }
   };
   auto send = [&](Load& to) {
+    // Before the rows' own loads: loads come back in their order, so waiting
+    // for these would be waiting for those.
+    Ids next;
+    find(next);
 #pragma unroll
     for (int i = 0; i < loads_m; ++i)
-      to.m[i] = load_valid<T, 8>(from_m + ids.m[i] * p.dy_stride, ids.m[i] >= 0 ? valid_m : 0);
+      to.m[i] = load_edge<T, 8, Narrow>(from_m + ids.m[i] * p.dy_stride,
+                                        ids.m[i] >= 0 ? valid_m : 0);
 #pragma unroll
     for (int i = 0; i < loads_n; ++i)
-      to.n[i] = load_valid<T, 8>(from_n + ids.n[i] * p.x_stride, ids.n[i] >= 0 ? valid_n : 0);
-    find();
+      to.n[i] = load_edge<T, 8, Narrow>(from_n + ids.n[i] * p.x_stride,
+                                        ids.n[i] >= 0 ? valid_n : 0);
+    ids = next;
   };
-  auto put = [&](const Load& from, T* to) {
+  auto settle_all = [&](Load& from) {
+#pragma unroll
+    for (int i = 0; i < loads_m; ++i) from.m[i] = settle<T, 8, Narrow>(from.m[i], valid_m);
+#pragma unroll
+    for (int i = 0; i < loads_n; ++i) from.n[i] = settle<T, 8, Narrow>(from.n[i], valid_n);
+  };
+  auto put = [&](Load& from, T* to) {
+    if (ragged) settle_all(from);
 #pragma unroll
     for (int i = 0; i < loads_m; ++i)
       if (apart_m * loads_m == Rows || row_m + i * apart_m < Rows)
@@ -370,14 +386,6 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   const bool sums = db && n0 == 0;
   f32x4 c[A][B];
   float sum[(A + 3) / 4];  // of the outputs of fragments wave % 4, + 4, ..
-  auto clear = [&]() {
-#pragma unroll
-    for (int i = 0; i < A; ++i)
-#pragma unroll
-      for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < (A + 3) / 4; ++i) sum[i] = 0.f;
-  };
   auto multiply_step = [&](const T* from) {
     constexpr int deep = Mma<T>::step;
 #pragma unroll
@@ -401,95 +409,119 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   };
 
   const int q = lane >> 4, i16 = lane & 15;
-  // Writes the tile of segment at.s and goes on to the next.
+  // Writes the tile of segment at.s.
   auto finish = [&]() __attribute__((always_inline)) {
     const int64_t low = line_at(g, at.s), high = line_at(g, at.s + 1);
     const bool whole = low >= at.from && high <= at.to;
-    const int64_t size = int64_t(p.outputs) * (int64_t(p.features) + 1);
-    float* const mine = partial + (2 * int64_t(share) + (low < at.from ? 0 : 1)) * size;
     const int64_t weights = int64_t(p.outputs) * p.features;
     const bool group = at.s > 0 && at.s <= g.groups;
+    float* const part =
+        partial + (2 * int64_t(share) + (low < at.from ? 0 : 1)) * (weights + p.outputs);
+    // The tile's corner; a lane's place from there on.
+    const int64_t corner = (m0 + wave_m) * int64_t(p.features) + n0 + wave_n;
+    float* const to_part = part + corner;
+    T* const to_dw = dw + ((at.s - 1) * weights + corner);
+    const uint32_t place = uint32_t(i16) * p.features + 4 * q;
+    const int rows_left = group ? p.outputs - m0 - wave_m - i16 : 0;
+    const int columns_left = p.features - n0 - wave_n - 4 * q;
 #pragma unroll
     for (int i = 0; i < A; ++i) {
-      const int m = m0 + wave_m + 16 * i + i16;
-      float total = sum[i / 4];
-      if (sums && (wave & 3) == (i & 3)) {
-        total += __shfl_xor(total, 16);
-        total += __shfl_xor(total, 32);
-      }
-      if (!group || m >= p.outputs) continue;
       // Lane 16 q + i holds features 4 q .. 4 q + 3 of output i of a fragment.
+      if (rows_left > 16 * i && (!whole || dw)) {
 #pragma unroll
-      for (int j = 0; j < B; ++j) {
-        const int n = n0 + wave_n + 16 * j + 4 * q;
-        const int valid = min(p.features - n, 4);
-        if (!whole) {
-          store_valid<float, 4>(mine + int64_t(m) * p.features + n, valid, c[i][j]);
-        } else if (dw) {
+        for (int j = 0; j < B; ++j) {
+          const uint32_t to = place + uint32_t(16 * i) * p.features + 16 * j;
           const vec<T, 4> v = {T(c[i][j][0]), T(c[i][j][1]), T(c[i][j][2]), T(c[i][j][3])};
-          store_valid<T, 4>(dw + (at.s - 1) * weights + int64_t(m) * p.features + n, valid, v);
+          if (columns_left >= 16 * j + 4) {
+            if (whole)
+              store_packed<T, 4>(to_dw + to, v);
+            else
+              store_packed<float, 4>(to_part + to, c[i][j]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 3; ++h)
+              if (columns_left > 16 * j + h) {
+                if (whole)
+                  to_dw[to + h] = v[h];
+                else
+                  to_part[to + h] = c[i][j][h];
+              }
+          }
         }
       }
-      if (sums && (wave & 3) == (i & 3) && q == 0) {
-        if (whole)
-          db[(at.s - 1) * int64_t(p.outputs) + m] = T(total);
-        else
-          mine[weights + m] = total;
+      if (sums && (wave & 3) == (i & 3)) {
+        float total = sum[i / 4];
+        total += __shfl_xor(total, 16);
+        total += __shfl_xor(total, 32);
+        const int m = m0 + wave_m + 16 * i + i16;
+        if (rows_left > 16 * i && q == 0) {
+          if (whole)
+            db[(at.s - 1) * int64_t(p.outputs) + m] = T(total);
+          else
+            part[weights + m] = total;
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);  // or all places are held at once
     }
-    clear();
-    at.open(g, at.s + 1);
   };
-  // Whether a step is left; segments without another row in this share are
-  // finished on the way.
-  auto more = [&]() __attribute__((always_inline)) {
-    while (at.next >= at.end && at.inside(g)) finish();
-    return at.inside(g);
-  };
-
-  clear();
-  find();
+  find(ids);
   send(ahead[0]);
   send(ahead[1]);
   put(ahead[0], lds);
   send(ahead[0]);
   __syncthreads();
-  while (more()) {
-    put(ahead[1], lds + buffer);
-    send(ahead[1]);
-    multiply_step(lds);
-    at.next += min(at.end - at.next, Rows);
-    __syncthreads();
-    if (!more()) return;
-    put(ahead[0], lds);
-    send(ahead[0]);
-    multiply_step(lds + buffer);
-    at.next += min(at.end - at.next, Rows);
-    __syncthreads();
+  for (; at.inside; at.open(g, at.s + 1)) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < (A + 3) / 4; ++i) sum[i] = 0.f;
+    for (int pair = pairs_of(at); pair; --pair) {
+      put(ahead[1], lds + buffer);
+      send(ahead[1]);
+      multiply_step(lds);
+      __syncthreads();
+      put(ahead[0], lds);
+      send(ahead[0]);
+      multiply_step(lds + buffer);
+      __syncthreads();
+    }
+    finish();
   }
 }
 
-// Adds the parts of the groups that lie in several shares. blockIdx.y: the
-// border between two shares that is the first within its group; blockIdx.x:
+// Adds the parts of the groups that lie in several shares. blockIdx.y: a
+// group, or where there are fewer borders between shares than groups a border,
+// which stands for the group that it is the first border within; blockIdx.x:
 // kThreads / Slices values of dW and db at a time, for which each slice of
 // the threads adds every Slices-th part.
 template <typename T, int Slices>
 __global__ __launch_bounds__(kThreads) void group_join_kernel(const float* __restrict__ partial,
                                                               Grouping g, GroupSum p,
-                                                              T* __restrict__ dw,
+                                                              bool by_border, T* __restrict__ dw,
                                                               T* __restrict__ db) {
   constexpr int columns = kThreads / Slices;
   __shared__ float sums[Slices][columns];
   const int64_t length = line_length(g);
-  const int border = blockIdx.y + 1;
-  const int64_t v = length * border / p.shares;
-  const int s = find_segment(segments_of(g), v, [&](int i) { return line_at(g, i); });
+  int s = blockIdx.y + 1;
+  int64_t border = s;
+  if (by_border)
+    s = find_segment(segments_of(g), length * border / p.shares,
+                     [&](int i) { return line_at(g, i); });
   const int64_t low = line_at(g, s), high = line_at(g, s + 1);
-  if (s < 1 || s > g.groups || v <= low || length * (border - 1) / p.shares > low) return;
+  if (!by_border) {  // the first border behind `low`
+    border = low * p.shares / length;
+    while (length * border / p.shares <= low) ++border;
+  }
+  const int64_t v = length * border / p.shares;
+  if (s < 1 || s > g.groups || border >= p.shares || v <= low || v >= high ||
+      length * (border - 1) / p.shares > low)
+    return;
   // Shares border - 1 (its tail) .. last (their heads).
-  int last = border;
+  int64_t last = border;
   while (last + 1 < p.shares && length * (last + 1) / p.shares < high) ++last;
-  const int count = last - border + 2;
+  const int count = int(last - border) + 2;
   const int64_t weights = int64_t(p.outputs) * p.features, size = weights + p.outputs;
   const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
   for (int64_t first = int64_t(blockIdx.x) * columns; first < size;
@@ -499,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void group_join_kernel(const float* __res
     if (i < size) {
 #pragma unroll 8
       for (int j = slice; j < count; j += Slices)
-        sum += partial[(j ? 2 * int64_t(border - 1 + j) : 2 * int64_t(border) - 1) * size + i];
+        sum += partial[(j ? 2 * (border - 1 + j) : 2 * border - 1) * size + i];
     }
     if constexpr (Slices > 1) {
       sums[slice][column] = sum;
@@ -653,10 +685,10 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     T* const dw = static_cast<T*>(grad_weight);
     T* const db = static_cast<T*>(grad_bias);
     float* const partial = static_cast<float*>(workspace);
-    auto launch = [&](auto a, auto b) {
+    auto launch = [&](auto a, auto b, auto narrow) {
       constexpr int step = a.value == 2 ? 64 : 32;
       constexpr size_t lds = 2 * step * (32 * a.value + 16 + 64 * b.value + 16) * sizeof(T);
-      auto* const kernel = &group_sum_kernel<T, a.value, b.value, step>;
+      auto* const kernel = &group_sum_kernel<T, a.value, b.value, step, narrow.value>;
       GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
       kernel<<<dim3{unsigned(blocks)}, kSumThreads, lds, s>>>(
           static_cast<const T*>(grad_y), static_cast<const T*>(x), g, p, partial, dw, db);
@@ -668,18 +700,30 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     using two = integral_constant<int, 2>;
     using four = integral_constant<int, 4>;
     const int shape = plan.a * 10 + plan.b;
-    if (shape == 21) GS_CHECK(launch(two{}, one{}));
-    if (shape == 22) GS_CHECK(launch(two{}, two{}));
-    if (shape == 41) GS_CHECK(launch(four{}, one{}));
-    if (shape == 42) GS_CHECK(launch(four{}, two{}));
+    // Rows of fewer than eight values have no place to load eight from.
+    const bool few = outputs < 8 || features < 8;
+    using wide = std::false_type;
+    using narrow = std::true_type;
+    if (shape == 21) GS_CHECK(few ? launch(two{}, one{}, narrow{}) : launch(two{}, one{}, wide{}));
+    if (shape == 22) GS_CHECK(few ? launch(two{}, two{}, narrow{}) : launch(two{}, two{}, wide{}));
+    if (shape == 41)
+      GS_CHECK(few ? launch(four{}, one{}, narrow{}) : launch(four{}, one{}, wide{}));
+    if (shape == 42) GS_CHECK(launch(four{}, two{}, wide{}));
     if constexpr (sizeof(T) == 2)
-      if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}));
+      if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}, wide{}));
     if (plan.shares == 1) return int(GS_OK);
     const int64_t size = outputs * (features + 1);
     auto join = [&](auto slices) {
-      const dim3 grid{unsigned(std::min<int64_t>(ceil_div(size, kThreads / slices.value), 1 << 14)),
-                      unsigned(plan.shares - 1)};
-      group_join_kernel<T, slices.value><<<grid, kThreads, 0, s>>>(partial, g, p, dw, db);
+      // Workgroups go on to further values: those of the groups that lie in
+      // one share have nothing to do, and a workgroup to each 64 values and
+      // border (100k x 256 -> 256 in 64 groups: 32,000) took 180 us to find
+      // that out.
+      const bool by_border = plan.shares - 1 < groups;
+      const int64_t each = by_border ? plan.shares - 1 : groups;
+      const int64_t chunks = ceil_div(size, kThreads / slices.value);
+      const dim3 grid{unsigned(std::min(chunks, ceil_div(4096, each))), unsigned(each)};
+      group_join_kernel<T, slices.value><<<grid, kThreads, 0, s>>>(partial, g, p, by_border, dw,
+                                                                  db);
     };
     size >= 512 * kThreads ? join(one{}) : join(four{});
     GS_LAUNCHED("group_join_kernel");
