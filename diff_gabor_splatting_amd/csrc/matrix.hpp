@@ -239,6 +239,25 @@ inline int64_t steps_of(size_t size, int64_t k) {
 }
 
 
+// Rows of a wave's tile, and fragments side by side of a panel of the matrix:
+// the widest panel that its k leaves room for in LDS, no wider than the
+// columns of C ask for, at least 128 bytes of a row of C; 0 where that does
+// not fit. With few rows, narrower ones, while that gives more workgroups (up
+// to one per compute unit) less to put in place.
+constexpr int kRowTile = 32;
+inline int panel_fragments(size_t size, int64_t rows, int64_t k, int64_t n) {
+  const int least = size == 4 ? 2 : 4;
+  int fragments = 8;
+  while (fragments >= least && steps_of(size, k) * 2048 * fragments > int64_t(kRowLds))
+    fragments /= 2;
+  if (fragments < least) return 0;
+  const int64_t tiles = ceil_div(rows, kRowTile);
+  while (fragments > least &&
+         (n <= 8 * fragments || tiles * ceil_div(n, 8 * fragments) <= 256))
+    fragments /= 2;
+  return fragments;
+}
+
 // --------------------------------------------------------------------------
 // Sums over rows
 
