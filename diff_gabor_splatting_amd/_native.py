@@ -269,6 +269,23 @@ _SIGNATURES = {
         [_c_int, _c_ptr, _c_i64, _c_ptr, _c_i64] + [_c_ptr] * 2 + [_c_i64] * 4 + [_c_ptr] * 3
         + [_c_size, _c_ptr],
     ),
+    "gs_adapted_linear_inner_size": (_c_size, [_c_i64] * 2),
+    "gs_adapted_linear_forward": (
+        _c_int,
+        [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 4 + [_c_float] + [_c_ptr] * 2 + [_c_i64] * 5
+        + [_c_ptr, _c_size] + [_c_ptr] * 2,
+    ),
+    "gs_adapted_linear_backward_input": (
+        _c_int,
+        [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 3 + [_c_float] + [_c_ptr] * 2 + [_c_i64] * 5
+        + [_c_ptr, _c_size] + [_c_ptr] * 2,
+    ),
+    "gs_adapted_linear_backward_adapters_workspace_size": (_c_size, [_c_i64] * 5),
+    "gs_adapted_linear_backward_adapters": (
+        _c_int,
+        [_c_int, _c_ptr, _c_i64, _c_ptr, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 5 + [_c_ptr] * 3
+        + [_c_size, _c_ptr],
+    ),
 }
 
 PROFILE_FAMILIES = {

@@ -1,0 +1,420 @@
+// Linear layers that all rows share, with a low-rank adapter of the row's
+// group beside them: y_i = W x_i + b + s B_g A_g x_i for the rows i of group g, and
+// the gradients dx_i = W^T dy_i + s A_g^T B_g^T dy_i, dA_g = s sum (B_g^T dy_i) x_i^T,
+// dB_g = s sum dy_i (A_g x_i)^T. Rows of no group have the shared layer alone.
+//
+// The inner rows, s A_g x_i and s B_g^T dy_i, are the sums that the other products
+// share: each is computed once, kept (see Inner) and met again by the product
+// with the other narrow matrix, in the accumulators of the wide one, and by
+// the narrow matrices' gradients.
+//
+//   few_inner_kernel, few_adapted_kernel  the forward pass of a few rows
+//   group_tile_kernel  inner rows; y and dx
+//   narrow_sum_kernel  dA and dB, a wave to 128 columns of a share of the rows
+#include "group_sums.hpp"
+#include "group_tile.hpp"
+
+namespace gs {
+namespace {
+
+// --------------------------------------------------------------------------
+// y of a few rows: a workgroup to an inner row, then a wave to an output.
+
+constexpr int kFewRows = 16;
+
+// The sum over k of a[k] b[k], in every lane of the wave.
+template <typename T>
+__device__ __forceinline__ float wave_dot(const T* a, const T* b, int k) {
+  const int lane = threadIdx.x & 63;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = lane * kChunk; c < k; c += 64 * kChunk) {
+    const int valid = min(k - c, kChunk);
+    float u[kChunk], v[kChunk];
+    load8<T>(a + c, valid, u);
+    load8<T>(b + c, valid, v);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) sum = __builtin_fmaf(u[j], v[j], sum);
+  }
+#pragma unroll
+  for (int step = 32; step; step >>= 1) sum += __shfl_xor(sum, step);
+  return sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void few_inner_kernel(const T* __restrict__ x,
+                                                             int64_t stride,
+                                                             const T* __restrict__ down,
+                                                             float scale, Grouping g, int k,
+                                                             Inner<T> inner) {
+  __shared__ float values[kMostRank];
+  const int position = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int s = find_segment(segments_of(g), position,
+                             [&](int i) { return int64_t(begin_of(g, i)); });
+  const bool member = s > 0 && s <= g.groups;
+  if (threadIdx.x < kMostRank) values[threadIdx.x] = 0.f;
+  __syncthreads();
+  if (member) {
+    const T* const row = x + row_at(g, position) * stride;
+    const T* const matrix = down + int64_t(s - 1) * inner.rank * k;
+    for (int r = wave; r < inner.rank; r += kThreads / 64) {
+      const float sum = wave_dot<T>(row, matrix + int64_t(r) * k, k);
+      if (lane == 0) values[r] = scale * sum;
+    }
+  }
+  __syncthreads();
+  if (wave) return;
+  float most = finite_size(values[lane]);
+#pragma unroll
+  for (int step = 32; step; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
+  const float up = inner.begin_row(position, most, member ? s - 1 : -1, lane == 0);
+  if (4 * lane >= 32 * inner.chunks()) return;
+  const float four[4] = {values[4 * lane], values[4 * lane + 1], values[4 * lane + 2],
+                         values[4 * lane + 3]};
+  inner.template put<4>(position, 4 * lane, four, up);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void few_adapted_kernel(
+    const T* __restrict__ x, int64_t stride, const T* __restrict__ w, const T* __restrict__ bias,
+    const T* __restrict__ up, Grouping g, int k, int n, Inner<T> inner, T* __restrict__ y) {
+  const int lane = threadIdx.x & 63, position = blockIdx.y;
+  const int output = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (output >= n) return;
+  const int64_t row = row_at(g, position);
+  const int group = inner.groups[position];
+  // The narrow sum: a value of the rank to a lane.
+  float narrow = 0.f;
+  if (group >= 0 && lane < inner.rank)
+    narrow = inner.get(position, lane) *
+             float(up[(int64_t(group) * n + output) * inner.rank + lane]);
+#pragma unroll
+  for (int step = 32; step; step >>= 1) narrow += __shfl_xor(narrow, step);
+  float sum = wave_dot<T>(x + row * stride, w + int64_t(output) * k, k) + narrow;
+  if (bias) sum += float(bias[output]);
+  if (lane == 0) y[row * n + output] = T(sum);
+}
+
+// --------------------------------------------------------------------------
+// Inner rows, y and dx by tiles
+
+template <typename T, bool NContiguous, int Mode>
+int launch_tiles(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
+                 const Grouping& g, int64_t k, int64_t n, const Adapters<T>& adapters, void* out,
+                 hipStream_t stream) {
+  const GroupProduct p{n, k, ceil_div(n, kEdge), stride};
+  const int64_t blocks = tile_numbers(g) * p.tiles_n;
+  GS_REQUIRE(blocks < (int64_t(1) << 32) / kThreads, GS_ERR_OVERFLOW, "%s: too many rows", name);
+  group_tile_kernel<T, NContiguous, Mode><<<dim3{unsigned(blocks)}, kThreads, 0, stream>>>(
+      static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), g, p,
+      adapters, static_cast<T*>(out));
+  GS_LAUNCHED(name);
+  return GS_OK;
+}
+
+// --------------------------------------------------------------------------
+// dA and dB: the sums over each group's rows of inner^T rows, [rank, width].
+//
+// A wave takes 128 columns (eight to each of 16 lanes) and four rows at a
+// time (one to each lane group), which is how memory holds them and how the
+// float32 matrix instruction takes them: no LDS, no turning, and products of
+// float32 inner values as they are. Waves share nothing; each has its own
+// share of the rows. The instruction's rate is the reading's at a rank of 16
+// and half of it at 64.
+
+constexpr int64_t kNarrowCost = 32;  // of a group's sums, in rows
+constexpr int kNarrowColumns = 128;
+constexpr int kNarrowRows = 16;  // of a step
+
+struct NarrowSum {
+  int64_t stride;
+  int width, blocks, shares;
+};
+
+// Turned: the result is [width, rank] (dB), not [rank, width] (dA). R: 16s of
+// the rank.
+template <typename T, int R, bool Turned, bool Narrow>
+__global__ __launch_bounds__(kThreads) void narrow_sum_kernel(Inner<T> inner,
+                                                              const T* __restrict__ rows,
+                                                              Grouping g, NarrowSum p,
+                                                              float* __restrict__ partial,
+                                                              T* __restrict__ out) {
+  constexpr int steps = kNarrowRows / 4;
+  const int64_t number = int64_t(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  const int block = __builtin_amdgcn_readfirstlane(int(number % p.blocks));
+  const int share = __builtin_amdgcn_readfirstlane(int(number / p.blocks));
+  if (share >= p.shares) return;
+  const int lane = threadIdx.x & 63, q = lane >> 4, i16 = lane & 15;
+  const int column = block * kNarrowColumns + 8 * i16;
+  const int valid = max(0, min(p.width - column, 8));
+  const int64_t length = line_length(g, kNarrowCost);
+  Share at{kNarrowCost};
+  at.from = length * share / p.shares;
+  at.to = length * (share + 1) / p.shares;
+  at.open(g, find_segment(segments_of(g), at.from,
+                          [&](int i) { return line_at(g, kNarrowCost, i); }));
+  const int64_t size = int64_t(inner.rank) * p.width;
+  for (; at.inside; at.open(g, at.s + 1)) {
+    f32x4 c[R][8];
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int64_t id[steps];
+    auto find = [&](int first) {
+#pragma unroll
+      for (int i = 0; i < steps; ++i) id[i] = row_at(g, min(first + 4 * i + q, at.end - 1));
+    };
+    if (at.next < at.end) find(at.next);
+    for (int first = at.next; first < at.end; first += kNarrowRows) {
+      vec<T, 8> raw[steps];
+      float a[steps][R];
+#pragma unroll
+      for (int i = 0; i < steps; ++i) {
+        const int position = first + 4 * i + q;
+        const bool live = position < at.end;
+        raw[i] = load_edge<T, 8, Narrow>(rows + id[i] * p.stride + column, live ? valid : 0);
+#pragma unroll
+        for (int t = 0; t < R; ++t) a[i][t] = live ? inner.get(position, 16 * t + i16) : 0.f;
+      }
+      if (first + kNarrowRows < at.end) find(first + kNarrowRows);
+#pragma unroll
+      for (int i = 0; i < steps; ++i) {
+        const bool live = first + 4 * i + q < at.end;
+        const vec<T, 8> v = settle<T, 8, Narrow>(raw[i], live ? valid : 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int t = 0; t < R; ++t)
+            c[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][t], float(v[j]), c[t][j], 0, 0, 0);
+      }
+    }
+    // Lane 16 q + i holds ranks 16 t + 4 q .. + 3 of columns 8 i .. 8 i + 7.
+    if (at.s < 1 || at.s > g.groups) continue;
+    const int64_t low = line_at(g, kNarrowCost, at.s), high = line_at(g, kNarrowCost, at.s + 1);
+    const bool whole = low >= at.from && high <= at.to;
+    float* const part = partial + (2 * int64_t(share) + (low < at.from ? 0 : 1)) * size;
+    T* const to = out + (at.s - 1) * size;
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      const int r0 = 16 * t + 4 * q;
+      if constexpr (Turned) {
+        const int left = max(0, min(inner.rank - r0, 4));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= valid) continue;
+          const int64_t place = int64_t(column + j) * inner.rank + r0;
+          if (whole)
+            store_valid<T, 4>(to + place, left, vec<T, 4>{T(c[t][j][0]), T(c[t][j][1]),
+                                                          T(c[t][j][2]), T(c[t][j][3])});
+          else
+            store_valid<float, 4>(part + place, left, c[t][j]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r0 + r >= inner.rank) continue;
+          const int64_t place = int64_t(r0 + r) * p.width + column;
+          const float v[8] = {c[t][0][r], c[t][1][r], c[t][2][r], c[t][3][r],
+                              c[t][4][r], c[t][5][r], c[t][6][r], c[t][7][r]};
+          if (whole)
+            store8<T>(to + place, valid, v);
+          else
+            store8<float>(part + place, valid, v);
+        }
+      }
+    }
+  }
+}
+
+// 4,096 waves: as many as the chip holds at a rank of 32, two rounds at 64.
+int64_t narrow_shares(const Grouping& g, int64_t width) {
+  const int64_t shares = std::max<int64_t>(1, 4096 / ceil_div(width, kNarrowColumns));
+  return std::min(shares, ceil_div(line_length(g, kNarrowCost), 2 * kNarrowCost));
+}
+
+template <typename T, bool Turned>
+int launch_narrow(const char* name, const Inner<T>& inner, const void* rows, int64_t stride,
+                  const Grouping& g, int64_t width, float* partial, void* out,
+                  hipStream_t stream) {
+  const NarrowSum p{stride, int(width), int(ceil_div(width, kNarrowColumns)),
+                    int(narrow_shares(g, width))};
+  const dim3 grid{unsigned(ceil_div(int64_t(p.blocks) * p.shares, kThreads / 64))};
+  auto launch = [&](auto r, auto narrow) {
+    narrow_sum_kernel<T, r.value, Turned, narrow.value><<<grid, kThreads, 0, stream>>>(
+        inner, static_cast<const T*>(rows), g, p, partial, static_cast<T*>(out));
+  };
+  auto by_width = [&](auto r) {
+    width < 8 ? launch(r, std::true_type{}) : launch(r, std::false_type{});
+  };
+  if (inner.rank <= 16)
+    by_width(std::integral_constant<int, 1>{});
+  else if (inner.rank <= 32)
+    by_width(std::integral_constant<int, 2>{});
+  else
+    by_width(std::integral_constant<int, 4>{});
+  GS_LAUNCHED(name);
+  return launch_join(partial, g, kNarrowCost, p.shares, inner.rank * width, 0,
+                     static_cast<T*>(out), static_cast<T*>(nullptr), stream);
+}
+
+int check_adapted(const char* name, int32_t dtype, const void* offsets, int64_t rows,
+                  int64_t groups, int64_t features, int64_t outputs, int64_t rank) {
+  GS_CHECK(check_grouping(name, offsets, rows, groups));
+  GS_CHECK(check_rows(name, dtype, rows, features, features));
+  GS_CHECK(check_rows(name, dtype, rows, outputs, outputs));
+  GS_REQUIRE(outputs <= kMostFeatures / 64 && features <= kMostFeatures / 64, GS_ERR_ARGUMENT,
+             "%s: at most %lld features and outputs", name, (long long)(kMostFeatures / 64));
+  GS_REQUIRE(rank >= 1 && rank <= kMostRank, GS_ERR_ARGUMENT, "%s: rank must be 1 through %d",
+             name, kMostRank);
+  return GS_OK;
+}
+
+int check_inner(const char* name, const void* inner, size_t bytes, int64_t rows, int64_t rank) {
+  GS_REQUIRE(inner && bytes >= Inner<float>::bytes(rows, rank), GS_ERR_WORKSPACE,
+             "inner rows too small for %s", name);
+  return GS_OK;
+}
+
+Grouping grouping(const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups) {
+  return {order, offsets, int32_t(rows), int32_t(groups)};
+}
+
+}  // namespace
+}  // namespace gs
+
+extern "C" {
+
+size_t gs_adapted_linear_inner_size(int64_t rows, int64_t rank) {
+  using namespace gs;
+  if (rows <= 0 || rank <= 0 || rank > kMostRank) return 0;
+  return Inner<float>::bytes(rows, rank);
+}
+
+int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const void* weight,
+                              const void* bias, const void* down, const void* up, float scale,
+                              const int32_t* order, const int32_t* offsets, int64_t rows,
+                              int64_t groups, int64_t features, int64_t outputs, int64_t rank,
+                              void* inner, size_t inner_bytes, void* y, void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_adapted_linear_forward";
+  GS_CHECK(check_adapted(name, dtype, offsets, rows, groups, features, outputs, rank));
+  GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
+  GS_REQUIRE(std::isfinite(scale), GS_ERR_ARGUMENT, "%s: scale must be finite", name);
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && weight && down && up && y, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  GS_CHECK(check_inner(name, inner, inner_bytes, rows, rank));
+  const Grouping g = grouping(order, offsets, rows, groups);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const Inner<T> held = Inner<T>::at(inner, rows, rank);
+    if (rows <= kFewRows) {
+      few_inner_kernel<T><<<dim3{unsigned(rows)}, kThreads, 0, s>>>(
+          static_cast<const T*>(x), row_stride, static_cast<const T*>(down), scale, g,
+          int(features), held);
+      GS_LAUNCHED(name);
+      const dim3 grid{unsigned(ceil_div(outputs, kThreads / 64)), unsigned(rows)};
+      few_adapted_kernel<T><<<grid, kThreads, 0, s>>>(
+          static_cast<const T*>(x), row_stride, static_cast<const T*>(weight),
+          static_cast<const T*>(bias), static_cast<const T*>(up), g, int(features), int(outputs),
+          held, static_cast<T*>(y));
+      GS_LAUNCHED(name);
+      return int(GS_OK);
+    }
+    GS_CHECK((launch_tiles<T, true, kInner>(name, x, row_stride, down, nullptr, g, features, rank,
+                                            Adapters<T>{held, nullptr, scale}, nullptr, s)));
+    return launch_tiles<T, true, kAdapted>(
+        name, x, row_stride, weight, bias, g, features, outputs,
+        Adapters<T>{held, static_cast<const T*>(up), 0.f}, y, s);
+  });
+}
+
+int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                     const void* weight, const void* down, const void* up,
+                                     float scale, const int32_t* order, const int32_t* offsets,
+                                     int64_t rows, int64_t groups, int64_t features,
+                                     int64_t outputs, int64_t rank, void* inner_grad,
+                                     size_t inner_bytes, void* grad_x, void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_adapted_linear_backward_input";
+  GS_CHECK(check_adapted(name, dtype, offsets, rows, groups, features, outputs, rank));
+  GS_CHECK(check_rows(name, dtype, rows, outputs, grad_stride));
+  GS_REQUIRE(std::isfinite(scale), GS_ERR_ARGUMENT, "%s: scale must be finite", name);
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(grad_y && up && (!grad_x || (weight && down)), GS_ERR_ARGUMENT,
+             "null pointer passed to %s", name);
+  GS_CHECK(check_inner(name, inner_grad, inner_bytes, rows, rank));
+  const Grouping g = grouping(order, offsets, rows, groups);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const Inner<T> held = Inner<T>::at(inner_grad, rows, rank);
+    GS_CHECK((launch_tiles<T, false, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
+                                             rank, Adapters<T>{held, nullptr, scale}, nullptr,
+                                             s)));
+    if (!grad_x) return int(GS_OK);
+    return launch_tiles<T, false, kAdapted>(
+        name, grad_y, grad_stride, weight, nullptr, g, outputs, features,
+        Adapters<T>{held, static_cast<const T*>(down), 0.f}, grad_x, s);
+  });
+}
+
+size_t gs_adapted_linear_backward_adapters_workspace_size(int64_t rows, int64_t groups,
+                                                          int64_t features, int64_t outputs,
+                                                          int64_t rank) {
+  using namespace gs;
+  if (rows < 0 || rows > kMostGroupedRows || groups <= 0 || groups > kMostGroupsOfRows ||
+      features <= 0 || outputs <= 0 || rank <= 0 || rank > kMostRank)
+    return 0;
+  const Grouping g = grouping(nullptr, nullptr, rows, groups);
+  auto bytes = [&](int64_t width) {
+    const int64_t shares = narrow_shares(g, width);
+    return shares == 1 ? 0 : size_t(2 * shares) * size_t(rank * width) * sizeof(float);
+  };
+  return std::max(bytes(features), bytes(outputs));
+}
+
+int gs_adapted_linear_backward_adapters(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                        const void* x, int64_t row_stride, const void* inner,
+                                        const void* inner_grad, const int32_t* order,
+                                        const int32_t* offsets, int64_t rows, int64_t groups,
+                                        int64_t features, int64_t outputs, int64_t rank,
+                                        void* grad_down, void* grad_up, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  using namespace gs;
+  clear_error();
+  const char* const name = "gs_adapted_linear_backward_adapters";
+  GS_CHECK(check_adapted(name, dtype, offsets, rows, groups, features, outputs, rank));
+  if (!grad_down && !grad_up) return GS_OK;
+  GS_REQUIRE(offsets, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  if (grad_down) {
+    GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
+    GS_REQUIRE(rows == 0 || (x && inner_grad), GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  }
+  if (grad_up) {
+    GS_CHECK(check_rows(name, dtype, rows, outputs, grad_stride));
+    GS_REQUIRE(rows == 0 || (grad_y && inner), GS_ERR_ARGUMENT, "null pointer passed to %s", name);
+  }
+  const size_t need =
+      gs_adapted_linear_backward_adapters_workspace_size(rows, groups, features, outputs, rank);
+  GS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), GS_ERR_WORKSPACE,
+             "workspace too small for %s", name);
+  const Grouping g = grouping(order, offsets, rows, groups);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  float* const partial = static_cast<float*>(workspace);
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    if (grad_down)
+      GS_CHECK((launch_narrow<T, false>(name, Inner<T>::at(const_cast<void*>(inner_grad), rows, rank),
+                                        x, row_stride, g, features, partial, grad_down, s)));
+    if (grad_up)
+      GS_CHECK((launch_narrow<T, true>(name, Inner<T>::at(const_cast<void*>(inner), rows, rank),
+                                       grad_y, grad_stride, g, outputs, partial, grad_up, s)));
+    return int(GS_OK);
+  });
+}
+
+}  // extern "C"

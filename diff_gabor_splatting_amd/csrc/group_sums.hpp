@@ -1,0 +1,145 @@
+// Sums over each group's rows, cut into shares that go by the rows and not by
+// the groups.
+//
+// Shares are cut from the line on which each segment takes `cost` + its rows,
+// so that what a group costs beside its rows counts too. A group whose part of
+// the line lies in one share is written by that share; the others' parts go to
+// two places that each share has, its head (the group began before it) and its
+// tail, and group_join_kernel adds them in their order. No atomics: results do not
+// depend on timing.
+#pragma once
+
+#include "groups.hpp"
+#include "kept8.hpp"
+
+namespace gs {
+
+__device__ __forceinline__ int64_t line_at(const Grouping& g, int64_t cost, int s) {
+  return begin_of(g, s) + cost * s;
+}
+__host__ __device__ __forceinline__ int64_t line_length(const Grouping& g, int64_t cost) {
+  return g.rows + cost * (int64_t(g.groups) + 2);
+}
+
+// Where a share stands: segment s, whose positions from `next` to `end` are its.
+struct Share {
+  int64_t cost;
+  int64_t from, to;  // on the line
+  int s, next, end;
+  bool inside;  // whether segment s begins before the share's end
+
+  __device__ __forceinline__ void open(const Grouping& g, int segment) {
+    s = segment;
+    next = end = 0;
+    inside = s < segments_of(g) && line_at(g, cost, s) < to;
+    if (!inside) return;
+    // A row at position i of segment s lies at i + cost (s + 1).
+    const int64_t shift = cost * (s + 1);
+    const int64_t low = begin_of(g, s), high = begin_of(g, s + 1);
+    const int64_t a = from - shift > low ? from - shift : low;
+    const int64_t b = to - shift < high ? to - shift : high;
+    const bool some = a < b && s > 0 && s <= g.groups;
+    next = some ? int(a) : 0;
+    end = some ? int(b) : 0;
+  }
+};
+
+// --------------------------------------------------------------------------
+
+constexpr int kJoinThreads = 256;
+
+struct JoinOf {
+  int64_t cost, shares;
+  int64_t weights, biases;  // values of a group: dW's, then db's
+  bool by_border;
+};
+
+// Adds the parts of the groups that lie in several shares. blockIdx.y: a
+// group, or where there are fewer borders between shares than groups a border,
+// which stands for the group that it is the first border within; blockIdx.x:
+// 4 kJoinThreads / Slices values of dW and db at a time, for which each slice of
+// the threads adds every Slices-th part.
+template <typename T, int Slices>
+__global__ __launch_bounds__(kJoinThreads) void group_join_kernel(const float* __restrict__ partial,
+                                                              Grouping g, JoinOf p,
+                                                              T* __restrict__ dw,
+                                                              T* __restrict__ db) {
+  constexpr int columns = kJoinThreads / Slices;
+  __shared__ vec<float, 4> sums[Slices][columns];
+  const int64_t length = line_length(g, p.cost);
+  int s = blockIdx.y + 1;
+  int64_t border = s;
+  if (p.by_border)
+    s = find_segment(segments_of(g), length * border / p.shares,
+                     [&](int i) { return line_at(g, p.cost, i); });
+  const int64_t low = line_at(g, p.cost, s), high = line_at(g, p.cost, s + 1);
+  if (!p.by_border) {  // the first border behind `low`
+    border = low * p.shares / length;
+    while (length * border / p.shares <= low) ++border;
+  }
+  const int64_t v = length * border / p.shares;
+  if (s < 1 || s > g.groups || border >= p.shares || v <= low || v >= high ||
+      length * (border - 1) / p.shares > low)
+    return;
+  // Shares border - 1 (its tail) .. last (their heads).
+  int64_t last = border;
+  while (last + 1 < p.shares && length * (last + 1) / p.shares < high) ++last;
+  const int count = int(last - border) + 2;
+  const int64_t weights = p.weights, size = weights + p.biases;
+  const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
+  for (int64_t first = int64_t(blockIdx.x) * 4 * columns; first < size;
+       first += int64_t(gridDim.x) * 4 * columns) {
+    const int64_t i = first + 4 * column;
+    const int valid = int(size - i < 4 ? size - i : 4);
+    vec<float, 4> sum = 0.f;
+#pragma unroll 8
+    for (int j = slice; j < count; j += Slices)
+      sum += load_valid<float, 4>(partial + (j ? 2 * (border - 1 + j) : 2 * border - 1) * size + i,
+                                  valid);
+    if constexpr (Slices > 1) {
+      sums[slice][column] = sum;
+      __syncthreads();
+      if (slice == 0)
+        for (int j = 1; j < Slices; ++j) sum += sums[j][column];
+      __syncthreads();
+    }
+    if (slice) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= valid) continue;
+      if (i + j < weights) {
+        if (dw) dw[(s - 1) * weights + i + j] = T(sum[j]);
+      } else if (db) {
+        db[(s - 1) * p.biases + (i + j - weights)] = T(sum[j]);
+      }
+    }
+  }
+}
+
+// partial: [shares, 2 (head, tail), weights + biases]. Either result may be null.
+template <typename T>
+int launch_join(const float* partial, const Grouping& g, int64_t cost, int64_t shares,
+                int64_t weights, int64_t biases, T* dw, T* db, hipStream_t stream) {
+  if (shares == 1) return GS_OK;
+  // Workgroups go on to further values: those of the groups that lie in one
+  // share have nothing to do, and a workgroup to each 64 values and border
+  // (100k x 256 -> 256 in 64 groups: 32,000) took 180 us to find that out.
+  const JoinOf p{cost, shares, weights, biases, shares - 1 < g.groups};
+  const int64_t each = p.by_border ? shares - 1 : g.groups;
+  auto join = [&](auto slices) {
+    const int64_t chunks = ceil_div(weights + biases, 4 * kJoinThreads / slices.value);
+    const dim3 grid{unsigned(std::min(chunks, ceil_div(4096, each))), unsigned(each)};
+    group_join_kernel<T, slices.value><<<grid, kJoinThreads, 0, stream>>>(partial, g, p, dw, db);
+  };
+  // As many slices as there may be parts to add.
+  if (shares < 4 * int64_t(g.groups))
+    join(std::integral_constant<int, 1>{});
+  else if (shares < 16 * int64_t(g.groups))
+    join(std::integral_constant<int, 4>{});
+  else
+    join(std::integral_constant<int, 16>{});
+  GS_LAUNCHED("group_join_kernel");
+  return GS_OK;
+}
+
+}  // namespace gs

@@ -13,8 +13,8 @@
 //                      partial sums group_join_kernel adds in their order
 //
 // No atomics: results do not depend on timing.
-#include "groups.hpp"
-#include "matrix.hpp"
+#include "group_sums.hpp"
+#include "group_tile.hpp"
 
 namespace gs {
 namespace {
@@ -22,140 +22,14 @@ namespace {
 // --------------------------------------------------------------------------
 // y and dx, a tile of 128 x 128 to a workgroup
 
-// Tiles are numbered without the groups' counts being added up: segment s
-// begins at tile B / 128 + s, B its first position, which leaves it room
-// enough (some numbers have no rows).
-__device__ __forceinline__ int64_t tile_key(const Grouping& g, int s) {
-  return begin_of(g, s) / kEdge + s;
-}
-int64_t tile_numbers(const Grouping& g) { return g.rows / kEdge + g.groups + 2; }
-
-// A tile of rows on its way from memory to LDS, eight columns to a chunk.
-template <typename T, int Columns>
-struct StagedRows {
-  static constexpr int across = Columns / kChunk;
-  static constexpr int count = kEdge * across / kThreads;
-  const T* row[count];  // null past the segment's end
-  vec<T, 8> v[count];
-
-  __device__ __forceinline__ void place(const Grouping& g, const T* data, int64_t stride,
-                                        int first, int end) {
-#pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int position = first + (i * kThreads + int(threadIdx.x)) / across;
-      row[i] = position < end ? data + row_at(g, position) * stride : nullptr;
-    }
-  }
-  __device__ __forceinline__ void load(int64_t column, int64_t columns) {
-#pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int64_t c = column + (i * kThreads + threadIdx.x) % across * kChunk;
-      const int64_t left = columns - c;
-      v[i] = load_valid<T, 8>(row[i] + c, row[i] ? int(left < kChunk ? left : kChunk) : 0);
-    }
-  }
-  template <int Pitch>
-  __device__ __forceinline__ void store(T* lds) const {
-#pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int id = i * kThreads + threadIdx.x;
-      *reinterpret_cast<vec<T, 8>*>(lds + id / across * Pitch + id % across * kChunk) = v[i];
-    }
-  }
-};
-
-struct GroupProduct {
-  int64_t n, k;      // columns of C, length of the sum
-  int64_t tiles_n;
-  int64_t stride;    // of the rows
-};
-
-// C[i][n] = sum_k x[i][k] W_g(n, k) (+ bias[g][n]); W_g is [n][k] in memory
-// (NContiguous) or [k][n].
-template <typename T, bool NContiguous>
-__global__ __launch_bounds__(kThreads) void group_tile_kernel(
-    const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ bias, Grouping g,
-    GroupProduct p, T* __restrict__ out) {
-  constexpr int depth = Mma<T>::depth;
-  __shared__ __align__(16) T m_lds[kTileSize<T, true>];
-  __shared__ __align__(16) T n_lds[kTileSize<T, NContiguous>];
-  const int64_t number = blockIdx.x / p.tiles_n, n0 = blockIdx.x % p.tiles_n * kEdge;
-  const int s = find_segment(segments_of(g), number, [&](int i) { return tile_key(g, i); });
-  const int begin = begin_of(g, s), end = begin_of(g, s + 1);
-  const int64_t first64 = begin + (number - tile_key(g, s)) * kEdge;
-  if (first64 < begin || first64 >= end) return;  // below only where offsets fall
-  const int first = int(first64);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wave_m = (wave >> 1) * kWaveEdge, wave_n = (wave & 1) * kWaveEdge;
-  const int64_t n = n0 + wave_n + 16 * (lane >> 4);
-  f32x4 c[kTiles][kTiles];  // [m][n]
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float offset[16] = {};
-  if (s > 0 && s <= g.groups) {
-    const int64_t group = s - 1;
-    const T* const matrix = w + group * p.n * p.k;
-    const Side<T> ns{matrix, NContiguous ? p.k : p.n, NContiguous ? p.n : p.k,
-                     NContiguous ? p.k : p.n};
-    StagedRows<T, depth> m_next;
-    Staged<T, NContiguous ? kEdge : depth, NContiguous ? depth : kEdge> n_next;
-    m_next.place(g, x, p.stride, first, end);
-    auto fetch = [&](int64_t k) {
-      m_next.load(k, p.k);
-      if constexpr (NContiguous)
-        n_next.load(ns, n0, k);
-      else
-        n_next.load(ns, k, n0);
-    };
-    fetch(0);
-    for (int64_t k = 0; k < p.k; k += depth) {
-      m_next.template store<kPitch<T, true>>(m_lds);
-      n_next.template store<kPitch<T, NContiguous>, true, NContiguous>(n_lds);
-      __syncthreads();
-      if (k + depth < p.k) fetch(k + depth);
-#pragma unroll
-      for (int step = 0; step < depth; step += Mma<T>::step) {
-        typename Mma<T>::Fragment a[kTiles], b[kTiles];
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          a[i] = fragment<T, true>(m_lds, wave_m + 16 * i, step);
-          b[i] = fragment<T, NContiguous>(n_lds, wave_n + 16 * i, step);
-        }
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) c[i][j] = Mma<T>::of(b[j], a[i], c[i][j]);
-      }
-      __syncthreads();
-    }
-    if (bias) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        offset[j] = n + j < p.n ? float(bias[group * p.n + n + j]) : 0.f;
-    }
-  }
-  // Lane 16 q + i holds, of fragment row i, the 16 columns from 16 q on.
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    const int64_t position = int64_t(first) + wave_m + 16 * i + (lane & 15);
-    if (position >= end) continue;
-    float row[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) row[j] = c[i][j >> 2][j & 3] + offset[j];
-    store_row<T>(out + row_at(g, int(position)) * p.n + n, p.n - n, row);
-  }
-}
-
 template <typename T, bool NContiguous>
 int launch_tiles(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
                  const Grouping& g, int64_t k, int64_t n, void* out, hipStream_t stream) {
   const GroupProduct p{n, k, ceil_div(n, kEdge), stride};
   const int64_t blocks = tile_numbers(g) * p.tiles_n;
   GS_REQUIRE(blocks < (int64_t(1) << 32) / kThreads, GS_ERR_OVERFLOW, "%s: too many rows", name);
-  group_tile_kernel<T, NContiguous><<<dim3{unsigned(blocks)}, kThreads, 0, stream>>>(
-      static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), g, p,
+  group_tile_kernel<T, NContiguous, kByGroup><<<dim3{unsigned(blocks)}, kThreads, 0, stream>>>(
+      static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), g, p, {},
       static_cast<T*>(out));
   GS_LAUNCHED(name);
   return GS_OK;
@@ -461,18 +335,10 @@ __global__ __launch_bounds__(kThreads) void group_few_kernel(
 // and one in LDS, run on across that. A share is cut from the line on which
 // each segment takes kGroupCost + its rows, so that writing a group's
 // tile counts too. A group whose part of the line lies in one share is
-// written at once; the others' parts go to the share's head (the group
-// began before it) or tail, and group_join_kernel adds them in their order.
+// written at once; the others' parts are joined after.
 
 constexpr int kSumThreads = 512;
 constexpr int64_t kGroupCost = 128;  // of a group's tile, in rows
-
-__device__ __forceinline__ int64_t line_at(const Grouping& g, int s) {
-  return begin_of(g, s) + kGroupCost * s;
-}
-__host__ __device__ __forceinline__ int64_t line_length(const Grouping& g) {
-  return g.rows + kGroupCost * (int64_t(g.groups) + 2);
-}
 
 struct GroupSum {
   int64_t dy_stride, x_stride;
@@ -484,28 +350,6 @@ struct GroupSum {
 // Rows of dy and x that are multiplied: the positions of one step.
 struct StepOf {
   int first, count;
-};
-
-// Where a share stands: segment s, whose positions from `next` to `end` are its.
-struct Share {
-  int64_t from, to;  // on the line
-  int s, next, end;
-  bool inside;  // whether segment s begins before the share's end
-
-  __device__ __forceinline__ void open(const Grouping& g, int segment) {
-    s = segment;
-    next = end = 0;
-    inside = s < segments_of(g) && line_at(g, s) < to;
-    if (!inside) return;
-    // A row at position i of segment s lies at i + kGroupCost (s + 1).
-    const int64_t shift = kGroupCost * (s + 1);
-    const int64_t low = begin_of(g, s), high = begin_of(g, s + 1);
-    const int64_t a = from - shift > low ? from - shift : low;
-    const int64_t b = to - shift < high ? to - shift : high;
-    const bool some = a < b && s > 0 && s <= g.groups;
-    next = some ? int(a) : 0;
-    end = some ? int(b) : 0;
-  }
 };
 
 // 16 rows by 16 columns of LDS as a fragment, k along the rows, `k` the first
@@ -550,11 +394,11 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   if (share >= p.shares) return;
   const int tile = shared_xcd ? in_xcd % tiles : int(blockIdx.x / unsigned(p.shares));
   const int m0 = tile / p.tiles_n * tile_m, n0 = tile % p.tiles_n * tile_n;
-  const int64_t length = line_length(g);
-  Share at;
+  const int64_t length = line_length(g, kGroupCost);
+  Share at{kGroupCost};
   at.from = length * share / p.shares;
   at.to = length * (share + 1) / p.shares;
-  at.open(g, find_segment(segments_of(g), at.from, [&](int i) { return line_at(g, i); }));
+  at.open(g, find_segment(segments_of(g), at.from, [&](int i) { return line_at(g, kGroupCost, i); }));
   // Steps come in pairs, for the two buffers: a group's last may be empty.
   auto pairs_of = [](const Share& of) { return (of.end - of.next + 2 * Rows - 1) / (2 * Rows); };
   Share ahead_at = at;
@@ -667,7 +511,7 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   const int q = lane >> 4, i16 = lane & 15;
   // Writes the tile of segment at.s.
   auto finish = [&]() __attribute__((always_inline)) {
-    const int64_t low = line_at(g, at.s), high = line_at(g, at.s + 1);
+    const int64_t low = line_at(g, kGroupCost, at.s), high = line_at(g, kGroupCost, at.s + 1);
     const bool whole = low >= at.from && high <= at.to;
     const int64_t weights = int64_t(p.outputs) * p.features;
     const bool group = at.s > 0 && at.s <= g.groups;
@@ -747,68 +591,6 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   }
 }
 
-// Adds the parts of the groups that lie in several shares. blockIdx.y: a
-// group, or where there are fewer borders between shares than groups a border,
-// which stands for the group that it is the first border within; blockIdx.x:
-// 4 kThreads / Slices values of dW and db at a time, for which each slice of
-// the threads adds every Slices-th part.
-template <typename T, int Slices>
-__global__ __launch_bounds__(kThreads) void group_join_kernel(const float* __restrict__ partial,
-                                                              Grouping g, GroupSum p,
-                                                              bool by_border, T* __restrict__ dw,
-                                                              T* __restrict__ db) {
-  constexpr int columns = kThreads / Slices;
-  __shared__ vec<float, 4> sums[Slices][columns];
-  const int64_t length = line_length(g);
-  int s = blockIdx.y + 1;
-  int64_t border = s;
-  if (by_border)
-    s = find_segment(segments_of(g), length * border / p.shares,
-                     [&](int i) { return line_at(g, i); });
-  const int64_t low = line_at(g, s), high = line_at(g, s + 1);
-  if (!by_border) {  // the first border behind `low`
-    border = low * p.shares / length;
-    while (length * border / p.shares <= low) ++border;
-  }
-  const int64_t v = length * border / p.shares;
-  if (s < 1 || s > g.groups || border >= p.shares || v <= low || v >= high ||
-      length * (border - 1) / p.shares > low)
-    return;
-  // Shares border - 1 (its tail) .. last (their heads).
-  int64_t last = border;
-  while (last + 1 < p.shares && length * (last + 1) / p.shares < high) ++last;
-  const int count = int(last - border) + 2;
-  const int64_t weights = int64_t(p.outputs) * p.features, size = weights + p.outputs;
-  const int slice = threadIdx.x / columns, column = threadIdx.x % columns;
-  for (int64_t first = int64_t(blockIdx.x) * 4 * columns; first < size;
-       first += int64_t(gridDim.x) * 4 * columns) {
-    const int64_t i = first + 4 * column;
-    const int valid = int(size - i < 4 ? size - i : 4);
-    vec<float, 4> sum = 0.f;
-#pragma unroll 8
-    for (int j = slice; j < count; j += Slices)
-      sum += load_valid<float, 4>(partial + (j ? 2 * (border - 1 + j) : 2 * border - 1) * size + i,
-                                  valid);
-    if constexpr (Slices > 1) {
-      sums[slice][column] = sum;
-      __syncthreads();
-      if (slice == 0)
-        for (int j = 1; j < Slices; ++j) sum += sums[j][column];
-      __syncthreads();
-    }
-    if (slice) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j >= valid) continue;
-      if (i + j < weights) {
-        if (dw) dw[(s - 1) * weights + i + j] = T(sum[j]);
-      } else if (db) {
-        db[(s - 1) * int64_t(p.outputs) + (i + j - weights)] = T(sum[j]);
-      }
-    }
-  }
-}
-
 // How dW's sums are cut: fragments of a wave's tile along the outputs and the
 // features, positions of a step, and shares of the line. As for one group:
 // the widest tiles where they leave little empty and there are rows enough.
@@ -830,7 +612,7 @@ GroupSumPlan sum_plan(size_t size, const Grouping& g, int64_t features, int64_t 
   p.tiles_n = ceil_div(features, 64 * p.b);
   const int64_t tiles = p.tiles_m * p.tiles_n;
   p.shares = std::max<int64_t>(1, (large ? 256 : 512) / tiles);
-  p.shares = std::min(p.shares, ceil_div(line_length(g), 2 * kGroupCost));
+  p.shares = std::min(p.shares, ceil_div(line_length(g, kGroupCost), 2 * kGroupCost));
   return p;
 }
 
@@ -981,28 +763,7 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     if constexpr (sizeof(T) == 2)
       if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}, wide{}));
     if (plan.shares == 1) return int(GS_OK);
-    const int64_t size = outputs * (features + 1);
-    auto join = [&](auto slices) {
-      // Workgroups go on to further values: those of the groups that lie in
-      // one share have nothing to do, and a workgroup to each 64 values and
-      // border (100k x 256 -> 256 in 64 groups: 32,000) took 180 us to find
-      // that out.
-      const bool by_border = plan.shares - 1 < groups;
-      const int64_t each = by_border ? plan.shares - 1 : groups;
-      const int64_t chunks = ceil_div(size, 4 * kThreads / slices.value);
-      const dim3 grid{unsigned(std::min(chunks, ceil_div(4096, each))), unsigned(each)};
-      group_join_kernel<T, slices.value><<<grid, kThreads, 0, s>>>(partial, g, p, by_border, dw,
-                                                                  db);
-    };
-    // As many slices as there may be parts to add.
-    if (plan.shares < 4 * groups)
-      join(one{});
-    else if (plan.shares < 16 * groups)
-      join(four{});
-    else
-      join(integral_constant<int, 16>{});
-    GS_LAUNCHED("group_join_kernel");
-    return int(GS_OK);
+    return launch_join(partial, g, kGroupCost, plan.shares, outputs * features, outputs, dw, db, s);
   });
 }
 

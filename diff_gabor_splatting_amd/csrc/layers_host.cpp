@@ -36,6 +36,11 @@ struct Api {
   decltype(&gs_grouped_linear_backward_input) grouped_backward_input = nullptr;
   decltype(&gs_grouped_linear_backward_weight_workspace_size) grouped_workspace = nullptr;
   decltype(&gs_grouped_linear_backward_weight) grouped_backward_weight = nullptr;
+  decltype(&gs_adapted_linear_inner_size) adapted_inner = nullptr;
+  decltype(&gs_adapted_linear_forward) adapted_forward = nullptr;
+  decltype(&gs_adapted_linear_backward_input) adapted_backward_input = nullptr;
+  decltype(&gs_adapted_linear_backward_adapters_workspace_size) adapted_workspace = nullptr;
+  decltype(&gs_adapted_linear_backward_adapters) adapted_backward_adapters = nullptr;
 };
 
 Api api;
@@ -602,6 +607,127 @@ at::Tensor grouped_linear(const at::Tensor& x, const at::Tensor& weight,
   return GroupedLinear::apply(x, weight, offsets, order, bias);
 }
 
+// --------------------------------------------------------------------------
+// Linear layers with low-rank adapters
+
+at::Tensor adapted_rows(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& down,
+                        const at::Tensor& up, const Groups& groups, const at::Tensor& bias,
+                        double scale, at::Tensor* kept) {
+  const c10::DeviceGuard guard(x.device());
+  const RowsOf r(x);
+  const at::Tensor w = dense(weight), b = dense(bias), a = dense(down), u = dense(up);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = w.size(0);
+  at::Tensor y = at::empty(shape, x.options());
+  at::Tensor inner = workspace(api.adapted_inner(r.rows, a.size(1)), x.device());
+  check(api.adapted_forward(type_of(x), r.data(), r.stride, w.data_ptr(), data_of(b),
+                            a.data_ptr(), u.data_ptr(), float(scale), groups.places(),
+                            groups.begins(), r.rows, groups.count(), r.features, w.size(0),
+                            a.size(1), inner.data_ptr(), size_t(inner.numel()), y.data_ptr(),
+                            stream_of(x.device())));
+  if (kept) *kept = inner;
+  return y;
+}
+
+struct AdaptedLinear : torch::autograd::Function<AdaptedLinear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                            const at::Tensor& weight, const at::Tensor& down,
+                            const at::Tensor& up, const at::Tensor& offsets,
+                            const std::optional<at::Tensor>& order,
+                            const std::optional<at::Tensor>& bias, double scale) {
+    const Groups groups{offsets, order.value_or(at::Tensor())};
+    const bool shared = weight.requires_grad() || (bias && bias->requires_grad());
+    at::Tensor inner;
+    at::Tensor y = adapted_rows(x, weight, down, up, groups, bias.value_or(at::Tensor()), scale,
+                                up.requires_grad() ? &inner : nullptr);
+    ctx->save_for_backward({shared || down.requires_grad() ? x : at::Tensor(), weight, down, up,
+                            offsets, groups.order, inner});
+    ctx->saved_data["order"] = order.has_value();
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    check_calls("adapted_linear", {&grads[0]});
+    const auto saved = ctx->get_saved_variables();
+    const bool has_order = ctx->saved_data["order"].toBool();
+    const bool has_bias = ctx->saved_data["bias"].toBool();
+    const at::Tensor& grad = grads[0];
+    const c10::DeviceGuard guard(grad.device());
+    const RowsOf g(grad);
+    const at::Tensor w = dense(saved[1]), a = dense(saved[2]), u = dense(saved[3]);
+    const Groups groups{saved[4], saved[5]};
+    const int64_t outputs = w.size(0), features = w.size(1), rank = a.size(1);
+    const int32_t type = type_of(grad);
+    void* const stream = stream_of(grad.device());
+    at::Tensor dx, dw, da, du, db, back;
+    std::optional<RowsOf> x;
+    if (saved[0].defined()) x.emplace(saved[0]);
+    if (ctx->needs_input_grad(0))
+      dx = at::empty(ctx->saved_data["shape"].toIntVector(), grad.options());
+    if (ctx->needs_input_grad(2)) da = at::empty(a.sizes(), grad.options());
+    if (ctx->needs_input_grad(3)) du = at::empty(u.sizes(), grad.options());
+    if (dx.defined() || da.defined()) {
+      back = workspace(api.adapted_inner(g.rows, rank), grad.device());
+      check(api.adapted_backward_input(
+          type, g.data(), g.stride, w.data_ptr(), a.data_ptr(), u.data_ptr(),
+          float(ctx->saved_data["scale"].toDouble()), groups.places(), groups.begins(), g.rows,
+          groups.count(), features, outputs, rank, back.data_ptr(), size_t(back.numel()),
+          const_cast<void*>(data_of(dx)), stream));
+    }
+    if (da.defined() || du.defined()) {
+      const at::Tensor space = workspace(
+          api.adapted_workspace(g.rows, groups.count(), features, outputs, rank), grad.device());
+      check(api.adapted_backward_adapters(
+          type, g.data(), g.stride, x ? x->data() : nullptr, x ? x->stride : features,
+          data_of(saved[6]), data_of(back), groups.places(), groups.begins(), g.rows,
+          groups.count(), features, outputs, rank, const_cast<void*>(data_of(da)),
+          const_cast<void*>(data_of(du)), space.data_ptr(), size_t(space.numel()), stream));
+    }
+    // The shared layer's gradients are linear's, of the input in 8 bits.
+    if (ctx->needs_input_grad(1)) dw = at::empty(w.sizes(), grad.options());
+    if (has_bias && ctx->needs_input_grad(has_order ? 6 : 5))
+      db = at::empty({outputs}, grad.options());
+    if (dw.defined() || db.defined()) {
+      const Kept kept = Kept::empty(g.rows, features, grad.device());
+      check(api.checkpoint_write(type, x->data(), x->stride, g.rows, features,
+                                 kept.values.data_ptr(), kept.exponents.data_ptr(), stream));
+      const at::Tensor space =
+          workspace(api.linear_workspace(type, g.rows, features, outputs), grad.device());
+      check(api.linear_backward_weight(
+          type, g.data(), g.stride, kept.values.data_ptr(), kept.exponents.data_ptr(), g.rows,
+          features, outputs, const_cast<void*>(data_of(dw)), const_cast<void*>(data_of(db)),
+          space.data_ptr(), size_t(space.numel()), stream));
+    }
+    return once({dx, dw, da, du, at::Tensor(), at::Tensor(), db, at::Tensor()},
+                "adapted_linear");
+  }
+};
+
+at::Tensor adapted_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& down,
+                          const at::Tensor& up, const at::Tensor& offsets,
+                          const std::optional<at::Tensor>& order,
+                          const std::optional<at::Tensor>& bias, double scale) {
+  const at::Tensor b = bias.value_or(at::Tensor());
+  const Groups groups{offsets, order.value_or(at::Tensor())};
+  check_calls("adapted_linear", {&x, &weight, &down, &up, &b});
+  check_input(x);
+  if (weight.dim() != 2 || weight.size(0) < 1)
+    throw py::value_error("weight must have shape (outputs, features)");
+  check_parameter("weight", weight, {weight.size(0), x.size(-1)}, x, false);
+  check_parameter("bias", b, {weight.size(0)}, x, false);
+  if (down.dim() != 3 || down.size(0) < 1 || down.size(1) < 1 || down.size(1) > 64)
+    throw py::value_error("down must have shape (groups, rank, features), rank at most 64");
+  check_parameter("down", down, {down.size(0), down.size(1), x.size(-1)}, x, false);
+  check_parameter("up", up, {down.size(0), weight.size(0), down.size(1)}, x, false);
+  groups.check(x, down.size(0));
+  if (!grad_wanted({&x, &weight, &down, &up, &b}))
+    return adapted_rows(x, weight, down, up, groups, b, scale, nullptr);
+  return AdaptedLinear::apply(x, weight, down, up, offsets, order, bias, scale);
+}
+
 }  // namespace
 
 void bind_layers(const py::dict& table) {
@@ -625,6 +751,11 @@ void bind_layers(const py::dict& table) {
   take(table, "gs_grouped_linear_backward_input", next.grouped_backward_input);
   take(table, "gs_grouped_linear_backward_weight_workspace_size", next.grouped_workspace);
   take(table, "gs_grouped_linear_backward_weight", next.grouped_backward_weight);
+  take(table, "gs_adapted_linear_inner_size", next.adapted_inner);
+  take(table, "gs_adapted_linear_forward", next.adapted_forward);
+  take(table, "gs_adapted_linear_backward_input", next.adapted_backward_input);
+  take(table, "gs_adapted_linear_backward_adapters_workspace_size", next.adapted_workspace);
+  take(table, "gs_adapted_linear_backward_adapters", next.adapted_backward_adapters);
   api = next;
 }
 
@@ -636,7 +767,10 @@ std::vector<std::string> layer_entry_points() {
           "gs_linear_backward_weight", "gs_dropout", "gs_row_groups_workspace_size",
           "gs_row_groups", "gs_grouped_linear_forward", "gs_grouped_linear_backward_input",
           "gs_grouped_linear_backward_weight_workspace_size",
-          "gs_grouped_linear_backward_weight"};
+          "gs_grouped_linear_backward_weight", "gs_adapted_linear_inner_size",
+          "gs_adapted_linear_forward", "gs_adapted_linear_backward_input",
+          "gs_adapted_linear_backward_adapters_workspace_size",
+          "gs_adapted_linear_backward_adapters"};
 }
 
 void define_layers(py::module_& m) {
@@ -654,6 +788,8 @@ void define_layers(py::module_& m) {
   m.def("row_groups", &row_groups, py::arg("index"), py::arg("groups"));
   m.def("grouped_linear", &grouped_linear, py::arg("x"), py::arg("weight"), py::arg("offsets"),
         py::arg("order"), py::arg("bias"));
+  m.def("adapted_linear", &adapted_linear, py::arg("x"), py::arg("weight"), py::arg("down"),
+        py::arg("up"), py::arg("offsets"), py::arg("order"), py::arg("bias"), py::arg("scale"));
 }
 
 }  // namespace gs_host

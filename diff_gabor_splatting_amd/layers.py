@@ -40,7 +40,7 @@ ACTIVATIONS = {"sine": 0, "gelu": 1, "silu": 2}
 _CHECKPOINTS = {"full": False, "8bit": True}
 
 __all__ = ["Checkpoint", "quantize", "dequantize", "activation", "layer_norm", "linear", "dropout",
-           "RowGroups", "row_groups", "grouped_linear"]
+           "RowGroups", "row_groups", "grouped_linear", "adapted_linear"]
 
 
 class Checkpoint:
@@ -205,3 +205,24 @@ def grouped_linear(x: Tensor, weight: Tensor, groups: RowGroups,
     groups = _groups(groups)
     return _host.grouped_linear(_tensor("x", x), _tensor("weight", weight), groups.offsets,
                                 groups.order, bias)
+
+
+def adapted_linear(x: Tensor, weight: Tensor, down: Tensor, up: Tensor, groups: RowGroups,
+                   bias: Optional[Tensor] = None, scale: float = 1.0) -> Tensor:
+    """``x weight^T + bias + scale (x down[g]^T) up[g]^T`` for the rows of group
+    g, without the last term for rows of no group: a linear layer that all rows
+    share, with an adapter of each row's group beside it. ``weight``
+    [outputs, features], ``bias`` [outputs], ``down`` [groups, rank, features]
+    and ``up`` [groups, outputs, rank] have the type of ``x``; the rank is at
+    most 64. The backward pass reads ``x`` itself for the adapters' gradients, and
+    the shared matrix's gradient is that of :func:`linear`, taken with the
+    input in 8 bits; none is computed that is not asked for. What an infinity
+    in an adapter's matrix meets is NaN."""
+    groups = _groups(groups)
+    _number("scale", scale)
+    # As the kernels take it: a larger number is an infinity there.
+    if not math.isfinite(scale) or abs(scale) > 3.4e38:
+        raise ValueError("scale must be finite in float32")
+    return _host.adapted_linear(_tensor("x", x), _tensor("weight", weight),
+                                _tensor("down", down), _tensor("up", up), groups.offsets,
+                                groups.order, bias, scale)

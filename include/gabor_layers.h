@@ -137,6 +137,41 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
                                       void* grad_bias, void* workspace, size_t workspace_bytes,
                                       void* stream);
 
+/* A linear layer with a low-rank adapter by group: y = x weight^T + bias +
+ * scale (x down[g]^T) up[g]^T for the rows of group g (weight [outputs,
+ * features], bias [outputs] or null, down [groups, rank, features], up
+ * [groups, outputs, rank]), all of one type; rows of no group have the first
+ * two terms. rank <= 64. inner (gs_adapted_linear_inner_size bytes, 16-byte
+ * aligned) receives scale x down[g]^T of every row, which the backward pass of
+ * `up` reads. */
+size_t gs_adapted_linear_inner_size(int64_t rows, int64_t rank);
+int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride,
+                              const void* weight, const void* bias, const void* down,
+                              const void* up, float scale, const int32_t* order,
+                              const int32_t* offsets, int64_t rows, int64_t groups,
+                              int64_t features, int64_t outputs, int64_t rank, void* inner,
+                              size_t inner_bytes, void* y, void* stream);
+/* inner_grad (as large as inner) receives scale grad_y up[g], and grad_x (may
+ * be null) grad_y weight + inner_grad down[g]. */
+int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                     const void* weight, const void* down, const void* up,
+                                     float scale, const int32_t* order, const int32_t* offsets,
+                                     int64_t rows, int64_t groups, int64_t features,
+                                     int64_t outputs, int64_t rank, void* inner_grad,
+                                     size_t inner_bytes, void* grad_x, void* stream);
+/* grad_down[g] = the sum over group g's rows of inner_grad^T x, grad_up[g] that
+ * of grad_y^T inner (either may be null, and then what it alone reads). */
+size_t gs_adapted_linear_backward_adapters_workspace_size(int64_t rows, int64_t groups,
+                                                          int64_t features, int64_t outputs,
+                                                          int64_t rank);
+int gs_adapted_linear_backward_adapters(int32_t dtype, const void* grad_y, int64_t grad_stride,
+                                        const void* x, int64_t row_stride, const void* inner,
+                                        const void* inner_grad, const int32_t* order,
+                                        const int32_t* offsets, int64_t rows, int64_t groups,
+                                        int64_t features, int64_t outputs, int64_t rank,
+                                        void* grad_down, void* grad_up, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

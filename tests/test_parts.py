@@ -513,3 +513,248 @@ def test_grouped_linear_refusals():
     (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="grouped_linear is differentiable once"):
         dx.sum().backward()
+
+
+# --------------------------------------------------------------------------
+# GPU: linear layers with adapters by group
+
+# An inner row of a 2-byte type is kept in two parts: to 2^-16 of its value in
+# bfloat16, whose first part is cut off, and in float16 to 2^-21 of its row's
+# largest (its second part may be below the type's normal range).
+INNER = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -21}
+
+
+def near_or_past(got, expected, error, dtype):
+    """near, but for what is past the type's largest: an infinity by the rounding
+    itself (float16: from 65520 on)."""
+    most = torch.finfo(dtype).max
+    past = expected.abs() - error > most * (1 + torch.finfo(dtype).eps / 2)
+    got = got.detach().cpu().double()
+    assert torch.equal(got[past], torch.sign(expected[past]) * math.inf)
+    edge = ~past & (expected.abs() + error >= most)
+    assert edge.sum() <= 1 + edge.numel() // 1000
+    fine = ~past & ~edge
+    near(got[fine], expected[fine], error[fine], dtype)
+
+
+def check_adapted(x, w, b, a, u, g, scale, members, y, grads):
+    """Errors: sums of float32, the inner rows' parts, and their own sums' errors
+    on the way through the other products."""
+    dtype, rank = x.dtype, a.shape[1]
+    rows, features, outputs = len(x), x.shape[1], w.shape[0]
+    want = oracle.adapted_linear(x, w, a, u, members, b, scale, g)
+    low, high = w.abs(), None if b is None else b.abs()
+    size = oracle.adapted_linear(x.abs(), low, a.abs(), u.abs(), members, high, abs(scale), g.abs())
+    terms = features + outputs + rank + 8
+
+    def inner_error(sum_error):
+        return sum_error * E + INNER[dtype]
+
+    inner = torch.zeros(rows, rank, dtype=torch.float64)
+    back = torch.zeros(rows, rank, dtype=torch.float64)
+    for group, at in enumerate(members):
+        inner[at] = abs(scale) * (x[at].double().abs() @ a[group].double().abs().t())
+        back[at] = abs(scale) * (g[at].double().abs() @ u[group].double().abs())
+    # float16's parts go by the row's largest.
+    if dtype == torch.float16:
+        inner, back = (t.amax(1, keepdim=True).expand_as(t) for t in (inner, back))
+    narrow = [torch.zeros(rows, outputs, dtype=torch.float64), torch.zeros(rows, features,
+                                                                         dtype=torch.float64),
+              torch.zeros_like(a, dtype=torch.float64), torch.zeros_like(u, dtype=torch.float64)]
+    for group, at in enumerate(members):
+        narrow[0][at] = inner[at] @ u[group].double().abs().t()
+        narrow[1][at] = back[at] @ a[group].double().abs()
+        narrow[2][group] = back[at].t() @ x[at].double().abs()
+        narrow[3][group] = g[at].double().abs().t() @ inner[at]
+    most = max([len(m) for m in members] + [1]) + 2
+    near_or_past(y.reshape(rows, outputs), want[0],
+         terms * E * size[0] + inner_error(features + 2) * narrow[0], dtype)
+    near_or_past(grads[0].reshape(rows, features), want[1],
+         terms * E * size[1] + inner_error(outputs + 2) * narrow[1], dtype)
+    near_or_past(grads[1], want[2], most * E * size[2] + inner_error(outputs + 2) * narrow[2], dtype)
+    near_or_past(grads[2], want[3], most * E * size[3] + inner_error(features + 2) * narrow[3], dtype)
+
+
+def adapted_case(rows, features, outputs, groups, rank, dtype, bias=True, seed=31, scale=0.7,
+                 index=None, by=None, size=1.0):
+    m = layers()
+    x = normal(rows, features, seed=seed, dtype=dtype)
+    w = normal(outputs, features, seed=seed + 1, dtype=dtype, scale=features ** -0.5)
+    b = normal(outputs, seed=seed + 2, dtype=dtype) if bias else None
+    a = normal(groups, rank, features, seed=seed + 3, dtype=dtype, scale=size * features ** -0.5)
+    u = normal(groups, outputs, rank, seed=seed + 4, dtype=dtype, scale=rank ** -0.5)
+    g = normal(rows, outputs, seed=seed + 5, dtype=dtype)
+    if by is None:
+        index = some_groups(rows, groups, seed) if index is None else index
+        by, members = grouped_by(index, groups)
+    else:
+        members = oracle.members(by.offsets, by.order, rows)
+    on, wc, ac, uc = (t.cuda().requires_grad_(i != 1) for i, t in enumerate((x, w, a, u)))
+    bc = None if b is None else b.cuda()
+    y = m.adapted_linear(on, wc, ac, uc, by, bc, scale)
+    grads = torch.autograd.grad(y, (on, ac, uc), g.cuda())
+    with torch.no_grad():
+        assert torch.equal(m.adapted_linear(on, wc, ac, uc, by, bc, scale), y)
+    check_adapted(x, w, b, a, u, g, scale, members, y, grads)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs,groups,rank", [
+    (1, 1, 1, 1, 1), (1, 1024, 57, 8, 16), (4, 64, 64, 8, 5), (16, 33, 18, 3, 64), (17, 8, 8, 5, 4),
+    (40, 5, 3, 2, 2), (64, 96, 57, 64, 16), (127, 130, 63, 4, 33), (300, 187, 18, 7, 5),
+    (1000, 40, 72, 300, 8), (2500, 264, 136, 6, 32), (1024, 64, 57, 16, 17), (5000, 128, 128, 12, 64),
+    (200, 1100, 40, 3, 16), (200, 40, 1100, 3, 16), (90, 1030, 1030, 2, 48), (700, 512, 512, 5, 16),
+    (900, 256, 256, 3, 31)])
+def test_adapted_linear(dtype, rows, features, outputs, groups, rank):
+    adapted_case(rows, features, outputs, groups, rank, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_adapted_linear_of_special_groups(dtype):
+    m = layers()
+    adapted_case(500, 64, 40, 5, 8, dtype, bias=False, scale=-2.0)
+    none = torch.full((200,), -1)
+    adapted_case(200, 64, 40, 5, 8, dtype, index=none)           # no row has an adapter
+    adapted_case(200, 64, 40, 5, 8, dtype, index=none + 4)       # one has all
+    adapted_case(3000, 64, 40, 5, 8, dtype, index=torch.arange(3000) % 5)
+    adapted_case(130, 64, 40, 130, 8, dtype, index=torch.arange(130))  # a row each
+    adapted_case(2000, 24, 8, 3000, 3, dtype)
+    adapted_case(300, 64, 40, 5, 8, dtype, scale=0.0)
+    offsets = torch.tensor([30, 30, 200, 455, 455, 690], dtype=torch.int32).cuda()
+    adapted_case(700, 64, 40, 5, 8, dtype, by=m.RowGroups(offsets))
+    adapted_case(10, 64, 40, 2, 8, dtype, by=m.RowGroups(
+        torch.tensor([1, 3, 8], dtype=torch.int32).cuda()))
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 12])
+def test_adapted_linear_of_small_and_large_inner_rows(dtype, size):
+    """Inner values far from 1, past float16's largest where `size` is 2^12:
+    their own range is float32's. Some of down's gradients are past it where
+    `size` is 2^-12 (scale 2^12)."""
+    adapted_case(400, 64, 40, 5, 8, dtype, size=size, scale=1 / size)
+    adapted_case(400, 64, 40, 5, 8, dtype, size=size, scale=32 / size ** 2)
+    adapted_case(9, 64, 40, 5, 8, dtype, size=size, scale=1 / size)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_adapted_linear_gradients_asked_for_one_by_one(dtype):
+    """The shared layer's are linear's."""
+    m = layers()
+    index = some_groups(900, 6, 3)
+    by, _ = grouped_by(index, 6)
+    tensors = [normal(900, 40, seed=1, dtype=dtype), normal(24, 40, seed=2, dtype=dtype),
+               normal(6, 8, 40, seed=3, dtype=dtype), normal(6, 24, 8, seed=4, dtype=dtype),
+               normal(24, seed=5, dtype=dtype)]
+    g = normal(900, 24, seed=6, dtype=dtype).cuda()
+    for groups in (by, m.RowGroups(by.offsets)):
+        every = [t.cuda().requires_grad_() for t in tensors]
+        want = torch.autograd.grad(m.adapted_linear(*every[:4], groups, every[4]), every, g)
+        plain = torch.autograd.grad(m.linear(every[0], every[1], every[4]), (every[1], every[4]), g)
+        assert torch.equal(want[1], plain[0]) and torch.equal(want[4], plain[1])
+        for i in range(5):
+            some = [t.cuda().requires_grad_(j == i) for j, t in enumerate(tensors)]
+            y = m.adapted_linear(*some[:4], groups, some[4])
+            (got,) = torch.autograd.grad(y, some[i], g)
+            assert torch.equal(got, want[i])
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_adapted_linear_keeps_bad_values_to_their_place(dtype):
+    m = layers()
+    index = torch.arange(400) % 4 - 1
+    by, _ = grouped_by(index, 3)
+    x, w = normal(400, 64, seed=1, dtype=dtype), normal(32, 64, seed=2, dtype=dtype)
+    a, u = normal(3, 8, 64, seed=3, dtype=dtype), normal(3, 32, 8, seed=4, dtype=dtype)
+    g = normal(400, 32, seed=5, dtype=dtype)
+    outs = []
+    for bad in (False, True):
+        held, grad = x.clone(), g.clone()
+        if bad:
+            held[4], grad[4] = math.nan, math.inf  # a row of no group
+            held[5] = math.nan                     # of group 0
+        on, ac, uc = (t.cuda().requires_grad_() for t in (held, a, u))
+        y = m.adapted_linear(on, w.cuda(), ac, uc, by)
+        outs.append((y, *torch.autograd.grad(y, (on, ac, uc), grad.cuda())))
+    (y0, dx0, da0, du0), (y1, dx1, da1, du1) = outs
+    rows = torch.ones(400, dtype=torch.bool, device="cuda")
+    rows[4:6] = False
+    assert torch.equal(y0[rows], y1[rows]) and y1[4:6].isnan().all()
+    assert torch.equal(dx0[rows], dx1[rows])
+    assert torch.equal(da0[1:], da1[1:]) and da1[0].isnan().all()
+    assert torch.equal(du0[1:], du1[1:]) and du1[0].isnan().all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [9, 600])
+def test_adapted_linear_shapes_and_strides(dtype, rows):
+    m = layers()
+    base = normal(rows, 4, 200, seed=1, dtype=dtype).cuda()
+    w = normal(40, 96, seed=2, dtype=dtype).cuda()
+    a, u = normal(3, 8, 96, seed=3, dtype=dtype).cuda(), normal(3, 40, 8, seed=4, dtype=dtype).cuda()
+    for view in (lambda t: t[:, 1, :96], lambda t: t[:, 2, 3:99], lambda t: t[:, :3, 8:104],
+                 lambda t: t[:1, 0, :96].expand(rows, 96)):
+        x = view(base)
+        by = m.row_groups((torch.arange(x.numel() // 96) % 4 - 1).cuda(), 3)
+        outs = []
+        for source, turned in ((x, False), (x.contiguous(), True)):
+            on, down, up = (t.detach().requires_grad_() for t in (
+                source, a.transpose(1, 2).contiguous().transpose(1, 2) if turned else a, u))
+            y = m.adapted_linear(on, w.t().contiguous().t() if turned else w, down, up, by)
+            outs.append((y, *torch.autograd.grad(
+                y, (on, down, up), torch.ones(1, dtype=dtype, device="cuda").expand_as(y))))
+        assert outs[0][0].shape == (*x.shape[:-1], 40)
+        for got, want in zip(*outs):
+            assert torch.equal(got, want)
+
+
+@gpu_test
+def test_adapted_linear_of_no_rows():
+    m = layers()
+    x = torch.zeros(0, 8, device="cuda", requires_grad=True)
+    w, b = torch.ones(4, 8, device="cuda", requires_grad=True), torch.ones(4, device="cuda")
+    a = torch.ones(3, 2, 8, device="cuda", requires_grad=True)
+    u = torch.ones(3, 4, 2, device="cuda", requires_grad=True)
+    by = m.row_groups(torch.zeros(0, dtype=torch.int64, device="cuda"), 3)
+    y = m.adapted_linear(x, w, a, u, by, b)
+    grads = torch.autograd.grad(y.sum(), (x, w, a, u))
+    assert y.shape == (0, 4) and not any(t.any() for t in grads)
+
+
+@gpu_test
+def test_adapted_linear_refusals():
+    m = layers()
+    x, w = torch.zeros(6, 8, device="cuda"), torch.zeros(4, 8, device="cuda")
+    a, u = torch.zeros(3, 2, 8, device="cuda"), torch.zeros(3, 4, 2, device="cuda")
+    by = m.row_groups(torch.zeros(6, dtype=torch.int32, device="cuda"), 3)
+    with pytest.raises(TypeError, match="RowGroups"):
+        m.adapted_linear(x, w, a, u, None)
+    with pytest.raises(TypeError, match="down must be"):
+        m.adapted_linear(x, w, None, u, by)
+    for down in (a[0], a[..., :7], torch.zeros(3, 65, 8, device="cuda")):
+        with pytest.raises(ValueError, match="down must have shape"):
+            m.adapted_linear(x, w, down, u, by)
+    for up in (u[:2], u.transpose(1, 2)):
+        with pytest.raises(ValueError, match="up must have shape"):
+            m.adapted_linear(x, w, a, up, by)
+    with pytest.raises(ValueError, match="type of x"):
+        m.adapted_linear(x, w, a.half(), u, by)
+    with pytest.raises(ValueError, match="weight must have shape"):
+        m.adapted_linear(x, w[:, :7], a, u, by)
+    with pytest.raises(ValueError, match="of 3 groups, not 2"):
+        m.adapted_linear(x, w, a[:2], u[:2], by)
+    for scale in (math.inf, math.nan, 1e39):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            m.adapted_linear(x, w, a, u, by, scale=scale)
+    with pytest.raises(ValueError, match="scale has no gradient"):
+        m.adapted_linear(x, w, a, u, by, scale=torch.ones((), requires_grad=True))
+    y = m.adapted_linear(x.requires_grad_(), w, a, u, by)
+    (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="adapted_linear is differentiable once"):
+        dx.sum().backward()
