@@ -9,8 +9,10 @@
 // the narrow matrices' gradients.
 //
 //   few_inner_kernel, few_adapted_kernel  the forward pass of a few rows
-//   group_tile_kernel  inner rows; y and dx
+//   group_rows_kernel  inner rows; y and dx
+//   group_tile_kernel  the same where a matrix has a side too long for that
 //   narrow_sum_kernel  dA and dB, a wave to 128 columns of a share of the rows
+#include "group_rows.hpp"
 #include "group_sums.hpp"
 #include "group_tile.hpp"
 
@@ -110,6 +112,82 @@ int launch_tiles(const char* name, const void* x, int64_t stride, const void* w,
       adapters, static_cast<T*>(out));
   GS_LAUNCHED(name);
   return GS_OK;
+}
+
+// --------------------------------------------------------------------------
+// Inner rows, y and dx with the matrix in LDS and the rows streamed past it
+
+// down [groups, rank, features] as [groups, features, rank], the layout in
+// which the product with the inner rows reads it.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void turn_kernel(const T* __restrict__ down, int64_t size,
+                                                        int rank, int features,
+                                                        T* __restrict__ out) {
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < size;
+       i += int64_t(gridDim.x) * kThreads) {
+    const int64_t row = i / features;  // of all groups' ranks
+    const int column = int(i - row * features);
+    const int64_t group = row / rank;
+    out[(group * features + column) * rank + (row - group * rank)] = down[i];
+  }
+}
+
+// `taken` is false where the matrix is too large to stay in LDS, or k less
+// than a lane's part of a fragment.
+template <typename T, bool Transposed, int Mode>
+int launch_rows(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
+                const Grouping& g, int64_t k, int64_t n, const Adapters<T>& adapters, void* out,
+                hipStream_t stream, bool& taken) {
+  const int64_t steps = steps_of(sizeof(T), k);
+  int fragments;
+  if constexpr (Mode == kInner) {
+    fragments = n <= 32 ? 2 : 4;  // all of the rank, at most 64
+    if (steps * 2048 * fragments > int64_t(kRowLds)) fragments = 0;
+  } else {
+    fragments = panel_fragments(sizeof(T), g.rows, k, n);
+  }
+  const int64_t panels = fragments ? ceil_div(n, 16 * fragments) : 0;
+  taken = fragments && panels <= 32 && k >= kPart<T>;
+  if (!taken) return GS_OK;
+  using std::integral_constant;
+  auto launch = [&](auto tn, auto ahead, auto tail) {
+    GroupRows p{stride, int(k), int(n), int(panels), 0, int(steps)};
+    // Inner rows are bound by reading: as many workgroups as LDS lets run.
+    const int64_t most = Mode == kInner ? (steps * 2048 * fragments > 48 * 1024 ? 256 : 512)
+                                        : 32 / panels * 8;
+    p.workers = int(std::min<int64_t>(most, ceil_div(g.rows, kRowTile)));
+    const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
+    const size_t lds = size_t(steps) * 2 * tn.value * 1024;
+    auto* const kernel = &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value, Mode>;
+    GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
+    kernel<<<grid, kRowThreads, lds, stream>>>(static_cast<const T*>(x), static_cast<const T*>(w),
+                                               static_cast<const T*>(bias), g, p, adapters,
+                                               static_cast<T*>(out));
+    GS_LAUNCHED(name);
+    return int(GS_OK);
+  };
+  using one = integral_constant<int, 1>;
+  using two = integral_constant<int, 2>;
+  using four = integral_constant<int, 4>;
+  auto by_tail = [&](auto tn, auto ahead) {
+    return k != steps * kStep<T> ? launch(tn, ahead, std::true_type{})
+                                 : launch(tn, ahead, std::false_type{});
+  };
+  auto by_ahead = [&](auto tn) {
+    switch (ahead_of(steps)) {
+      case 1: return by_tail(tn, one{});
+      case 2: return by_tail(tn, two{});
+      default: return by_tail(tn, four{});
+    }
+  };
+  switch (fragments) {
+    case 8:
+      if constexpr (Mode == kAdapted) return by_ahead(integral_constant<int, 8>{});
+    case 4: return by_ahead(four{});
+    default:
+      if constexpr (sizeof(T) == 4 || Mode == kInner) return by_ahead(two{});
+      return int(GS_OK);  // not reached: panel_fragments gives no such panel
+  }
 }
 
 // --------------------------------------------------------------------------
@@ -270,12 +348,6 @@ int check_adapted(const char* name, int32_t dtype, const void* offsets, int64_t 
   return GS_OK;
 }
 
-int check_inner(const char* name, const void* inner, size_t bytes, int64_t rows, int64_t rank) {
-  GS_REQUIRE(inner && bytes >= Inner<float>::bytes(rows, rank), GS_ERR_WORKSPACE,
-             "inner rows too small for %s", name);
-  return GS_OK;
-}
-
 Grouping grouping(const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups) {
   return {order, offsets, int32_t(rows), int32_t(groups)};
 }
@@ -291,6 +363,16 @@ size_t gs_adapted_linear_inner_size(int64_t rows, int64_t rank) {
   return Inner<float>::bytes(rows, rank);
 }
 
+size_t gs_adapted_linear_inner_grad_size(int32_t dtype, int64_t rows, int64_t groups,
+                                         int64_t features, int64_t rank) {
+  using namespace gs;
+  if (groups <= 0 || groups > kMostGroupsOfRows || features <= 0 || features > kMostFeatures)
+    return 0;
+  const size_t size = gs_adapted_linear_inner_size(rows, rank);
+  // And down, turned.
+  return size ? size + size_t(groups * rank * features) * (dtype == GS_FLOAT32 ? 4 : 2) : 0;
+}
+
 int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const void* weight,
                               const void* bias, const void* down, const void* up, float scale,
                               const int32_t* order, const int32_t* offsets, int64_t rows,
@@ -304,7 +386,8 @@ int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, 
   GS_REQUIRE(std::isfinite(scale), GS_ERR_ARGUMENT, "%s: scale must be finite", name);
   if (rows == 0) return GS_OK;
   GS_REQUIRE(x && weight && down && up && y, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
-  GS_CHECK(check_inner(name, inner, inner_bytes, rows, rank));
+  GS_REQUIRE(inner && inner_bytes >= gs_adapted_linear_inner_size(rows, rank), GS_ERR_WORKSPACE,
+             "inner rows too small for %s", name);
   const Grouping g = grouping(order, offsets, rows, groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto zero) {
@@ -323,11 +406,19 @@ int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, 
       GS_LAUNCHED(name);
       return int(GS_OK);
     }
-    GS_CHECK((launch_tiles<T, true, kInner>(name, x, row_stride, down, nullptr, g, features, rank,
-                                            Adapters<T>{held, nullptr, scale}, nullptr, s)));
-    return launch_tiles<T, true, kAdapted>(
-        name, x, row_stride, weight, bias, g, features, outputs,
-        Adapters<T>{held, static_cast<const T*>(up), 0.f}, y, s);
+    const Adapters<T> first{held, nullptr, scale};
+    const Adapters<T> second{held, static_cast<const T*>(up), 0.f};
+    bool taken = false;
+    GS_CHECK((launch_rows<T, false, kInner>(name, x, row_stride, down, nullptr, g, features, rank,
+                                            first, nullptr, s, taken)));
+    if (!taken)
+      GS_CHECK((launch_tiles<T, true, kInner>(name, x, row_stride, down, nullptr, g, features,
+                                              rank, first, nullptr, s)));
+    GS_CHECK((launch_rows<T, false, kAdapted>(name, x, row_stride, weight, bias, g, features,
+                                              outputs, second, y, s, taken)));
+    if (taken) return int(GS_OK);
+    return launch_tiles<T, true, kAdapted>(name, x, row_stride, weight, bias, g, features,
+                                           outputs, second, y, s);
   });
 }
 
@@ -346,19 +437,39 @@ int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
   if (rows == 0) return GS_OK;
   GS_REQUIRE(grad_y && up && (!grad_x || (weight && down)), GS_ERR_ARGUMENT,
              "null pointer passed to %s", name);
-  GS_CHECK(check_inner(name, inner_grad, inner_bytes, rows, rank));
+  GS_REQUIRE(inner_grad && inner_bytes >= gs_adapted_linear_inner_grad_size(
+                                              dtype, rows, groups, features, rank),
+             GS_ERR_WORKSPACE, "inner rows too small for %s", name);
   const Grouping g = grouping(order, offsets, rows, groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const Inner<T> held = Inner<T>::at(inner_grad, rows, rank);
-    GS_CHECK((launch_tiles<T, false, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
-                                             rank, Adapters<T>{held, nullptr, scale}, nullptr,
-                                             s)));
+    const Adapters<T> first{held, nullptr, scale};
+    Adapters<T> second{held, static_cast<const T*>(down), 0.f};
+    bool taken = false;
+    GS_CHECK((launch_rows<T, true, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
+                                           rank, first, nullptr, s, taken)));
+    if (!taken)
+      GS_CHECK((launch_tiles<T, false, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
+                                               rank, first, nullptr, s)));
     if (!grad_x) return int(GS_OK);
-    return launch_tiles<T, false, kAdapted>(
-        name, grad_y, grad_stride, weight, nullptr, g, outputs, features,
-        Adapters<T>{held, static_cast<const T*>(down), 0.f}, grad_x, s);
+    if (panel_fragments(sizeof(T), rows, outputs, features) && outputs >= kPart<T>) {
+      T* const turned = reinterpret_cast<T*>(static_cast<char*>(inner_grad) +
+                                             Inner<T>::bytes(rows, rank));
+      const int64_t size = groups * rank * features;
+      turn_kernel<T><<<dim3{unsigned(std::min<int64_t>(ceil_div(size, kThreads), 1 << 16))},
+                       kThreads, 0, s>>>(static_cast<const T*>(down), size, int(rank),
+                                         int(features), turned);
+      GS_LAUNCHED(name);
+      second.matrix = turned;
+      GS_CHECK((launch_rows<T, true, kAdapted>(name, grad_y, grad_stride, weight, nullptr, g,
+                                               outputs, features, second, grad_x, s, taken)));
+      if (taken) return int(GS_OK);
+      second.matrix = static_cast<const T*>(down);
+    }
+    return launch_tiles<T, false, kAdapted>(name, grad_y, grad_stride, weight, nullptr, g,
+                                            outputs, features, second, grad_x, s);
   });
 }
 

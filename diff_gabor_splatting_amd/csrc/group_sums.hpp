@@ -74,16 +74,15 @@ __global__ __launch_bounds__(kJoinThreads) void group_join_kernel(const float* _
                      [&](int i) { return line_at(g, p.cost, i); });
   const int64_t low = line_at(g, p.cost, s), high = line_at(g, p.cost, s + 1);
   if (!p.by_border) {  // the first border behind `low`
-    border = low * p.shares / length;
-    while (length * border / p.shares <= low) ++border;
+    border = ((low + 1) * p.shares + length - 1) / length;
   }
   const int64_t v = length * border / p.shares;
   if (s < 1 || s > g.groups || border >= p.shares || v <= low || v >= high ||
       length * (border - 1) / p.shares > low)
     return;
   // Shares border - 1 (its tail) .. last (their heads).
-  int64_t last = border;
-  while (last + 1 < p.shares && length * (last + 1) / p.shares < high) ++last;
+  int64_t last = (high * p.shares - 1) / length;
+  if (last >= p.shares) last = p.shares - 1;
   const int count = int(last - border) + 2;
   const int64_t weights = p.weights, size = weights + p.biases;
   const int slice = threadIdx.x / columns, column = threadIdx.x % columns;

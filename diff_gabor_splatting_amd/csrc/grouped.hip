@@ -13,6 +13,7 @@
 //                      partial sums group_join_kernel adds in their order
 //
 // No atomics: results do not depend on timing.
+#include "group_rows.hpp"
 #include "group_sums.hpp"
 #include "group_tile.hpp"
 
@@ -38,208 +39,6 @@ int launch_tiles(const char* name, const void* x, int64_t stride, const void* w,
 // --------------------------------------------------------------------------
 // y and dx, a group's matrix in LDS and its rows streamed past it
 
-// A workgroup takes a panel of the columns and a share of the rows, whatever
-// groups they are in, and puts another matrix in place where another group
-// begins; a wave takes 32 rows at a time and, but for that, needs no other
-// wave. Shares are cut from the line on which each segment takes kStageCost +
-// its rows, so that putting a matrix in place counts too.
-constexpr int64_t kStageCost = 64;  // of a matrix, in rows
-
-__device__ __forceinline__ int64_t stage_line(const Grouping& g, int s) {
-  return begin_of(g, s) + kStageCost * s;
-}
-
-struct GroupRows {
-  int64_t stride;
-  int k, n;          // length of the sum and columns of C
-  int panels;        // workgroups side by side, each with its columns of C
-  int workers;       // workgroups to a panel
-  int steps;         // of the sum, see steps_of
-};
-
-// Where the line's place v lies in segment s, as a position: from the
-// segment's begin on a whole number of tiles, so that the shares on both sides
-// of it agree and few tiles are partly filled.
-__device__ __forceinline__ int cut_at(int64_t v, int s, int low, int high) {
-  const int64_t into = v - kStageCost * (s + 1) - low;
-  if (into <= 0) return low;
-  const int64_t up = (into + kRowTile - 1) / kRowTile * kRowTile;
-  return up < high - low ? low + int(up) : high;
-}
-
-// Ahead: steps on their way. Tail: k is no whole number of steps.
-template <typename T, int TN, int Ahead, bool Transposed, bool Tail>
-__global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
-    const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ bias, Grouping g,
-    GroupRows p, T* __restrict__ out) {
-  constexpr int TM = kRowTile / 16;
-  constexpr int part = kPart<T>, step = kStep<T>, columns = 16 * TN;
-  constexpr int loads = 2 * TM;  // of eight rows each
-  typedef vec<T, part> Part;
-  extern __shared__ __align__(16) char shared[];
-  Part* const panel = reinterpret_cast<Part*>(shared);
-  __shared__ Part turns[kRowWaves][128];
-  __shared__ float offset[columns];
-  // Workgroups go to the eight XCDs in turn: those that take the same rows
-  // share one, and its L2.
-  const int xcd = blockIdx.x & 7, in_xcd = blockIdx.x >> 3;
-  const int at = in_xcd % p.panels;
-  const int worker = in_xcd / p.panels * 8 + xcd;
-  if (worker >= p.workers) return;
-  const int n0 = at * columns;
-  const int64_t length = g.rows + kStageCost * segments_of(g);
-  const int64_t from_line = length * worker / p.workers;
-  const int64_t to_line = length * (worker + 1) / p.workers;
-
-  const int lane = threadIdx.x & 63, q = lane >> 4, i16 = lane & 15;
-  const int row8 = lane >> 3, piece = lane & 7;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Part* const turn = turns[wave];
-
-  int s = find_segment(segments_of(g), from_line, [&](int i) { return stage_line(g, i); });
-  for (; s < segments_of(g) && stage_line(g, s) < to_line; ++s) {
-    const int low = begin_of(g, s), high = max(begin_of(g, s + 1), low);
-    const int first = cut_at(from_line, s, low, high), end = cut_at(to_line, s, low, high);
-    if (first >= end) continue;
-    if (s == 0 || s > g.groups) {  // rows of no group
-      constexpr int pieces = columns / part;
-      for (int64_t id = threadIdx.x; id < int64_t(end - first) * pieces; id += kRowThreads) {
-        const int n = n0 + int(id % pieces) * part;
-        store_valid<T, part>(out + row_at(g, first + int(id / pieces)) * p.n + n,
-                             min(p.n - n, part), Part(T(0)));
-      }
-      continue;
-    }
-    const int tiles = (end - first + kRowTile - 1) / kRowTile;
-
-    // What is on its way: the loop below takes ring[u] and sends for the step
-    // `Ahead` later in its place. Past the wave's last tile it sends for that
-    // one again, so that the number of loads under way is always the same.
-    // The rows' places are asked for a tile before they are needed.
-    int now[loads], sent_rows[loads], after[loads];
-    auto places = [&](int tile, int (&to)[loads]) {
-#pragma unroll
-      for (int j = 0; j < loads; ++j)  // positions past the end repeat the last one
-        to[j] = int(row_at(g, min(first + tile * kRowTile + 8 * j + row8, end - 1)));
-    };
-    const T* from[loads];
-    auto turn_to = [&]() {
-#pragma unroll
-      for (int j = 0; j < loads; ++j) from[j] = x + sent_rows[j] * p.stride + piece * part;
-    };
-    int sent = min(wave, tiles - 1), sent_step = 0;
-    auto send = [&](Part (&to)[loads]) {
-      if (sent_step == p.steps) {
-        sent_step = 0;
-        if (sent + kRowWaves < tiles) {
-          sent += kRowWaves;
-#pragma unroll
-          for (int j = 0; j < loads; ++j) sent_rows[j] = after[j];
-        }
-        turn_to();
-        places(min(sent + kRowWaves, tiles - 1), after);
-      }
-      if (!Tail || (sent_step + 1) * step <= p.k) {
-#pragma unroll
-        for (int j = 0; j < loads; ++j)
-          to[j] = load_packed<T, part>(from[j] + sent_step * step);
-      } else {
-        const int left = min(p.k - sent_step * step - piece * part, part);
-#pragma unroll
-        for (int j = 0; j < loads; ++j)
-          to[j] = load_edge<T, part, false>(from[j] + sent_step * step, left);
-      }
-      ++sent_step;
-    };
-    Part ring[Ahead][loads];
-    places(sent, sent_rows);
-    places(min(sent + kRowWaves, tiles - 1), after);
-#pragma unroll
-    for (int j = 0; j < loads; ++j) now[j] = sent_rows[j];
-    turn_to();
-
-    // The matrix, once no wave reads the one before.
-    __syncthreads();
-    stage_panel<T, TN, Transposed>(w + int64_t(s - 1) * p.n * p.k, p.k, p.n, p.steps, n0, panel);
-    if (threadIdx.x < columns)
-      offset[threadIdx.x] = bias && n0 + int(threadIdx.x) < p.n
-                                ? float(bias[int64_t(s - 1) * p.n + n0 + threadIdx.x])
-                                : 0.f;
-#pragma unroll
-    for (int u = 0; u < Ahead; ++u) send(ring[u]);
-    __syncthreads();
-
-    for (int tile = wave; tile < tiles; tile += kRowWaves) {
-      f32x4 c[TM][TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int t = 0; t < TN; ++t) c[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int s0 = 0; s0 < p.steps; s0 += Ahead) {
-#pragma unroll
-        for (int u = 0; u < Ahead; ++u) {
-          const int st = s0 + u;
-          if (Tail && (st + 1) * step > p.k) {
-            const int left = min(p.k - st * step - piece * part, part);
-#pragma unroll
-            for (int j = 0; j < loads; ++j) ring[u][j] = settle<T, part, false>(ring[u][j], left);
-          }
-          Part b[TM][2];
-#pragma unroll
-          for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              turn[turn_place(8 * j + row8, piece >> 2, piece & 3)] = ring[u][2 * i + j];
-            wave_order();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) b[i][h] = turn[turn_place(i16, h, q)];
-            wave_order();
-          }
-          send(ring[u]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < TN; ++t) {
-              const Part a = panel[((2 * st + h) * TN + t) * 64 + lane];
-#pragma unroll
-              for (int i = 0; i < TM; ++i) c[i][t] = multiply<T>(a, b[i][h], c[i][t]);
-            }
-        }
-      }
-      // Lane group q has, of every 64 bytes of the columns, the q-th 16.
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int v = 0; v < 4 * TN; v += 2 * part) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            Part r;
-#pragma unroll
-            for (int j = 0; j < part; ++j) {
-              const int from_fragment = v + h * part + j;
-              r[j] = T(c[i][from_fragment >> 2][j & 3] +
-                       offset[4 * (v + h * part) + q * part + j]);
-            }
-            turn[turn_place(i16, h, q)] = r;
-          }
-          wave_order();
-          const int n = n0 + 4 * v + piece * part;
-          const int inside = min(p.n - n, part);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const bool row = first + tile * kRowTile + 16 * i + 8 * j + row8 < end;
-            const Part r = turn[turn_place(8 * j + row8, piece >> 2, piece & 3)];
-            store_valid<T, part>(out + int64_t(now[2 * i + j]) * p.n + n, row ? inside : 0, r);
-          }
-          wave_order();
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < loads; ++j) now[j] = sent_rows[j];
-    }
-  }
-}
-
 // `taken` is false where the matrix is too large to stay in LDS, or k less
 // than a lane's part of a fragment.
 template <typename T, bool Transposed>
@@ -257,10 +56,10 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
     p.workers = int(std::min<int64_t>(32 / panels * 8, ceil_div(rows, kRowTile)));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
     const size_t lds = size_t(p.steps) * 2 * tn.value * 1024;
-    auto* const kernel = &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value>;
+    auto* const kernel = &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value, kByGroup>;
     GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
     kernel<<<grid, kRowThreads, lds, stream>>>(static_cast<const T*>(x), static_cast<const T*>(w),
-                                               static_cast<const T*>(bias), g, p,
+                                               static_cast<const T*>(bias), g, p, {},
                                                static_cast<T*>(out));
     GS_LAUNCHED(name);
     return int(GS_OK);
