@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void few_inner_kernel(const T* __restrict
   float most = finite_size(values[lane]);
 #pragma unroll
   for (int step = 32; step; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
-  const float up = inner.begin_row(position, most, member ? s - 1 : -1, lane == 0);
+  const float up = inner.begin_row(position, most, lane == 0);
   if (4 * lane >= 32 * inner.chunks()) return;
   const float four[4] = {values[4 * lane], values[4 * lane + 1], values[4 * lane + 2],
                          values[4 * lane + 3]};
@@ -84,12 +84,13 @@ __global__ __launch_bounds__(kThreads) void few_adapted_kernel(
   const int output = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (output >= n) return;
   const int64_t row = row_at(g, position);
-  const int group = inner.groups[position];
+  const int s = find_segment(segments_of(g), position,
+                             [&](int i) { return int64_t(begin_of(g, i)); });
   // The narrow sum: a value of the rank to a lane.
   float narrow = 0.f;
-  if (group >= 0 && lane < inner.rank)
+  if (s > 0 && s <= g.groups && lane < inner.rank)
     narrow = inner.get(position, lane) *
-             float(up[(int64_t(group) * n + output) * inner.rank + lane]);
+             float(up[(int64_t(s - 1) * n + output) * inner.rank + lane]);
 #pragma unroll
   for (int step = 32; step; step >>= 1) narrow += __shfl_xor(narrow, step);
   float sum = wave_dot<T>(x + row * stride, w + int64_t(output) * k, k) + narrow;
@@ -138,27 +139,44 @@ template <typename T, bool Transposed, int Mode>
 int launch_rows(const char* name, const void* x, int64_t stride, const void* w, const void* bias,
                 const Grouping& g, int64_t k, int64_t n, const Adapters<T>& adapters, void* out,
                 hipStream_t stream, bool& taken) {
-  const int64_t steps = steps_of(sizeof(T), k);
+  // kAdapted's steps need no even number: the adapters' chunks are among them.
+  const int64_t steps = Mode == kInner ? steps_of(sizeof(T), k) : ceil_div(k, kStep<T>);
+  const int64_t chunks = Mode == kInner ? 0 : adapters.inner.chunks();
   int fragments;
   if constexpr (Mode == kInner) {
     fragments = n <= 32 ? 2 : 4;  // all of the rank, at most 64
     if (steps * 2048 * fragments > int64_t(kRowLds)) fragments = 0;
   } else {
+    // The adapter's matrix and what the waves turn their rows in lie beside.
     fragments = panel_fragments(sizeof(T), g.rows, k, n);
+    auto bytes = [&](int64_t of) {
+      return of * 1024 * (2 * steps + chunks * (sizeof(T) == 4 ? 2 : 1)) +
+             kRowWaves * 2048 + of * 64;
+    };
+    while (fragments && bytes(fragments) > 160 * 1024) fragments /= 2;
+    if (fragments < (sizeof(T) == 4 ? 2 : 4)) fragments = 0;
   }
+  // Steps under way: those that leave the fewest to be filled up.
+  int64_t ahead = Mode == kInner ? ahead_of(steps) : 4;
+  if constexpr (Mode == kAdapted)
+    for (int64_t of = 3; of >= 2; --of)
+      if (ceil_div(steps + chunks, of) * of < ceil_div(steps + chunks, ahead) * ahead) ahead = of;
+  const int64_t all = ceil_div(steps + chunks, ahead) * ahead;
   const int64_t panels = fragments ? ceil_div(n, 16 * fragments) : 0;
   taken = fragments && panels <= 32 && k >= kPart<T>;
   if (!taken) return GS_OK;
   using std::integral_constant;
-  auto launch = [&](auto tn, auto ahead, auto tail) {
-    GroupRows p{stride, int(k), int(n), int(panels), 0, int(steps)};
+  auto launch = [&](auto tn, auto under_way, auto tail) {
+    GroupRows p{stride, int(k), int(n), int(panels), 0, int(steps), int(all)};
     // Inner rows are bound by reading: as many workgroups as LDS lets run.
     const int64_t most = Mode == kInner ? (steps * 2048 * fragments > 48 * 1024 ? 256 : 512)
                                         : 32 / panels * 8;
     p.workers = int(std::min<int64_t>(most, ceil_div(g.rows, kRowTile)));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
-    const size_t lds = size_t(steps) * 2 * tn.value * 1024;
-    auto* const kernel = &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value, Mode>;
+    const size_t lds =
+        size_t(2 * steps + chunks * (sizeof(T) == 4 ? 2 : 1)) * tn.value * 1024;
+    auto* const kernel =
+        &group_rows_kernel<T, tn.value, under_way.value, Transposed, tail.value, Mode>;
     GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
     kernel<<<grid, kRowThreads, lds, stream>>>(static_cast<const T*>(x), static_cast<const T*>(w),
                                                static_cast<const T*>(bias), g, p, adapters,
@@ -168,17 +186,19 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
   };
   using one = integral_constant<int, 1>;
   using two = integral_constant<int, 2>;
+  using three = integral_constant<int, 3>;
   using four = integral_constant<int, 4>;
-  auto by_tail = [&](auto tn, auto ahead) {
-    return k != steps * kStep<T> ? launch(tn, ahead, std::true_type{})
-                                 : launch(tn, ahead, std::false_type{});
+  auto by_tail = [&](auto tn, auto under_way) {
+    return k != steps * kStep<T> ? launch(tn, under_way, std::true_type{})
+                                 : launch(tn, under_way, std::false_type{});
   };
   auto by_ahead = [&](auto tn) {
-    switch (ahead_of(steps)) {
-      case 1: return by_tail(tn, one{});
-      case 2: return by_tail(tn, two{});
-      default: return by_tail(tn, four{});
+    if constexpr (Mode == kInner) {
+      if (ahead == 1) return by_tail(tn, one{});
+    } else {
+      if (ahead == 3) return by_tail(tn, three{});
     }
+    return ahead == 2 ? by_tail(tn, two{}) : by_tail(tn, four{});
   };
   switch (fragments) {
     case 8:

@@ -22,7 +22,9 @@ struct GroupRows {
   int k, n;          // length of the sum and columns of C
   int panels;        // workgroups side by side, each with its columns of C
   int workers;       // workgroups to a panel
-  int steps;         // of the sum, see steps_of
+  int steps;         // of the sum, of 128 bytes of a row
+  int all;           // those, the adapters' chunks, and as many as make the
+                     // whole a multiple of those under way
 };
 
 // Where the line's place v lies in segment s, as a position: from the
@@ -48,7 +50,7 @@ __device__ __forceinline__ int panel_column(int t, int i) {
 // Sixteen rows' columns as inner rows: lane 16 q + i has row i.
 template <typename T, int TN>
 __device__ __forceinline__ void put_inner(const Adapters<T>& adapters, int position, int end,
-                                          int group, f32x4 (&c)[TN]) {
+                                          f32x4 (&c)[TN]) {
   const int q = (threadIdx.x & 63) >> 4;
   const Inner<T>& inner = adapters.inner;
   float most = 0.f;
@@ -64,7 +66,7 @@ __device__ __forceinline__ void put_inner(const Adapters<T>& adapters, int posit
     most = fmaxf(most, __shfl_xor(most, 32));
   }
   if (position >= end) return;
-  const float up = inner.begin_row(position, most, group, q == 0);
+  const float up = inner.begin_row(position, most, q == 0);
 #pragma unroll
   for (int t = 0; t < TN; ++t) {
     const int n = panel_column<T>(t, 4 * q);
@@ -74,92 +76,20 @@ __device__ __forceinline__ void put_inner(const Adapters<T>& adapters, int posit
   }
 }
 
-// Adds inner B_g to a wave's tile, whose first row is at `first`. The tile's
-// rows may be of several groups: each group's product is taken with the
-// others' inner rows as zeros, which costs 4 matrix instructions to a
-// fragment of columns where the tile's own product has `steps` times that.
+// The adapter's matrix of a group, [n][rank], as fragments beside those of the
+// panel: one to 16 columns and chunk for the 2-byte types, whose two parts of
+// an inner row meet the same values, two for float32.
 template <typename T, int TN>
-__device__ __forceinline__ void add_adapters(const Adapters<T>& adapters, const Grouping& g,
-                                             const GroupRows& p, int first, int end, int n0,
-                                             f32x4 (&c)[kRowTile / 16][TN]) {
-  constexpr int TM = kRowTile / 16, part = kPart<T>;
-  typedef vec<T, part> Part;
-  const Inner<T>& inner = adapters.inner;
-  const int lane = threadIdx.x & 63, q = lane >> 4, i16 = lane & 15;
-  int position[TM], group[TM];
-  float scale[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int at = first + 16 * i + i16;
-    position[i] = min(at, end - 1);
-    group[i] = at < end ? inner.groups[position[i]] : -1;
-    if constexpr (Inner<T>::scaled) scale[i] = inner.scales[position[i]];
-  }
-  if constexpr (Inner<T>::scaled) {
-    // Powers of two, and far enough inside float32.
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int t = 0; t < TN; ++t) c[i][t] *= 1.f / scale[i];
-  }
-  for (int chunk = 0; chunk < inner.chunks(); ++chunk) {
-    Part b[TM][2];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[i][h] = *reinterpret_cast<const Part*>(
-            inner.rows + position[i] * inner.stride() +
-            (chunk * kInnerBytes + h * 64 + q * 16) / int(sizeof(T)));
-    bool left[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) left[i] = group[i] >= 0;
-    for (;;) {
-      // The next group of the tile's rows.
-      int of = -1;
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const uint64_t lanes = __ballot(left[i]);
-        if (of < 0 && lanes)
-          of = __builtin_amdgcn_readlane(group[i], int(__builtin_ctzll(lanes)));
-      }
-      if (of < 0) break;
-      Part mine[TM][2];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const bool here = group[i] == of;
-        left[i] = left[i] && !here;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) mine[i][h] = here ? b[i][h] : Part(T(0));
-      }
-      const T* const matrix = adapters.matrix + int64_t(of) * p.n * inner.rank;
-#pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        const int n = n0 + panel_column<T>(t, i16);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          // The two parts of the 2-byte types meet the same values.
-          const int k = 32 * chunk + part * q + (sizeof(T) == 4 ? 16 * h : 0);
-          Part a;
-          if (sizeof(T) == 4 || h == 0)
-            a = load_valid<T, part>(matrix + int64_t(n) * inner.rank + k,
-                                    n < p.n ? inner.rank - k : 0);
-#pragma unroll
-          for (int i = 0; i < TM; ++i) c[i][t] = multiply<T>(a, mine[i][h], c[i][t]);
-          if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) c[i][t] = multiply<T>(a, mine[i][1], c[i][t]);
-            break;
-          }
-        }
-      }
-    }
-  }
-  if constexpr (Inner<T>::scaled) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int t = 0; t < TN; ++t) c[i][t] *= scale[i];
+__device__ __forceinline__ void stage_adapter(const T* __restrict__ matrix, int n, int rank,
+                                              int chunks, int n0, vec<T, kPart<T>>* lds) {
+  constexpr int part = kPart<T>, columns = 16 * TN, parts = 32 / part;
+  for (int id = threadIdx.x; id < columns * parts * chunks; id += kRowThreads) {
+    const int column = id / (parts * chunks), c = id - column * (parts * chunks);
+    const int k = c * part;
+    const vec<T, part> v = load_valid<T, part>(matrix + int64_t(n0 + column) * rank + k,
+                                               n0 + column < n ? rank - k : 0);
+    const FragmentPlace to = place_in_panel<T>(column);
+    lds[((c >> 2) * TN + to.t) * 64 + (c & 3) * 16 + to.i] = v;
   }
 }
 
@@ -192,26 +122,25 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part* const turn = turns[wave];
 
-  int s = Mode == kAdapted
-              ? 1
-              : find_segment(segments_of(g), from_line, [&](int i) { return stage_line(g, i); });
-  for (; Mode == kAdapted ? s == 1 : s < segments_of(g) && stage_line(g, s) < to_line; ++s) {
-    int first, end;
-    if constexpr (Mode == kAdapted) {  // one matrix for all rows
-      first = cut_at(int64_t(g.rows) * worker / p.workers, -1, 0, g.rows);
-      end = cut_at(int64_t(g.rows) * (worker + 1) / p.workers, -1, 0, g.rows);
-    } else {
-      const int low = begin_of(g, s), high = max(begin_of(g, s + 1), low);
-      first = cut_at(from_line, s, low, high);
-      end = cut_at(to_line, s, low, high);
-    }
+  bool staged = false;
+  int s = find_segment(segments_of(g), from_line, [&](int i) { return stage_line(g, i); });
+  for (; s < segments_of(g) && stage_line(g, s) < to_line; ++s) {
+    const int low = begin_of(g, s), high = max(begin_of(g, s + 1), low);
+    const int first = cut_at(from_line, s, low, high), end = cut_at(to_line, s, low, high);
     if (first >= end) continue;
-    if (Mode == kInner && (s == 0 || s > g.groups)) {
-      for (int64_t id = threadIdx.x; id < end - first; id += kRowThreads)
-        adapters.inner.begin_row(first + id, 0.f, -1, true);
-      continue;  // nothing reads the rest
+    const bool member = s > 0 && s <= g.groups;
+    if (Mode == kInner && !member) {
+      const Inner<T>& inner = adapters.inner;
+      const int fours = 8 * inner.chunks();
+      const float none[4] = {};
+      for (int64_t id = threadIdx.x; id < int64_t(end - first) * fours; id += kRowThreads) {
+        const int64_t position = first + id / fours;
+        const int n = int(id % fours) * 4;
+        inner.template put<4>(position, n, none, inner.begin_row(position, 0.f, n == 0));
+      }
+      continue;
     }
-    if (Mode == kByGroup && (s == 0 || s > g.groups)) {  // rows of no group
+    if (Mode == kByGroup && !member) {
       constexpr int pieces = columns / part;
       for (int64_t id = threadIdx.x; id < int64_t(end - first) * pieces; id += kRowThreads) {
         const int n = n0 + int(id % pieces) * part;
@@ -225,31 +154,42 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
     // What is on its way: the loop below takes ring[u] and sends for the step
     // `Ahead` later in its place. Past the wave's last tile it sends for that
     // one again, so that the number of loads under way is always the same.
-    // The rows' places are asked for a tile before they are needed.
-    int now[loads], sent_rows[loads], after[loads];
-    auto places = [&](int tile, int (&to)[loads]) {
-#pragma unroll
-      for (int j = 0; j < loads; ++j)  // positions past the end repeat the last one
-        to[j] = int(row_at(g, min(first + tile * kRowTile + 8 * j + row8, end - 1)));
+    // The rows' places are asked for a tile before they are needed; lane i
+    // has that of the tile's row i % 32.
+    auto places = [&](int tile) {  // positions past the end repeat the last one
+      return int(row_at(g, min(first + tile * kRowTile + (lane & 31), end - 1)));
     };
+    int sent = min(wave, tiles - 1), sent_step = 0;
+    int sent_rows = places(sent), now = sent_rows;
+    int after = places(min(sent + kRowWaves, tiles - 1));
     const T* from[loads];
     auto turn_to = [&]() {
 #pragma unroll
-      for (int j = 0; j < loads; ++j) from[j] = x + sent_rows[j] * p.stride + piece * part;
+      for (int j = 0; j < loads; ++j)
+        from[j] = x + __shfl(sent_rows, 8 * j + row8) * p.stride + piece * part;
     };
-    int sent = min(wave, tiles - 1), sent_step = 0;
     auto send = [&](Part (&to)[loads]) {
-      if (sent_step == p.steps) {
+      if (sent_step == p.all) {
         sent_step = 0;
         if (sent + kRowWaves < tiles) {
           sent += kRowWaves;
-#pragma unroll
-          for (int j = 0; j < loads; ++j) sent_rows[j] = after[j];
+          sent_rows = after;
         }
         turn_to();
-        places(min(sent + kRowWaves, tiles - 1), after);
+        after = places(min(sent + kRowWaves, tiles - 1));
       }
-      if (!Tail || (sent_step + 1) * step <= p.k) {
+      if (Mode == kAdapted && sent_step >= p.steps) {
+        const int chunk = min(sent_step - p.steps, adapters.inner.chunks() - 1);
+        const int in_tile = first + sent * kRowTile;
+        const T* const rows = adapters.inner.rows + in_tile * adapters.inner.stride() +
+                              (chunk * kInnerBytes) / int(sizeof(T));
+        const int last = min(end - in_tile, kRowTile) - 1;
+#pragma unroll
+        for (int j = 0; j < loads; ++j)
+          to[j] = load_packed<T, part>(
+              rows + uint32_t(min(8 * j + row8, last) * int(adapters.inner.stride()) +
+                              piece * part));
+      } else if (!Tail || (sent_step + 1) * step <= p.k) {
 #pragma unroll
         for (int j = 0; j < loads; ++j)
           to[j] = load_packed<T, part>(from[j] + sent_step * step);
@@ -262,19 +202,27 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
       ++sent_step;
     };
     Part ring[Ahead][loads];
-    places(sent, sent_rows);
-    places(min(sent + kRowWaves, tiles - 1), after);
-#pragma unroll
-    for (int j = 0; j < loads; ++j) now[j] = sent_rows[j];
     turn_to();
 
-    // The matrix, once no wave reads the one before.
+    // The matrix, once no wave reads the one before; the shared one of
+    // kAdapted once.
     __syncthreads();
-    stage_panel<T, TN, Transposed>(w + int64_t(s - 1) * p.n * p.k, p.k, p.n, p.steps, n0, panel);
-    if (threadIdx.x < columns)
-      offset[threadIdx.x] = bias && n0 + int(threadIdx.x) < p.n
-                                ? float(bias[int64_t(s - 1) * p.n + n0 + threadIdx.x])
-                                : 0.f;
+    if (Mode != kAdapted || !staged) {
+      const int64_t of = Mode == kAdapted ? 0 : s - 1;
+      stage_panel<T, TN, Transposed>(w + of * p.n * p.k, p.k, p.n, p.steps, n0, panel);
+      if (Mode != kInner && threadIdx.x < columns)
+        offset[threadIdx.x] = bias && n0 + int(threadIdx.x) < p.n
+                                  ? float(bias[of * p.n + n0 + threadIdx.x])
+                                  : 0.f;
+      staged = true;
+    }
+    Part* const narrow = panel + p.steps * 2 * TN * 64;
+    if constexpr (Mode == kAdapted) {
+      const int rank = adapters.inner.rank;
+      // Rows of no group meet zeros.
+      stage_adapter<T, TN>(adapters.matrix + int64_t(member ? s - 1 : 0) * p.n * rank,
+                           member ? p.n : 0, rank, adapters.inner.chunks(), n0, narrow);
+    }
 #pragma unroll
     for (int u = 0; u < Ahead; ++u) send(ring[u]);
     __syncthreads();
@@ -285,11 +233,17 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int t = 0; t < TN; ++t) c[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int s0 = 0; s0 < p.steps; s0 += Ahead) {
+      float scale[TM];
+      if constexpr (Mode == kAdapted && Inner<T>::scaled) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          scale[i] = adapters.inner.scales[min(first + tile * kRowTile + 16 * i + i16, end - 1)];
+      }
+      for (int s0 = 0; s0 < p.all; s0 += Ahead) {
 #pragma unroll
         for (int u = 0; u < Ahead; ++u) {
           const int st = s0 + u;
-          if (Tail && (st + 1) * step > p.k) {
+          if (Tail && (st + 1) * step > p.k && (Mode != kAdapted || st < p.steps)) {
             const int left = min(p.k - st * step - piece * part, part);
 #pragma unroll
             for (int j = 0; j < loads; ++j) ring[u][j] = settle<T, part, false>(ring[u][j], left);
@@ -306,22 +260,46 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
             wave_order();
           }
           send(ring[u]);
+          // Where the step's fragments lie, and those of its second half.
+          const Part* fragments = panel + 2 * st * TN * 64 + lane;
+          int second = TN * 64;
+          if constexpr (Mode == kAdapted) {
+            const int chunk = st - p.steps;
+            if (chunk >= adapters.inner.chunks()) continue;
+            if (chunk >= 0) {
+              if constexpr (sizeof(T) == 2) {
+                fragments = narrow + chunk * TN * 64 + lane;
+                second = 0;
+              }
+              if (Inner<T>::scaled && chunk == 0) {
+                // Powers of two, and far enough inside float32.
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                  for (int t = 0; t < TN; ++t) c[i][t] *= 1.f / scale[i];
+              }
+            }
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
-              const Part a = panel[((2 * st + h) * TN + t) * 64 + lane];
+              const Part a = fragments[h * second + t * 64];
 #pragma unroll
               for (int i = 0; i < TM; ++i) c[i][t] = multiply<T>(a, b[i][h], c[i][t]);
             }
         }
       }
-      if constexpr (Mode == kAdapted)
-        add_adapters<T, TN>(adapters, g, p, first + tile * kRowTile, end, n0, c);
+      if constexpr (Mode == kAdapted && Inner<T>::scaled) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int t = 0; t < TN; ++t) c[i][t] *= scale[i];
+      }
       if constexpr (Mode == kInner) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
-          put_inner<T, TN>(adapters, first + tile * kRowTile + 16 * i + i16, end, s - 1, c[i]);
+          put_inner<T, TN>(adapters, first + tile * kRowTile + 16 * i + i16, end, c[i]);
       }
       if constexpr (Mode != kInner) {
       // Lane group q has, of every 64 bytes of the columns, the q-th 16.
@@ -347,13 +325,13 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
           for (int j = 0; j < 2; ++j) {
             const bool row = first + tile * kRowTile + 16 * i + 8 * j + row8 < end;
             const Part r = turn[turn_place(8 * j + row8, piece >> 2, piece & 3)];
-            store_valid<T, part>(out + int64_t(now[2 * i + j]) * p.n + n, row ? inside : 0, r);
+            store_valid<T, part>(out + int64_t(__shfl(now, 16 * i + 8 * j + row8)) * p.n + n,
+                                 row ? inside : 0, r);
           }
           wave_order();
         }
       }
-#pragma unroll
-      for (int j = 0; j < loads; ++j) now[j] = sent_rows[j];
+        now = sent_rows;
       }
     }
   }

@@ -34,7 +34,6 @@ struct Inner {
   static constexpr bool scaled = std::is_same_v<T, f16>;
   T* rows;          // [positions, chunks, kInnerBytes]
   float* scales;    // [positions], float16 alone
-  int32_t* groups;  // [positions]: the row's group, -1 of none
   int rank;
 
   __host__ __device__ __forceinline__ int chunks() const { return (rank + 31) / 32; }
@@ -42,21 +41,18 @@ struct Inner {
     return int64_t(chunks()) * (kInnerBytes / sizeof(T));
   }
   static size_t bytes(int64_t count, int64_t rank) {
-    return size_t(count) * (size_t(ceil_div(rank, 32)) * kInnerBytes + 2 * sizeof(float));
+    return size_t(count) * (size_t(ceil_div(rank, 32)) * kInnerBytes + sizeof(float));
   }
   static Inner at(void* memory, int64_t count, int64_t rank) {
-    Inner i{static_cast<T*>(memory), nullptr, nullptr, int(rank)};
+    Inner i{static_cast<T*>(memory), nullptr, int(rank)};
     i.scales = reinterpret_cast<float*>(static_cast<char*>(memory) +
                                         size_t(count) * size_t(i.chunks()) * kInnerBytes);
-    i.groups = reinterpret_cast<int32_t*>(i.scales + count);
     return i;
   }
 
-  // Writes the row's group and scale (`writes`: one lane does), whose largest
-  // finite magnitude is `most`; returns what its values are multiplied by.
-  __device__ __forceinline__ float begin_row(int64_t position, float most, int group,
-                                             bool writes) const {
-    if (writes) groups[position] = group;
+  // Writes the scale of a row (`writes`: one lane does) whose largest finite
+  // magnitude is `most`; returns what its values are multiplied by.
+  __device__ __forceinline__ float begin_row(int64_t position, float most, bool writes) const {
     if constexpr (scaled) {
       // most = m 2^e with 1/2 <= m < 1; between 2^-60 and 2^60 both powers
       // stay far inside float32.
@@ -307,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void group_tile_kernel(
       most = fmaxf(most, __shfl_xor(most, 16));
       most = fmaxf(most, __shfl_xor(most, 32));
       if (position >= end) continue;
-      const float up = inner.begin_row(position, most, int(member ? group : -1), lane >> 4 == 0);
+      const float up = inner.begin_row(position, most, lane >> 4 == 0);
       if (n >= 32 * inner.chunks()) continue;
       inner.template put<16>(position, int(n), row, up);
     } else {

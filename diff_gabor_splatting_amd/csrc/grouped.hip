@@ -52,7 +52,8 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
   if (!taken) return GS_OK;
   using std::integral_constant;
   auto launch = [&](auto tn, auto ahead, auto tail) {
-    GroupRows p{stride, int(k), int(n), int(panels), 0, int(steps_of(sizeof(T), k))};
+    const int steps = int(steps_of(sizeof(T), k));
+    GroupRows p{stride, int(k), int(n), int(panels), 0, steps, steps};
     p.workers = int(std::min<int64_t>(32 / panels * 8, ceil_div(rows, kRowTile)));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
     const size_t lds = size_t(p.steps) * 2 * tn.value * 1024;
