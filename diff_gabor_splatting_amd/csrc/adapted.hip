@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(Inner<T> inner,
                                                               Grouping g, NarrowSum p,
                                                               float* __restrict__ partial,
                                                               T* __restrict__ out) {
-  constexpr int steps = kNarrowRows / 4;
+  constexpr int fours = kNarrowRows / 4;  // one row of each to a lane group
   const int64_t number = int64_t(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
   const int block = __builtin_amdgcn_readfirstlane(int(number % p.blocks));
   const int share = __builtin_amdgcn_readfirstlane(int(number / p.blocks));
@@ -258,34 +258,61 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(Inner<T> inner,
     for (int t = 0; t < R; ++t)
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int64_t id[steps];
-    auto find = [&](int first) {
-#pragma unroll
-      for (int i = 0; i < steps; ++i) id[i] = row_at(g, min(first + 4 * i + q, at.end - 1));
+    // Rows and inner rows of a step are on their way while the step before is
+    // multiplied; the rows' places, 64 at a time, a whole 64 before.
+    struct Step {
+      vec<T, 8> rows[fours];
+      typename Inner<T>::Raw inner[fours][R];
+      float scales[fours];
     };
-    if (at.next < at.end) find(at.next);
-    for (int first = at.next; first < at.end; first += kNarrowRows) {
-      vec<T, 8> raw[steps];
-      float a[steps][R];
-#pragma unroll
-      for (int i = 0; i < steps; ++i) {
-        const int position = first + 4 * i + q;
-        const bool live = position < at.end;
-        raw[i] = load_edge<T, 8, Narrow>(rows + id[i] * p.stride + column, live ? valid : 0);
-#pragma unroll
-        for (int t = 0; t < R; ++t) a[i][t] = live ? inner.get(position, 16 * t + i16) : 0.f;
+    const int first = at.next, count = at.end - at.next;
+    auto find = [&](int of) {
+      return count > 0 ? int(row_at(g, first + min(64 * of + lane, count - 1))) : 0;
+    };
+    int id = 0, next_id = find(0);
+    auto load = [&](Step& to, int step) {
+      if (step % 4 == 0) {
+        id = next_id;
+        next_id = find(step / 4 + 1);
       }
-      if (first + kNarrowRows < at.end) find(first + kNarrowRows);
 #pragma unroll
-      for (int i = 0; i < steps; ++i) {
-        const bool live = first + 4 * i + q < at.end;
-        const vec<T, 8> v = settle<T, 8, Narrow>(raw[i], live ? valid : 8);
+      for (int i = 0; i < fours; ++i) {
+        const int place = step * kNarrowRows + 4 * i + q;
+        const int64_t row = __shfl(id, place % 64);
+        const bool live = place < count;
+        to.rows[i] = load_edge<T, 8, Narrow>(rows + row * p.stride + column, live ? valid : 0);
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+          to.inner[i][t] = inner.raw(first + min(place, count - 1), 16 * t + i16);
+        if constexpr (Inner<T>::scaled)
+          to.scales[i] = inner.scales[first + min(place, count - 1)];
+      }
+    };
+    auto multiply_step = [&](const Step& of, int step) {
+#pragma unroll
+      for (int i = 0; i < fours; ++i) {
+        const bool live = step * kNarrowRows + 4 * i + q < count;
+        const vec<T, 8> v = settle<T, 8, Narrow>(of.rows[i], live ? valid : 8);
+        float a[R];
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+          a[t] = live ? of.inner[i][t].sum() : 0.f;
+          if constexpr (Inner<T>::scaled) a[t] *= of.scales[i];
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int t = 0; t < R; ++t)
-            c[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][t], float(v[j]), c[t][j], 0, 0, 0);
+            c[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], float(v[j]), c[t][j], 0, 0, 0);
       }
+    };
+    Step ahead[2];
+    if (count > 0) load(ahead[0], 0);
+    for (int step = 0; step * kNarrowRows < count; step += 2) {
+      load(ahead[1], step + 1);
+      multiply_step(ahead[0], step);
+      load(ahead[0], step + 2);
+      multiply_step(ahead[1], step + 1);
     }
     // Lane 16 q + i holds ranks 16 t + 4 q .. + 3 of columns 8 i .. 8 i + 7.
     if (at.s < 1 || at.s > g.groups) continue;

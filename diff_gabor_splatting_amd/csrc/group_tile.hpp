@@ -89,12 +89,26 @@ struct Inner {
       if constexpr (sizeof(T) == 2) *reinterpret_cast<vec<T, 4>*>(to + 32 + h) = low;
     }
   }
-  // Value n of a row.
-  __device__ __forceinline__ float get(int64_t position, int n) const {
+  // Value n of a row as it is kept, but for its row's scale.
+  struct Raw {
+    T parts[4 / sizeof(T)];
+    __device__ __forceinline__ float sum() const {
+      if constexpr (sizeof(T) == 4)
+        return parts[0];
+      else
+        return float(parts[0]) + float(parts[1]);
+    }
+  };
+  __device__ __forceinline__ Raw raw(int64_t position, int n) const {
     const T* const from =
         rows + position * stride() + n / 32 * (kInnerBytes / int(sizeof(T))) + n % 32;
-    if constexpr (sizeof(T) == 4) return float(from[0]);
-    const float sum = float(from[0]) + float(from[32]);
+    if constexpr (sizeof(T) == 4)
+      return {{from[0]}};
+    else
+      return {{from[0], from[32]}};
+  }
+  __device__ __forceinline__ float get(int64_t position, int n) const {
+    const float sum = raw(position, n).sum();
     return scaled ? sum * scales[position] : sum;
   }
 };
