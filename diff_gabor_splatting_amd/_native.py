@@ -270,7 +270,6 @@ _SIGNATURES = {
         + [_c_size, _c_ptr],
     ),
     "gs_adapted_linear_inner_size": (_c_size, [_c_i64] * 2),
-    "gs_adapted_linear_inner_grad_size": (_c_size, [_c_int] + [_c_i64] * 4),
     "gs_adapted_linear_forward": (
         _c_int,
         [_c_int, _c_ptr, _c_i64] + [_c_ptr] * 4 + [_c_float] + [_c_ptr] * 2 + [_c_i64] * 5

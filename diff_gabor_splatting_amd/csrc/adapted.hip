@@ -118,21 +118,6 @@ int launch_tiles(const char* name, const void* x, int64_t stride, const void* w,
 // --------------------------------------------------------------------------
 // Inner rows, y and dx with the matrix in LDS and the rows streamed past it
 
-// down [groups, rank, features] as [groups, features, rank], the layout in
-// which the product with the inner rows reads it.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void turn_kernel(const T* __restrict__ down, int64_t size,
-                                                        int rank, int features,
-                                                        T* __restrict__ out) {
-  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < size;
-       i += int64_t(gridDim.x) * kThreads) {
-    const int64_t row = i / features;  // of all groups' ranks
-    const int column = int(i - row * features);
-    const int64_t group = row / rank;
-    out[(group * features + column) * rank + (row - group * rank)] = down[i];
-  }
-}
-
 // `taken` is false where the matrix is too large to stay in LDS, or k less
 // than a lane's part of a fragment.
 template <typename T, bool Transposed, int Mode>
@@ -224,19 +209,30 @@ constexpr int64_t kNarrowCost = 32;  // of a group's sums, in rows
 constexpr int kNarrowColumns = 128;
 constexpr int kNarrowRows = 16;  // of a step
 
+template <typename T>
 struct NarrowSum {
+  Inner<T> inner;
+  const T* rows;
   int64_t stride;
+  float* partial;
+  T* out;
   int width, blocks, shares;
+  bool turned;  // the result is [width, rank] (dB), not [rank, width] (dA)
 };
 
-// Turned: the result is [width, rank] (dB), not [rank, width] (dA). R: 16s of
-// the rank.
-template <typename T, int R, bool Turned, bool Narrow>
-__global__ __launch_bounds__(kThreads) void narrow_sum_kernel(Inner<T> inner,
-                                                              const T* __restrict__ rows,
-                                                              Grouping g, NarrowSum p,
-                                                              float* __restrict__ partial,
-                                                              T* __restrict__ out) {
+template <typename T>
+struct NarrowSums {
+  NarrowSum<T> of[2];
+};
+
+// blockIdx.y: which of two sums. R: 16s of the rank.
+template <typename T, int R, bool Narrow>
+__global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums, Grouping g) {
+  const NarrowSum<T> p = sums.of[blockIdx.y];
+  const Inner<T> inner = p.inner;
+  const T* __restrict__ const rows = p.rows;
+  float* __restrict__ const partial = p.partial;
+  T* __restrict__ const out = p.out;
   constexpr int fours = kNarrowRows / 4;  // one row of each to a lane group
   const int64_t number = int64_t(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
   const int block = __builtin_amdgcn_readfirstlane(int(number % p.blocks));
@@ -323,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(Inner<T> inner,
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       const int r0 = 16 * t + 4 * q;
-      if constexpr (Turned) {
+      if (p.turned) {
         const int left = max(0, min(inner.rank - r0, 4));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -358,29 +354,41 @@ int64_t narrow_shares(const Grouping& g, int64_t width) {
   return std::min(shares, ceil_div(line_length(g, kNarrowCost), 2 * kNarrowCost));
 }
 
-template <typename T, bool Turned>
-int launch_narrow(const char* name, const Inner<T>& inner, const void* rows, int64_t stride,
-                  const Grouping& g, int64_t width, float* partial, void* out,
+// dA and dB in one launch, and their joins in another: with few rows a launch
+// is most of the time.
+template <typename T>
+int launch_narrow(const char* name, NarrowSum<T>* sums, int count, const Grouping& g,
                   hipStream_t stream) {
-  const NarrowSum p{stride, int(width), int(ceil_div(width, kNarrowColumns)),
-                    int(narrow_shares(g, width))};
-  const dim3 grid{unsigned(ceil_div(int64_t(p.blocks) * p.shares, kThreads / 64))};
+  NarrowSums<T> both{};
+  Join<T> joins[2];
+  int64_t waves = 0;
+  bool narrow = false;
+  for (int i = 0; i < count; ++i) {
+    NarrowSum<T>& p = sums[i];
+    p.blocks = int(ceil_div(p.width, kNarrowColumns));
+    p.shares = int(narrow_shares(g, p.width));
+    waves = std::max(waves, int64_t(p.blocks) * p.shares);
+    narrow = narrow || p.width < 8;
+    both.of[i] = p;
+    joins[i] = {p.partial, p.out, nullptr, kNarrowCost, p.shares,
+                int64_t(p.inner.rank) * p.width, 0};
+  }
+  const dim3 grid{unsigned(ceil_div(waves, kThreads / 64)), unsigned(count)};
   auto launch = [&](auto r, auto narrow) {
-    narrow_sum_kernel<T, r.value, Turned, narrow.value><<<grid, kThreads, 0, stream>>>(
-        inner, static_cast<const T*>(rows), g, p, partial, static_cast<T*>(out));
+    narrow_sum_kernel<T, r.value, narrow.value><<<grid, kThreads, 0, stream>>>(both, g);
   };
   auto by_width = [&](auto r) {
-    width < 8 ? launch(r, std::true_type{}) : launch(r, std::false_type{});
+    narrow ? launch(r, std::true_type{}) : launch(r, std::false_type{});
   };
-  if (inner.rank <= 16)
+  const int rank = sums[0].inner.rank;
+  if (rank <= 16)
     by_width(std::integral_constant<int, 1>{});
-  else if (inner.rank <= 32)
+  else if (rank <= 32)
     by_width(std::integral_constant<int, 2>{});
   else
     by_width(std::integral_constant<int, 4>{});
   GS_LAUNCHED(name);
-  return launch_join(partial, g, kNarrowCost, p.shares, inner.rank * width, 0,
-                     static_cast<T*>(out), static_cast<T*>(nullptr), stream);
+  return launch_joins(joins, count, g, stream);
 }
 
 int check_adapted(const char* name, int32_t dtype, const void* offsets, int64_t rows,
@@ -408,16 +416,6 @@ size_t gs_adapted_linear_inner_size(int64_t rows, int64_t rank) {
   using namespace gs;
   if (rows <= 0 || rank <= 0 || rank > kMostRank) return 0;
   return Inner<float>::bytes(rows, rank);
-}
-
-size_t gs_adapted_linear_inner_grad_size(int32_t dtype, int64_t rows, int64_t groups,
-                                         int64_t features, int64_t rank) {
-  using namespace gs;
-  if (groups <= 0 || groups > kMostGroupsOfRows || features <= 0 || features > kMostFeatures)
-    return 0;
-  const size_t size = gs_adapted_linear_inner_size(rows, rank);
-  // And down, turned.
-  return size ? size + size_t(groups * rank * features) * (dtype == GS_FLOAT32 ? 4 : 2) : 0;
 }
 
 int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, const void* weight,
@@ -484,8 +482,7 @@ int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
   if (rows == 0) return GS_OK;
   GS_REQUIRE(grad_y && up && (!grad_x || (weight && down)), GS_ERR_ARGUMENT,
              "null pointer passed to %s", name);
-  GS_REQUIRE(inner_grad && inner_bytes >= gs_adapted_linear_inner_grad_size(
-                                              dtype, rows, groups, features, rank),
+  GS_REQUIRE(inner_grad && inner_bytes >= gs_adapted_linear_inner_size(rows, rank),
              GS_ERR_WORKSPACE, "inner rows too small for %s", name);
   const Grouping g = grouping(order, offsets, rows, groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -493,7 +490,7 @@ int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
     using T = decltype(zero);
     const Inner<T> held = Inner<T>::at(inner_grad, rows, rank);
     const Adapters<T> first{held, nullptr, scale};
-    Adapters<T> second{held, static_cast<const T*>(down), 0.f};
+    const Adapters<T> second{held, static_cast<const T*>(down), 0.f};
     bool taken = false;
     GS_CHECK((launch_rows<T, true, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
                                            rank, first, nullptr, s, taken)));
@@ -501,20 +498,9 @@ int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
       GS_CHECK((launch_tiles<T, false, kInner>(name, grad_y, grad_stride, up, nullptr, g, outputs,
                                                rank, first, nullptr, s)));
     if (!grad_x) return int(GS_OK);
-    if (panel_fragments(sizeof(T), rows, outputs, features) && outputs >= kPart<T>) {
-      T* const turned = reinterpret_cast<T*>(static_cast<char*>(inner_grad) +
-                                             Inner<T>::bytes(rows, rank));
-      const int64_t size = groups * rank * features;
-      turn_kernel<T><<<dim3{unsigned(std::min<int64_t>(ceil_div(size, kThreads), 1 << 16))},
-                       kThreads, 0, s>>>(static_cast<const T*>(down), size, int(rank),
-                                         int(features), turned);
-      GS_LAUNCHED(name);
-      second.matrix = turned;
-      GS_CHECK((launch_rows<T, true, kAdapted>(name, grad_y, grad_stride, weight, nullptr, g,
-                                               outputs, features, second, grad_x, s, taken)));
-      if (taken) return int(GS_OK);
-      second.matrix = static_cast<const T*>(down);
-    }
+    GS_CHECK((launch_rows<T, true, kAdapted>(name, grad_y, grad_stride, weight, nullptr, g,
+                                             outputs, features, second, grad_x, s, taken)));
+    if (taken) return int(GS_OK);
     return launch_tiles<T, false, kAdapted>(name, grad_y, grad_stride, weight, nullptr, g,
                                             outputs, features, second, grad_x, s);
   });
@@ -532,7 +518,7 @@ size_t gs_adapted_linear_backward_adapters_workspace_size(int64_t rows, int64_t 
     const int64_t shares = narrow_shares(g, width);
     return shares == 1 ? 0 : size_t(2 * shares) * size_t(rank * width) * sizeof(float);
   };
-  return std::max(bytes(features), bytes(outputs));
+  return bytes(features) + bytes(outputs);
 }
 
 int gs_adapted_linear_backward_adapters(int32_t dtype, const void* grad_y, int64_t grad_stride,
@@ -565,13 +551,20 @@ int gs_adapted_linear_backward_adapters(int32_t dtype, const void* grad_y, int64
   float* const partial = static_cast<float*>(workspace);
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
+    NarrowSum<T> sums[2];
+    int count = 0;
     if (grad_down)
-      GS_CHECK((launch_narrow<T, false>(name, Inner<T>::at(const_cast<void*>(inner_grad), rows, rank),
-                                        x, row_stride, g, features, partial, grad_down, s)));
-    if (grad_up)
-      GS_CHECK((launch_narrow<T, true>(name, Inner<T>::at(const_cast<void*>(inner), rows, rank),
-                                       grad_y, grad_stride, g, outputs, partial, grad_up, s)));
-    return int(GS_OK);
+      sums[count++] = {Inner<T>::at(const_cast<void*>(inner_grad), rows, rank),
+                       static_cast<const T*>(x), row_stride, partial,
+                       static_cast<T*>(grad_down), int(features), 0, 0, false};
+    if (grad_up) {
+      const int64_t shares = narrow_shares(g, features);
+      sums[count++] = {Inner<T>::at(const_cast<void*>(inner), rows, rank),
+                       static_cast<const T*>(grad_y), grad_stride,
+                       partial + (shares == 1 ? 0 : 2 * shares * rank * features),
+                       static_cast<T*>(grad_up), int(outputs), 0, 0, true};
+    }
+    return launch_narrow(name, sums, count, g, s);
   });
 }
 

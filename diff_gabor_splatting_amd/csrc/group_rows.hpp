@@ -76,20 +76,46 @@ __device__ __forceinline__ void put_inner(const Adapters<T>& adapters, int posit
   }
 }
 
-// The adapter's matrix of a group, [n][rank], as fragments beside those of the
-// panel: one to 16 columns and chunk for the 2-byte types, whose two parts of
-// an inner row meet the same values, two for float32.
-template <typename T, int TN>
-__device__ __forceinline__ void stage_adapter(const T* __restrict__ matrix, int n, int rank,
-                                              int chunks, int n0, vec<T, kPart<T>>* lds) {
-  constexpr int part = kPart<T>, columns = 16 * TN, parts = 32 / part;
-  for (int id = threadIdx.x; id < columns * parts * chunks; id += kRowThreads) {
-    const int column = id / (parts * chunks), c = id - column * (parts * chunks);
-    const int k = c * part;
-    const vec<T, part> v = load_valid<T, part>(matrix + int64_t(n0 + column) * rank + k,
-                                               n0 + column < n ? rank - k : 0);
+// The adapter's matrix of a group, [n][rank] or (Transposed) [rank][n], as
+// fragments beside those of the panel: one to 16 columns and chunk for the
+// 2-byte types, whose two parts of an inner row meet the same values, two for
+// float32. Without `some` it is zeros.
+template <typename T, int TN, bool Transposed>
+__device__ __forceinline__ void stage_adapter(const T* __restrict__ matrix, bool some, int n,
+                                              int rank, int chunks, int n0,
+                                              vec<T, kPart<T>>* lds) {
+  constexpr int part = kPart<T>, columns = 16 * TN;
+  const int parts = chunks * (32 / part);
+  auto place = [&](int column, int c) {
     const FragmentPlace to = place_in_panel<T>(column);
-    lds[((c >> 2) * TN + to.t) * 64 + (c & 3) * 16 + to.i] = v;
+    return ((c >> 2) * TN + to.t) * 64 + (c & 3) * 16 + to.i;
+  };
+  if constexpr (!Transposed) {
+    for (int id = threadIdx.x; id < columns * parts; id += kRowThreads) {
+      const int column = id / parts, c = id - column * parts;
+      lds[place(column, c)] =
+          load_valid<T, part>(matrix + int64_t(n0 + column) * rank + c * part,
+                              some && n0 + column < n ? rank - c * part : 0);
+    }
+  } else {
+    // Four columns of `part` ranks at a time, turned in registers.
+    for (int id = threadIdx.x; id < columns / 4 * parts; id += kRowThreads) {
+      const int c = id / (columns / 4), column = 4 * (id - c * (columns / 4));
+      vec<T, 4> v[part];
+#pragma unroll
+      for (int j = 0; j < part; ++j) {
+        const int k = c * part + j;
+        v[j] = load_valid<T, 4>(matrix + int64_t(k) * n + n0 + column,
+                                some && k < rank ? n - n0 - column : 0);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        vec<T, part> turned;
+#pragma unroll
+        for (int j = 0; j < part; ++j) turned[j] = v[j][b];
+        lds[place(column, c) + b] = turned;
+      }
+    }
   }
 }
 
@@ -220,8 +246,9 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
     if constexpr (Mode == kAdapted) {
       const int rank = adapters.inner.rank;
       // Rows of no group meet zeros.
-      stage_adapter<T, TN>(adapters.matrix + int64_t(member ? s - 1 : 0) * p.n * rank,
-                           member ? p.n : 0, rank, adapters.inner.chunks(), n0, narrow);
+      stage_adapter<T, TN, Transposed>(
+          adapters.matrix + int64_t(member ? s - 1 : 0) * p.n * rank, member, p.n, rank,
+          adapters.inner.chunks(), n0, narrow);
     }
 #pragma unroll
     for (int u = 0; u < Ahead; ++u) send(ring[u]);

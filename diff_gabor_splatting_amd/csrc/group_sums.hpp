@@ -48,10 +48,24 @@ struct Share {
 
 constexpr int kJoinThreads = 256;
 
-struct JoinOf {
+// Parts [shares, 2 (head, tail), weights + biases] of a group's values, dW's and
+// then db's; either result may be null.
+template <typename T>
+struct Join {
+  const float* partial;
+  T* dw;
+  T* db;
   int64_t cost, shares;
-  int64_t weights, biases;  // values of a group: dW's, then db's
-  bool by_border;
+  int64_t weights, biases;
+  __host__ __device__ bool by_border(const Grouping& g) const { return shares - 1 < g.groups; }
+  __host__ __device__ int64_t each(const Grouping& g) const {
+    return by_border(g) ? shares - 1 : g.groups;
+  }
+};
+
+template <typename T>
+struct Joins {
+  Join<T> of[2];
 };
 
 // Adds the parts of the groups that lie in several shares. blockIdx.y: a
@@ -60,20 +74,23 @@ struct JoinOf {
 // 4 kJoinThreads / Slices values of dW and db at a time, for which each slice of
 // the threads adds every Slices-th part.
 template <typename T, int Slices>
-__global__ __launch_bounds__(kJoinThreads) void group_join_kernel(const float* __restrict__ partial,
-                                                              Grouping g, JoinOf p,
-                                                              T* __restrict__ dw,
-                                                              T* __restrict__ db) {
+__global__ __launch_bounds__(kJoinThreads) void group_join_kernel(Joins<T> joins, Grouping g) {
   constexpr int columns = kJoinThreads / Slices;
   __shared__ vec<float, 4> sums[Slices][columns];
+  const Join<T> p = joins.of[blockIdx.z];
+  const float* __restrict__ const partial = p.partial;
+  T* __restrict__ const dw = p.dw;
+  T* __restrict__ const db = p.db;
+  const bool by_border = p.by_border(g);
+  if (blockIdx.y >= p.each(g)) return;
   const int64_t length = line_length(g, p.cost);
   int s = blockIdx.y + 1;
   int64_t border = s;
-  if (p.by_border)
+  if (by_border)
     s = find_segment(segments_of(g), length * border / p.shares,
                      [&](int i) { return line_at(g, p.cost, i); });
   const int64_t low = line_at(g, p.cost, s), high = line_at(g, p.cost, s + 1);
-  if (!p.by_border) {  // the first border behind `low`
+  if (!by_border) {  // the first border behind `low`
     border = ((low + 1) * p.shares + length - 1) / length;
   }
   const int64_t v = length * border / p.shares;
@@ -115,28 +132,36 @@ __global__ __launch_bounds__(kJoinThreads) void group_join_kernel(const float* _
   }
 }
 
-// partial: [shares, 2 (head, tail), weights + biases]. Either result may be null.
+// Joins up to two results in one launch; those of one share have no parts.
 template <typename T>
-int launch_join(const float* partial, const Grouping& g, int64_t cost, int64_t shares,
-                int64_t weights, int64_t biases, T* dw, T* db, hipStream_t stream) {
-  if (shares == 1) return GS_OK;
-  // Workgroups go on to further values: those of the groups that lie in one
-  // share have nothing to do, and a workgroup to each 64 values and border
-  // (100k x 256 -> 256 in 64 groups: 32,000) took 180 us to find that out.
-  const JoinOf p{cost, shares, weights, biases, shares - 1 < g.groups};
-  const int64_t each = p.by_border ? shares - 1 : g.groups;
-  auto join = [&](auto slices) {
-    const int64_t chunks = ceil_div(weights + biases, 4 * kJoinThreads / slices.value);
-    const dim3 grid{unsigned(std::min(chunks, ceil_div(4096, each))), unsigned(each)};
-    group_join_kernel<T, slices.value><<<grid, kJoinThreads, 0, stream>>>(partial, g, p, dw, db);
+int launch_joins(const Join<T>* join, int count, const Grouping& g, hipStream_t stream) {
+  Joins<T> joins{};
+  int some = 0;
+  int64_t each = 0, values = 0, parts = 0;
+  for (int i = 0; i < count; ++i) {
+    if (join[i].shares == 1) continue;
+    joins.of[some++] = join[i];
+    each = std::max(each, join[i].each(g));
+    values = std::max(values, join[i].weights + join[i].biases);
+    parts = std::max(parts, join[i].shares);
+  }
+  if (!some) return GS_OK;
+  auto launch = [&](auto slices) {
+    // Workgroups go on to further values: those of the groups that lie in one
+    // share have nothing to do, and a workgroup to each 64 values and border
+    // (100k x 256 -> 256 in 64 groups: 32,000) took 180 us to find that out.
+    const int64_t chunks = ceil_div(values, 4 * kJoinThreads / slices.value);
+    const dim3 grid{unsigned(std::min(chunks, ceil_div(4096, each))), unsigned(each),
+                    unsigned(some)};
+    group_join_kernel<T, slices.value><<<grid, kJoinThreads, 0, stream>>>(joins, g);
   };
   // As many slices as there may be parts to add.
-  if (shares < 4 * int64_t(g.groups))
-    join(std::integral_constant<int, 1>{});
-  else if (shares < 16 * int64_t(g.groups))
-    join(std::integral_constant<int, 4>{});
+  if (parts < 4 * int64_t(g.groups))
+    launch(std::integral_constant<int, 1>{});
+  else if (parts < 16 * int64_t(g.groups))
+    launch(std::integral_constant<int, 4>{});
   else
-    join(std::integral_constant<int, 16>{});
+    launch(std::integral_constant<int, 16>{});
   GS_LAUNCHED("group_join_kernel");
   return GS_OK;
 }

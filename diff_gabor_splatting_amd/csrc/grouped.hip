@@ -388,10 +388,10 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
 }
 
 // How dW's sums are cut: fragments of a wave's tile along the outputs and the
-// features, positions of a step, and shares of the line. As for one group:
+// features, and shares of the line. As for one group:
 // the widest tiles where they leave little empty and there are rows enough.
 struct GroupSumPlan {
-  int a, b, step;
+  int a, b;
   int64_t tiles_m, tiles_n, shares;
 };
 
@@ -403,7 +403,6 @@ GroupSumPlan sum_plan(size_t size, const Grouping& g, int64_t features, int64_t 
                      double(g.rows) * double(outputs) * double(features) >= 2e10;
   p.a = large ? 8 : outputs <= 64 ? 2 : 4;
   p.b = large ? 4 : features <= 64 ? 1 : 2;
-  p.step = p.a == 2 ? 64 : 32;
   p.tiles_m = ceil_div(outputs, 32 * p.a);
   p.tiles_n = ceil_div(features, 64 * p.b);
   const int64_t tiles = p.tiles_m * p.tiles_n;
@@ -533,7 +532,7 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     T* const db = static_cast<T*>(grad_bias);
     float* const partial = static_cast<float*>(workspace);
     auto launch = [&](auto a, auto b, auto narrow) {
-      constexpr int step = a.value == 2 ? 64 : 32;
+      constexpr int step = a.value == 2 || (a.value == 4 && sizeof(T) == 2) ? 64 : 32;
       constexpr size_t lds = 2 * step * (32 * a.value + 16 + 64 * b.value + 16) * sizeof(T);
       auto* const kernel = &group_sum_kernel<T, a.value, b.value, step, narrow.value>;
       GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
@@ -559,7 +558,8 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     if constexpr (sizeof(T) == 2)
       if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}, wide{}));
     if (plan.shares == 1) return int(GS_OK);
-    return launch_join(partial, g, kGroupCost, plan.shares, outputs * features, outputs, dw, db, s);
+    const Join<T> join{partial, dw, db, kGroupCost, plan.shares, outputs * features, outputs};
+    return launch_joins(&join, 1, g, s);
   });
 }
 

@@ -37,7 +37,6 @@ struct Api {
   decltype(&gs_grouped_linear_backward_weight_workspace_size) grouped_workspace = nullptr;
   decltype(&gs_grouped_linear_backward_weight) grouped_backward_weight = nullptr;
   decltype(&gs_adapted_linear_inner_size) adapted_inner = nullptr;
-  decltype(&gs_adapted_linear_inner_grad_size) adapted_inner_grad = nullptr;
   decltype(&gs_adapted_linear_forward) adapted_forward = nullptr;
   decltype(&gs_adapted_linear_backward_input) adapted_backward_input = nullptr;
   decltype(&gs_adapted_linear_backward_adapters_workspace_size) adapted_workspace = nullptr;
@@ -671,8 +670,7 @@ struct AdaptedLinear : torch::autograd::Function<AdaptedLinear> {
     if (ctx->needs_input_grad(2)) da = at::empty(a.sizes(), grad.options());
     if (ctx->needs_input_grad(3)) du = at::empty(u.sizes(), grad.options());
     if (dx.defined() || da.defined()) {
-      back = workspace(api.adapted_inner_grad(type, g.rows, groups.count(), features, rank),
-                       grad.device());
+      back = workspace(api.adapted_inner(g.rows, rank), grad.device());
       check(api.adapted_backward_input(
           type, g.data(), g.stride, w.data_ptr(), a.data_ptr(), u.data_ptr(),
           float(ctx->saved_data["scale"].toDouble()), groups.places(), groups.begins(), g.rows,
@@ -754,7 +752,6 @@ void bind_layers(const py::dict& table) {
   take(table, "gs_grouped_linear_backward_weight_workspace_size", next.grouped_workspace);
   take(table, "gs_grouped_linear_backward_weight", next.grouped_backward_weight);
   take(table, "gs_adapted_linear_inner_size", next.adapted_inner);
-  take(table, "gs_adapted_linear_inner_grad_size", next.adapted_inner_grad);
   take(table, "gs_adapted_linear_forward", next.adapted_forward);
   take(table, "gs_adapted_linear_backward_input", next.adapted_backward_input);
   take(table, "gs_adapted_linear_backward_adapters_workspace_size", next.adapted_workspace);
@@ -771,7 +768,7 @@ std::vector<std::string> layer_entry_points() {
           "gs_row_groups", "gs_grouped_linear_forward", "gs_grouped_linear_backward_input",
           "gs_grouped_linear_backward_weight_workspace_size",
           "gs_grouped_linear_backward_weight", "gs_adapted_linear_inner_size",
-          "gs_adapted_linear_inner_grad_size", "gs_adapted_linear_forward", "gs_adapted_linear_backward_input",
+          "gs_adapted_linear_forward", "gs_adapted_linear_backward_input",
           "gs_adapted_linear_backward_adapters_workspace_size",
           "gs_adapted_linear_backward_adapters"};
 }

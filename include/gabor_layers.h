@@ -151,11 +151,8 @@ int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride,
                               const int32_t* offsets, int64_t rows, int64_t groups,
                               int64_t features, int64_t outputs, int64_t rank, void* inner,
                               size_t inner_bytes, void* y, void* stream);
-/* inner_grad (gs_adapted_linear_inner_grad_size bytes, 16-byte aligned)
- * receives scale grad_y up[g], and grad_x (may be null) grad_y weight +
- * inner_grad down[g]. */
-size_t gs_adapted_linear_inner_grad_size(int32_t dtype, int64_t rows, int64_t groups,
-                                         int64_t features, int64_t rank);
+/* inner_grad (as large as inner) receives scale grad_y up[g], and grad_x (may
+ * be null) grad_y weight + inner_grad down[g]. */
 int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_stride,
                                      const void* weight, const void* down, const void* up,
                                      float scale, const int32_t* order, const int32_t* offsets,
