@@ -156,7 +156,9 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
     // Inner rows are bound by reading: as many workgroups as LDS lets run.
     const int64_t most = Mode == kInner ? (steps * 2048 * fragments > 48 * 1024 ? 256 : 512)
                                         : 32 / panels * 8;
-    p.workers = int(std::min<int64_t>(most, ceil_div(g.rows, kRowTile)));
+    // A worker to each tile, or to each group where those are fewer rows.
+    p.workers = int(std::min<int64_t>(
+        most, ceil_div(g.rows, kRowTile) + std::min(g.groups, g.rows)));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
     const size_t lds =
         size_t(2 * steps + chunks * (sizeof(T) == 4 ? 2 : 1)) * tn.value * 1024;
@@ -207,7 +209,8 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
 // parts need no scale, through its own, 16 rows at a time and once for each
 // part, four times as fast (rank 64, 1M x 512: 790 us and 262).
 
-constexpr int64_t kNarrowCost = 32;  // of a group's sums, in rows
+constexpr int64_t kNarrowCost = 32;   // of a group's sums, in rows
+constexpr int64_t kNarrowUncut = 96;  // on the line: groups of up to 64 rows
 constexpr int kNarrowColumns = 128;
 constexpr int kNarrowRows = 16;  // of a step
 
@@ -246,8 +249,8 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
   const int valid = max(0, min(p.width - column, 8));
   const int64_t length = line_length(g, kNarrowCost);
   Share at{kNarrowCost};
-  at.from = length * share / p.shares;
-  at.to = length * (share + 1) / p.shares;
+  at.from = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share);
+  at.to = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share + 1);
   at.open(g, find_segment(segments_of(g), at.from,
                           [&](int i) { return line_at(g, kNarrowCost, i); }));
   const int64_t size = int64_t(inner.rank) * p.width;
@@ -377,10 +380,15 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
   }
 }
 
-// 4,096 waves: as many as the chip holds at a rank of 32, two rounds at 64.
+// Up to 4,096 waves, of 256 rows each, or of 64 for up to 512 shares: with fewer
+// rows a wave's time counts, with more its parts (100k rows of 256 at rank 16, dA,
+// dB and what they take: 82 us at 64 rows, 56 at 256; 33k of 187 and 57 at
+// rank 5: 35 and 44).
 int64_t narrow_shares(const Grouping& g, int64_t width) {
-  const int64_t shares = std::max<int64_t>(1, 4096 / ceil_div(width, kNarrowColumns));
-  return std::min(shares, ceil_div(line_length(g, kNarrowCost), 2 * kNarrowCost));
+  const int64_t most = std::max<int64_t>(1, 4096 / ceil_div(width, kNarrowColumns));
+  const int64_t length = line_length(g, kNarrowCost);
+  return std::min(most, std::max(ceil_div(length, 256),
+                                 std::min<int64_t>(512, ceil_div(length, 64))));
 }
 
 // dA and dB in one launch, and their joins in another: with few rows a launch
@@ -399,8 +407,8 @@ int launch_narrow(const char* name, NarrowSum<T>* sums, int count, const Groupin
     waves = std::max(waves, int64_t(p.blocks) * p.shares);
     narrow = narrow || p.width < 8;
     both.of[i] = p;
-    joins[i] = {p.partial, p.out, nullptr, kNarrowCost, p.shares,
-                int64_t(p.inner.rank) * p.width, 0};
+    joins[i] = {p.partial, p.out,    nullptr, kNarrowCost,
+                kNarrowUncut, p.shares, int64_t(p.inner.rank) * p.width, 0};
   }
   const dim3 grid{unsigned(ceil_div(waves, kThreads / 64)), unsigned(count)};
   auto launch = [&](auto r, auto narrow) {

@@ -21,6 +21,20 @@ __host__ __device__ __forceinline__ int64_t line_length(const Grouping& g, int64
   return g.rows + cost * (int64_t(g.groups) + 2);
 }
 
+// Border b of the shares on the line. One that lies in a segment of up to
+// `uncut` goes to that segment's nearer end: small groups are written at once,
+// where a part of each would be as much as the whole (50k rows of 128 -> 128 in
+// 512 groups: 60 MB of parts beside 58 MB of inputs and results).
+__device__ __forceinline__ int64_t border_at(const Grouping& g, int64_t cost, int64_t uncut,
+                                             int64_t length, int64_t shares, int64_t b) {
+  const int64_t v = length * b / shares;
+  if (!uncut || b == 0 || b == shares) return v;
+  const int s = find_segment(segments_of(g), v, [&](int i) { return line_at(g, cost, i); });
+  const int64_t low = line_at(g, cost, s), high = line_at(g, cost, s + 1);
+  if (high - low > uncut) return v;
+  return v - low < high - v ? low : high;
+}
+
 // Where a share stands: segment s, whose positions from `next` to `end` are its.
 struct Share {
   int64_t cost;
@@ -55,7 +69,7 @@ struct Join {
   const float* partial;
   T* dw;
   T* db;
-  int64_t cost, shares;
+  int64_t cost, uncut, shares;
   int64_t weights, biases;
   __host__ __device__ bool by_border(const Grouping& g) const { return shares - 1 < g.groups; }
   __host__ __device__ int64_t each(const Grouping& g) const {
@@ -90,6 +104,7 @@ __global__ __launch_bounds__(kJoinThreads) void group_join_kernel(Joins<T> joins
     s = find_segment(segments_of(g), length * border / p.shares,
                      [&](int i) { return line_at(g, p.cost, i); });
   const int64_t low = line_at(g, p.cost, s), high = line_at(g, p.cost, s + 1);
+  if (high - low <= p.uncut) return;
   if (!by_border) {  // the first border behind `low`
     border = ((low + 1) * p.shares + length - 1) / length;
   }

@@ -64,26 +64,31 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const I* __restrict__ i
 }
 
 // Each group's counts become what the blocks before have of it, and its
-// total. 16 groups to a workgroup, 16 shares of the blocks.
-__global__ __launch_bounds__(kThreads) void column_kernel(Sorted s, int32_t* __restrict__ counts,
-                                                          int32_t* __restrict__ totals) {
-  __shared__ int sums[16][16];
+// total. 16 groups to a workgroup, 64 shares of the blocks.
+constexpr int kColumnThreads = 1024;
+constexpr int kShares = kColumnThreads / 16;
+
+__global__ __launch_bounds__(kColumnThreads) void column_kernel(Sorted s,
+                                                                int32_t* __restrict__ counts,
+                                                                int32_t* __restrict__ totals) {
+  __shared__ int sums[kShares][16];
   const int column = threadIdx.x & 15, share = threadIdx.x >> 4;
   const int g = blockIdx.x * 16 + column;
-  const int64_t each = (s.blocks + 15) / 16;
+  const int64_t each = (s.blocks + kShares - 1) / kShares;
   const int64_t from = share * each, to = from + each < s.blocks ? from + each : s.blocks;
   int sum = 0;
   if (g <= s.groups) {
-#pragma unroll 8
+#pragma unroll 4
     for (int64_t b = from; b < to; ++b) sum += counts[b * (s.groups + 1) + g];
   }
   sums[share][column] = sum;
   __syncthreads();
   if (g > s.groups) return;
   int before = 0;
-  for (int i = 0; i < share; ++i) before += sums[i][column];
-  if (share == 15) totals[g] = before + sum;
-#pragma unroll 8
+#pragma unroll 16
+  for (int i = 0; i < kShares; ++i) before += i < share ? sums[i][column] : 0;
+  if (share == kShares - 1) totals[g] = before + sum;
+#pragma unroll 4
   for (int64_t b = from; b < to; ++b) {
     int32_t* const at = counts + b * (s.groups + 1) + g;
     const int here = *at;
@@ -178,9 +183,9 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ i
   }
 }
 
-// Rows of a wave's round of 64: 16 rounds where there are rows enough for a
-// workgroup to each compute unit (1M rows), 4 below.
-int rounds_of(int64_t rows) { return rows > (int64_t(1) << 18) ? 16 : 4; }
+// Rounds of 64 rows of a wave: 8 where there are rows enough for a workgroup to
+// each compute unit, 4 below.
+int rounds_of(int64_t rows) { return rows > (int64_t(1) << 18) ? 8 : 4; }
 
 }  // namespace
 }  // namespace gs
@@ -222,7 +227,7 @@ int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups,
     if (!single) {
       count_kernel<I, count.value><<<grid, kThreads, lds, s>>>(from, sorted, counts);
       GS_LAUNCHED("row groups count");
-      column_kernel<<<dim3{unsigned(ceil_div(groups + 1, 16))}, kThreads, 0, s>>>(sorted, counts,
+      column_kernel<<<dim3{unsigned(ceil_div(groups + 1, 16))}, kColumnThreads, 0, s>>>(sorted, counts,
                                                                                   totals);
       GS_LAUNCHED("row groups columns");
     }
@@ -234,7 +239,7 @@ int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups,
     return int(GS_OK);
   };
   using four = std::integral_constant<int, 4>;
-  using all = std::integral_constant<int, 16>;
+  using all = std::integral_constant<int, 8>;
   if (wide)
     return rounds == 4 ? launch(int64_t(0), four{}) : launch(int64_t(0), all{});
   return rounds == 4 ? launch(int32_t(0), four{}) : launch(int32_t(0), all{});
