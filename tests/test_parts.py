@@ -758,3 +758,310 @@ def test_adapted_linear_refusals():
     (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="adapted_linear is differentiable once"):
         dx.sum().backward()
+
+
+# --------------------------------------------------------------------------
+# GPU: all of them
+
+
+def parts_step(dtype=torch.bfloat16, rows=700, seed=51, offsets_only=False):
+    """Leaves and a function that runs the operators as a decoder in parts does:
+    a layer by part, dropout, a shared layer with the parts' adapters."""
+    m = layers()
+    x = normal(rows, 72, seed=seed, dtype=dtype)
+    w, b = normal(6, 64, 72, seed=seed + 1, dtype=dtype, scale=0.1), normal(6, 64, seed=seed + 2,
+                                                                          dtype=dtype)
+    shared = normal(57, 64, seed=seed + 3, dtype=dtype, scale=0.1)
+    bias = normal(57, seed=seed + 4, dtype=dtype)
+    down = normal(6, 8, 64, seed=seed + 5, dtype=dtype, scale=0.1)
+    up = normal(6, 57, 8, seed=seed + 6, dtype=dtype, scale=0.3)
+    index = some_groups(rows, 6, seed)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b, shared, bias, down, up)]
+    on_device = index.cuda()
+    grad = normal(rows, 57, seed=seed + 7, dtype=dtype).cuda()
+
+    def run(keep=None):
+        x, w, b, shared, bias, down, up = leaves
+        by = m.row_groups(on_device, 6)
+        h = m.grouped_linear(x, w, by, b)
+        d = m.dropout(h, 0.25, 99)
+        y = m.adapted_linear(d, shared, down, up, by, bias, scale=0.5)
+        if keep is not None:
+            keep.update(by=by, h=h, d=d)
+            h.retain_grad()
+            d.retain_grad()
+        return y
+
+    return leaves, grad, run
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operators_together(dtype):
+    """Each operator against its formula at what the one before gave it, forward
+    and backward."""
+    m = layers()
+    leaves, grad, run = parts_step(dtype)
+    kept = {}
+    y = run(kept)
+    y.backward(grad)
+    x, w, b, shared, bias, down, up = (t.detach().cpu() for t in leaves)
+    h, d = kept["h"].detach().cpu(), kept["d"].detach().cpu()
+    members = oracle.members(kept["by"].offsets, kept["by"].order, len(x))
+    check_grouped(x, w, b, kept["h"].grad.cpu(), members, kept["h"],
+                  [leaves[0].grad, leaves[1].grad, leaves[2].grad])
+    check_dropout(h, kept["d"].grad.cpu(), 0.25, 99, kept["d"], kept["h"].grad)
+    check_adapted(d, shared, bias, down, up, grad.cpu(), 0.5, members, y,
+                  [kept["d"].grad, leaves[5].grad, leaves[6].grad])
+    plain = torch.autograd.grad(m.linear(kept["d"].detach(), leaves[3], leaves[4]), leaves[3:5],
+                                grad)
+    assert torch.equal(leaves[3].grad, plain[0]) and torch.equal(leaves[4].grad, plain[1])
+
+
+@gpu_test
+def test_results_repeat_bit_for_bit_on_any_stream():
+    leaves, grad, run = parts_step()
+    want = None
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            y = run()
+            got = (y, *torch.autograd.grad(y, leaves, grad))
+        torch.cuda.current_stream().wait_stream(stream)
+        torch.cuda.synchronize()
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu_test
+def test_operators_in_graphs():
+    """Two graphs of the forward and backward passes, replayed in turn with
+    eager work between, over inputs and groups that change."""
+    steps = [parts_step(rows=700), parts_step(torch.float32, rows=9000, seed=81)]
+    graphs, outs = [], []
+    for leaves, grad, run in steps:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(run(), leaves, grad)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = run()
+            out = (y.detach(), *torch.autograd.grad(y, leaves, grad))
+        del y
+        graphs.append(graph)
+        outs.append(out)
+    for round_ in range(3):
+        for (leaves, grad, run), graph, out in zip(steps, graphs, outs):
+            with torch.no_grad():
+                for t in leaves:
+                    t.mul_(1 + 0.25 * round_)
+            graph.replay()
+            torch.cuda.synchronize()
+            y = run()
+            want = (y, *torch.autograd.grad(y, leaves, grad))
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+            del y, want
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_against_differences(dtype):
+    """The operators are linear in each of their inputs, and small whole numbers
+    leave nothing to round: differences give the gradients exactly."""
+    m = layers()
+    gen = torch.Generator().manual_seed(3)
+
+    def whole(*shape, most=1):
+        return torch.randint(-most, most + 1, shape, generator=gen).to(dtype).cuda()
+
+    by, _ = grouped_by(some_groups(40, 3, 4), 3)
+    cases = [(lambda *t: m.grouped_linear(t[0], t[1], by, t[2]),
+              [whole(40, 12), whole(3, 9, 12), whole(3, 9)], whole(40, 9)),
+             (lambda *t: m.adapted_linear(t[0], w, t[1], t[2], by, scale=2.0),
+              [whole(40, 12), whole(3, 2, 12), whole(3, 9, 2)], whole(40, 9))]
+    w = whole(9, 12)
+    for call, inputs, g in cases:
+        for t in inputs:
+            t.requires_grad_()
+        grads = torch.autograd.grad(call(*inputs), inputs, g)
+        for i, grad in enumerate(grads):
+            step = whole(*inputs[i].shape)
+            with torch.no_grad():
+                moved = [[t + sign * step if j == i else t for j, t in enumerate(inputs)]
+                         for sign in (1, -1)]
+                up, down = ((call(*at).double() * g.double()).sum() for at in moved)
+            assert (up - down) / 2 == (grad.double() * step.double()).sum()
+
+
+@gpu_test
+def test_offsets_past_32_bits():
+    """Rows that lie over 2^32 values apart, and results of more values."""
+    m = layers()
+    rows, stride = 70_000, 65_536
+    base = torch.empty(rows, stride, dtype=torch.float16, device="cuda")  # 9.2 GB
+    x = base[:, 100:140]
+    x.copy_(normal(rows, 40, seed=1, dtype=torch.float16))
+    dense = x.contiguous()
+    by = m.row_groups((torch.arange(rows) % 5 - 1).cuda(), 4)
+    w, b = normal(4, 24, 40, seed=2, dtype=torch.float16).cuda(), None
+    a, u = (normal(4, 8, 40, seed=3, dtype=torch.float16).cuda(),
+            normal(4, 24, 8, seed=4, dtype=torch.float16).cuda())
+    g = normal(rows, 24, seed=5, dtype=torch.float16).cuda()
+    outs = []
+    for source in (x, dense):
+        t, wt, at, ut = (v.detach().requires_grad_() for v in (source, w, a, u))
+        y = m.grouped_linear(t, wt, by, b)
+        z = m.adapted_linear(t, w[0], at, ut, by)
+        outs.append((y, z, *torch.autograd.grad(y, (t, wt), g), *torch.autograd.grad(z, (t, at, ut), g),
+                     m.dropout(source, 0.5, 3)))
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+    del outs, base, x, y, z
+    rows = 4_300_000
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 4_194_303, 4_194_304, rows - 1], device="cuda")
+    x[at] = 1
+    w = torch.ones(2, 1024, 8, dtype=torch.bfloat16, device="cuda")
+    w[1] = 2
+    index = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    index[at[2:]] = 1
+    y = m.grouped_linear(x, w, m.row_groups(index, 2))  # 4.4e9 values
+    want = torch.tensor([8.0, 8, 16, 16, 16], device="cuda", dtype=torch.bfloat16)
+    assert torch.equal(y[at], want[:, None].expand(5, 1024)) and int(y[:, 5].count_nonzero()) == 5
+    kept = m.dropout(y[at[2:4]], 0.5, 3)
+    whole = m.dropout(y, 0.5, 3)
+    some = oracle.dropout(y[at].cpu().float(), 0.5, 3, rows=at.tolist())
+    assert torch.equal(whole[at].cpu().double(), some) and kept.shape == (2, 1024)
+
+
+@gpu_test
+def test_wrong_groups_stay_inside():
+    """Offsets that fall or pass the rows, and rows that are not there: results
+    are not defined, but every access is held to what exists, and later calls are
+    right."""
+    m = layers()
+    leaves, grad, run = parts_step()
+    want = run()
+    x, w, b, shared, bias, down, up = leaves
+    rows = len(x)
+    for offsets, order in (([0, 300, 100, 50, 600, 650, 700], None),
+                           ([-5, 10, 2_000_000, 20, 30, 1 << 30, 700], None),
+                           ([700] * 7, None), ([0] * 7, None),
+                           ([0, 100, 200, 300, 400, 500, 700], [-1, 1 << 30, 5, 5] * 175)):
+        by = m.RowGroups(torch.tensor(offsets, dtype=torch.int32).cuda(),
+                         None if order is None else torch.tensor(order, dtype=torch.int32).cuda())
+        for few in (rows, 12):
+            groups = by if order is None or few == rows else m.RowGroups(by.offsets,
+                                                                       by.order[:few].contiguous())
+            for y in (m.grouped_linear(x[:few], w, groups, b),
+                      m.adapted_linear(leaves[0][:few, :64], shared, down, up, groups, bias)):
+                torch.autograd.grad(y.sum(), leaves, allow_unused=True)
+    torch.cuda.synchronize()
+    assert torch.equal(run(), want)
+
+
+@gpu_test
+def test_lazily_negated_views():
+    m = layers()
+    z = torch.complex(normal(50, 24, seed=1), normal(50, 24, seed=2)).cuda()
+    view = z.conj().imag
+    assert view.is_neg()
+    by = m.row_groups((torch.arange(50) % 3).cuda(), 3)
+    w, a, u = (normal(3, 16, 24, seed=3).cuda(), normal(3, 4, 24, seed=4).cuda(),
+               normal(3, 16, 4, seed=5).cuda())
+    plain = view.resolve_neg()
+    assert torch.equal(m.grouped_linear(view, w, by), m.grouped_linear(plain, w, by))
+    assert torch.equal(m.adapted_linear(view, w[0], a, u, by), m.adapted_linear(plain, w[0], a, u, by))
+    assert torch.equal(m.dropout(view, 0.5, 1), m.dropout(plain, 0.5, 1))
+
+
+def parts_calls(device="cpu"):
+    m = layers()
+    w, a = torch.ones(2, 4, 8, device=device), torch.ones(2, 3, 8, device=device)
+    u, shared = torch.ones(2, 4, 3, device=device), torch.ones(4, 8, device=device)
+    by = m.RowGroups(torch.tensor([0, 1, 2], dtype=torch.int32, device=device))
+    return {"dropout": lambda t: m.dropout(t, 0.5, 1),
+            "grouped_linear": lambda t: m.grouped_linear(t, w, by),
+            "adapted_linear": lambda t: m.adapted_linear(t, shared, a, u, by)}
+
+
+def test_forward_mode_and_tracing_are_refused():
+    from test_layers import refuses_what_would_lose_a_result
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    m = layers()
+    refuses_what_would_lose_a_result(parts_calls(), torch.zeros(2, 8))
+    with pytest.raises(RuntimeError, match="row_groups cannot be traced"):
+        make_fx(lambda t: m.row_groups(t, 2).order)(torch.zeros(4, dtype=torch.int32))
+
+
+@gpu_test
+def test_forward_mode_and_tracing_are_refused_on_the_device():
+    from test_layers import refuses_what_would_lose_a_result
+
+    refuses_what_would_lose_a_result(parts_calls("cuda"), torch.ones(2, 8, device="cuda"))
+
+
+@gpu_test
+def test_second_derivatives_are_refused():
+    m = layers()
+    x = normal(4, 32, seed=1).cuda().requires_grad_()
+    (dx,) = torch.autograd.grad(m.dropout(x, 0.5, 1).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="dropout is differentiable once"):
+        dx.sum().backward()
+
+
+def test_c_entry_points_of_layers_by_group_refuse_bad_arguments():
+    from diff_gabor_splatting_amd import _native
+
+    lib, p = _native.lib, ctypes.c_void_p(256)
+    forward = lambda *t: lib.gs_grouped_linear_forward(*t, None)  # noqa: E731
+    refused(lib, forward(3, p, 8, p, p, p, p, 4, 2, 8, 8, p), 1, "unknown type")
+    refused(lib, forward(0, p, 7, p, p, p, p, 4, 2, 8, 8, p), 1, "overlap")
+    refused(lib, forward(0, p, 8, p, p, p, None, 4, 2, 8, 8, p), 1, "null")
+    refused(lib, forward(0, p, 8, None, p, p, p, 4, 2, 8, 8, p), 1, "null")
+    refused(lib, forward(0, p, 8, p, p, p, p, 1 << 31, 2, 8, 8, p), 2, "rows")
+    refused(lib, forward(0, p, 8, p, p, p, p, 4, 0, 8, 8, p), 1, "groups")
+    refused(lib, forward(0, p, 8, p, p, p, p, 4, (1 << 20) + 1, 8, 8, p), 1, "groups")
+    refused(lib, forward(0, p, 8, p, p, p, p, 4, 2, 8, 1 << 20, p), 1, "at most")
+    assert forward(0, None, 8, None, None, None, None, 0, 2, 8, 8, None) == 0
+    refused(lib, lib.gs_grouped_linear_backward_input(0, p, 8, p, p, p, 4, 2, 8, 8, None, None), 1,
+            "null")
+    need = lib.gs_grouped_linear_backward_weight_workspace_size(0, 5000, 4, 64, 64)
+    assert need > 0
+    refused(lib, lib.gs_grouped_linear_backward_weight(0, p, 64, p, 64, p, p, 5000, 4, 64, 64, p, p,
+                                                       p, need - 1, None), 4, "workspace")
+    refused(lib, lib.gs_grouped_linear_backward_weight(0, p, 64, None, 64, p, p, 5000, 4, 64, 64, p,
+                                                       p, p, need, None), 1, "null")
+    size = lib.gs_adapted_linear_inner_size(100, 16)
+    assert size >= 100 * 16 * 4
+
+    def adapted(dtype=0, scale=1.0, rank=16, bytes=size, inner=p, up=p):
+        return lib.gs_adapted_linear_forward(dtype, p, 8, p, p, p, up, scale, p, p, 100, 2, 8, 8,
+                                             rank, inner, bytes, p, None)
+
+    refused(lib, adapted(dtype=7), 1, "unknown type")
+    refused(lib, adapted(scale=math.inf), 1, "scale")
+    refused(lib, adapted(rank=65), 1, "rank")
+    refused(lib, adapted(rank=0), 1, "rank")
+    refused(lib, adapted(bytes=size - 1), 4, "inner rows")
+    refused(lib, adapted(inner=None), 4, "inner rows")
+    refused(lib, adapted(up=None), 1, "null")
+    refused(lib, lib.gs_adapted_linear_backward_input(0, p, 8, None, p, p, 1.0, p, p, 100, 2, 8, 8,
+                                                      16, p, size, p, None), 1, "null")
+    need = lib.gs_adapted_linear_backward_adapters_workspace_size(5000, 2, 64, 64, 16)
+    assert need > 0
+    refused(lib, lib.gs_adapted_linear_backward_adapters(0, p, 64, p, 64, p, p, p, p, 5000, 2, 64,
+                                                         64, 16, p, p, p, need - 1, None), 4,
+            "workspace")
+    refused(lib, lib.gs_adapted_linear_backward_adapters(0, p, 64, p, 64, None, p, p, p, 5000, 2, 64,
+                                                         64, 16, p, p, p, need, None), 1, "null")
+
+
+def test_python_layers_by_group_refuse_cpu_tensors():
+    for call in parts_calls().values():
+        with pytest.raises(ValueError, match="on a HIP device"):
+            call(torch.zeros(2, 8))
