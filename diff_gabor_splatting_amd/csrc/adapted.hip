@@ -440,6 +440,14 @@ int check_adapted(const char* name, int32_t dtype, const void* offsets, int64_t 
   return GS_OK;
 }
 
+int check_inner(const char* name, const void* inner, size_t bytes, int64_t rows, int64_t rank) {
+  GS_REQUIRE(inner && bytes >= Inner<float>::bytes(rows, rank), GS_ERR_WORKSPACE,
+             "inner rows too small for %s", name);
+  GS_REQUIRE(reinterpret_cast<uintptr_t>(inner) % 16 == 0, GS_ERR_ARGUMENT,
+             "inner rows are not 16-byte aligned in %s", name);
+  return GS_OK;
+}
+
 Grouping grouping(const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups) {
   return {order, offsets, int32_t(rows), int32_t(groups)};
 }
@@ -468,8 +476,7 @@ int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, 
   GS_REQUIRE(std::isfinite(scale), GS_ERR_ARGUMENT, "%s: scale must be finite", name);
   if (rows == 0) return GS_OK;
   GS_REQUIRE(x && weight && down && up && y, GS_ERR_ARGUMENT, "null pointer passed to %s", name);
-  GS_REQUIRE(inner && inner_bytes >= gs_adapted_linear_inner_size(rows, rank), GS_ERR_WORKSPACE,
-             "inner rows too small for %s", name);
+  GS_CHECK(check_inner(name, inner, inner_bytes, rows, rank));
   const Grouping g = grouping(order, offsets, rows, groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto zero) {
@@ -519,8 +526,7 @@ int gs_adapted_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
   if (rows == 0) return GS_OK;
   GS_REQUIRE(grad_y && up && (!grad_x || (weight && down)), GS_ERR_ARGUMENT,
              "null pointer passed to %s", name);
-  GS_REQUIRE(inner_grad && inner_bytes >= gs_adapted_linear_inner_size(rows, rank),
-             GS_ERR_WORKSPACE, "inner rows too small for %s", name);
+  GS_CHECK(check_inner(name, inner_grad, inner_bytes, rows, rank));
   const Grouping g = grouping(order, offsets, rows, groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto zero) {

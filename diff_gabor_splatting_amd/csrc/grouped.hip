@@ -289,8 +289,31 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wave_m = (wave >> 2) * 16 * A, wave_n = (wave & 3) * 16 * B;
   const bool sums = db && n0 == 0;
-  f32x4 c[A][B];
+  // float32 sums go over to others every kFold pairs of steps: a sum of n
+  // values in one go is off by about sqrt(n / 8) half units, which shows in
+  // float32 alone (1M rows of 512 -> 512: 62,000 to a share).
+  constexpr bool folds = sizeof(T) == 4;
+  constexpr int kFold = 16;
+  f32x4 c[A][B], far[A][B];
   float sum[(A + 3) / 4];  // of the outputs of fragments wave % 4, + 4, ..
+  float far_sum[(A + 3) / 4];
+  auto clear = [&](auto& values, auto& sums) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) values[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < (A + 3) / 4; ++i) sums[i] = 0.f;
+  };
+  auto add_far = [&](auto& values, auto& sums, const auto& from, const auto& from_sums)
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) values[i][j] += from[i][j];
+#pragma unroll
+    for (int i = 0; i < (A + 3) / 4; ++i) sums[i] += from_sums[i];
+  };
   auto multiply_step = [&](const T* from) {
     constexpr int deep = Mma<T>::step;
 #pragma unroll
@@ -377,12 +400,8 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   send(ahead[0], ids[0]);
   __syncthreads();
   for (; at.inside; at.open(g, at.s + 1)) {
-#pragma unroll
-    for (int i = 0; i < A; ++i)
-#pragma unroll
-      for (int j = 0; j < B; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < (A + 3) / 4; ++i) sum[i] = 0.f;
+    clear(c, sum);
+    if constexpr (folds) clear(far, far_sum);
     for (int pair = pairs_of(at); pair; --pair) {
       put(ahead[1], lds + buffer);
       send(ahead[1], ids[1]);
@@ -392,7 +411,12 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
       send(ahead[0], ids[0]);
       multiply_step(lds + buffer);
       __syncthreads();
+      if (folds && pair % kFold == 0) {
+        add_far(far, far_sum, c, sum);
+        clear(c, sum);
+      }
     }
+    if constexpr (folds) add_far(c, sum, far, far_sum);
     finish();
   }
 }

@@ -13,8 +13,8 @@
 
 namespace gs {
 
-// Positions are 32-bit.
-constexpr int64_t kMostGroupedRows = 0x7fffffff;
+// Positions are 32-bit, with room for the last tile's rows past the end.
+constexpr int64_t kMostGroupedRows = 0x7ffff000;
 constexpr int64_t kMostGroupsOfRows = int64_t(1) << 20;
 
 struct Grouping {

@@ -517,7 +517,7 @@ struct Groups {
       throw py::value_error("groups has offsets of " + std::to_string(count()) + " groups, not " +
                             std::to_string(groups));
     const int64_t rows = x.numel() / x.size(-1);
-    if (rows > 0x7fffffff) throw py::value_error("x has more than 2^31 - 1 rows");
+    if (rows > 0x7ffff000) throw py::value_error("x has more than 2^31 - 4096 rows");
     if (order.defined() && order.numel() != rows)
       throw py::value_error("groups has an order of " + std::to_string(order.numel()) +
                             " rows, x has " + std::to_string(rows));

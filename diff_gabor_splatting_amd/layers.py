@@ -16,6 +16,11 @@ nearest integer multiple of it (ties to even). The error of a value is at most
 kept value is exact in the type it came from and does not depend on how a scale
 was rounded). A group with an infinity or a NaN reads back as NaN.
 
+Surfels that belong to parts go through ``grouped_linear`` (a matrix to each
+group of rows) or ``adapted_linear`` (a shared matrix, a low-rank adapter to
+each group) by the :class:`RowGroups` that :func:`row_groups` makes; these keep
+their input whole. ``dropout`` keeps nothing.
+
 All work is queued on the current stream; nothing synchronises. Inputs whose
 features are contiguous and whose leading dimensions collapse are read in
 place, others are copied first. ``include/gabor_layers.h`` has the C entry
@@ -181,7 +186,7 @@ class RowGroups:
 def row_groups(index: Tensor, groups: int) -> RowGroups:
     """The rows by group: ``index`` (int32 or int64, any shape) is each row's
     group, 0 through ``groups - 1``, and any other number puts a row in none.
-    Rows keep their order within a group. At most 4096 groups and 2^31 - 1
+    Rows keep their order within a group. At most 4096 groups and 2^31 - 4096
     rows."""
     groups = operator.index(groups)
     if not 1 <= groups <= 4096:

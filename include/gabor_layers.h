@@ -103,7 +103,7 @@ int gs_dropout(int32_t dtype, double p, int64_t seed, const void* seed_at, const
  * order is null), group g has the positions offsets[g] .. offsets[g + 1] - 1,
  * and the rows at other positions are in no group. order is a permutation of
  * the rows, offsets [groups + 1] does not fall; both are held to the rows
- * that exist. rows < 2^31.
+ * that exist. rows <= 2^31 - 4096.
  *
  * gs_row_groups makes both of each row's group (index, int32 or with `wide`
  * int64; outside 0 .. groups - 1: of none, behind the last group), each
