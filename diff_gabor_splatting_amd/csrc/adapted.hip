@@ -24,9 +24,9 @@ namespace {
 
 constexpr int kFewRows = 16;
 
-// The sum over k of a[k] b[k], in every lane of the wave.
+// A lane's part of the sum over k of a[k] b[k], and the whole of such parts.
 template <typename T>
-__device__ __forceinline__ float wave_dot(const T* a, const T* b, int k) {
+__device__ __forceinline__ float dot_part(const T* a, const T* b, int k) {
   const int lane = threadIdx.x & 63;
   float sum = 0.f;
 #pragma unroll 4
@@ -38,13 +38,19 @@ __device__ __forceinline__ float wave_dot(const T* a, const T* b, int k) {
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) sum = __builtin_fmaf(u[j], v[j], sum);
   }
+  return sum;
+}
+__device__ __forceinline__ float all_lanes(float sum) {
 #pragma unroll
   for (int step = 32; step; step >>= 1) sum += __shfl_xor(sum, step);
   return sum;
 }
 
+// A wave to one of the rank, or to several of more than 16.
+constexpr int kInnerThreads = 1024;
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void few_inner_kernel(const T* __restrict__ x,
+__global__ __launch_bounds__(kInnerThreads) void few_inner_kernel(const T* __restrict__ x,
                                                              int64_t stride,
                                                              const T* __restrict__ down,
                                                              float scale, Grouping g, int k,
@@ -59,8 +65,8 @@ __global__ __launch_bounds__(kThreads) void few_inner_kernel(const T* __restrict
   if (member) {
     const T* const row = x + row_at(g, position) * stride;
     const T* const matrix = down + int64_t(s - 1) * inner.rank * k;
-    for (int r = wave; r < inner.rank; r += kThreads / 64) {
-      const float sum = wave_dot<T>(row, matrix + int64_t(r) * k, k);
+    for (int r = wave; r < inner.rank; r += kInnerThreads / 64) {
+      const float sum = all_lanes(dot_part<T>(row, matrix + int64_t(r) * k, k));
       if (lane == 0) values[r] = scale * sum;
     }
   }
@@ -86,14 +92,12 @@ __global__ __launch_bounds__(kThreads) void few_adapted_kernel(
   const int64_t row = row_at(g, position);
   const int s = find_segment(segments_of(g), position,
                              [&](int i) { return int64_t(begin_of(g, i)); });
-  // The narrow sum: a value of the rank to a lane.
-  float narrow = 0.f;
+  // The shared sum, and the narrow one, a value of the rank to a lane.
+  float sum = dot_part<T>(x + row * stride, w + int64_t(output) * k, k);
   if (s > 0 && s <= g.groups && lane < inner.rank)
-    narrow = inner.get(position, lane) *
-             float(up[(int64_t(s - 1) * n + output) * inner.rank + lane]);
-#pragma unroll
-  for (int step = 32; step; step >>= 1) narrow += __shfl_xor(narrow, step);
-  float sum = wave_dot<T>(x + row * stride, w + int64_t(output) * k, k) + narrow;
+    sum = __builtin_fmaf(inner.get(position, lane),
+                         float(up[(int64_t(s - 1) * n + output) * inner.rank + lane]), sum);
+  sum = all_lanes(sum);
   if (bias) sum += float(bias[output]);
   if (lane == 0) y[row * n + output] = T(sum);
 }
@@ -249,10 +253,10 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
   const int valid = max(0, min(p.width - column, 8));
   const int64_t length = line_length(g, kNarrowCost);
   Share at{kNarrowCost};
-  at.from = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share);
-  at.to = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share + 1);
-  at.open(g, find_segment(segments_of(g), at.from,
-                          [&](int i) { return line_at(g, kNarrowCost, i); }));
+  int from_segment, to_segment;
+  at.from = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share, from_segment);
+  at.to = border_at(g, kNarrowCost, kNarrowUncut, length, p.shares, share + 1, to_segment);
+  at.open(g, from_segment);
   const int64_t size = int64_t(inner.rank) * p.width;
   for (; at.inside; at.open(g, at.s + 1)) {
     f32x4 c[R][8];
@@ -483,7 +487,7 @@ int gs_adapted_linear_forward(int32_t dtype, const void* x, int64_t row_stride, 
     using T = decltype(zero);
     const Inner<T> held = Inner<T>::at(inner, rows, rank);
     if (rows <= kFewRows) {
-      few_inner_kernel<T><<<dim3{unsigned(rows)}, kThreads, 0, s>>>(
+      few_inner_kernel<T><<<dim3{unsigned(rows)}, kInnerThreads, 0, s>>>(
           static_cast<const T*>(x), row_stride, static_cast<const T*>(down), scale, g,
           int(features), held);
       GS_LAUNCHED(name);

@@ -206,9 +206,10 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
   const int m0 = tile / p.tiles_n * tile_m, n0 = tile % p.tiles_n * tile_n;
   const int64_t length = line_length(g, kGroupCost);
   Share at{kGroupCost};
-  at.from = border_at(g, kGroupCost, kGroupUncut, length, p.shares, share);
-  at.to = border_at(g, kGroupCost, kGroupUncut, length, p.shares, share + 1);
-  at.open(g, find_segment(segments_of(g), at.from, [&](int i) { return line_at(g, kGroupCost, i); }));
+  int from_segment, to_segment;
+  at.from = border_at(g, kGroupCost, kGroupUncut, length, p.shares, share, from_segment);
+  at.to = border_at(g, kGroupCost, kGroupUncut, length, p.shares, share + 1, to_segment);
+  at.open(g, from_segment);
   // Steps come in pairs, for the two buffers: a group's last may be empty.
   auto pairs_of = [](const Share& of) { return (of.end - of.next + 2 * Rows - 1) / (2 * Rows); };
   Share ahead_at = at;
