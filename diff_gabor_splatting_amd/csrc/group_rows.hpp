@@ -10,7 +10,13 @@ namespace gs {
 // groups they are in, and puts another matrix in place where another group
 // begins; a wave takes 32 rows at a time and, but for that, needs no other
 // wave. Shares are cut from the line on which each segment takes kStageCost +
-// its rows, so that putting a matrix in place counts too.
+// its rows, so that putting a matrix in place counts too (64 to 1,024 rows give
+// the same times).
+//
+// 1M x 512 -> 512 bfloat16 in 32 groups: y 615 us, dx 592 (850 to 890 TFLOP/s),
+// as long as with one matrix for all rows: matrix cores 41% busy, LDS 46%, the
+// address unit 62%. With the adapters' steps (rank 16) 670 and 660; inner rows
+// 243 and 253, bound by the address unit (80%).
 constexpr int64_t kStageCost = 64;  // of a matrix, in rows
 
 __device__ __forceinline__ int64_t stage_line(const Grouping& g, int s) {

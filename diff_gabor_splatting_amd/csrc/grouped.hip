@@ -66,7 +66,8 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
     p.workers = int(std::min<int64_t>(32 / panels * 8, ceil_div(rows, kRowTile)));
     const dim3 grid{unsigned(ceil_div(p.workers, 8) * panels * 8)};
     const size_t lds = size_t(p.steps) * 2 * tn.value * 1024;
-    auto* const kernel = &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value, kByGroup>;
+    auto* const kernel =
+        &group_rows_kernel<T, tn.value, ahead.value, Transposed, tail.value, kByGroup>;
     GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), lds));
     kernel<<<grid, kRowThreads, lds, stream>>>(static_cast<const T*>(x), static_cast<const T*>(w),
                                                static_cast<const T*>(bias), g, p, {},
@@ -100,7 +101,10 @@ int launch_rows(const char* name, const void* x, int64_t stride, const void* w, 
 }
 
 // --------------------------------------------------------------------------
-// y of a few rows: a wave to a row's output, its lanes along the features.
+// y of a few rows: a wave to a row's output, its lanes along the features. 4 rows
+// of 1024 -> 1024 bfloat16: 3.9 us, launch and loads that wait for each other.
+// More than 16 rows have a matrix put in LDS (32 to 380 rows of 1024 -> 1024 in
+// 8 groups: 13 to 15 us).
 
 constexpr int kFewRows = 16;
 
@@ -145,6 +149,12 @@ __global__ __launch_bounds__(kThreads) void group_few_kernel(
 // each segment takes kGroupCost + its rows, so that writing a group's
 // tile counts too. A group whose part of the line lies in one share is
 // written at once; the others' parts are joined after.
+//
+// 1M x 512 -> 512 bfloat16 in 32 groups: 824 us (636 TFLOP/s), matrix cores 30%
+// busy, LDS 20%: the waves wait at a step's barrier and for what lies between
+// LDS and its first product. 100k x 256 -> 256 in 64 groups: 48 us, and 14 for the
+// joining. One loop for both halves of a pair of steps: groups that end in
+// either half cost 80 registers more.
 
 constexpr int kSumThreads = 512;
 constexpr int64_t kGroupCost = 128;   // of a group's tile, in rows
@@ -595,7 +605,8 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
     if constexpr (sizeof(T) == 2)
       if (shape == 84) GS_CHECK(launch(integral_constant<int, 8>{}, four{}, wide{}));
     if (plan.shares == 1) return int(GS_OK);
-    const Join<T> join{partial, dw, db, kGroupCost, kGroupUncut, plan.shares, outputs * features, outputs};
+    const Join<T> join{partial,     dw,          db,      kGroupCost,
+                       kGroupUncut, plan.shares, outputs * features, outputs};
     return launch_joins(&join, 1, g, s);
   });
 }

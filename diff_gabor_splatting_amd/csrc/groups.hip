@@ -8,7 +8,9 @@
 // each group are summed over the blocks (column_kernel), and the blocks place
 // their rows (place_kernel): bytes read twice and written once, 16 to 20 a row.
 // One block's rows need the last kernel alone. Ranks within 64 rows come from
-// ballots over the bits of the group, so nothing depends on timing.
+// ballots over the bits of the group, so nothing depends on timing. 100k rows in
+// 64 groups 13.6 us, 1M rows in 512 groups 24.3 (3 launches): latency, of the
+// counters in LDS and of the rounds that follow each other.
 #include "groups.hpp"
 #include "layers_api.hpp"
 
@@ -17,7 +19,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int64_t kMostGroups = 4096;  // their counters for four waves, and their beginnings, in LDS
+constexpr int64_t kMostGroups = 4096;  // counters for four waves, and beginnings, in LDS
 
 struct Sorted {
   int64_t rows;
@@ -227,8 +229,8 @@ int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups,
     if (!single) {
       count_kernel<I, count.value><<<grid, kThreads, lds, s>>>(from, sorted, counts);
       GS_LAUNCHED("row groups count");
-      column_kernel<<<dim3{unsigned(ceil_div(groups + 1, 16))}, kColumnThreads, 0, s>>>(sorted, counts,
-                                                                                  totals);
+      column_kernel<<<dim3{unsigned(ceil_div(groups + 1, 16))}, kColumnThreads, 0, s>>>(
+          sorted, counts, totals);
       GS_LAUNCHED("row groups columns");
     }
     auto* const kernel = &place_kernel<I, count.value>;
