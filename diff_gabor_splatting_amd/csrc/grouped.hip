@@ -363,19 +363,20 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
     const uint32_t place = uint32_t(i16) * p.features + 4 * q;
     const int rows_left = group ? p.outputs - m0 - wave_m - i16 : 0;
     const int columns_left = p.features - n0 - wave_n - 4 * q;
-#pragma unroll
-    for (int i = 0; i < A; ++i) {
+    // Fragment i of the outputs.
+    auto put_fragment = [&](int i, const f32x4 (&f)[B], float total)
+        __attribute__((always_inline)) {
       // Lane 16 q + i holds features 4 q .. 4 q + 3 of output i of a fragment.
       if (rows_left > 16 * i && (!whole || dw)) {
 #pragma unroll
         for (int j = 0; j < B; ++j) {
           const uint32_t to = place + uint32_t(16 * i) * p.features + 16 * j;
-          const vec<T, 4> v = {T(c[i][j][0]), T(c[i][j][1]), T(c[i][j][2]), T(c[i][j][3])};
+          const vec<T, 4> v = {T(f[j][0]), T(f[j][1]), T(f[j][2]), T(f[j][3])};
           if (columns_left >= 16 * j + 4) {
             if (whole)
               store_packed<T, 4>(to_dw + to, v);
             else
-              store_packed<float, 4>(to_part + to, c[i][j]);
+              store_packed<float, 4>(to_part + to, f[j]);
           } else {
 #pragma unroll
             for (int h = 0; h < 3; ++h)
@@ -383,13 +384,12 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
                 if (whole)
                   to_dw[to + h] = v[h];
                 else
-                  to_part[to + h] = c[i][j][h];
+                  to_part[to + h] = f[j][h];
               }
           }
         }
       }
       if (sums && (wave & 3) == (i & 3)) {
-        float total = sum[i / 4];
         total += __shfl_xor(total, 16);
         total += __shfl_xor(total, 32);
         const int m = m0 + wave_m + 16 * i + i16;
@@ -400,7 +400,25 @@ __global__ __launch_bounds__(kSumThreads) void group_sum_kernel(
             part[weights + m] = total;
         }
       }
-      __builtin_amdgcn_sched_barrier(0);  // or all places are held at once
+    };
+    if constexpr (A * B < 32) {
+#pragma unroll
+      for (int i = 0; i < A; ++i) {
+        put_fragment(i, c[i], sum[i / 4]);
+        __builtin_amdgcn_sched_barrier(0);  // or all places are held at once
+      }
+    } else {
+      // From c[0], the others moved up: all of it in succession is 25 KB of code
+      // that a workgroup runs once a group and fetches each time (100k x 512 ->
+      // 512 in 64 groups: 181 us, 157 so; tiles a quarter as large: 61, 64).
+#pragma unroll 1
+      for (int i = 0; i < A; ++i) {
+        put_fragment(i, c[0], i < 4 ? sum[0] : sum[(A + 3) / 4 - 1]);
+#pragma unroll
+        for (int k = 0; k + 1 < A; ++k)
+#pragma unroll
+          for (int j = 0; j < B; ++j) c[k][j] = c[k + 1][j];
+      }
     }
   };
   find(ids[0]);
