@@ -612,6 +612,25 @@ def test_adapted_linear(dtype, rows, features, outputs, groups, rank):
 
 @gpu_test
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("features,outputs,rank", [
+    (64, 256, 16), (128, 512, 16), (190, 256, 40), (256, 256, 16), (256, 256, 33), (320, 200, 8),
+    (512, 512, 16), (512, 512, 40)])
+def test_adapted_linear_of_wide_panels(dtype, features, outputs, rank):
+    """Rows enough for the widest panels, steps that the adapters' chunks make a
+    whole number of those under way and others, and matrices that leave no room in
+    LDS for the adapters beside the widest."""
+    adapted_case(3000, features, outputs, 5, rank, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("features,outputs", [(64, 256), (190, 512), (512, 512), (256, 300)])
+def test_grouped_linear_of_wide_panels(dtype, features, outputs):
+    grouped_case(3000, features, outputs, 5, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_adapted_linear_of_special_groups(dtype):
     m = layers()
     adapted_case(500, 64, 40, 5, 8, dtype, bias=False, scale=-2.0)
