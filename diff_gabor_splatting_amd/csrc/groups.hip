@@ -5,12 +5,13 @@
 //
 // A row of no group (an index outside 0 .. groups - 1) is sorted as group
 // `groups`. Blocks of rows count their groups (count_kernel), the counts of
-// each group are summed over the blocks (column_kernel), and the blocks place
-// their rows (place_kernel): bytes read twice and written once, 16 to 20 a row.
-// One block's rows need the last kernel alone. Ranks within 64 rows come from
-// ballots over the bits of the group, so nothing depends on timing. 100k rows in
-// 64 groups 13.6 us, 1M rows in 512 groups 24.3 (3 launches): latency, of the
-// counters in LDS and of the rounds that follow each other.
+// each group are summed over the blocks (column_kernel, or where they are few
+// each block of the next kernel for itself), and the blocks place their rows
+// (place_kernel): bytes read twice and written once, 12 to 20 a row. One block's
+// rows need the last kernel alone. Ranks within 64 rows come from ballots over
+// the bits of the group, so nothing depends on timing. 100k rows in 64 groups
+// 10.8 us a call, 1M rows in 512 groups 25: latency, of the counters in LDS and
+// of the rounds that follow each other.
 #include "groups.hpp"
 #include "layers_api.hpp"
 
@@ -26,6 +27,7 @@ struct Sorted {
   int groups;   // without the rows of none
   int bits;     // of a group's number, `groups` included
   int64_t blocks;
+  bool direct;  // every block of place_kernel sums the counts for itself
 };
 
 template <typename I>
@@ -126,7 +128,8 @@ __device__ __forceinline__ void begin_of_groups(const Sorted& s, int* begin, F v
   }
 }
 
-// counts: what the blocks before have of each group (null: there is one block).
+// counts: each block's groups (null: there is one block), or but for `direct`
+// what the blocks before have of them.
 template <typename I, int Rounds>
 __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ index, Sorted s,
                                                          const int32_t* __restrict__ counts,
@@ -137,7 +140,11 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ i
   const int size = s.groups + 1;
   int* const at = shared;                   // [kWaves][size]: next place
   int* const begin = shared + kWaves * size;
+  int* const all = begin + size;            // direct: each group's rows,
+  int* const earlier = all + size;          // and those of the blocks before
   for (int i = threadIdx.x; i < kWaves * size; i += kThreads) at[i] = 0;
+  if (s.direct)
+    for (int i = threadIdx.x; i < 2 * size; i += kThreads) all[i] = 0;
   int key[Rounds];
   load_keys<I, Rounds>(index, s, key);
   __syncthreads();
@@ -147,7 +154,27 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ i
   for (int r = 0; r < Rounds; ++r)
     if (key[r] >= 0) atomicAdd(&mine[key[r]], 1);
   __syncthreads();
+  if (s.direct) {
+    // 16 counts of a thread at a time; whole numbers have the same sum in any
+    // order.
+    const int entries = int(s.blocks) * size, mine_from = int(blockIdx.x) * size;
+    for (int first = threadIdx.x; first < entries; first += 16 * kThreads) {
+      int count[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        count[u] = first + u * kThreads < entries ? counts[first + u * kThreads] : 0;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int entry = first + u * kThreads, g = entry % size;
+        if (!count[u]) continue;
+        atomicAdd(&all[g], count[u]);
+        if (entry < mine_from) atomicAdd(&earlier[g], count[u]);
+      }
+    }
+    __syncthreads();
+  }
   begin_of_groups(s, begin, [&](int g) {
+    if (s.direct) return all[g];
     if (counts) return totals[g];
     int sum = 0;
     for (int w = 0; w < kWaves; ++w) sum += at[w * size + g];
@@ -156,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ i
   const int32_t* const before = counts ? counts + blockIdx.x * int64_t(size) : nullptr;
   for (int g = threadIdx.x; g <= s.groups; g += kThreads) {
     if (blockIdx.x == 0) offsets[g] = begin[g];
-    int place = begin[g] + (before ? before[g] : 0);
+    int place = begin[g] + (s.direct ? earlier[g] : before ? before[g] : 0);
     for (int w = 0; w < kWaves; ++w) {
       const int here = at[w * size + g];
       at[w * size + g] = place;
@@ -184,6 +211,11 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ i
     wave_order();
   }
 }
+
+// Counts up to which every block sums them for itself, which saves a launch:
+// 100k rows in 64 groups (6,370 counts) 12.7 us to 10.8, 1M in 8 (4,401) 16.1 to
+// 14.1; 100k in 150 (14,798) 13.0 and 14.9, 1M in 32 (16,137) 17.5 and 18.9.
+constexpr int64_t kDirect = 8192;
 
 // Rounds of 64 rows of a wave: 8 where there are rows enough for a workgroup to
 // each compute unit, 4 below.
@@ -216,7 +248,9 @@ int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups,
              "workspace too small for gs_row_groups");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rounds = rounds_of(rows);
-  Sorted sorted{rows, int(groups), 0, std::max<int64_t>(1, ceil_div(rows, kThreads * rounds))};
+  Sorted sorted{rows, int(groups), 0, std::max<int64_t>(1, ceil_div(rows, kThreads * rounds)),
+                false};
+  sorted.direct = sorted.blocks > 1 && sorted.blocks * (groups + 1) <= kDirect;
   while (groups >> sorted.bits) ++sorted.bits;
   const bool single = sorted.blocks == 1;
   int32_t* const counts = single ? nullptr : static_cast<int32_t*>(workspace);
@@ -229,14 +263,16 @@ int gs_row_groups(int32_t wide, const void* index, int64_t rows, int64_t groups,
     if (!single) {
       count_kernel<I, count.value><<<grid, kThreads, lds, s>>>(from, sorted, counts);
       GS_LAUNCHED("row groups count");
+    }
+    if (!single && !sorted.direct) {
       column_kernel<<<dim3{unsigned(ceil_div(groups + 1, 16))}, kColumnThreads, 0, s>>>(
           sorted, counts, totals);
       GS_LAUNCHED("row groups columns");
     }
     auto* const kernel = &place_kernel<I, count.value>;
-    GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), (kWaves + 1) * lds));
-    kernel<<<grid, kThreads, (kWaves + 1) * lds, s>>>(from, sorted, counts, totals, order,
-                                                      offsets);
+    const size_t all_lds = (kWaves + (sorted.direct ? 3 : 1)) * lds;
+    GS_CHECK(allow_lds(reinterpret_cast<const void*>(kernel), all_lds));
+    kernel<<<grid, kThreads, all_lds, s>>>(from, sorted, counts, totals, order, offsets);
     GS_LAUNCHED("row groups place");
     return int(GS_OK);
   };
