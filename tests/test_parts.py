@@ -997,6 +997,22 @@ def test_lazily_negated_views():
     assert torch.equal(m.dropout(view, 0.5, 1), m.dropout(plain, 0.5, 1))
 
 
+@gpu_test
+def test_groups_may_not_change_before_the_backward_pass():
+    m = layers()
+    x = normal(30, 8, seed=1).cuda().requires_grad_()
+    w = normal(2, 4, 8, seed=2).cuda()
+    a, u = normal(2, 3, 8, seed=3).cuda(), normal(2, 4, 3, seed=4).cuda()
+    for call in (lambda by: m.grouped_linear(x, w, by),
+                 lambda by: m.adapted_linear(x, w[0], a, u, by)):
+        for change in ("offsets", "order"):
+            by = m.row_groups((torch.arange(30) % 2).cuda(), 2)
+            y = call(by)
+            getattr(by, change).add_(0)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()
+
+
 def parts_calls(device="cpu"):
     m = layers()
     w, a = torch.ones(2, 4, 8, device=device), torch.ones(2, 3, 8, device=device)
