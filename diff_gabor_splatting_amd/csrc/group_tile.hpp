@@ -1,7 +1,7 @@
 // Products of rows with the matrix of their group, a tile of 128 x 128 to a
 // workgroup (50k x 128 -> 128 float16 in 512 groups: 18 us each way, bound by
-// latency; 1M x 512 -> 512 bfloat16 in 32 groups: y 1,045, dx 1,171); and the adapters' inner rows, which such a product gives and
-// another takes.
+// latency; 1M x 512 -> 512 bfloat16 in 32 groups: y 1,045, dx 1,171); and the
+// adapters' inner rows, which such a product gives and another takes.
 #pragma once
 
 #include "groups.hpp"

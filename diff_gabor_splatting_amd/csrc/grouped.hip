@@ -8,7 +8,8 @@
 //
 //   group_few_kernel   y of a few rows: a wave to a row's output
 //   group_rows_kernel  y and dx: a group's matrix in LDS, its rows streamed past
-//   group_tile_kernel  y and dx where a matrix has a side too long for that
+//   group_tile_kernel  y and dx where a matrix has a side too long for that, or
+//                      there are many groups of few rows
 //   group_sum_kernel   dW and db: tiles of dW over shares of all rows, whose
 //                      partial sums group_join_kernel adds in their order
 //

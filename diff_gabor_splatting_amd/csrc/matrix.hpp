@@ -183,8 +183,8 @@ __device__ __forceinline__ FragmentPlace place_in_panel(int n) {
 
 // The matrix as fragments. Transposed: `w` is [k][n] in memory, else [n][k].
 template <typename T, int TN, bool Transposed>
-__device__ __forceinline__ void stage_panel(const T* __restrict__ w, int wk, int wn, int steps, int n0,
-                                            vec<T, kPart<T>>* lds) {
+__device__ __forceinline__ void stage_panel(const T* __restrict__ w, int wk, int wn, int steps,
+                                            int n0, vec<T, kPart<T>>* lds) {
   constexpr int part = kPart<T>, columns = 16 * TN;
   const int parts = steps * 8;
   if constexpr (!Transposed) {
