@@ -64,7 +64,7 @@ __device__ __forceinline__ void put_inner(const Adapters<T>& adapters, int posit
   for (int t = 0; t < TN; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      c[t][j] *= adapters.scale;
+      c[t][j] = inner.value(panel_column<T>(t, 4 * q) + j, c[t][j], adapters.scale);
       most = fmaxf(most, finite_size(c[t][j]));
     }
   if constexpr (Inner<T>::scaled) {

@@ -51,6 +51,11 @@ struct Inner {
     return i;
   }
 
+  // Value n of a row, of its sum. Past the rank it is zero, and not the sum:
+  // that is of products with zeros, which an infinity of the row makes NaN.
+  __device__ __forceinline__ float value(int n, float sum, float scale) const {
+    return n < rank ? scale * sum : 0.f;
+  }
   // Writes the scale of a row (`writes`: one lane does) whose largest finite
   // magnitude is `most`; returns what its values are multiplied by.
   __device__ __forceinline__ float begin_row(int64_t position, float most, bool writes) const {
@@ -312,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void group_tile_kernel(
       float most = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        row[j] *= adapters.scale;
+        row[j] = inner.value(int(n) + j, row[j], adapters.scale);
         most = fmaxf(most, finite_size(row[j]));
       }
       most = fmaxf(most, __shfl_xor(most, 16));
