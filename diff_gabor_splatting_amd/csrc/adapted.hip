@@ -312,8 +312,18 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           b[j] = __builtin_bit_cast(raw, vec<T, 4>{v[0][j], v[1][j], v[2][j], v[3][j]});
+        // Infinities of the rows meet the first parts alone: a second part may
+        // be zero, or of the other sign.
+        uint32_t largest = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < fours; ++i) largest = max(largest, largest_of<T, 8>(v[i]));
+        const bool infinite = __ballot(largest >= 0x7f800000u) != 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h && infinite) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (b[j] & 0x7f80) == 0x7f80 ? raw(0) : b[j];
+          }
 #pragma unroll
           for (int t = 0; t < R; ++t) {
             vec<T, 4> a;
@@ -325,6 +335,7 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
               c[t][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(raw, a), b[j],
                                                                   c[t][j], 0, 0, 0);
           }
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < fours; ++i) {

@@ -67,3 +67,12 @@ def test_adapted_linear_of_rows_with_infinities(dtype, rows, features, rank):
     results, error = infinite_rows(dtype, rows, features, rank)
     for got, expected in results[:2]:
         infinite_where_expected(got, expected, error, dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@INFINITE_CASES
+def test_adapters_gradients_of_rows_with_infinities(dtype, rows, features, rank):
+    results, error = infinite_rows(dtype, rows, features, rank)
+    for got, expected in results[2:]:
+        infinite_where_expected(got, expected, error, dtype)
