@@ -264,10 +264,6 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
   const int64_t size = int64_t(inner.rank) * p.width;
   for (; at.inside; at.open(g, at.s + 1)) {
     f32x4 c[R][8];
-#pragma unroll
-    for (int t = 0; t < R; ++t)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // Rows and inner rows of a step are on their way while the step before is
     // multiplied; the rows' places, 64 at a time, a whole 64 before.
     struct Step {
@@ -279,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
     auto find = [&](int of) {
       return count > 0 ? int(row_at(g, first + min(64 * of + lane, count - 1))) : 0;
     };
-    int id = 0, next_id = find(0);
+    int id, next_id;
     auto load = [&](Step& to, int step) {
       if (step % 4 == 0) {
         id = next_id;
@@ -298,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
           to.scales[i] = inner.scales[first + min(place, count - 1)];
       }
     };
-    auto multiply_step = [&](const Step& of, int step) {
+    auto multiply_step = [&](const Step& of, int step, auto infinite) {
       vec<T, 8> v[fours];
       bool live[fours];
 #pragma unroll
@@ -312,15 +308,9 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           b[j] = __builtin_bit_cast(raw, vec<T, 4>{v[0][j], v[1][j], v[2][j], v[3][j]});
-        // Infinities of the rows meet the first parts alone: a second part may
-        // be zero, or of the other sign.
-        uint32_t largest = 0;
-#pragma unroll
-        for (int i = 0; i < fours; ++i) largest = max(largest, largest_of<T, 8>(v[i]));
-        const bool infinite = __ballot(largest >= 0x7f800000u) != 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (h && infinite) {
+          if (infinite.value && h) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) b[j] = (b[j] & 0x7f80) == 0x7f80 ? raw(0) : b[j];
           }
@@ -354,13 +344,35 @@ __global__ __launch_bounds__(kThreads) void narrow_sum_kernel(NarrowSums<T> sums
         }
       }
     };
-    Step ahead[2];
-    if (count > 0) load(ahead[0], 0);
-    for (int step = 0; step * kNarrowRows < count; step += 2) {
-      load(ahead[1], step + 1);
-      multiply_step(ahead[0], step);
-      load(ahead[0], step + 2);
-      multiply_step(ahead[1], step + 1);
+    auto sum = [&](auto infinite) {
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      id = 0;
+      next_id = find(0);
+      Step ahead[2];
+      if (count > 0) load(ahead[0], 0);
+      for (int step = 0; step * kNarrowRows < count; step += 2) {
+        load(ahead[1], step + 1);
+        multiply_step(ahead[0], step, infinite);
+        load(ahead[0], step + 2);
+        multiply_step(ahead[1], step + 1, infinite);
+      }
+    };
+    sum(std::false_type{});
+    if constexpr (parts) {
+      // An infinity of a row times a second part, which may be zero or of the
+      // other sign, is a NaN that the formula has not: sums that came out bad are
+      // taken again, and infinities of the rows meet the first parts alone.
+      float bad = 0.f;
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(c[t][j][r], 0.f, bad);
+      if (__ballot(bad != bad)) sum(std::true_type{});
     }
     // Lane 16 q + i holds ranks 16 t + 4 q .. + 3 of columns 8 i .. 8 i + 7.
     if (at.s < 1 || at.s > g.groups) continue;
