@@ -305,7 +305,8 @@ __global__ __launch_bounds__(kRowThreads) void group_rows_kernel(
                 second = 0;
               }
               if (Inner<T>::scaled && chunk == 0) {
-                // Powers of two, and far enough inside float32.
+                // Powers of two: what is lost of the sum is below 2^-149 of a
+                // scale of at most 2^113, far below float16's own steps.
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll

@@ -60,9 +60,11 @@ struct Inner {
   // magnitude is `most`; returns what its values are multiplied by.
   __device__ __forceinline__ float begin_row(int64_t position, float most, bool writes) const {
     if constexpr (scaled) {
-      // most = m 2^e with 1/2 <= m < 1; between 2^-60 and 2^60 both powers
-      // stay far inside float32.
-      const int e = min(max(__builtin_amdgcn_frexp_expf(most), -60), 60);
+      // most = m 2^e with 1/2 <= m < 1. Up to 2^113, so that the largest of
+      // float32 comes to below 2^15; from 2^-60 on, so that the shared sum over
+      // the scale stays inside float32 (2^50 at most). Both powers are normal
+      // numbers.
+      const int e = min(max(__builtin_amdgcn_frexp_expf(most), -60), 113);
       if (writes) scales[position] = __uint_as_float(uint32_t(127 + e) << 23);
       return __uint_as_float(uint32_t(127 - e) << 23);
     }

@@ -12,7 +12,7 @@ import torch
 
 from oracle import parts as oracle
 from test_layers import DTYPES, E, gpu_test, layers, near, normal
-from test_parts import INNER, grouped_by
+from test_parts import INNER, adapted_case, grouped_by, some_groups
 
 # --------------------------------------------------------------------------
 # Infinities
@@ -76,3 +76,67 @@ def test_adapters_gradients_of_rows_with_infinities(dtype, rows, features, rank)
     results, error = infinite_rows(dtype, rows, features, rank)
     for got, expected in results[2:]:
         infinite_where_expected(got, expected, error, dtype)
+
+# --------------------------------------------------------------------------
+# Scales far from one
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [2.0 ** -90, 2.0 ** 90, -(2.0 ** 100)])
+def test_adapted_linear_of_scales_far_from_one(dtype, scale):
+    """Inner values in float32's range, whatever the type: float16's results
+    are infinities there, and no NaN."""
+    adapted_case(400, 64, 40, 5, 8, dtype, scale=scale)
+    adapted_case(9, 64, 40, 5, 8, dtype, scale=scale)
+
+
+@gpu_test
+@pytest.mark.parametrize("scale", [2.0 ** 90, -(2.0 ** 100)])
+def test_wide_float16_layers_of_large_scales(scale):
+    """Sums of 1100 terms by tiles. Where the formula's value is past float16's
+    largest by more than the sums' error, it is an infinity of its sign. The
+    error is (1100 + 2) e of what the magnitudes add up to, 8 (the rank) * 21
+    (1100 products of mean 0.64 / sqrt(1100)) * 0.28 (of `up`) = 48 times the
+    scale, and as much again of the shared terms' bound: 6e-3 of values whose
+    spread is about 1, so half a percent of them say nothing."""
+    m, dtype = layers(), torch.float16
+    rows, features, outputs, groups, rank = 60, 1100, 40, 3, 8
+    x, g = normal(rows, features, seed=31, dtype=dtype), normal(rows, outputs, seed=36, dtype=dtype)
+    w = normal(outputs, features, seed=32, dtype=dtype, scale=features ** -0.5)
+    a = normal(groups, rank, features, seed=34, dtype=dtype, scale=features ** -0.5)
+    u = normal(groups, outputs, rank, seed=35, dtype=dtype, scale=rank ** -0.5)
+    by, members = grouped_by(some_groups(rows, groups, 31), groups)
+    on = x.cuda().requires_grad_()
+    y = m.adapted_linear(on, w.cuda(), a.cuda(), u.cuda(), by, scale=scale)
+    (dx,) = torch.autograd.grad(y, on, g.cuda())
+    want = oracle.adapted_linear(x, w, a, u, members, None, scale, g)
+    size = oracle.adapted_linear(x.abs(), w.abs(), a.abs(), u.abs(), members, None, abs(scale),
+                                 g.abs())
+    inside = torch.cat(members)
+    for got, expected, total in zip((y, dx), want, size):
+        got, error = got.detach().cpu().double(), 2 * (features + outputs) * E * total
+        assert not got.isnan().any()
+        past = expected.abs() - error > 65520
+        assert torch.equal(got[past], torch.sign(expected[past]) * math.inf)
+        assert past[inside].double().mean() > 0.97
+        none = torch.ones(rows, dtype=torch.bool)
+        none[inside] = False
+        near(got[none], expected[none], error[none], dtype)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features", [(9, 64), (400, 64), (60, 1100)])
+def test_adapted_linear_of_large_inner_rows_that_meet_zeros(dtype, rows, features):
+    """Adapters whose `up` is still zero, as training begins: the shared layer's
+    values, whatever the inner rows are."""
+    m = layers()
+    by, _ = grouped_by(some_groups(rows, 3, 4), 3)
+    x, w = normal(rows, features, seed=1, dtype=dtype).cuda(), normal(40, features, seed=2,
+                                                                   dtype=dtype).cuda()
+    a = normal(3, 8, features, seed=3, dtype=dtype).cuda()
+    u = torch.zeros(3, 40, 8, dtype=dtype, device="cuda")
+    want = m.adapted_linear(x, w, a, u, by, scale=0.0)
+    for scale in (1.0, 2.0 ** 20, 2.0 ** 60, 2.0 ** 80, 2.0 ** 110):
+        assert torch.equal(m.adapted_linear(x, w, a, u, by, scale=scale), want), scale
