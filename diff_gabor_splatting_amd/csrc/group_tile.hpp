@@ -14,9 +14,10 @@ namespace gs {
 //
 // They are float32 sums that go into another product. For float32 they are
 // kept as they are, 32 of the rank to a chunk of 128 bytes. For the 2-byte
-// types a chunk has two parts of 32, whose sum stands for the value to 16 bits
-// and more: the matrix instructions take both, so the inner rounding stays below
-// that of the output (one part would be a rounding as large as it). The
+// types a chunk has two parts of 32, each rounded to the nearest, whose sum stands
+// for the value to 17 bits or (float16) 22: the matrix instructions take both, so
+// the inner rounding, 2^-18 or 2^-23 of the largest, stays far below that of the
+// output (one part would be a rounding as large as it). The
 // rank's rest of the last chunk is zero. float16 could not hold large values, nor a
 // second part of small ones: its rows are divided by a power of two
 // that brings the largest value to 1/2 .. 1, and `scales` has it.
@@ -84,12 +85,11 @@ struct Inner {
         if constexpr (sizeof(T) == 4) {
           high[j] = f;
         } else {
-          // bfloat16's first part is cut off, so that it is never past the
-          // largest; the second then has the value's sign.
-          float first = f;
+          high[j] = T(f);
+          // Cut off where bfloat16's rounding would pass its largest.
           if constexpr (!scaled)
-            if (f == f) first = __uint_as_float(__float_as_uint(f) & 0xffff0000u);
-          high[j] = T(first);
+            if (finite_size(f) > 0.f && __builtin_fabsf(float(high[j])) == __builtin_inff())
+              high[j] = T(__uint_as_float(__float_as_uint(f) & 0xffff0000u));
           low[j] = finite_size(f) == __builtin_fabsf(f) ? T(f - float(high[j])) : T(0.f);
         }
       }

@@ -140,3 +140,32 @@ def test_adapted_linear_of_large_inner_rows_that_meet_zeros(dtype, rows, feature
     want = m.adapted_linear(x, w, a, u, by, scale=0.0)
     for scale in (1.0, 2.0 ** 20, 2.0 ** 60, 2.0 ** 80, 2.0 ** 110):
         assert torch.equal(m.adapted_linear(x, w, a, u, by, scale=scale), want), scale
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [9, 300])
+def test_inner_rows_hold_17_bits(dtype, rows):
+    """131071 is 17 ones: y is what is left of it beside 131072, forward and
+    backward."""
+    m = layers()
+    by, _ = grouped_by(torch.zeros(rows, dtype=torch.int64), 1)
+    x = torch.zeros(rows, 64, dtype=dtype)
+    x[:, :2] = torch.tensor([1.0, -1.0])
+    a = torch.zeros(1, 2, 64, dtype=dtype)
+    a[0, 0, 0], a[0, 0, 1], a[0, 1, 0] = 512, 2.0 ** -8, 512  # 512 - 2^-8 and 512
+    u = torch.zeros(1, 40, 2, dtype=dtype)
+    u[0, :, 0], u[0, :, 1] = 1, -1
+    on, w = x.cuda().requires_grad_(), torch.zeros(40, 64, dtype=dtype, device="cuda")
+    y = m.adapted_linear(on, w, a.cuda(), u.cuda(), by, scale=256.0)
+    assert (y == -1).all()
+    # The gradient's inner row: 131071 for rank 0 and 131072 for rank 1.
+    u = torch.zeros(1, 40, 2, dtype=dtype)
+    u[0, 0, 0], u[0, 1, 0], u[0, 0, 1] = 512, 2.0 ** -8, 512
+    a = torch.zeros(1, 2, 64, dtype=dtype)
+    a[0, 0], a[0, 1] = 1, -1
+    g = torch.zeros(rows, 40, dtype=dtype)
+    g[:, 0], g[:, 1] = 1, -1
+    y = m.adapted_linear(on, w, a.cuda(), u.cuda(), by, scale=256.0)
+    (dx,) = torch.autograd.grad(y, on, g.cuda())
+    assert (dx == -1).all()
