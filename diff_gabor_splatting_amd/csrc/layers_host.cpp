@@ -543,10 +543,11 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
                             const at::Tensor& weight, const at::Tensor& offsets,
                             const std::optional<at::Tensor>& order,
                             const std::optional<at::Tensor>& bias) {
-    const bool keep = weight.requires_grad() || (bias && bias->requires_grad());
     const Groups groups{offsets, order.value_or(at::Tensor())};
     at::Tensor y = grouped_rows(x, weight, groups, bias.value_or(at::Tensor()));
-    ctx->save_for_backward({keep ? x : at::Tensor(), weight, offsets, groups.order});
+    // The bias's gradient takes no rows of x.
+    ctx->save_for_backward(
+        {weight.requires_grad() ? x : at::Tensor(), weight, offsets, groups.order});
     ctx->saved_data["order"] = order.has_value();
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["shape"] = x.sizes().vec();
@@ -579,13 +580,15 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     if (has_bias && ctx->needs_input_grad(bias_at))
       db = at::empty({groups.count(), outputs}, grad.options());
     if (dw.defined() || db.defined()) {
-      const RowsOf r(saved[0]);
+      std::optional<RowsOf> r;
+      if (dw.defined()) r.emplace(saved[0]);
       const at::Tensor space = workspace(
           api.grouped_workspace(type, g.rows, groups.count(), features, outputs), grad.device());
       check(api.grouped_backward_weight(
-          type, g.data(), g.stride, r.data(), r.stride, groups.places(), groups.begins(), g.rows,
-          groups.count(), features, outputs, const_cast<void*>(data_of(dw)),
-          const_cast<void*>(data_of(db)), space.data_ptr(), size_t(space.numel()), stream));
+          type, g.data(), g.stride, r ? r->data() : nullptr, r ? r->stride : features,
+          groups.places(), groups.begins(), g.rows, groups.count(), features, outputs,
+          const_cast<void*>(data_of(dw)), const_cast<void*>(data_of(db)), space.data_ptr(),
+          size_t(space.numel()), stream));
     }
     return once({dx, dw, at::Tensor(), at::Tensor(), db}, "grouped_linear");
   }

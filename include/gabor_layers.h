@@ -126,7 +126,8 @@ int gs_grouped_linear_backward_input(int32_t dtype, const void* grad_y, int64_t 
                                      int64_t features, int64_t outputs, void* grad_x,
                                      void* stream);
 /* grad_weight[g] = the sum over group g's rows of grad_y^T x, grad_bias[g] the
- * sum of grad_y (either may be null; zero for a group without rows). */
+ * sum of grad_y (either may be null, and without grad_weight x, too; zero for a
+ * group without rows). */
 size_t gs_grouped_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows,
                                                         int64_t groups, int64_t features,
                                                         int64_t outputs);

@@ -5,6 +5,7 @@ change under a captured graph, and memory beside the results.
 Tolerances as in test_parts.py.
 """
 
+import ctypes
 import math
 
 import pytest
@@ -169,3 +170,44 @@ def test_inner_rows_hold_17_bits(dtype, rows):
     y = m.adapted_linear(on, w, a.cuda(), u.cuda(), by, scale=256.0)
     (dx,) = torch.autograd.grad(y, on, g.cuda())
     assert (dx == -1).all()
+
+# --------------------------------------------------------------------------
+# Gradients asked for alone
+
+
+def db_needs_no_rows(backward_weight, need, kept):
+    """The bias's gradient of no rows' values: `x` (or what is kept of it) is not
+    asked for. (On the CPU: a call that is refused for another reason.)"""
+    from diff_gabor_splatting_amd import _native
+
+    status = backward_weight(kept, need - 1)
+    assert status == 4 and "workspace" in _native.lib.gs_last_error().decode()
+
+
+def test_grouped_bias_gradient_takes_no_rows():
+    from diff_gabor_splatting_amd import _native
+
+    lib, p = _native.lib, ctypes.c_void_p(256)
+    need = lib.gs_grouped_linear_backward_weight_workspace_size(0, 5000, 4, 64, 64)
+    db_needs_no_rows(lambda x, size: lib.gs_grouped_linear_backward_weight(
+        0, p, 64, x, 64, p, p, 5000, 4, 64, 64, None, p, p, size, None), need, None)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs,groups", [
+    (900, 40, 24, 6), (3000, 300, 5, 4), (3000, 5, 300, 4), (700, 700, 130, 3),
+    (130_000, 512, 512, 7), (3000, 1030, 40, 300)])
+def test_grouped_bias_gradient_alone(dtype, rows, features, outputs, groups):
+    """The sums of dy, whatever the shares; the rows are not kept for them."""
+    m = layers()
+    by, members = grouped_by(some_groups(rows, groups, 3), groups)
+    x = normal(rows, features, seed=1, dtype=dtype).cuda()
+    w = normal(groups, outputs, features, seed=2, dtype=dtype).cuda()
+    b = normal(groups, outputs, seed=3, dtype=dtype).cuda().requires_grad_()
+    g = normal(rows, outputs, seed=4, dtype=dtype)
+    y = m.grouped_linear(x, w, by, b)
+    x.mul_(2)  # raises in the backward pass where x is kept
+    (got,) = torch.autograd.grad(y, b, g.cuda())
+    want, size = (torch.stack([t.double()[at].sum(0) for at in members]) for t in (g, g.abs()))
+    near(got, want, max(len(at) for at in members) * E * size, dtype)
