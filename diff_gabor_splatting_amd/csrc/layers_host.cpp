@@ -383,9 +383,9 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& weight, const at::
 struct Linear : torch::autograd::Function<Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
                             const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
-    const bool keep = weight.requires_grad() || (bias && bias->requires_grad());
-    Kept kept;
-    at::Tensor y = linear_rows(x, weight, bias.value_or(at::Tensor()), keep ? &kept : nullptr);
+    Kept kept;  // the bias's gradient takes none
+    at::Tensor y = linear_rows(x, weight, bias.value_or(at::Tensor()),
+                               weight.requires_grad() ? &kept : nullptr);
     ctx->save_for_backward({weight, kept.values, kept.exponents});
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["shape"] = x.sizes().vec();
@@ -639,12 +639,13 @@ struct AdaptedLinear : torch::autograd::Function<AdaptedLinear> {
                             const std::optional<at::Tensor>& order,
                             const std::optional<at::Tensor>& bias, double scale) {
     const Groups groups{offsets, order.value_or(at::Tensor())};
-    const bool shared = weight.requires_grad() || (bias && bias->requires_grad());
+    // The bias's gradient takes no rows of x.
+    const bool keep = weight.requires_grad() || down.requires_grad();
     at::Tensor inner;
     at::Tensor y = adapted_rows(x, weight, down, up, groups, bias.value_or(at::Tensor()), scale,
                                 up.requires_grad() ? &inner : nullptr);
-    ctx->save_for_backward({shared || down.requires_grad() ? x : at::Tensor(), weight, down, up,
-                            offsets, groups.order, inner});
+    ctx->save_for_backward({keep ? x : at::Tensor(), weight, down, up, offsets, groups.order,
+                            inner});
     ctx->saved_data["order"] = order.has_value();
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["scale"] = scale;
@@ -694,13 +695,16 @@ struct AdaptedLinear : torch::autograd::Function<AdaptedLinear> {
     if (has_bias && ctx->needs_input_grad(has_order ? 6 : 5))
       db = at::empty({outputs}, grad.options());
     if (dw.defined() || db.defined()) {
-      const Kept kept = Kept::empty(g.rows, features, grad.device());
-      check(api.checkpoint_write(type, x->data(), x->stride, g.rows, features,
-                                 kept.values.data_ptr(), kept.exponents.data_ptr(), stream));
+      Kept kept;
+      if (dw.defined()) {
+        kept = Kept::empty(g.rows, features, grad.device());
+        check(api.checkpoint_write(type, x->data(), x->stride, g.rows, features,
+                                   kept.values.data_ptr(), kept.exponents.data_ptr(), stream));
+      }
       const at::Tensor space =
           workspace(api.linear_workspace(type, g.rows, features, outputs), grad.device());
       check(api.linear_backward_weight(
-          type, g.data(), g.stride, kept.values.data_ptr(), kept.exponents.data_ptr(), g.rows,
+          type, g.data(), g.stride, data_of(kept.values), data_of(kept.exponents), g.rows,
           features, outputs, const_cast<void*>(data_of(dw)), const_cast<void*>(data_of(db)),
           space.data_ptr(), size_t(space.numel()), stream));
     }

@@ -615,6 +615,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict_
 // at least to each, 128 from eight tiles on. Where the shares are no multiple of
 // the eight XCDs some XCDs have one more of them than others (600 -> 600: 20
 // shares of 25 tiles, 390 us for 200k rows where 127 would do).
+//
+// The bias's gradient alone goes by one feature's plan and reads none: the grid
+// has one column of tiles, which multiplies zeros (a pass of 1M x 512 -> 512
+// bfloat16 197 us, 589 with the matrix's gradient).
 struct SumPlan {
   int a, b, step;
   int64_t tiles_m, tiles_n, splits, share;
@@ -859,8 +863,11 @@ size_t gs_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows, int
   using namespace gs;
   if (rows <= 0 || features <= 0 || outputs <= 0) return 0;
   const size_t size = dtype == GS_FLOAT32 ? 4 : 2;
-  return size_t(sum_plan(size, rows, features, outputs).splits) *
-         size_t(outputs * (features + 1)) * sizeof(float);
+  auto bytes = [&](int64_t planned, int64_t values) {
+    return size_t(sum_plan(size, rows, planned, outputs).splits) * size_t(outputs * values) *
+           sizeof(float);
+  };
+  return std::max(bytes(features, features + 1), bytes(1, 1));
 }
 
 int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_stride,
@@ -873,7 +880,7 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
   GS_CHECK(check_linear("gs_linear_backward_weight", dtype, rows, features, outputs));
   GS_CHECK(check_rows("gs_linear_backward_weight", dtype, rows, outputs, grad_stride));
   if (!grad_weight && !grad_bias) return GS_OK;
-  GS_REQUIRE(rows == 0 || (grad_y && values && exponents), GS_ERR_ARGUMENT,
+  GS_REQUIRE(rows == 0 || (grad_y && ((values && exponents) || !grad_weight)), GS_ERR_ARGUMENT,
              "null pointer passed to gs_linear_backward_weight");
   const size_t need =
       gs_linear_backward_weight_workspace_size(dtype, rows, features, outputs);
@@ -883,10 +890,11 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     int64_t splits = 0;
+    const int64_t across = grad_weight ? features : 0;
     if (rows > 0) {
-      const SumPlan plan = sum_plan(sizeof(T), rows, features, outputs);
+      const SumPlan plan = sum_plan(sizeof(T), rows, grad_weight ? features : 1, outputs);
       splits = plan.splits;
-      const SumProduct p{rows, grad_stride, int(outputs), int(features), int(plan.tiles_m),
+      const SumProduct p{rows, grad_stride, int(outputs), int(across), int(plan.tiles_m),
                          int(plan.tiles_n), int(splits), plan.share};
       const int64_t blocks =
           (splits >= 8 ? ceil_div(splits, 8) * 8 : splits) * plan.tiles_m * plan.tiles_n;
@@ -923,7 +931,7 @@ int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_st
         if (shape == 44) GS_CHECK(launch(four{}, four{}, wide{}));
       }
     }
-    const int64_t weights = outputs * features, size = weights + outputs;
+    const int64_t weights = outputs * across, size = weights + outputs;
     // Enough workgroups to fill the chip with few values, too: 65,792 values of
     // 128 partial results take 9.2 us with one slice and 6.2 with four, 147,840
     // 7.1 and 7.2.

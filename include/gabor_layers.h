@@ -79,7 +79,7 @@ int gs_linear_backward_input(int32_t dtype, const void* grad_y, int64_t grad_str
                              const void* weight, int64_t rows, int64_t features, int64_t outputs,
                              void* grad_x, void* stream);
 /* grad_weight = grad_y^T (kept x), grad_bias = the sum of grad_y's rows
- * (either may be null). */
+ * (either may be null, and without grad_weight the kept x, too). */
 size_t gs_linear_backward_weight_workspace_size(int32_t dtype, int64_t rows, int64_t features,
                                                 int64_t outputs);
 int gs_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t grad_stride,

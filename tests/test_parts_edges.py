@@ -211,3 +211,39 @@ def test_grouped_bias_gradient_alone(dtype, rows, features, outputs, groups):
     (got,) = torch.autograd.grad(y, b, g.cuda())
     want, size = (torch.stack([t.double()[at].sum(0) for at in members]) for t in (g, g.abs()))
     near(got, want, max(len(at) for at in members) * E * size, dtype)
+
+
+def test_linear_bias_gradient_takes_no_rows():
+    from diff_gabor_splatting_amd import _native
+
+    lib, p = _native.lib, ctypes.c_void_p(256)
+    need = lib.gs_linear_backward_weight_workspace_size(0, 5000, 64, 64)
+    db_needs_no_rows(lambda kept, size: lib.gs_linear_backward_weight(
+        0, p, 64, kept, kept, 5000, 64, 64, None, p, p, size, None), need, None)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs", [(900, 40, 24), (3000, 300, 5), (3000, 5, 300),
+                                                   (700, 700, 130), (130_000, 512, 512)])
+def test_shared_bias_gradient_alone(dtype, rows, features, outputs):
+    """Of linear and of adapted_linear: the sums of dy, and nothing of the rows is
+    kept for them."""
+    m = layers()
+    by, _ = grouped_by(some_groups(rows, 5, 3), 5)
+    x = normal(rows, features, seed=1, dtype=dtype).cuda()
+    w, b = normal(outputs, features, seed=2, dtype=dtype).cuda(), normal(outputs, seed=3,
+                                                                       dtype=dtype).cuda()
+    a, u = normal(5, 4, features, seed=5, dtype=dtype).cuda(), normal(5, outputs, 4, seed=6,
+                                                                     dtype=dtype).cuda()
+    g = normal(rows, outputs, seed=4, dtype=dtype)
+    b.requires_grad_()
+    before = torch.cuda.memory_allocated()
+    y = m.linear(x, w, b)
+    # (Memory is handed out in steps of 512 bytes.)
+    assert torch.cuda.memory_allocated() - before < y.nbytes + rows * features
+    z = m.adapted_linear(x, w, a, u, by, b)
+    x.mul_(2)  # raises in the backward pass where x is kept
+    for out in (y, z):
+        (got,) = torch.autograd.grad(out, b, g.cuda())
+        near(got, g.double().sum(0), rows * E * g.double().abs().sum(0), dtype)
