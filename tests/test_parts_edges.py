@@ -247,3 +247,81 @@ def test_shared_bias_gradient_alone(dtype, rows, features, outputs):
     for out in (y, z):
         (got,) = torch.autograd.grad(out, b, g.cuda())
         near(got, g.double().sum(0), rows * E * g.double().abs().sum(0), dtype)
+
+# --------------------------------------------------------------------------
+# Many rows: small whole numbers, whose sums float32 holds exactly in any order
+
+
+def whole_numbers(seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def whole(*shape, dtype):
+        return torch.randint(-1, 2, shape, generator=gen, device="cuda").to(dtype)
+
+    return whole
+
+
+def rows_of(by, group, bounds):
+    return by.order[bounds[group]:bounds[group + 1]].long()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype,rows,features,outputs,groups", [
+    # The widest tiles of dW, 256 x 256: one with empty edges, several with
+    # both edges ragged, and groups that end within a share.
+    *((d, *size) for d in (torch.bfloat16, torch.float16)
+      for size in ((600_001, 200, 200, 5), (100_003, 500, 508, 64), (60_000, 700, 508, 200))),
+    # Parts joined by 64, 16 and 4 slices.
+    *((d, 70_001, 40, 24, groups) for d in DTYPES for groups in (3, 6, 20))])
+def test_grouped_linear_of_many_rows(dtype, rows, features, outputs, groups):
+    m, whole = layers(), whole_numbers(rows + groups)
+    x, g = whole(rows, features, dtype=dtype).requires_grad_(), whole(rows, outputs, dtype=dtype)
+    w = whole(groups, outputs, features, dtype=dtype).requires_grad_()
+    b = whole(groups, outputs, dtype=dtype).requires_grad_()
+    by = m.row_groups(some_groups(rows, groups, 5, none=0.01).cuda(), groups)
+    y = m.grouped_linear(x, w, by, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    bounds = by.offsets.tolist()
+    for group in range(groups):
+        at = rows_of(by, group, bounds)
+        part, d, matrix = x[at].detach().double(), g[at].double(), w[group].detach().double()
+        assert torch.equal(y[at], (part @ matrix.t() + b[group].double()).to(dtype))
+        assert torch.equal(dx[at], (d @ matrix).to(dtype))
+        assert torch.equal(dw[group], (d.t() @ part).to(dtype))
+        assert torch.equal(db[group], d.sum(0).to(dtype))
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,outputs,groups,rank", [
+    (70_001, 40, 24, 3, 5),      # 64 slices
+    (70_001, 40, 24, 12, 16),    # 16
+    (70_001, 40, 24, 40, 33),    # 4
+    (300_001, 72, 57, 7, 40),
+    (300_001, 256, 136, 9, 64)])
+def test_adapted_linear_of_many_rows(dtype, rows, features, outputs, groups, rank):
+    """Inner values are whole halves below 2^15, which two parts hold."""
+    m, whole = layers(), whole_numbers(rows + groups)
+    x, g = whole(rows, features, dtype=dtype).requires_grad_(), whole(rows, outputs, dtype=dtype)
+    w, b = whole(outputs, features, dtype=dtype), whole(outputs, dtype=dtype)
+    a = whole(groups, rank, features, dtype=dtype).requires_grad_()
+    u = whole(groups, outputs, rank, dtype=dtype).requires_grad_()
+    by = m.row_groups(some_groups(rows, groups, 5, none=0.01).cuda(), groups)
+    y = m.adapted_linear(x, w, a, u, by, b, scale=0.5)
+    dx, da, du = torch.autograd.grad(y, (x, a, u), g)
+    bounds = by.offsets.tolist()
+    inside = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    shared = w.double()
+    for group in range(groups):
+        at = rows_of(by, group, bounds)
+        inside[at] = True
+        part, d = x[at].detach().double(), g[at].double()
+        down, up = a[group].detach().double(), u[group].detach().double()
+        inner, back = 0.5 * part @ down.t(), 0.5 * d @ up
+        assert torch.equal(y[at], (part @ shared.t() + b.double() + inner @ up.t()).to(dtype))
+        assert torch.equal(dx[at], (d @ shared + back @ down).to(dtype))
+        assert torch.equal(da[group], (back.t() @ part).to(dtype))
+        assert torch.equal(du[group], (d.t() @ inner).to(dtype))
+    rest = ~inside
+    assert torch.equal(y[rest], (x[rest].double() @ shared.t() + b.double()).to(dtype))
+    assert torch.equal(dx[rest], (g[rest].double() @ shared).to(dtype))
