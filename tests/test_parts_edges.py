@@ -325,3 +325,49 @@ def test_adapted_linear_of_many_rows(dtype, rows, features, outputs, groups, ran
     rest = ~inside
     assert torch.equal(y[rest], (x[rest].double() @ shared.t() + b.double()).to(dtype))
     assert torch.equal(dx[rest], (g[rest].double() @ shared).to(dtype))
+
+# --------------------------------------------------------------------------
+# Groups that change under a captured graph
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype,rows", [(torch.bfloat16, 700), (torch.float32, 9000)])
+def test_graphs_take_the_groups_of_each_replay(dtype, rows):
+    """A captured launch holds any groups: each replay sorts the rows anew and
+    goes by what it finds."""
+    m = layers()
+    x = normal(rows, 72, seed=1, dtype=dtype)
+    w, b = normal(6, 64, 72, seed=2, dtype=dtype, scale=0.1), normal(6, 64, seed=3, dtype=dtype)
+    shared, bias = normal(57, 64, seed=4, dtype=dtype, scale=0.1), normal(57, seed=5, dtype=dtype)
+    down = normal(6, 8, 64, seed=6, dtype=dtype, scale=0.1)
+    up = normal(6, 57, 8, seed=7, dtype=dtype, scale=0.3)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b, shared, bias, down, up)]
+    grad = normal(rows, 57, seed=8, dtype=dtype).cuda()
+    index = some_groups(rows, 6, 9).cuda()
+
+    def step(index):
+        x, w, b, shared, bias, down, up = leaves
+        by = m.row_groups(index, 6)
+        h = m.grouped_linear(x, w, by, b)
+        y = m.adapted_linear(h, shared, down, up, by, bias, scale=0.5)
+        grads = torch.autograd.grad(y, leaves, grad)
+        return (y.detach(), h.detach(), by.order, by.offsets, *grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(index)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(index)
+    all_rows = torch.full((rows,), 4)
+    uneven = torch.where(torch.arange(rows) == 17, 5, 0)
+    for other in (some_groups(rows, 6, 10), all_rows, all_rows - 5, torch.arange(rows) % 6, uneven,
+                  some_groups(rows, 6, 9)):
+        index.copy_(other)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step(index.clone())):
+            assert torch.equal(got, want)
