@@ -371,3 +371,93 @@ def test_graphs_take_the_groups_of_each_replay(dtype, rows):
         torch.cuda.synchronize()
         for got, want in zip(out, step(index.clone())):
             assert torch.equal(got, want)
+
+# --------------------------------------------------------------------------
+# Memory beside the results
+
+SENTINEL, MARGIN = 0x5A, 1 << 16
+
+
+class Guarded:
+    """`count` bytes between margins that a call must leave as they are."""
+
+    def __init__(self, count):
+        self.count = count
+        self.all = torch.full((count + 2 * MARGIN,), SENTINEL, dtype=torch.uint8, device="cuda")
+
+    @property
+    def pointer(self):
+        return ctypes.c_void_p(self.all.data_ptr() + MARGIN)
+
+    def intact(self):
+        return bool((self.all[:MARGIN] == SENTINEL).all()) and \
+            bool((self.all[MARGIN + self.count:] == SENTINEL).all())
+
+
+def malformed_groups(rows, groups):
+    """Offsets that fall, pass the rows or are below zero, and places that are
+    not rows."""
+    gen = torch.Generator().manual_seed(rows + groups)
+    wild = lambda *shape: torch.randint(-(1 << 31), 1 << 31, shape, generator=gen)  # noqa: E731
+    near_by = lambda *shape: torch.randint(-40, rows + 40, shape, generator=gen)  # noqa: E731
+    for offsets in (wild(groups + 1), near_by(groups + 1), near_by(groups + 1).sort().values,
+                    near_by(groups + 1).sort(descending=True).values,
+                    torch.full((groups + 1,), rows), torch.full((groups + 1,), 1 << 30)):
+        for order in (None, wild(rows), near_by(rows)):
+            yield (offsets.to(torch.int32).cuda(),
+                   None if order is None else order.to(torch.int32).cuda())
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,features,outputs,groups,rank", [
+    (12, 72, 57, 6, 8), (700, 72, 57, 6, 8), (700, 72, 130, 130, 40), (3000, 1100, 40, 5, 8),
+    (3000, 40, 1100, 5, 33)])
+def test_wrong_groups_write_nothing_beside_the_results(dtype, rows, features, outputs, groups, rank):
+    """The C entry points with groups that are none: what is written is the
+    results, the inner rows and the workspace."""
+    from diff_gabor_splatting_amd import _native
+
+    lib, size = _native.lib, 4 if dtype == 0 else 2
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    held = {name: torch.zeros(count * size, dtype=torch.uint8, device="cuda") for name, count in (
+        ("x", rows * features), ("g", rows * outputs), ("w", groups * outputs * features),
+        ("b", groups * outputs), ("down", groups * rank * features),
+        ("up", groups * outputs * rank))}
+    p = {name: ctypes.c_void_p(t.data_ptr()) for name, t in held.items()}
+    inner_size = lib.gs_adapted_linear_inner_size(rows, rank)
+    sum_size = lib.gs_grouped_linear_backward_weight_workspace_size(dtype, rows, groups, features,
+                                                                    outputs)
+    narrow_size = lib.gs_adapted_linear_backward_adapters_workspace_size(rows, groups, features,
+                                                                         outputs, rank)
+    for offsets, order in malformed_groups(rows, groups):
+        at = ctypes.c_void_p(offsets.data_ptr())
+        by = None if order is None else ctypes.c_void_p(order.data_ptr())
+        y, dx, z, dz = (Guarded(rows * n * size) for n in (outputs, features, outputs, features))
+        dw, db = Guarded(groups * outputs * features * size), Guarded(groups * outputs * size)
+        da, du = Guarded(groups * rank * features * size), Guarded(groups * outputs * rank * size)
+        inner, back = Guarded(inner_size), Guarded(inner_size)
+        sums, narrow = Guarded(sum_size), Guarded(narrow_size)
+        calls = (
+            lib.gs_grouped_linear_forward(dtype, p["x"], features, p["w"], p["b"], by, at, rows,
+                                          groups, features, outputs, y.pointer, stream),
+            lib.gs_grouped_linear_backward_input(dtype, p["g"], outputs, p["w"], by, at, rows, groups,
+                                                 features, outputs, dx.pointer, stream),
+            lib.gs_grouped_linear_backward_weight(
+                dtype, p["g"], outputs, p["x"], features, by, at, rows, groups, features, outputs,
+                dw.pointer, db.pointer, sums.pointer, sum_size, stream),
+            lib.gs_adapted_linear_forward(
+                dtype, p["x"], features, p["w"], p["b"], p["down"], p["up"], 0.5, by, at, rows,
+                groups, features, outputs, rank, inner.pointer, inner_size, z.pointer, stream),
+            lib.gs_adapted_linear_backward_input(
+                dtype, p["g"], outputs, p["w"], p["down"], p["up"], 0.5, by, at, rows, groups,
+                features, outputs, rank, back.pointer, inner_size, dz.pointer, stream),
+            lib.gs_adapted_linear_backward_adapters(
+                dtype, p["g"], outputs, p["x"], features, inner.pointer, back.pointer, by, at, rows,
+                groups, features, outputs, rank, da.pointer, du.pointer, narrow.pointer, narrow_size,
+                stream))
+        assert calls == (0,) * 6, lib.gs_last_error()
+        torch.cuda.synchronize()
+        for name, buffer in dict(y=y, dx=dx, z=z, dz=dz, dw=dw, db=db, da=da, du=du, inner=inner,
+                                 back=back, sums=sums, narrow=narrow).items():
+            assert buffer.intact(), name
