@@ -9,8 +9,8 @@
 // 65536 / (65536 - t), so the mean is that of x whatever p was rounded to.
 // 16 bits a value and not 32: the ten rounds of two 32 x 32 products each are
 // what a lane spends its time on beside its loads, and they serve eight
-// values this way. 1M x 512 bfloat16: 367 to 405 us a pass, 5.6 TB/s at the
-// least; the vector units issue for 71% of it.
+// values this way. 1M x 512 bfloat16: 367 us a pass, 5.6 TB/s (410 under the
+// profiler); the vector units issue for 72% of it.
 #include "layers_api.hpp"
 
 namespace gs {

@@ -13,10 +13,10 @@ namespace gs {
 // its rows, so that putting a matrix in place counts too (64 to 1,024 rows give
 // the same times).
 //
-// 1M x 512 -> 512 bfloat16 in 32 groups: y 615 us, dx 592 (850 to 890 TFLOP/s),
-// as long as with one matrix for all rows: matrix cores 41% busy, LDS 46%, the
-// address unit 62%. With the adapters' steps (rank 16) 670 and 660; inner rows
-// 243 and 253, bound by the address unit (80%).
+// 1M x 512 -> 512 bfloat16 in 32 groups: y 613 us, dx 591 (850 to 890 TFLOP/s),
+// as long as with one matrix for all rows: matrix cores 40% busy, LDS 46%, the
+// address unit 64%. With the adapters' steps (rank 16) 665 and 654; inner rows
+// 242 and 254, bound by the address unit (80%).
 constexpr int64_t kStageCost = 64;  // of a matrix, in rows
 
 __device__ __forceinline__ int64_t stage_line(const Grouping& g, int s) {
@@ -27,7 +27,8 @@ struct GroupRows {
   int64_t stride;
   int k, n;          // length of the sum and columns of C
   int panels;        // workgroups side by side, each with its columns of C
-  int workers;       // workgroups to a panel
+  int workers;       // workgroups to a panel, 32 / panels to an XCD at most: with
+                     // 17 panels 15 of its compute units have none
   int steps;         // of the sum, of 128 bytes of a row
   int all;           // those, the adapters' chunks, and as many as make the
                      // whole a multiple of those under way

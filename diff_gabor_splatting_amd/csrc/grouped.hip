@@ -151,8 +151,8 @@ __global__ __launch_bounds__(kThreads) void group_few_kernel(
 // tile counts too. A group whose part of the line lies in one share is
 // written at once; the others' parts are joined after.
 //
-// 1M x 512 -> 512 bfloat16 in 32 groups: 824 us (636 TFLOP/s), matrix cores 30%
-// busy, LDS 20%: the waves wait at a step's barrier and for what lies between
+// 1M x 512 -> 512 bfloat16 in 32 groups: 794 us (660 TFLOP/s), matrix cores 30%
+// busy, LDS 21%: the waves wait at a step's barrier and for what lies between
 // LDS and its first product. 100k x 256 -> 256 in 64 groups: 48 us, and 14 for the
 // joining. One loop for both halves of a pair of steps: groups that end in
 // either half cost 80 registers more.

@@ -125,7 +125,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:
     """``x weight^T + bias`` with ``weight`` [outputs, features], all of one
     type. The weight's gradient is taken with the input as kept in 8 bits; the
-    input's gradient does not depend on it."""
+    other gradients do not depend on it."""
     return _host.linear(_tensor("x", x), _tensor("weight", weight), bias)
 
 
@@ -205,8 +205,8 @@ def grouped_linear(x: Tensor, weight: Tensor, groups: RowGroups,
     """``x weight[g]^T + bias[g]`` for the rows of group g, 0 for rows of no
     group (whose gradient is 0, too). ``weight`` [groups, outputs, features]
     and ``bias`` [groups, outputs] have the type of ``x``. Rows are read and
-    written where they lie. The backward pass reads ``x`` itself, which the
-    parameters' gradients are those of."""
+    written where they lie. The backward pass reads ``x`` itself, for the
+    matrices' gradients."""
     groups = _groups(groups)
     return _host.grouped_linear(_tensor("x", x), _tensor("weight", weight), groups.offsets,
                                 groups.order, bias)
@@ -221,8 +221,8 @@ def adapted_linear(x: Tensor, weight: Tensor, down: Tensor, up: Tensor, groups: 
     and ``up`` [groups, outputs, rank] have the type of ``x``; the rank is at
     most 64. The backward pass reads ``x`` itself for the adapters' gradients, and
     the shared matrix's gradient is that of :func:`linear`, taken with the
-    input in 8 bits; none is computed that is not asked for. What an infinity
-    in an adapter's matrix meets is NaN."""
+    input in 8 bits; none is computed that is not asked for. An infinity in an
+    adapter's matrix may give NaN where the formula has an infinity."""
     groups = _groups(groups)
     _number("scale", scale)
     # As the kernels take it: a larger number is an infinity there.
