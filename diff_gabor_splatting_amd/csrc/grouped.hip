@@ -581,7 +581,7 @@ int gs_grouped_linear_backward_weight(int32_t dtype, const void* grad_y, int64_t
   const char* const name = "gs_grouped_linear_backward_weight";
   GS_CHECK(check_grouped(name, dtype, offsets, rows, groups, features, outputs));
   GS_CHECK(check_rows(name, dtype, rows, outputs, grad_stride));
-  GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
+  if (grad_weight) GS_CHECK(check_rows(name, dtype, rows, features, row_stride));
   if (!grad_weight && !grad_bias) return GS_OK;
   GS_REQUIRE(offsets && (rows == 0 || (grad_y && (x || !grad_weight))), GS_ERR_ARGUMENT,
              "null pointer passed to %s", name);

@@ -190,7 +190,7 @@ def test_grouped_bias_gradient_takes_no_rows():
     lib, p = _native.lib, ctypes.c_void_p(256)
     need = lib.gs_grouped_linear_backward_weight_workspace_size(0, 5000, 4, 64, 64)
     db_needs_no_rows(lambda x, size: lib.gs_grouped_linear_backward_weight(
-        0, p, 64, x, 64, p, p, 5000, 4, 64, 64, None, p, p, size, None), need, None)
+        0, p, 64, x, 0, p, p, 5000, 4, 64, 64, None, p, p, size, None), need, None)
 
 
 @gpu_test
